@@ -358,6 +358,109 @@ int wf_attn_dense_bf16(const void* q, int64_t lq, int32_t n_heads,
                        float softmax_scale, void* out, int64_t ldo,
                        void* stream);
 
+/* ---------------------------------------------------------------------
+ * A batch of sequences over one page pool
+ *
+ * Several generation streams in one launch.  Sequence b (b < n_seqs) owns the
+ * rows cu_new[b] .. cu_new[b + 1] of the ragged row tensors (cu_new int32
+ * [n_seqs + 1], cu_new[0] = 0, not decreasing; rows from cu_new[n_seqs] on
+ * are padding and are left as they are).  kv_lens[b] (int32) positions are
+ * in its cache, those of its rows last: row i of the sequence stands at
+ * position kv_lens[b] - (cu_new[b + 1] - cu_new[b]) + i.  Position p lives in
+ * physical page tables[b][p / page_tokens] (int32 [n_seqs][ld_table]), row
+ * p % page_tokens, of pools laid out as for wf_fp8_kv_pack with n_kv_heads
+ * heads; a position that is negative, past the table or on a page outside
+ * [0, pool_pages) is not written, and read as above (gather: the row is left
+ * as it is; attention: zero K and V).  cu_new, kv_lens and tables are read on
+ * the device when the work runs, so a captured graph follows their contents.
+ * head_dim is 128; a pool has fewer than 2^31 (position, head) rows and may
+ * have any size in bytes; page_tokens >= 1.
+ *
+ * Formats of a page:
+ *   WF_KV_E4M3  wf_fp8_kv_pack's codes and scales;
+ *   WF_KV_INT8  s = max(max|x| / 127, 1e-8), code = clamp(rint(x / s), -127,
+ *               127) (fp32; wf_act_quant_i8's arithmetic per (token, head)),
+ *               the codes as signed bytes.
+ * ------------------------------------------------------------------- */
+
+#define WF_KV_E4M3 0
+#define WF_KV_INT8 1
+
+/* Quantize the rows of K and V (bf16 [n_rows][n_kv_heads][128], row stride
+ * ld_kv; V may be NULL with its pools) into their positions' pages.  A row
+ * of a head that holds a NaN or an infinity is stored as scale NaN and zero
+ * codes, and reads back as NaN.  Positions of different rows must differ.
+ * The reference appends one sequence's chunk per call
+ * (wave_rt/denoiser/exchange/paged.py:120-145). */
+int wf_kv_batch_append(const void* k, const void* v, int64_t n_rows,
+                       int32_t n_kv_heads, int32_t head_dim, int64_t ld_kv,
+                       int32_t format, const int32_t* cu_new,
+                       const int32_t* kv_lens, int64_t n_seqs,
+                       const int32_t* tables, int64_t ld_table,
+                       int32_t page_tokens, uint8_t* k_codes,
+                       uint8_t* v_codes, float* k_scales, float* v_scales,
+                       int64_t pool_pages, void* stream);
+
+/* The rows' positions read back: bf16(float(code) * s), K and V (V may be
+ * NULL) bf16 [n_rows][n_kv_heads][128] with row stride ld_out.  With
+ * cu_new the running sum of kv_lens, the sequences' whole caches. */
+int wf_kv_batch_gather(const uint8_t* k_codes, const uint8_t* v_codes,
+                       const float* k_scales, const float* v_scales,
+                       int64_t pool_pages, int32_t format,
+                       int32_t page_tokens, const int32_t* cu_new,
+                       const int32_t* kv_lens, int64_t n_seqs,
+                       const int32_t* tables, int64_t ld_table,
+                       int64_t n_rows, int32_t n_kv_heads, int32_t head_dim,
+                       void* k_out, void* v_out, int64_t ld_out, void* stream);
+
+/* Workspace bytes of wf_attn_paged_batch (paged != 0) or wf_attn_cross_batch
+ * (paged == 0) with these sizes, into *bytes (host memory). */
+int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads,
+                            int32_t n_kv_heads, int64_t n_seqs,
+                            int64_t max_new, int64_t max_kv, int32_t paged,
+                            int64_t* bytes);
+
+/* Attention of the rows' queries q [n_rows][n_heads][128] (row stride ldq)
+ * over their sequences' caches, query head h on key head
+ * h / (n_heads / n_kv_heads):
+ *   out = softmax_j(softmax_scale * <q, code_k[j] s_k[j]>) . code_v[j] s_v[j]
+ * over the keys j < lim, lim = kv_lens[b] when block == 0, else
+ * min(kv_lens[b], (p / block + 1) * block) for the row's position p: every
+ * key, causal (block 1), or causal by blocks of `block` positions (a frame,
+ * a chunk).  Rows without a key are zero; keys a row does not see do not
+ * reach it, whatever they hold.  fp32 scores, softmax and sums; the weights
+ * p_j s_v[j] are rounded to bf16 for the second product.  max_new and max_kv
+ * bound the sequences' rows and keys; they choose the split, and results
+ * stay right where the device's lengths pass them.  ws: ws_bytes of scratch,
+ * 16-byte aligned, at least wf_attn_batch_workspace's.  The attention of
+ * wf_attn_paged_fp8 for a batch (wave_rt/runtime/backend.py:141-148), with
+ * the block-causal mask of naive_rt/rolling_forcing/wan/modules/
+ * causal_model.py as an argument. */
+int wf_attn_paged_batch(const void* q, int64_t n_rows, int32_t n_heads,
+                        int32_t n_kv_heads, int32_t head_dim, int64_t ldq,
+                        int32_t format, const uint8_t* k_codes,
+                        const uint8_t* v_codes, const float* k_scales,
+                        const float* v_scales, int64_t pool_pages,
+                        int32_t page_tokens, const int32_t* cu_new,
+                        const int32_t* kv_lens, int64_t n_seqs,
+                        const int32_t* tables, int64_t ld_table,
+                        int64_t max_new, int64_t max_kv, int32_t block,
+                        float softmax_scale, void* out, int64_t ldo, void* ws,
+                        int64_t ws_bytes, void* stream);
+
+/* The same over dense bf16 keys: sequence b's are the rows cu_kv[b] ..
+ * cu_kv[b + 1] of k and v [n_kv_rows][n_kv_heads][128] (row stride ldkv), all
+ * of them visible to its query rows cu_q[b] .. cu_q[b + 1].  The text
+ * cross-attention with each prompt's own length (naive_rt/rolling_forcing/
+ * wan/modules/model.py:165-189). */
+int wf_attn_cross_batch(const void* q, int64_t n_rows, int32_t n_heads,
+                        int32_t n_kv_heads, int32_t head_dim, int64_t ldq,
+                        const void* k, const void* v, int64_t n_kv_rows,
+                        int64_t ldkv, const int32_t* cu_q,
+                        const int32_t* cu_kv, int64_t n_seqs, int64_t max_q,
+                        int64_t max_kv, float softmax_scale, void* out,
+                        int64_t ldo, void* ws, int64_t ws_bytes, void* stream);
+
 /* ------------------------------------------------- block row-wise stages */
 
 /* y = LayerNorm(x) (fp32 statistics, optional bf16 affine w/b, rounded to

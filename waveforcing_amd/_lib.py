@@ -106,6 +106,23 @@ SIGNATURES: dict[str, list] = {
     "wf_attn_dense_bf16": [
         _c_void_p, _i64, _i32, _i32, _i64, _c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p, _i64, _c_void_p,
     ],
+    "wf_kv_batch_append": [
+        _c_void_p, _c_void_p, _i64, _i32, _i32, _i64, _i32, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i32,
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p,
+    ],
+    "wf_kv_batch_gather": [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
+        _i64, _i32, _i32, _c_void_p, _c_void_p, _i64, _c_void_p,
+    ],
+    "wf_attn_batch_workspace": [_i64, _i32, _i32, _i64, _i64, _i64, _i32, _c_void_p],
+    "wf_attn_paged_batch": [
+        _c_void_p, _i64, _i32, _i32, _i32, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32,
+        _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i32, _f32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+    ],
+    "wf_attn_cross_batch": [
+        _c_void_p, _i64, _i32, _i32, _i32, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64,
+        _i64, _f32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+    ],
     "wf_ln_modulate_quant": [
         _c_void_p, _i64, _i32, _i64, _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32,
         _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p,
@@ -132,6 +149,8 @@ FP8_AMAX_PARTIALS = 1024
 BF16_SILU_IN = 1
 BF16_SILU_OUT = 2
 BF16_GELU_OUT = 4
+KV_E4M3 = 0
+KV_INT8 = 1
 W8A8_STATIC_MAX_CODES = 64 << 20
 W8A8_STATIC_MAX_ROWS = 65536
 
@@ -191,3 +210,15 @@ def stream_handle(device=None) -> int:
     if isinstance(device, torch.device) and device.type == "cuda" and device.index is not None:
         return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(device, name: str, *args) -> None:
+    """:func:`call` with the current stream of ``device`` (a torch.device with an index) as the last argument, made
+    with that device current."""
+    import torch
+
+    if torch._C._cuda_getDevice() == device.index:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device.index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))

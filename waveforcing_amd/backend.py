@@ -28,7 +28,7 @@ from typing import Callable
 import torch
 
 from . import _lib
-from .kv import PagedKV
+from .kv import CrossBatch, PagedBatch, PagedKV
 
 ATTENTION_BACKENDS = ("torch_sdpa", "fa_custom", "sa", "fa", "fa2", "hip_fp8", "hip_fp8_qk", "hip_fp8_qkpv")
 
@@ -80,6 +80,8 @@ def attn_paged_fp8(q: torch.Tensor, k: PagedKV, v: PagedKV | None = None, causal
         raise ValueError(f"q must be bf16 [1, Lq, H, D] or [Lq, H, D], got {tuple(q.shape)} {q.dtype}")
     Lq, H, D = q3.shape
     pool = k.pool
+    if pool.format != _lib.KV_E4M3:
+        raise TypeError("hip_fp8 attention reads e4m3 pages; int8 pages are attended through attn_paged_batch")
     if H != pool.n_heads or D != pool.head_dim:
         raise ValueError(f"q heads/dim ({H}, {D}) differ from the pool ({pool.n_heads}, {pool.head_dim})")
     if q3.stride(2) != 1 or q3.stride(1) != D or q3.data_ptr() % 16 or q3.stride(0) % 8:
@@ -122,6 +124,97 @@ def attn_dense_bf16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_s
     o = out if out is not None else torch.empty((Lq, H, D), dtype=torch.bfloat16, device=q.device)
     _lib.call("wf_attn_dense_bf16", q.data_ptr(), Lq, H, D, q.stride(0), k.data_ptr(), v.data_ptr(), k.shape[0],
               k.stride(0), float(softmax_scale), o.data_ptr(), o.stride(0), _lib.stream_handle(q.device))
+    return o
+
+
+def _batch_rows(q: torch.Tensor, out: torch.Tensor | None, rows: int, device):
+    """Query rows [N, H, 128] (N >= rows) as the batch kernels read them, and the output rows."""
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != 128:
+        raise ValueError(f"q must be bf16 [rows, heads, 128], got {tuple(q.shape)} {q.dtype}")
+    if q.device != device:
+        raise ValueError(f"q is on {q.device}, the batch on {device}")
+    N, H, D = q.shape
+    if N < rows:
+        raise ValueError(f"q has {N} rows, the batch {rows}")
+    if q.stride(2) != 1 or q.stride(1) != D or q.data_ptr() % 16 or q.stride(0) % 8 or (N > 1 and q.stride(0) < H * D):
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((N, H, D), dtype=torch.bfloat16, device=device)
+        if N > rows:
+            out[rows:].zero_()
+    elif (out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != device or out.stride(2) != 1
+          or out.stride(1) != D or out.data_ptr() % 8 or out.stride(0) % 4 or (N > 1 and out.stride(0) < H * D)):
+        raise ValueError(f"out must be bf16 {tuple(q.shape)} on {device} with dense heads and a row stride that 4 divides")
+    return q, out, (q.stride(0) if N > 1 else H * D), (out.stride(0) if N > 1 else H * D)
+
+
+def attn_paged_batch(q: torch.Tensor, batch: PagedBatch, block: int = 0, softmax_scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a batch's new rows over their sequences' cached positions (wf_attn_paged_batch).
+
+    q [rows, heads, 128] bf16, the sequences' rows one after the other; the pool's heads divide ``heads`` and
+    query head h reads key head h // (heads // pool heads).  A row at position p of its sequence sees every
+    position (``block`` 0), those up to its own (1: causal), or those up to the end of its block of ``block``
+    positions (a frame's or a chunk's tokens: the block-causal mask).  The rows' own K/V are read from the
+    cache (:meth:`PagedBatch.append` first).  A row that sees nothing is zero; rows behind the batch's are left
+    as they are in ``out`` (zero in a new output).  For one call geometry the results are the same bits on
+    every run; how long caches are split, and with it the order of the sums, goes by the batch's sizes.
+    """
+    if not isinstance(batch, PagedBatch):
+        raise TypeError("attn_paged_batch takes a PagedBatch")
+    pool = batch.pool
+    q, o, ldq, ldo = _batch_rows(q, out, batch.n_new, batch.device)
+    H = q.shape[1]
+    if H % pool.n_heads or not H:
+        raise ValueError(f"{H} query heads do not group over the pool's {pool.n_heads}")
+    if not 0 <= block < 1 << 31:
+        raise ValueError(f"block={block} must be 0 (every position), 1 (causal) or a block's positions")
+    n = batch.workspace_bytes(H)
+    ws = torch.empty((n,), dtype=torch.uint8, device=batch.device) if n else None
+    cu, lens, n_seqs, tables, wide = batch._geom
+    _lib.call_on(batch.device, "wf_attn_paged_batch", q.data_ptr(), batch.n_new, H, pool.n_heads, 128, ldq, pool.format,
+                 pool._k_codes_p, pool._v_codes_p, pool._k_scales_p, pool._v_scales_p, pool.pool_pages, pool.page_tokens,
+                 cu, lens, n_seqs, tables, wide, batch.max_new, batch.max_kv, block,
+                 128 ** -0.5 if softmax_scale is None else float(softmax_scale), o.data_ptr(), ldo, _lib.ptr(ws), n)
+    return o
+
+
+def attn_cross_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: CrossBatch,
+                     softmax_scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a batch's query rows to their sequences' encoder rows (wf_attn_cross_batch): the text
+    cross-attention of several streams, each with its prompt's own length.
+
+    q [rows, heads, 128]; k, v [encoder rows, key heads, 128], all bf16, the sequences' rows one after the other
+    as ``batch`` counts them; key heads group over ``heads``.  A sequence without encoder rows gets zeros.
+    """
+    if not isinstance(batch, CrossBatch):
+        raise TypeError("attn_cross_batch takes a CrossBatch")
+    q, o, ldq, ldo = _batch_rows(q, out, batch.n_q, batch.device)
+    H = q.shape[1]
+    for name, t in (("k", k), ("v", v)):
+        if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[2] != 128 or t.device != batch.device:
+            raise ValueError(f"{name} must be bf16 [rows, heads, 128] on {batch.device}, got {tuple(t.shape)} {t.dtype} on "
+                             f"{t.device}")
+    if k.shape != v.shape or k.shape[0] < batch.n_kv:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must match and hold the batch's {batch.n_kv} rows")
+    rows, hkv, D = k.shape
+    if not hkv or H % hkv or not H:
+        raise ValueError(f"{H} query heads do not group over {hkv} key heads")
+
+    def dense(t):
+        if t.stride(2) != 1 or t.stride(1) != D or t.stride(0) % 8 or t.data_ptr() % 16 or (rows > 1 and t.stride(0) < hkv * D):
+            t = t.contiguous()
+        return t
+
+    k, v = dense(k), dense(v)
+    if rows > 1 and k.stride(0) != v.stride(0):
+        k, v = k.contiguous(), v.contiguous()
+    cu_q, cu_kv, n_seqs, max_q, max_kv = batch._geom
+    n = batch.workspace_bytes(H, hkv)
+    ws = torch.empty((n,), dtype=torch.uint8, device=batch.device) if n else None
+    _lib.call_on(batch.device, "wf_attn_cross_batch", q.data_ptr(), batch.n_q, H, hkv, 128, ldq, k.data_ptr(), v.data_ptr(),
+                 batch.n_kv, k.stride(0) if rows > 1 else hkv * D, cu_q, cu_kv, n_seqs, max_q, max_kv,
+                 128 ** -0.5 if softmax_scale is None else float(softmax_scale), o.data_ptr(), ldo, _lib.ptr(ws), n)
     return o
 
 

@@ -43,13 +43,13 @@
 // rounds the rotated K to bf16 (`.type_as(v)`, common.py:86-88).
 #include "fastdiv.hpp"
 #include "fp8_codec.hpp"
+#include "kv_row.hpp"
 #include "rows.hpp"
 #include "wf_common.hpp"
 
 namespace wf {
 namespace {
 
-constexpr int kHeadDim = 128;
 // Non-temporal hints, chosen by sweeps on MI355X (rows per lane group
 // {1, 2, 4, 8}, persistent grids, block-to-XCD maps, hints): streaming
 // stores for pack (6.0 TB/s over 30 layers in one launch), streaming loads
@@ -100,21 +100,6 @@ __device__ inline bool locate(const PageGeom& g, uint32_t r, int64_t& code_row, 
   return true;
 }
 
-// Four e4m3 codes of bf16-exact values x[0..3] with scale s (r within one ulp of 1/s).
-__device__ inline uint32_t quant4f(const float* x, float s, float r) {
-  float q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float ax = fabsf(x[i]);
-    float qi = ax * r;
-    const float e = fmaf(-qi, s, ax);
-    qi = fmaf(e, r, qi);
-    qi = fminf(qi, kE4M3Max);
-    q[i] = bits_f32(f32_bits(qi) | (f32_bits(x[i]) & 0x80000000u));
-  }
-  return e4m3_pack4_hw(q[0], q[1], q[2], q[3]);
-}
-
 __device__ inline uint32_t quant4(uint32_t w01, uint32_t w23, float s, float r) {
   const float x[4] = {bf16_lo_to_f32(w01), bf16_hi_to_f32(w01), bf16_lo_to_f32(w23), bf16_hi_to_f32(w23)};
   return quant4f(x, s, r);
@@ -147,35 +132,6 @@ __device__ inline float absmax8(const uint4& a, const uint4& b) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(bf16_lo_to_f32(w[i])), fabsf(bf16_hi_to_f32(w[i]))));
   return m;
-}
-
-// bf16(amax / 448) as bf16(amax * RN(1/448)) (see above), floored at bf16(1e-8).
-constexpr float kInvE4M3Max = 1.0f / kE4M3Max;
-__device__ inline float scale_from_amax(float amax) {
-  const float s = bf16_bits_to_f32(static_cast<uint16_t>(pack_bf16x2_hw(amax * kInvE4M3Max, 0.f)));
-  return fmaxf(s, bf16_bits_to_f32(kScaleFloorBf16Bits));
-}
-
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-
-template <bool NT>
-__device__ inline uint4 ld16(const uint4* p) {
-  if constexpr (NT) {
-    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-    return make_uint4(v[0], v[1], v[2], v[3]);
-  } else {
-    return *p;
-  }
-}
-
-template <bool NT>
-__device__ inline void st16(uint4* p, const uint4& v) {
-  if constexpr (NT) {
-    const u32x4 w = {v.x, v.y, v.z, v.w};
-    __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
-  } else {
-    *p = v;
-  }
 }
 
 // ROPE: K rows are rotated first, token t by row t % rope_rows of cos/sin
@@ -401,18 +357,6 @@ __global__ __launch_bounds__(256) void k_norm_rope_pack_kernel(KNormPackArgs a) 
       if (ch < n_chunks) rows::st16(qrow + ch * 8, rows::pack8(x));
     }
   }
-}
-
-__device__ inline uint2 dequant4(uint32_t w, float s) {
-  typedef float f2 __attribute__((ext_vector_type(2)));
-  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-  float v0, v1, v2, v3;
-  e4m3_unpack4_hw(w, v0, v1, v2, v3);
-  const f2 lo = {v0 * s, v1 * s};
-  const f2 hi = {v2 * s, v3 * s};
-  const b2 blo = __builtin_convertvector(lo, b2);
-  const b2 bhi = __builtin_convertvector(hi, b2);
-  return make_uint2(__builtin_bit_cast(uint32_t, blo), __builtin_bit_cast(uint32_t, bhi));
 }
 
 template <bool NT_LOAD, bool NT_STORE>

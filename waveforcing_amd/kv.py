@@ -22,6 +22,9 @@ slabs); the HIP kernels never allocate.
 
 from __future__ import annotations
 
+import collections
+import ctypes
+import itertools
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -92,6 +95,8 @@ def _rope_tables(rope, T: int, D: int, device, tiled: bool = False):
 
 class Fp8PagePool:
     """K and V page pools in HBM with pack / gather-dequant through the HIP kernels."""
+
+    format = _lib.KV_E4M3
 
     def __init__(
         self,
@@ -267,6 +272,208 @@ class Fp8PagePool:
             _lib.stream_handle(self.device),
         )
         return (out_k, out_v) if with_v else out_k
+
+
+class Int8PagePool(Fp8PagePool):
+    """The pools with signed int8 codes in place of e4m3 ones (scale max|x| / 127 per (token, head)): the same bytes
+    with 8 significant bits at a row's maximum where e4m3 keeps 4 at every magnitude.  Written, read and attended
+    through :class:`PagedBatch`; the one-sequence forms take e4m3 pages."""
+
+    format = _lib.KV_INT8
+
+    def _one_sequence(self, *args, **kwargs):
+        raise TypeError("int8 pages are written and read through PagedBatch (append, gather)")
+
+    pack = pack_k_norm_rope = unpack = _one_sequence
+
+
+def _int32_list(xs, name: str) -> list[int]:
+    out = [int(x) for x in xs]
+    for x in out:
+        if x < 0 or x >= 1 << 31:
+            raise ValueError(f"{name} holds {x}: expected 0 <= {name} < 2^31")
+    return out
+
+
+def _starts(lens: Sequence[int]) -> list[int]:
+    return [0, *itertools.accumulate(lens)]
+
+
+class PagedBatch:
+    """Several sequences over one page pool: their page lists, cached lengths and new rows, on host and device.
+
+    Sequence b has ``kv_lens[b]`` positions in its cache, stored in the pages ``pages[b]`` in order; the last
+    ``new_lens[b]`` of them (default: one each) are those of its new rows, which :meth:`append` writes and the
+    attention (backend.attn_paged_batch) takes as queries.  Row tensors hold the sequences' new rows one after
+    the other; rows behind the last sequence's are padding and are left as they are.  Sequences may share pages
+    that no row of the batch is written to (a common prefix).
+
+    The kernels read the lengths and tables on the device: ``cu_new`` int32 [n + 1], ``kv_lens_dev`` int32 [n],
+    ``tables`` int32 [n, pages].  A captured graph replays with what they hold then (:meth:`set_lens`, or the
+    caller's own kernels); ``max_kv`` (default: the longest of ``kv_lens``) should bound the lengths it will see,
+    since it chooses how long caches are split.
+    """
+
+    def __init__(self, pool: Fp8PagePool, pages: Sequence[Sequence[int]], kv_lens: Sequence[int],
+                 new_lens: Sequence[int] | None = None, max_kv: int | None = None) -> None:
+        self.pool = pool
+        self.pages = [_int32_list(p, "page id") for p in pages]
+        for ids in self.pages:
+            for i in ids:
+                if i >= pool.pool_pages:
+                    raise RuntimeError(f"page id {i} outside pool of {pool.pool_pages} pages")
+        self.n_seqs = len(self.pages)
+        self.device = pool.k_codes.device
+        wide = max((len(p) for p in self.pages), default=0)
+        self._check_lens(kv_lens, [1] * self.n_seqs if new_lens is None else new_lens)
+        n = self.n_seqs
+        flat = [*_starts(self.new_lens), *self.kv_lens]
+        for ids in self.pages:
+            flat += ids
+            flat += [-1] * (wide - len(ids))
+        dev = torch.tensor(flat, dtype=torch.int32).to(self.device)
+        self.cu_new, self.kv_lens_dev = dev[:n + 1], dev[n + 1:2 * n + 1]
+        self.tables = dev[2 * n + 1:].view(n, wide)
+        self._lens_dev = dev[:2 * n + 1]
+        self._geom = (self.cu_new.data_ptr(), self.kv_lens_dev.data_ptr(), n, self.tables.data_ptr() if wide else None,
+                      wide)
+        self._set_bounds(max_kv)
+
+    def _check_lens(self, kv_lens, new_lens) -> None:
+        kv, new = _int32_list(kv_lens, "kv_lens"), _int32_list(new_lens, "new_lens")
+        if not len(kv) == len(new) == self.n_seqs:
+            raise ValueError(f"{self.n_seqs} page lists, {len(kv)} kv_lens and {len(new)} new_lens")
+        for b, (t, n, ids) in enumerate(zip(kv, new, self.pages)):
+            if n > t:
+                raise ValueError(f"sequence {b}: {n} new rows among {t} cached positions")
+            if t > len(ids) * self.pool.page_tokens:
+                raise RuntimeError(f"page table of {len(ids)} pages cannot hold {t} tokens (sequence {b})")
+        self.kv_lens, self.new_lens = kv, new
+        self.n_new = sum(new)
+        if self.n_new >= 1 << 31:
+            raise ValueError(f"{self.n_new} new rows")
+        self._writable = False
+
+    def _set_bounds(self, max_kv) -> None:
+        longest = max(self.kv_lens, default=0)
+        if max_kv is not None and max_kv < longest:
+            raise ValueError(f"max_kv={max_kv} is below a sequence's {longest} positions")
+        self.max_kv = longest if max_kv is None else int(max_kv)
+        self.max_new = max(self.new_lens, default=0)
+        self._ws: dict = {}
+
+    def set_lens(self, kv_lens: Sequence[int], new_lens: Sequence[int] | None = None, max_kv: int | None = None) -> None:
+        """The lengths of the next step (``new_lens``: as they are by default); one copy to the device, ordered on the
+        current stream."""
+        self._check_lens(kv_lens, self.new_lens if new_lens is None else new_lens)
+        self._set_bounds(max_kv)
+        self._lens_dev.copy_(torch.tensor([*_starts(self.new_lens), *self.kv_lens], dtype=torch.int32))
+
+    def _check_written_pages(self) -> None:
+        """Every page that a new row is written to belongs to one place of one sequence."""
+        if self._writable:
+            return
+        uses = collections.Counter(itertools.chain.from_iterable(self.pages))
+        pt = self.pool.page_tokens
+        for b, (t, n) in enumerate(zip(self.kv_lens, self.new_lens)):
+            if n:
+                for i in self.pages[b][(t - n) // pt:(t - 1) // pt + 1]:
+                    if uses[i] > 1:
+                        raise RuntimeError(f"page {i} of sequence {b} would be written but is used {uses[i]} times")
+        self._writable = True
+
+    def _rows(self, x: torch.Tensor, name: str):
+        t, addr, shape, ld = _as_thd(x, name)
+        if shape[1:] != (self.pool.n_heads, self.pool.head_dim):
+            raise ValueError(f"{name} has heads/dim {shape[1:]}; the pool {(self.pool.n_heads, self.pool.head_dim)}")
+        if shape[0] < self.n_new:
+            raise ValueError(f"{name} has {shape[0]} rows, the batch {self.n_new}")
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, the pool on {self.device}")
+        return t, addr, ld
+
+    def append(self, k: torch.Tensor, v: torch.Tensor | None) -> None:
+        """Quantize the new rows K (and V) [rows, heads, 128] bf16 into their positions' pages (wf_kv_batch_append).
+        A (row, head) with a NaN or an infinity is stored so that it reads back as NaN."""
+        self._check_written_pages()
+        pool = self.pool
+        kt, kp, ld = self._rows(k, "k")
+        vt, vp = None, None
+        if v is not None:
+            vt, vp, vld = self._rows(v, "v")
+            if vld != ld:   # one row stride serves K and V
+                kt, vt = kt.reshape(-1, pool.n_heads, 128).contiguous(), vt.reshape(-1, pool.n_heads, 128).contiguous()
+                kp, vp, ld = kt.data_ptr(), vt.data_ptr(), pool.n_heads * 128
+        _lib.call_on(self.device, "wf_kv_batch_append", kp, vp, self.n_new, pool.n_heads, pool.head_dim, ld, pool.format,
+                     *self._geom, pool.page_tokens, pool._k_codes_p, pool._v_codes_p, pool._k_scales_p,
+                     pool._v_scales_p, pool.pool_pages)
+
+    def gather(self, with_v: bool = True, out_k: torch.Tensor | None = None, out_v: torch.Tensor | None = None):
+        """The new rows' positions read back as bf16 [rows, heads, 128] (wf_kv_batch_gather): what is cached there.
+        A batch whose ``new_lens`` are its ``kv_lens`` reads the whole caches.  Given outputs may have more rows
+        (left as they are) and a row stride of their own."""
+        pool = self.pool
+        outs = []
+        for name, t in (("out_k", out_k), ("out_v", out_v)):
+            if name == "out_v" and not with_v:
+                outs.append(None)
+                continue
+            if t is None:
+                t = torch.empty((self.n_new, pool.n_heads, pool.head_dim), dtype=torch.bfloat16, device=self.device)
+            at, addr, ld = self._rows(t, name)
+            if at is not t:
+                raise ValueError(f"{name} must have dense heads, 16-byte alignment and a row stride that 8 divides")
+            outs.append((t, addr, ld))
+        (k, kp, ld), v = outs
+        if v is not None and v[2] != ld:
+            raise ValueError(f"out_k and out_v have different row strides ({ld} and {v[2]})")
+        _lib.call_on(self.device, "wf_kv_batch_gather", pool._k_codes_p, pool._v_codes_p, pool._k_scales_p,
+                     pool._v_scales_p, pool.pool_pages, pool.format, pool.page_tokens, *self._geom, self.n_new,
+                     pool.n_heads, pool.head_dim, kp, None if v is None else v[1], ld)
+        return k if v is None else (k, v[0])
+
+    def workspace_bytes(self, n_heads: int) -> int:
+        """Scratch of the attention over this batch with ``n_heads`` query heads."""
+        n = self._ws.get(n_heads)
+        if n is None:
+            n = self._ws[n_heads] = _attn_workspace(self.n_new, n_heads, self.pool.n_heads, self.n_seqs, self.max_new,
+                                                    self.max_kv, True)
+        return n
+
+
+def _attn_workspace(rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv, paged: bool) -> int:
+    n = ctypes.c_int64()
+    _lib.call("wf_attn_batch_workspace", rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv, int(paged), ctypes.addressof(n))
+    return n.value
+
+
+class CrossBatch:
+    """Row counts of several sequences for the attention to encoder states (backend.attn_cross_batch): sequence b has
+    ``q_lens[b]`` query rows and ``kv_lens[b]`` encoder rows (0: its output is zero), one sequence after the
+    other in the row tensors; ``cu_q`` and ``cu_kv`` (int32 [n + 1]) hold their starts on the device."""
+
+    def __init__(self, q_lens: Sequence[int], kv_lens: Sequence[int], device="cuda") -> None:
+        self.q_lens, self.kv_lens = _int32_list(q_lens, "q_lens"), _int32_list(kv_lens, "kv_lens")
+        if len(self.q_lens) != len(self.kv_lens):
+            raise ValueError(f"{len(self.q_lens)} q_lens and {len(self.kv_lens)} kv_lens")
+        self.n_seqs = len(self.q_lens)
+        self.n_q, self.n_kv = sum(self.q_lens), sum(self.kv_lens)
+        if max(self.n_q, self.n_kv) >= 1 << 31:
+            raise ValueError(f"{self.n_q} query rows and {self.n_kv} encoder rows")
+        self.max_q, self.max_kv = max(self.q_lens, default=0), max(self.kv_lens, default=0)
+        dev = torch.tensor(_starts(self.q_lens) + _starts(self.kv_lens), dtype=torch.int32).to(device)
+        self.device = dev.device
+        self.cu_q, self.cu_kv = dev[:self.n_seqs + 1], dev[self.n_seqs + 1:]
+        self._geom = (self.cu_q.data_ptr(), self.cu_kv.data_ptr(), self.n_seqs, self.max_q, self.max_kv)
+        self._ws: dict = {}
+
+    def workspace_bytes(self, n_heads: int, n_kv_heads: int) -> int:
+        """Scratch of the attention with these heads."""
+        n = self._ws.get((n_heads, n_kv_heads))
+        if n is None:
+            n = self._ws[n_heads, n_kv_heads] = _attn_workspace(self.n_q, n_heads, n_kv_heads, self.n_seqs, self.max_q,
+                                                                self.max_kv, False)
+        return n
 
 
 @dataclass
