@@ -413,12 +413,11 @@ int wf_kv_batch_gather(const uint8_t* k_codes, const uint8_t* v_codes,
                        int64_t n_rows, int32_t n_kv_heads, int32_t head_dim,
                        void* k_out, void* v_out, int64_t ld_out, void* stream);
 
-/* Workspace bytes of wf_attn_paged_batch (paged != 0) or wf_attn_cross_batch
- * (paged == 0) with these sizes, into *bytes (host memory). */
+/* Workspace bytes of wf_attn_paged_batch or wf_attn_cross_batch
+ * with these sizes, into *bytes (host memory). */
 int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads,
                             int32_t n_kv_heads, int64_t n_seqs,
-                            int64_t max_new, int64_t max_kv, int32_t paged,
-                            int64_t* bytes);
+                            int64_t max_new, int64_t max_kv, int64_t* bytes);
 
 /* Attention of the rows' queries q [n_rows][n_heads][128] (row stride ldq)
  * over their sequences' caches, query head h on key head

@@ -56,6 +56,12 @@ def attend(q, k, v, limits, scale):
     the fp32 sums of 128 products of the parts run in any order (256 roundings of 2^-24 of twice the sum of the
     magnitudes: 2^-15); 2^-20 more for the exponential, and 2^-14 for the fp32 running sums over the keys (up to
     2^10 tiles' roundings).  The quotient of two sums doubles e.  The result is rounded to bf16 once: 2^-8.
+
+    Two absolute terms come with fp16 (many rows), whose numbers are 2^-24 apart below 2^-14, half a step 2^-25.  A
+    weight is held as 64 times its ratio to a maximum that the row's largest weight reaches, so it is off by at most
+    2^-25 / 64 = 2^-31 of that largest weight: together 2^-31 w_max sum_j |v_j| over the seen keys.  A value is held
+    as V 2^-E with 2^E at most a quarter of the largest scale of V, which is at most max|V| / 127: it is off by at most
+    2^-25 2^E <= 2^-27 max|V| / 127 < 2^-33 max|V|, and so is their weighted mean.
     """
     q, k, v = q.double(), k.double(), v.double()
     n, heads, _ = q.shape
@@ -83,5 +89,8 @@ def attend(q, k, v, limits, scale):
         bad = (seen.double() @ (~torch.isfinite(vg)).double()) > 0
         out[:, h] = out[:, h].masked_fill(bad, float("nan"))
         A = w @ vz.abs()
-        bound[:, h] = A * (2.0 ** -8 + 2 * e * (1 + 2.0 ** -8) + 2.0 ** -13) + out[:, h].abs() * 2.0 ** -8 * (1 + 2.0 ** -6) + 1e-30
+        small = torch.zeros_like(A)
+        if len(key):
+            small = 2.0 ** -31 * w.amax(-1, keepdim=True) * (seen.double() @ vz.abs()) + 2.0 ** -33 * vz.abs().max()
+        bound[:, h] = small + A * (2.0 ** -8 + 2 * e * (1 + 2.0 ** -8) + 2.0 ** -13) + out[:, h].abs() * 2.0 ** -8 * (1 + 2.0 ** -6) + 1e-30
     return out, bound

@@ -139,7 +139,7 @@ CROSS = dict(q=16, rows=4, heads=4, kv_heads=2, dim=128, ldq=512, k=32, v=48, kv
     ("wf_attn_paged_batch", PAGED, dict(ldq=504), "ldq/ldo"),
     ("wf_attn_paged_batch", PAGED, dict(q=24), "16-byte"),
     ("wf_attn_paged_batch", PAGED, dict(ks=None), "null pointer"),
-    ("wf_attn_paged_batch", PAGED, dict(max_kv=-1), "negative bound"),
+    ("wf_attn_paged_batch", PAGED, dict(max_kv=-1), "bad bound"),
     ("wf_attn_paged_batch", PAGED, dict(rows=1 << 30), "reaches 2"),
     ("wf_attn_cross_batch", CROSS, dict(kv_rows=-1), "key rows"),
     ("wf_attn_cross_batch", CROSS, dict(ldkv=128), "ldkv=128"),

@@ -114,7 +114,7 @@ SIGNATURES: dict[str, list] = {
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
         _i64, _i32, _i32, _c_void_p, _c_void_p, _i64, _c_void_p,
     ],
-    "wf_attn_batch_workspace": [_i64, _i32, _i32, _i64, _i64, _i64, _i32, _c_void_p],
+    "wf_attn_batch_workspace": [_i64, _i32, _i32, _i64, _i64, _i64, _c_void_p],
     "wf_attn_paged_batch": [
         _c_void_p, _i64, _i32, _i32, _i32, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32,
         _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i32, _f32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,

@@ -1,0 +1,630 @@
+// Batched attention, many rows: tiles of 256 (row, head) rows of a sequence over one key head.  Bound by the matrix cores
+// and by the issue of the vector work between their instructions.
+//
+// Eight waves of 32 rows; keys in tiles of 64 through two LDS stages, staged by all threads (thread t: key t / 8, 16
+// values t % 8 of its row) one tile ahead of the products, with the loads of the tile after in flight.  S^T = K Q^T on
+// 32x32 products leaves a lane with one row and 32 keys, so a row's maximum is an in-lane maximum and one lane swap, and
+// its weights are directly the second operand of O^T += V^T P^T, whose first operand comes from the staged rows by
+// transposing reads (attn_paged.hip has the layouts).
+//
+// What is rounded, and where:
+//   e4m3 keys  the codes go to the fp8 matrix cores as they are, Q as the sum of two e4m3 parts under a power-of-two scale
+//              of the row: q = 2^e (q1 + q2 / 16), exact where q's last bit is not below 2^-13 of 2^e (|q| < 2^8 2^e);
+//              the product is that of the codes with Q in fp32, and s_k c multiplies the score in fp32.  Staging K costs
+//              no conversion and half the LDS.
+//   int8 keys  the codes are exact in bf16, as Q is.
+//   V          fp16(code s_v 2^-E), 11 significant bits, E a power of two of the workgroup's keys so far: staged values
+//              stay below 2^16, and a tile whose scales pass the limit raises E first, rescales O and is staged again
+//              (a power of two moves no bit of them; values below 2^-29 of the largest lose their last ones).
+//   weights    fp16(64 p), p <= 2^kTau: eight times finer than bf16, down to 2^-31 of the row's largest; the row sum
+//              adds the rounded weights.
+//   dense      K, V, Q and the weights are bf16.
+// A NaN or infinite scale makes the key's score NaN and its V zero, so the rows that see the key become NaN and no
+// others; in tiles that some row does not see whole, so does a NaN code of V.
+#include <utility>
+
+#include "attn_batch.hpp"
+
+namespace wf {
+namespace attn_batch {
+namespace {
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+constexpr int BKV = 64;
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+constexpr int R = 32 * kWaves;
+constexpr int kXcds = 8;
+constexpr int kRun = 4;  // neighbouring row tiles that one XCD takes, which read the same keys
+static_assert(kThreads == BKV * 8, "one thread per key and 16 values of its row");
+
+template <int SRC>
+struct Lds {
+  static constexpr bool codes = SRC == SRC_E4M3;              // K as codes
+  static constexpr int k_pitch = codes ? D + 16 : 2 * D + 16;
+  static constexpr int v_pitch = 2 * D + 64;
+  static constexpr int v_off = BKV * k_pitch;
+  static constexpr int u_off = v_off + BKV * v_pitch;         // u [64], the staging waves' maxima of u [8] and of s_v [8]
+  static constexpr int stage = u_off + (BKV + 8 + 8) * 4;
+  static constexpr int o_pitch = 2 * D + 8;
+  static constexpr int out = kWaves * 32 * o_pitch;
+  static constexpr int bytes = 2 * stage > out ? 2 * stage : out;
+};
+
+__device__ inline uint32_t pk_mul_f16(uint32_t a, v2h f) {
+  return __builtin_bit_cast(uint32_t, static_cast<v2h>(__builtin_bit_cast(v2h, a) * f));
+}
+
+// 4 codes as 4 fp16 (exact).
+template <int SRC>
+__device__ inline uint2 codes_f16(uint32_t w) {
+  if constexpr (SRC == SRC_E4M3) {
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)));
+  } else {
+    // code + 128 as the last byte of 1024 + it, less 1152
+    const uint32_t x = w ^ 0x80808080u;
+    const v2h k = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    const uint32_t lo = __builtin_amdgcn_perm(x, 0x64646464u, 0x00050004u), hi = __builtin_amdgcn_perm(x, 0x64646464u, 0x00070006u);
+    return make_uint2(__builtin_bit_cast(uint32_t, static_cast<v2h>(__builtin_bit_cast(v2h, lo) + k)),
+                      __builtin_bit_cast(uint32_t, static_cast<v2h>(__builtin_bit_cast(v2h, hi) + k)));
+  }
+}
+
+// 4 int8 codes as 4 bf16 (exact).
+__device__ inline uint2 i8_bf16(uint32_t w) {
+  return make_uint2(cvt_bf16x2(static_cast<float>(static_cast<int8_t>(w)), static_cast<float>(static_cast<int8_t>(w >> 8))),
+                    cvt_bf16x2(static_cast<float>(static_cast<int8_t>(w >> 16)), static_cast<float>(static_cast<int8_t>(w >> 24))));
+}
+
+__device__ inline uint32_t cvt_f16x2(float lo, float hi) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
+}
+
+// Maximum over the 8 keys (lanes 8 k) that a wave stages.
+__device__ inline float keys_max(float v) {
+  const int i = static_cast<int>(f32_bits(v));
+  v = fmaxf(v, bits_f32(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(i, i, 0x128, 0xF, 0xF, false))));  // lane ^ 8
+  return max32(max16(v));
+}
+
+__device__ inline bool finite(float v) { return (f32_bits(v) & 0x7f800000u) != 0x7f800000u; }
+
+template <int SRC>
+__global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
+  using L = Lds<SRC>;
+  constexpr bool kDense = SRC == SRC_DENSE;
+  constexpr bool kCodes = SRC == SRC_E4M3;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[L::bytes];
+
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, half = lane >> 5;
+
+  // Item: runs of kRun neighbouring row tiles go to the XCDs in turn (workgroups are dealt to them round-robin), the
+  // last tiles of a sequence, whose causal rows see most, first.
+  const int n_items = a.n_tiles * a.n_kv_heads * a.n_splits;
+  const int xcd = static_cast<int>(blockIdx.x) % kXcds, slot = static_cast<int>(blockIdx.x) / kXcds;
+  const int i_run = (slot / kRun) * kXcds + xcd;
+  const int i_lin = i_run * kRun + slot % kRun;
+  if (i_lin >= n_items) return;
+  const int w = a.n_tiles - 1 - i_lin % a.n_tiles;
+  const int hs = i_lin / a.n_tiles;
+  const int head = hs % a.n_kv_heads, split = hs / a.n_kv_heads;
+  Tile t;
+  if (!find_tile<kDense>(a, w, t)) return;
+  const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
+  const int splits = used_splits(a, lim_max);
+  if (split >= splits) return;
+  const int k_lo = split * a.split_keys;
+  const int k_hi = split == splits - 1 ? lim_max : k_lo + a.split_keys;
+  const int tile_lo = k_lo / BKV, tile_hi = (k_hi + BKV - 1) / BKV;
+
+  // this wave's rows: the lane's own, and the largest limit
+  const int my_first = t.first + 32 * wave;
+  const int r = my_first + l32;
+  const bool row_ok = r < t.count;
+  uint32_t qi, gi;
+  a.group_div.divmod(static_cast<uint32_t>(row_ok ? r : t.first), qi, gi);
+  const int lim = row_ok ? row_limit(a, t, static_cast<int>(qi)) : 0;
+  int wave_max = 0;
+  if (my_first < t.count) wave_max = row_limit(a, t, static_cast<int>(a.group_div.div(min(my_first + 32, t.count) - 1)));
+  wave_max = __builtin_amdgcn_readfirstlane(wave_max);
+
+  // ---- staging: key skey of the tile, values 16 schunk .. + 15
+  const int skey = tid >> 3, schunk = tid & 7;
+  struct Staged {
+    u32x4 k0, v0, k1, v1;
+    float sk, sv;
+  };
+  Staged sreg;
+  // Where a tile's keys live (uniform).  Keys before `cut` are rows tok + key of the pool (scales sc + key), `n` of them to
+  // be read; a page boundary inside the tile makes cut < 64, and then every lane finds its own key.
+  struct Cursor {
+    int at, cut, tok, sc, n;
+  };
+  const int pt = a.geom.page_tokens;
+  const int32_t* table = a.geom.tables + static_cast<int64_t>(t.b) * a.geom.ld_table;
+  auto cursor_at = [&](int tile) -> Cursor {
+    if constexpr (kDense) return Cursor{0, BKV, 0, 0, 0};
+    uint32_t lp, at;
+    a.geom.page.divmod(static_cast<uint32_t>(tile) * BKV, lp, at);
+    const int i = static_cast<int>(lp);
+    int page = -1;
+    if (i < a.geom.ld_table) page = table[i];
+    page = __builtin_amdgcn_readfirstlane(page);
+    asm volatile("" ::"s"(page));  // awaited here, not among the LDS reads of the tile
+    const bool ok = page >= 0 && page < a.geom.pool_pages;
+    const int pg = ok ? page : 0, r0 = static_cast<int>(at);
+    return Cursor{r0, min(pt - r0, BKV), pg * pt + r0, (pg * a.n_kv_heads + head) * pt + r0, ok ? BKV : 0};
+  };
+  auto cursor_next = [&](const Cursor& c, int tile) -> Cursor {
+    if constexpr (kDense) return c;
+    if (c.at + BKV >= pt) return cursor_at(tile);
+    return Cursor{c.at + BKV, min(pt - c.at - BKV, BKV), c.tok + BKV, c.sc + BKV, c.n};
+  };
+  Cursor ahead{};
+  const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(kDense ? a.ldkv * 2 : a.n_kv_heads * D) +
+                            (kDense ? 32 : 16) * schunk;  // bytes; rows of a tile stay below 2^31 (checked on the host)
+  constexpr int kWord3 = 0x00020000;  // raw buffer, 32-bit data format
+  // The loads of a tile.  Within one page a buffer of the tile's rows that are there reads the others as zero, and a
+  // lane's offset never changes.
+  auto load_tile = [&](int tile, const Cursor& c, Staged& x) {
+    const int n = min(max(k_hi - tile * BKV, 0), BKV);
+    if constexpr (kDense) {
+      const int64_t first = static_cast<int64_t>(t.key0 + (n ? tile * BKV : 0)) * a.ldkv + head * D;
+      const int bytes = n ? (n - 1) * static_cast<int>(a.ldkv) * 2 + 2 * D : 0;
+      const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.k_dense + first), 0, bytes, kWord3);
+      const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.v_dense + first), 0, bytes, kWord3);
+      x.k0 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row, 0, 0);
+      x.k1 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row + 16, 0, 0);
+      x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
+      x.v1 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row + 16, 0, 0);
+    } else if (c.cut == BKV) {
+      const int m = min(n, c.n);
+      const int64_t first = static_cast<int64_t>(c.tok * a.n_kv_heads + head) * D;
+      const int bytes = m ? ((m - 1) * a.n_kv_heads + 1) * D : 0;
+      const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.k_codes + first), 0, bytes, kWord3);
+      const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.v_codes + first), 0, bytes, kWord3);
+      const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.k_scales + c.sc), 0, 4 * m, kWord3);
+      const auto sv = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.v_scales + c.sc), 0, 4 * m, kWord3);
+      x.k0 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row, 0, 0);
+      x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
+      x.sk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * skey, 0, 0));
+      x.sv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * skey, 0, 0));
+    } else {
+      x.k0 = x.v0 = u32x4{0, 0, 0, 0};
+      x.sk = x.sv = 0.f;
+      int page, at;
+      if (skey < n && pool_row(a.geom, t.b, tile * BKV + skey, page, at)) {
+        const int64_t off = static_cast<int64_t>((page * pt + at) * a.n_kv_heads + head) * D + 16 * schunk;
+        const int sc = (page * a.n_kv_heads + head) * pt + at;
+        x.k0 = *reinterpret_cast<const u32x4*>(a.k_codes + off);
+        x.v0 = *reinterpret_cast<const u32x4*>(a.v_codes + off);
+        x.sk = a.k_scales[sc];
+        x.sv = a.v_scales[sc];
+      }
+    }
+  };
+
+  int ev = 0;            // E: staged V = V 2^-E
+  float sv_lim = 0.f;    // the largest scale of V that E allows: 448 2^7 < 65504
+  auto set_exponent = [&](float top) {  // puts the scale `top` below 2^3
+    ev = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top) - 3);
+    sv_lim = __builtin_ldexpf(1.f, ev + 7);
+  };
+
+  struct Ready {
+    uint4 k0, k1, v0, v1;
+    float u, sv;
+  };
+  // The staged tile as it goes to LDS.  PARTIAL: some row may not see all of it.
+  auto convert = [&](Staged x, Ready& y, auto PARTIAL) {
+    if constexpr (kDense) {
+      y.k0 = make_uint4(x.k0[0], x.k0[1], x.k0[2], x.k0[3]);
+      y.k1 = make_uint4(x.k1[0], x.k1[1], x.k1[2], x.k1[3]);
+      y.v0 = make_uint4(x.v0[0], x.v0[1], x.v0[2], x.v0[3]);
+      y.v1 = make_uint4(x.v1[0], x.v1[1], x.v1[2], x.v1[3]);
+    } else {
+      bool poison = !finite(x.sv);
+      if constexpr (SRC == SRC_E4M3 && decltype(PARTIAL)::value) {
+        const bool nan = has_nan_code(x.v0[0]) || has_nan_code(x.v0[1]) || has_nan_code(x.v0[2]) || has_nan_code(x.v0[3]);
+        const uint64_t any = __ballot(nan);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.v0[e] = without_nan_codes(x.v0[e]);
+        poison = poison || (any >> (lane & 56) & 0xffu);
+      }
+      y.sv = poison ? 0.f : x.sv;
+      y.u = poison ? bits_f32(0x7fc00000u) : x.sk * a.c;
+      const float f = __builtin_ldexpf(y.sv, -ev);
+      const v2h ff = {static_cast<_Float16>(f), static_cast<_Float16>(f)};
+      if constexpr (kCodes) {
+        y.k0 = make_uint4(x.k0[0], x.k0[1], x.k0[2], x.k0[3]);
+      } else {
+        const uint2 p = i8_bf16(x.k0[0]), q = i8_bf16(x.k0[1]), s = i8_bf16(x.k0[2]), v = i8_bf16(x.k0[3]);
+        y.k0 = make_uint4(p.x, p.y, q.x, q.y);
+        y.k1 = make_uint4(s.x, s.y, v.x, v.y);
+      }
+      const uint2 p = codes_f16<SRC>(x.v0[0]), q = codes_f16<SRC>(x.v0[1]), s = codes_f16<SRC>(x.v0[2]), v = codes_f16<SRC>(x.v0[3]);
+      y.v0 = make_uint4(pk_mul_f16(p.x, ff), pk_mul_f16(p.y, ff), pk_mul_f16(q.x, ff), pk_mul_f16(q.y, ff));
+      y.v1 = make_uint4(pk_mul_f16(s.x, ff), pk_mul_f16(s.y, ff), pk_mul_f16(v.x, ff), pk_mul_f16(v.y, ff));
+    }
+  };
+  auto write = [&](int buf, const Ready& y) {
+    uint8_t* st = lds + buf * L::stage;
+    uint4* dv = reinterpret_cast<uint4*>(st + L::v_off + skey * L::v_pitch + schunk * 32);
+    if constexpr (kCodes) {
+      *reinterpret_cast<uint4*>(st + skey * L::k_pitch + schunk * 16) = y.k0;
+    } else {
+      uint4* dk = reinterpret_cast<uint4*>(st + skey * L::k_pitch + schunk * 32);
+      dk[0] = y.k0;
+      dk[1] = y.k1;
+    }
+    dv[0] = y.v0;
+    dv[1] = y.v1;
+    if constexpr (!kDense) {
+      // the key's factor, and the largest factor (of those that are numbers) and scale of V of the wave's 8 keys; lanes
+      // of one key write the same word
+      float* u = reinterpret_cast<float*>(st + L::u_off);
+      u[skey] = y.u;
+      u[BKV + wave] = keys_max(finite(y.u) ? y.u : 0.f);
+      u[BKV + 8 + wave] = keys_max(y.sv);
+    }
+  };
+
+  // ---- Q, the second operand of the scores, for the whole kernel
+  v8bf qb[kCodes ? 1 : 8];
+  v8i q1[kCodes ? 2 : 1], q2[kCodes ? 2 : 1];
+  int q_scale = 127;     // e4m3: E8M0 scale of q1
+  {
+    const uint16_t* qp = a.q + static_cast<int64_t>(t.row0 + static_cast<int>(qi)) * a.ldq + (head * a.group + static_cast<int>(gi)) * D;
+    uint4 raw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // e4m3: values 64 (i / 4) + 32 half + 8 (i % 4) .. + 7; else 16 i + 8 half .. + 7
+      raw[i] = *reinterpret_cast<const uint4*>(qp + (kCodes ? 64 * (i >> 2) + 32 * half + 8 * (i & 3) : 16 * i + 8 * half));
+      if (!row_ok) raw[i] = make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (!kCodes) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qb[i] = __builtin_bit_cast(v8bf, raw[i]);
+    } else {
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo_to_f32(x[e])), fabsf(bf16_hi_to_f32(x[e]))));
+      }
+      amax = max32(amax);
+      const int E = __builtin_amdgcn_frexp_expf(amax);  // amax < 2^E
+      // q = 2^e (q1 + q2 / 16), e = E - 8: |q| 2^-e < 256
+      const int e = amax > 0.f ? min(max(E - 8, -122), 126) : 0;
+      q_scale = 127 + e;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        uint32_t c1[8], c2[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 x = raw[4 * m + i];
+          const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float v[4] = {__builtin_ldexpf(bf16_lo_to_f32(y[2 * j]), -e), __builtin_ldexpf(bf16_hi_to_f32(y[2 * j]), -e),
+                                __builtin_ldexpf(bf16_lo_to_f32(y[2 * j + 1]), -e),
+                                __builtin_ldexpf(bf16_hi_to_f32(y[2 * j + 1]), -e)};
+            const uint32_t hi = e4m3_pack4_hw(v[0], v[1], v[2], v[3]);
+            float b0, b1, b2, b3;
+            e4m3_unpack4_hw(hi, b0, b1, b2, b3);
+            c1[2 * i + j] = hi;
+            c2[2 * i + j] = e4m3_pack4_hw((v[0] - b0) * 16.f, (v[1] - b1) * 16.f, (v[2] - b2) * 16.f, (v[3] - b3) * 16.f);
+          }
+        }
+        q1[m] = v8i{static_cast<int>(c1[0]), static_cast<int>(c1[1]), static_cast<int>(c1[2]), static_cast<int>(c1[3]),
+                    static_cast<int>(c1[4]), static_cast<int>(c1[5]), static_cast<int>(c1[6]), static_cast<int>(c1[7])};
+        q2[m] = v8i{static_cast<int>(c2[0]), static_cast<int>(c2[1]), static_cast<int>(c2[2]), static_cast<int>(c2[3]),
+                    static_cast<int>(c2[4]), static_cast<int>(c2[5]), static_cast<int>(c2[6]), static_cast<int>(c2[7])};
+      }
+    }
+  }
+
+  // Per-lane LDS offsets: K fragment of key block b, step s; V^T operand of d block db, 16-key step, read 0 / 1
+  const int k_lane = kCodes ? l32 * L::k_pitch + half * 32 : l32 * L::k_pitch + half * 16;
+  const int v_lane = L::v_off + (4 * half + ((lane & 15) >> 2)) * L::v_pitch + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+
+  v16f o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  float m_use = -INFINITY;  // the row's maximum in the exponents, log2 units
+  float l_run = 0.f;        // this half's row sum
+  constexpr float kShift = kDense ? 0.f : 6.f;  // weights are 2^kShift p
+  float neg_m = kShift;
+
+  // E is too small for the tile of stage `buf`, whose largest scale is `top`: raise it, rescale O, stage the tile's V again.
+  auto raise = [&](int tile, int buf, float top) {
+    const int e_old = ev;
+    set_exponent(top);
+    const float f = __builtin_ldexpf(1.f, max(e_old - ev, -200));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= f;
+    Staged x;
+    Ready y;
+    load_tile(tile, cursor_at(tile), x);
+    convert(x, y, std::true_type{});
+    uint4* dv = reinterpret_cast<uint4*>(lds + buf * L::stage + L::v_off + skey * L::v_pitch + schunk * 32);
+    dv[0] = y.v0;
+    dv[1] = y.v1;
+    __syncthreads();
+  };
+  auto max8 = [&](const float* p) {
+    const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+    return fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+  };
+  auto check_exponent = [&](int tile, int buf, float top) {
+    if constexpr (!kDense) {
+      top = bits_f32(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(f32_bits(top)))));
+      if (top > sv_lim) raise(tile, buf, top);
+    }
+  };
+
+  // One tile: scores with the conversion of the next tile among their matrix instructions; the next tile into the other
+  // stage and the loads of the one after; the row maxima; the weights with O^T += V^T P^T.  PARTIAL: some row may not see
+  // all of this tile or of the next.
+  auto body = [&](int tile, auto PARTIAL) {
+    const int cur = tile & 1;
+    const uint8_t* st = lds + cur * L::stage;
+    const float* us = reinterpret_cast<const float*>(st + L::u_off);
+    Ready nxt;
+    v16f s[2];
+    float top_sv = 0.f;
+    if constexpr (!kDense) top_sv = max8(us + BKV + 8);  // first of the LDS reads: the branch waits for it alone
+#pragma unroll
+    for (int b = 0; b < 2; ++b) s[b] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    if constexpr (kCodes) {
+      v8i kf[2][2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const uint8_t* p = st + k_lane + b * 32 * L::k_pitch + 64 * m;
+          const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 16);
+          kf[b][m] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+      check_exponent(tile, cur, top_sv);
+      convert(sreg, nxt, PARTIAL);
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q2[m], s[b], 0, 0, 0, 127, 0, q_scale - 4);
+          s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q1[m], s[b], 0, 0, 0, 127, 0, q_scale);
+        }
+    } else {
+      uint4 kf[2][8];
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) kf[b][ks] = *reinterpret_cast<const uint4*>(st + k_lane + b * 32 * L::k_pitch + ks * 32);
+      check_exponent(tile, cur, top_sv);
+      convert(sreg, nxt, PARTIAL);
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, kf[b][ks]), qb[ks], s[b], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    write(cur ^ 1, nxt);
+    load_tile(tile + 2, ahead, sreg);
+    // V^T operands of the first two 16-key steps and the keys' factors of the first, in flight during the maxima; those
+    // of step k + 2 (k + 1) are read at step k
+    uint4 vf[2][4];
+    float4 uf[2][2];
+    auto read_v = [&](int k) {
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        const uint8_t* p = st + v_lane + 16 * k * L::v_pitch + db * 64;
+        vf[k & 1][db] = __builtin_bit_cast(uint4, __builtin_shufflevector(read_tr16(p), read_tr16(p + 8 * L::v_pitch), 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    };
+    auto read_u = [&](int k) {
+      if constexpr (!kDense) {
+        uf[k & 1][0] = *reinterpret_cast<const float4*>(us + 16 * k + 4 * half);
+        uf[k & 1][1] = *reinterpret_cast<const float4*>(us + 16 * k + 8 + 4 * half);
+      }
+    };
+    float top_u = 0.f;
+    if constexpr (!kDense) top_u = max8(us + BKV);
+    read_u(0);
+    read_v(0);
+    read_v(1);
+    if constexpr (decltype(PARTIAL)::value) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          s[b][e] = tile * BKV + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= lim ? -INFINITY : s[b][e];
+    }
+    auto factor = [&](float u, float x) {  // a key that the row does not see has a score of -inf and may have any factor
+      if constexpr (decltype(PARTIAL)::value) return x == -INFINITY ? 1.f : u;
+      return u;
+    };
+    // An upper bound of the row's largest exponent from the largest score and the largest factor (0 where every score is
+    // negative); the exact one is taken only when the bound asks for a rescale.
+    float mt = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[b][e]);
+    if constexpr (kDense)
+      mt *= a.c;
+    else
+      mt = mt >= 0.f ? mt * top_u : mt == -INFINITY ? mt : 0.f;
+    mt = max32(mt);
+    const bool fire = mt > m_use + kTau;
+    if (__ballot(fire)) {
+      if constexpr (!kDense) {
+        mt = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 x = *reinterpret_cast<const float4*>(us + 32 * b + 8 * g + 4 * half);
+            const float u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mt = fmaxf(mt, s[b][4 * g + e] * factor(u[e], s[b][4 * g + e]));
+          }
+        mt = max32(mt);
+      }
+      const float m_new = fire ? fmaxf(m_use, mt) : m_use;
+      const float alpha = !fire || m_new == m_use ? 1.f : m_use == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_use - m_new);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] *= alpha;
+      l_run *= alpha;
+      m_use = m_new;
+      neg_m = m_new == -INFINITY ? kShift : kShift - m_new;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int b = k >> 1;
+      if (k < 3) read_u(k + 1);
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = s[b][8 * (k & 1) + e];
+        if constexpr (kDense) {
+          p[e] = __builtin_amdgcn_exp2f(fmaf(x, a.c, neg_m));
+        } else {
+          const float4 y = uf[k & 1][e >> 2];
+          const float u[4] = {y.x, y.y, y.z, y.w};
+          p[e] = __builtin_amdgcn_exp2f(fmaf(x, factor(u[e & 3], x), neg_m));
+        }
+      }
+      uint32_t x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (kDense) {
+          const v2bf one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+          x[e] = cvt_bf16x2(p[2 * e], p[2 * e + 1]);
+          l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, x[e]), one, l_run, false);
+        } else {
+          const v2h one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+          x[e] = cvt_f16x2(p[2 * e], p[2 * e + 1]);
+          l_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, x[e]), one, l_run, false);
+        }
+      }
+      const uint4 pw = make_uint4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        if constexpr (kDense)
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, vf[k & 1][db]), __builtin_bit_cast(v8bf, pw), o[db], 0, 0, 0);
+        else
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[k & 1][db]), __builtin_bit_cast(v8h, pw), o[db], 0, 0, 0);
+      }
+      if (k < 2) read_v(k + 2);
+    }
+  };
+  // A tile that none of the wave's rows sees: its share of the staging.
+  auto stage_only = [&](int tile) {
+    const int cur = tile & 1;
+    if constexpr (!kDense) check_exponent(tile, cur, max8(reinterpret_cast<const float*>(lds + cur * L::stage + L::u_off) + BKV + 8));
+    Ready nxt;
+    convert(sreg, nxt, std::true_type{});
+    write(cur ^ 1, nxt);
+    load_tile(tile + 2, ahead, sreg);
+  };
+
+  if (tile_lo < tile_hi) {
+    Cursor c = cursor_at(tile_lo);
+    load_tile(tile_lo, c, sreg);
+    if constexpr (!kDense) {  // E from the first tile's largest scale of V
+      float* u = reinterpret_cast<float*>(lds + L::u_off);
+      u[BKV + 8 + wave] = keys_max(finite(sreg.sv) ? sreg.sv : 0.f);
+      __syncthreads();
+      set_exponent(max8(u + BKV + 8));
+      __syncthreads();
+    }
+    Ready y;
+    convert(sreg, y, std::true_type{});
+    write(tile_lo & 1, y);
+    c = cursor_next(c, tile_lo + 1);
+    load_tile(tile_lo + 1, c, sreg);
+    ahead = cursor_next(c, tile_lo + 2);
+    __syncthreads();
+    // whole: tiles that every row sees, and the next one too
+    const int whole = min(max(lim_min / BKV - 1, tile_lo), tile_hi);
+    for (int tile = tile_lo; tile < whole; ++tile) {
+      body(tile, std::false_type{});
+      ahead = cursor_next(ahead, tile + 3);
+      __syncthreads();
+    }
+    for (int tile = whole; tile < tile_hi; ++tile) {
+      if (tile * BKV >= wave_max)
+        stage_only(tile);
+      else
+        body(tile, std::true_type{});
+      ahead = cursor_next(ahead, tile + 3);
+      __syncthreads();
+    }
+  }
+
+  // the rows' results: through LDS as bf16 rows (every wave its own; the last barrier has retired the stages), or, with
+  // several splits, in fp32 to the workspace
+  const float l_tot = sum32(l_run);
+  const float inv = l_tot == 0.f ? 0.f : __builtin_ldexpf(1.0f / l_tot, ev);
+  if (splits > 1) {
+    if (!row_ok) return;
+    const int64_t at = ((static_cast<int64_t>(w) * a.n_kv_heads + head) * a.n_splits + split) * R + 32 * wave + l32;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(a.part_o + at * D + 32 * db + 8 * g + 4 * half) =
+            make_float4(o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
+    if (half == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_use, l_tot);
+    return;
+  }
+  uint8_t* ow = lds + wave * 32 * L::o_pitch;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<uint2*>(ow + l32 * L::o_pitch + 64 * db + 16 * g + 8 * half) =
+          make_uint2(cvt_bf16x2(o[db][4 * g] * inv, o[db][4 * g + 1] * inv), cvt_bf16x2(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = 2 * i + half;
+    const uint2 v = *reinterpret_cast<const uint2*>(ow + row * L::o_pitch + 8 * l32);
+    if (my_first + row < t.count) {
+      uint32_t qj, gj;
+      a.group_div.divmod(static_cast<uint32_t>(my_first + row), qj, gj);
+      *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(t.row0 + static_cast<int>(qj)) * a.ldo +
+                                (head * a.group + static_cast<int>(gj)) * D + 4 * l32) = v;
+    }
+  }
+}
+
+}  // namespace
+
+int launch_wide(const Args& a, int src, hipStream_t stream) {
+  const int64_t items = static_cast<int64_t>(a.n_tiles) * a.n_kv_heads * a.n_splits;
+  constexpr int64_t per = kXcds * kRun;
+  const dim3 grid(static_cast<uint32_t>((items + per - 1) / per * per));
+  switch (src) {
+    case SRC_E4M3: hipLaunchKernelGGL(attn_wide_kernel<SRC_E4M3>, grid, dim3(kThreads), 0, stream, a); break;
+    case SRC_INT8: hipLaunchKernelGGL(attn_wide_kernel<SRC_INT8>, grid, dim3(kThreads), 0, stream, a); break;
+    default: hipLaunchKernelGGL(attn_wide_kernel<SRC_DENSE>, grid, dim3(kThreads), 0, stream, a); break;
+  }
+  return check_launch("wf_attn_batch (many rows)");
+}
+
+}  // namespace attn_batch
+}  // namespace wf

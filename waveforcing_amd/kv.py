@@ -287,11 +287,14 @@ class Int8PagePool(Fp8PagePool):
     pack = pack_k_norm_rope = unpack = _one_sequence
 
 
+_MOST = (1 << 31) - 1024   # positions and rows the kernels count in 32 bits, with the tiles they load ahead
+
+
 def _int32_list(xs, name: str) -> list[int]:
     out = [int(x) for x in xs]
     for x in out:
-        if x < 0 or x >= 1 << 31:
-            raise ValueError(f"{name} holds {x}: expected 0 <= {name} < 2^31")
+        if x < 0 or x >= _MOST:
+            raise ValueError(f"{name} holds {x}: expected 0 <= {name} < 2^31 - 1024")
     return out
 
 
@@ -350,7 +353,7 @@ class PagedBatch:
                 raise RuntimeError(f"page table of {len(ids)} pages cannot hold {t} tokens (sequence {b})")
         self.kv_lens, self.new_lens = kv, new
         self.n_new = sum(new)
-        if self.n_new >= 1 << 31:
+        if self.n_new >= _MOST:
             raise ValueError(f"{self.n_new} new rows")
         self._writable = False
 
@@ -437,13 +440,13 @@ class PagedBatch:
         n = self._ws.get(n_heads)
         if n is None:
             n = self._ws[n_heads] = _attn_workspace(self.n_new, n_heads, self.pool.n_heads, self.n_seqs, self.max_new,
-                                                    self.max_kv, True)
+                                                    self.max_kv)
         return n
 
 
-def _attn_workspace(rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv, paged: bool) -> int:
+def _attn_workspace(rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv) -> int:
     n = ctypes.c_int64()
-    _lib.call("wf_attn_batch_workspace", rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv, int(paged), ctypes.addressof(n))
+    _lib.call("wf_attn_batch_workspace", rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv, ctypes.addressof(n))
     return n.value
 
 
@@ -458,7 +461,7 @@ class CrossBatch:
             raise ValueError(f"{len(self.q_lens)} q_lens and {len(self.kv_lens)} kv_lens")
         self.n_seqs = len(self.q_lens)
         self.n_q, self.n_kv = sum(self.q_lens), sum(self.kv_lens)
-        if max(self.n_q, self.n_kv) >= 1 << 31:
+        if max(self.n_q, self.n_kv) >= _MOST:
             raise ValueError(f"{self.n_q} query rows and {self.n_kv} encoder rows")
         self.max_q, self.max_kv = max(self.q_lens, default=0), max(self.kv_lens, default=0)
         dev = torch.tensor(_starts(self.q_lens) + _starts(self.kv_lens), dtype=torch.int32).to(device)
@@ -472,7 +475,7 @@ class CrossBatch:
         n = self._ws.get((n_heads, n_kv_heads))
         if n is None:
             n = self._ws[n_heads, n_kv_heads] = _attn_workspace(self.n_q, n_heads, n_kv_heads, self.n_seqs, self.max_q,
-                                                                self.max_kv, False)
+                                                                self.max_kv)
         return n
 
 
