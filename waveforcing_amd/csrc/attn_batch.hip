@@ -70,7 +70,7 @@ Plan make_plan(int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_se
   int64_t keys = (max_kv * units + want - 1) / want;
   keys = std::max<int64_t>((keys + 127) / 128 * 128, least);
   p.n_splits = std::max<int64_t>(1, (max_kv + keys - 1) / keys);
-  p.split_keys = p.n_splits == 1 ? std::max<int64_t>(128, (max_kv + 127) / 128 * 128) : keys;
+  p.split_keys = std::max<int64_t>(128, ((max_kv + p.n_splits - 1) / p.n_splits + 127) / 128 * 128);
   p.bytes = p.n_splits == 1 ? 0 : ((p.n_tiles * n_kv_heads * p.n_splits) << p.tile_shift) * (D + 2) * 4;
   return p;
 }

@@ -49,11 +49,12 @@ struct Lds {
   static constexpr int k_pitch = codes ? D + 16 : 2 * D + 16;
   static constexpr int v_pitch = 2 * D + 64;
   static constexpr int v_off = BKV * k_pitch;
-  static constexpr int u_off = v_off + BKV * v_pitch;         // u [64], the staging waves' maxima of u [8] and of s_v [8]
-  static constexpr int stage = u_off + (BKV + 8 + 8) * 4;
+  static constexpr int u_off = v_off + BKV * v_pitch;         // u [64], then a word of every staging wave: E is too small
+  static constexpr int stage = u_off + (BKV + 8) * 4;
   static constexpr int o_pitch = 2 * D + 8;
   static constexpr int out = kWaves * 32 * o_pitch;
-  static constexpr int bytes = 2 * stage > out ? 2 * stage : out;
+  static constexpr int bytes = 3 * stage + 32;  // three stages, and the waves' largest scales of V
+  static_assert(bytes >= out, "the results are staged in the same LDS");
 };
 
 __device__ inline uint32_t pk_mul_f16(uint32_t a, v2h f) {
@@ -88,16 +89,22 @@ __device__ inline uint32_t cvt_f16x2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
 }
 
-// Maximum over the 8 keys (lanes 8 k) that a wave stages.
-__device__ inline float keys_max(float v) {
-  const int i = static_cast<int>(f32_bits(v));
-  v = fmaxf(v, bits_f32(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(i, i, 0x128, 0xF, 0xF, false))));  // lane ^ 8
-  return max32(max16(v));
+// Maximum over the 8 keys (lanes 8 k) that a wave stages, of numbers that are not negative: their bits order as they do.
+__device__ inline uint32_t keys_max(float v) {
+  uint32_t i = f32_bits(v);
+  i = max(i, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(i), static_cast<int>(i), 0x128, 0xF, 0xF, false)));  // lane ^ 8
+  float x = bits_f32(i), y = x;
+  swap16(x, y);
+  i = max(f32_bits(x), f32_bits(y));
+  x = y = bits_f32(i);
+  swap32(x, y);
+  return max(f32_bits(x), f32_bits(y));
 }
 
 __device__ inline bool finite(float v) { return (f32_bits(v) & 0x7f800000u) != 0x7f800000u; }
 
-template <int SRC>
+// SMALL: pages of fewer than 64 positions, where every lane finds its own key's page.
+template <int SRC, bool SMALL>
 __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   using L = Lds<SRC>;
   constexpr bool kDense = SRC == SRC_DENSE;
@@ -153,8 +160,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   };
   const int pt = a.geom.page_tokens;
   const int32_t* table = a.geom.tables + static_cast<int64_t>(t.b) * a.geom.ld_table;
-  auto cursor_at = [&](int tile) -> Cursor {
-    if constexpr (kDense) return Cursor{0, BKV, 0, 0, 0};
+  auto cursor_at = [&](int tile) __attribute__((always_inline)) -> Cursor {
+    if constexpr (kDense || SMALL) return Cursor{0, 0, 0, 0, 0};
     uint32_t lp, at;
     a.geom.page.divmod(static_cast<uint32_t>(tile) * BKV, lp, at);
     const int i = static_cast<int>(lp);
@@ -166,8 +173,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     const int pg = ok ? page : 0, r0 = static_cast<int>(at);
     return Cursor{r0, min(pt - r0, BKV), pg * pt + r0, (pg * a.n_kv_heads + head) * pt + r0, ok ? BKV : 0};
   };
-  auto cursor_next = [&](const Cursor& c, int tile) -> Cursor {
-    if constexpr (kDense) return c;
+  auto cursor_next = [&](const Cursor& c, int tile) __attribute__((always_inline)) -> Cursor {
+    if constexpr (kDense || SMALL) return c;
     if (c.at + BKV >= pt) return cursor_at(tile);
     return Cursor{c.at + BKV, min(pt - c.at - BKV, BKV), c.tok + BKV, c.sc + BKV, c.n};
   };
@@ -175,9 +182,17 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(kDense ? a.ldkv * 2 : a.n_kv_heads * D) +
                             (kDense ? 32 : 16) * schunk;  // bytes; rows of a tile stay below 2^31 (checked on the host)
   constexpr int kWord3 = 0x00020000;  // raw buffer, 32-bit data format
-  // The loads of a tile.  Within one page a buffer of the tile's rows that are there reads the others as zero, and a
-  // lane's offset never changes.
-  auto load_tile = [&](int tile, const Cursor& c, Staged& x) {
+  // SMALL: the page of this lane's key in the tile that is loaded next (-1: none), asked for a tile ahead
+  int lane_page = -1;
+  auto find_page = [&](int tile) __attribute__((always_inline)) {
+    const int j = tile * BKV + skey;
+    const int lp = static_cast<int>(a.geom.page.div(static_cast<uint32_t>(j)));
+    lane_page = -1;
+    if (j < k_hi && lp < a.geom.ld_table) lane_page = table[lp];
+  };
+  // The loads of a tile.  Within one page (ONE) a buffer of the tile's rows that are there reads the others as zero, and
+  // a lane's offset never changes.
+  auto load_tile = [&](int tile, const Cursor& c, Staged& x, auto ONE) __attribute__((always_inline)) {
     const int n = min(max(k_hi - tile * BKV, 0), BKV);
     if constexpr (kDense) {
       const int64_t first = static_cast<int64_t>(t.key0 + (n ? tile * BKV : 0)) * a.ldkv + head * D;
@@ -188,7 +203,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       x.k1 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row + 16, 0, 0);
       x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
       x.v1 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row + 16, 0, 0);
-    } else if (c.cut == BKV) {
+    } else if (decltype(ONE)::value || (!SMALL && c.cut == BKV)) {
       const int m = min(n, c.n);
       const int64_t first = static_cast<int64_t>(c.tok * a.n_kv_heads + head) * D;
       const int bytes = m ? ((m - 1) * a.n_kv_heads + 1) * D : 0;
@@ -201,12 +216,19 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       x.sk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * skey, 0, 0));
       x.sv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * skey, 0, 0));
     } else {
-      x.k0 = x.v0 = u32x4{0, 0, 0, 0};
+      int page = lane_page;
+      uint32_t lp, at;
+      a.geom.page.divmod(static_cast<uint32_t>(tile * BKV + skey), lp, at);
+      if constexpr (!SMALL) page = skey < n && static_cast<int>(lp) < a.geom.ld_table ? table[lp] : -1;
+      const bool there = page >= 0 && page < a.geom.pool_pages;
+      page = there ? page : 0;
+      const int64_t off = static_cast<int64_t>((page * pt + static_cast<int>(at)) * a.n_kv_heads + head) * D + 16 * schunk;
+      const int sc = (page * a.n_kv_heads + head) * pt + static_cast<int>(at);
+      const u32x4 zero = {0, 0, 0, 0};
+      x.k0 = zero;
+      x.v0 = zero;
       x.sk = x.sv = 0.f;
-      int page, at;
-      if (skey < n && pool_row(a.geom, t.b, tile * BKV + skey, page, at)) {
-        const int64_t off = static_cast<int64_t>((page * pt + at) * a.n_kv_heads + head) * D + 16 * schunk;
-        const int sc = (page * a.n_kv_heads + head) * pt + at;
+      if (there) {
         x.k0 = *reinterpret_cast<const u32x4*>(a.k_codes + off);
         x.v0 = *reinterpret_cast<const u32x4*>(a.v_codes + off);
         x.sk = a.k_scales[sc];
@@ -217,7 +239,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 
   int ev = 0;            // E: staged V = V 2^-E
   float sv_lim = 0.f;    // the largest scale of V that E allows: 448 2^7 < 65504
-  auto set_exponent = [&](float top) {  // puts the scale `top` below 2^3
+  auto set_exponent = [&](float top) __attribute__((always_inline)) {  // puts the scale `top` below 2^3
     ev = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top) - 3);
     sv_lim = __builtin_ldexpf(1.f, ev + 7);
   };
@@ -227,7 +249,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     float u, sv;
   };
   // The staged tile as it goes to LDS.  PARTIAL: some row may not see all of it.
-  auto convert = [&](Staged x, Ready& y, auto PARTIAL) {
+  auto convert = [&](Staged x, Ready& y, auto PARTIAL) __attribute__((always_inline)) {
     if constexpr (kDense) {
       y.k0 = make_uint4(x.k0[0], x.k0[1], x.k0[2], x.k0[3]);
       y.k1 = make_uint4(x.k1[0], x.k1[1], x.k1[2], x.k1[3]);
@@ -258,8 +280,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       y.v1 = make_uint4(pk_mul_f16(s.x, ff), pk_mul_f16(s.y, ff), pk_mul_f16(v.x, ff), pk_mul_f16(v.y, ff));
     }
   };
-  auto write = [&](int buf, const Ready& y) {
-    uint8_t* st = lds + buf * L::stage;
+  auto write = [&](int stage, const Ready& y) __attribute__((always_inline)) {
+    uint8_t* st = lds + stage;
     uint4* dv = reinterpret_cast<uint4*>(st + L::v_off + skey * L::v_pitch + schunk * 32);
     if constexpr (kCodes) {
       *reinterpret_cast<uint4*>(st + skey * L::k_pitch + schunk * 16) = y.k0;
@@ -271,12 +293,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     dv[0] = y.v0;
     dv[1] = y.v1;
     if constexpr (!kDense) {
-      // the key's factor, and the largest factor (of those that are numbers) and scale of V of the wave's 8 keys; lanes
-      // of one key write the same word
       float* u = reinterpret_cast<float*>(st + L::u_off);
-      u[skey] = y.u;
-      u[BKV + wave] = keys_max(finite(y.u) ? y.u : 0.f);
-      u[BKV + 8 + wave] = keys_max(y.sv);
+      u[skey] = y.u;  // (the lanes of one key write the same word)
+      reinterpret_cast<uint32_t*>(u)[BKV + wave] = __ballot(y.sv > sv_lim) ? 1u : 0u;
     }
   };
 
@@ -345,241 +364,322 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   for (int i = 0; i < 4; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   float m_use = -INFINITY;  // the row's maximum in the exponents, log2 units
   float l_run = 0.f;        // this half's row sum
-  constexpr float kShift = kDense ? 0.f : 6.f;  // weights are 2^kShift p
+  // Weights are 2^kShift p, and a tile's sum of them (of a lane's 32 keys) at most kMostSum: fp16 ends at 65504.
+  constexpr float kShift = kDense ? 0.f : 6.f;
+  constexpr float kMostSum = kDense ? 256.f : 32768.f;
   float neg_m = kShift;
 
-  // E is too small for the tile of stage `buf`, whose largest scale is `top`: raise it, rescale O, stage the tile's V again.
-  auto raise = [&](int tile, int buf, float top) {
-    const int e_old = ev;
-    set_exponent(top);
-    const float f = __builtin_ldexpf(1.f, max(e_old - ev, -200));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] *= f;
+  float pend = 1.f, o_scale = 1.f;
+  float* top_lds = reinterpret_cast<float*>(lds + 3 * L::stage);
+  // The largest scale of V of a staged tile, over the whole workgroup.
+  auto tile_top = [&](const Staged& x) __attribute__((always_inline)) {
+    reinterpret_cast<uint32_t*>(top_lds)[wave] = keys_max(finite(x.sv) ? x.sv : 0.f);
+    __syncthreads();
+    const uint4 p = *reinterpret_cast<const uint4*>(top_lds), q = *reinterpret_cast<const uint4*>(top_lds + 4);
+    return bits_f32(max(max(max(p.x, p.y), max(p.z, p.w)), max(max(q.x, q.y), max(q.z, q.w))));
+  };
+  // E is too small for the tile of stage `buf`: raise it, note that O is to be rescaled (with the next change of a
+  // maximum: one place that rescales keeps O in its registers), stage the tile's V again.
+  auto raise = [&](int tile, int stage) __attribute__((always_inline)) {
     Staged x;
     Ready y;
-    load_tile(tile, cursor_at(tile), x);
+    const int page_ahead = lane_page;
+    if constexpr (SMALL) find_page(tile);
+    load_tile(tile, cursor_at(tile), x, std::false_type{});
+    lane_page = page_ahead;
+    const int e_old = ev;
+    set_exponent(tile_top(x));
+    ev = max(ev, e_old);
+    pend *= __builtin_ldexpf(1.f, max(e_old - ev, -200));
     convert(x, y, std::true_type{});
-    uint4* dv = reinterpret_cast<uint4*>(lds + buf * L::stage + L::v_off + skey * L::v_pitch + schunk * 32);
+    uint4* dv = reinterpret_cast<uint4*>(lds + stage + L::v_off + skey * L::v_pitch + schunk * 32);
     dv[0] = y.v0;
     dv[1] = y.v1;
     __syncthreads();
   };
-  auto max8 = [&](const float* p) {
-    const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
-    return fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+  auto too_small = [&](int stage) __attribute__((always_inline)) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(lds + stage + L::u_off) + BKV;
+    const uint4 x = *reinterpret_cast<const uint4*>(p), y = *reinterpret_cast<const uint4*>(p + 4);
+    return (x.x | x.y | x.z | x.w) | (y.x | y.y | y.z | y.w);
   };
-  auto check_exponent = [&](int tile, int buf, float top) {
+  auto check_exponent = [&](int tile, int stage) __attribute__((always_inline)) {
     if constexpr (!kDense) {
-      top = bits_f32(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(f32_bits(top)))));
-      if (top > sv_lim) raise(tile, buf, top);
+      if (__builtin_amdgcn_readfirstlane(static_cast<int>(too_small(stage)))) raise(tile, stage);
     }
   };
 
-  // One tile: scores with the conversion of the next tile among their matrix instructions; the next tile into the other
-  // stage and the loads of the one after; the row maxima; the weights with O^T += V^T P^T.  PARTIAL: some row may not see
-  // all of this tile or of the next.
-  auto body = [&](int tile, auto PARTIAL) {
-    const int cur = tile & 1;
-    const uint8_t* st = lds + cur * L::stage;
-    const float* us = reinterpret_cast<const float*>(st + L::u_off);
-    Ready nxt;
-    v16f s[2];
-    float top_sv = 0.f;
-    if constexpr (!kDense) top_sv = max8(us + BKV + 8);  // first of the LDS reads: the branch waits for it alone
+  // Stages (bytes in LDS) of the tiles t - 1, t and t + 1.
+  int st_prev = 0, st_cur = L::stage, st_next = 2 * L::stage;
+  v16f s[2];        // scores of a tile, between its products and its weights
+  uint32_t pw[16];  // weights of a tile, between them and their product with V
 #pragma unroll
-    for (int b = 0; b < 2; ++b) s[b] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    if constexpr (kCodes) {
-      v8i kf[2][2];
+  for (int i = 0; i < 16; ++i) pw[i] = 0;
+
+  uint4 vf[2][4];
+  auto read_v = [&](int stage, int k) __attribute__((always_inline)) {  // V^T operands of 16-key step k
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const uint8_t* p = st + k_lane + b * 32 * L::k_pitch + 64 * m;
-          const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 16);
-          kf[b][m] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-      check_exponent(tile, cur, top_sv);
-      convert(sreg, nxt, PARTIAL);
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q2[m], s[b], 0, 0, 0, 127, 0, q_scale - 4);
-          s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q1[m], s[b], 0, 0, 0, 127, 0, q_scale);
-        }
-    } else {
-      uint4 kf[2][8];
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) kf[b][ks] = *reinterpret_cast<const uint4*>(st + k_lane + b * 32 * L::k_pitch + ks * 32);
-      check_exponent(tile, cur, top_sv);
-      convert(sreg, nxt, PARTIAL);
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, kf[b][ks]), qb[ks], s[b], 0, 0, 0);
+    for (int db = 0; db < 4; ++db) {
+      const uint8_t* p = lds + stage + v_lane + 16 * k * L::v_pitch + db * 64;
+      vf[k & 1][db] = __builtin_bit_cast(uint4, __builtin_shufflevector(read_tr16(p), read_tr16(p + 8 * L::v_pitch), 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    __builtin_amdgcn_sched_barrier(0);
-    write(cur ^ 1, nxt);
-    load_tile(tile + 2, ahead, sreg);
-    // V^T operands of the first two 16-key steps and the keys' factors of the first, in flight during the maxima; those
-    // of step k + 2 (k + 1) are read at step k
-    uint4 vf[2][4];
-    float4 uf[2][2];
-    auto read_v = [&](int k) {
+  };
+  // O^T += V^T P^T of the tile in `stage`; steps 0 and 1 of its V are being read.
+  auto pv = [&](int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint4 w = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
-        const uint8_t* p = st + v_lane + 16 * k * L::v_pitch + db * 64;
-        vf[k & 1][db] = __builtin_bit_cast(uint4, __builtin_shufflevector(read_tr16(p), read_tr16(p + 8 * L::v_pitch), 0, 1, 2, 3, 4, 5, 6, 7));
+        if constexpr (kDense)
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, vf[k & 1][db]), __builtin_bit_cast(v8bf, w), o[db], 0, 0, 0);
+        else
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[k & 1][db]), __builtin_bit_cast(v8h, w), o[db], 0, 0, 0);
+      }
+      if (k < 2) read_v(stage, k + 2);
+    }
+  };
+
+  // The matrix half of tile t: O += the tile before (steps 0 and 1 of its V have been asked for), the scores of t, and
+  // among the products the staging of tile t + 1 and the loads of t + 2.  PARTIAL: some row may not see all of t + 1, the
+  // wave may see none of t, or the tile to be loaded may span pages; without it the half is one block of instructions.
+  float4 uf[2][2];
+  auto read_u = [&](int stage, int k) __attribute__((always_inline)) {  // factors of the lane's keys in 16-key step k
+    if constexpr (!kDense) {
+      const float* us = reinterpret_cast<const float*>(lds + stage + L::u_off);
+      uf[k & 1][0] = *reinterpret_cast<const float4*>(us + 16 * k + 4 * half);
+      uf[k & 1][1] = *reinterpret_cast<const float4*>(us + 16 * k + 8 + 4 * half);
+    }
+  };
+  auto products = [&](int tile, auto PARTIAL) __attribute__((always_inline)) {
+    constexpr bool kPartial = decltype(PARTIAL)::value;
+    using One = std::bool_constant<!kPartial && !SMALL>;
+    const uint8_t* st = lds + st_cur;
+    Ready nxt;
+    o_scale *= pend;
+    pend = 1.f;
+    __builtin_amdgcn_s_setprio(1);
+    auto scores = [&](const auto& kf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) s[b] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int m = i >> 2, b = i & 1;
+          if (i & 2)
+            s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q1[m], s[b], 0, 0, 0, 127, 0, q_scale);
+          else
+            s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q2[m], s[b], 0, 0, 0, 127, 0, q_scale - 4);
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, kf[b][ks]), qb[ks], s[b], 0, 0, 0);
       }
     };
-    auto read_u = [&](int k) {
-      if constexpr (!kDense) {
-        uf[k & 1][0] = *reinterpret_cast<const float4*>(us + 16 * k + 4 * half);
-        uf[k & 1][1] = *reinterpret_cast<const float4*>(us + 16 * k + 8 + 4 * half);
+    std::conditional_t<kCodes, v8i, uint4> kf[2][kCodes ? 2 : 8];
+#pragma unroll
+    for (int i = 0; i < (kCodes ? 2 : 8); ++i)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if constexpr (kCodes) {
+          const uint8_t* p = st + k_lane + b * 32 * L::k_pitch + 64 * i;
+          const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 16);
+          kf[b][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+          kf[b][i] = *reinterpret_cast<const uint4*>(st + k_lane + b * 32 * L::k_pitch + i * 32);
+        }
       }
-    };
-    float top_u = 0.f;
-    if constexpr (!kDense) top_u = max8(us + BKV);
-    read_u(0);
-    read_v(0);
-    read_v(1);
-    if constexpr (decltype(PARTIAL)::value) {
+    pv(st_prev);
+    convert(sreg, nxt, PARTIAL);
+    if constexpr (!kPartial) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction, an LDS read or two, some vector work
+        __builtin_amdgcn_sched_group_barrier(0x100, kCodes ? 2 : 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (!kPartial || tile * BKV < wave_max) scores(kf);
+    write(st_next, nxt);
+    load_tile(tile + 2, ahead, sreg, One{});
+    if constexpr (SMALL) find_page(tile + 3);
+    read_u(st_cur, 0);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // The vector half: the weights of tile t (in `stage`) from its scores.
+  auto weigh = [&](int tile, int stage, auto PARTIAL) __attribute__((always_inline)) {
+    constexpr bool kPartial = decltype(PARTIAL)::value;
+    const float* us = reinterpret_cast<const float*>(lds + stage + L::u_off);
+    if (kPartial && tile * BKV >= wave_max) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pw[i] = 0;
+      read_v(stage, 0);
+      read_v(stage, 1);
+      return;
+    }
+    if constexpr (kPartial) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           s[b][e] = tile * BKV + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= lim ? -INFINITY : s[b][e];
     }
-    auto factor = [&](float u, float x) {  // a key that the row does not see has a score of -inf and may have any factor
-      if constexpr (decltype(PARTIAL)::value) return x == -INFINITY ? 1.f : u;
+    auto factor = [&](float u, float x) __attribute__((always_inline)) {  // a key that the row does not see has a score of -inf and may have any factor
+      if constexpr (kPartial) return x == -INFINITY ? 1.f : u;
       return u;
     };
-    // An upper bound of the row's largest exponent from the largest score and the largest factor (0 where every score is
-    // negative); the exact one is taken only when the bound asks for a rescale.
-    float mt = -INFINITY;
+    // The weights against the maximum so far.  Whether it still serves shows in their sum: a weight past the limit makes
+    // the sum reach it, and then (as before a row's first key) the exact maximum is taken and the weights are computed
+    // again.  So no tile pays for a maximum that does not change.
+    float l_tile;
+    auto weights = [&]() __attribute__((always_inline)) {
+      l_tile = 0.f;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int k = 0; k < 4; ++k) {
+        const int b = k >> 1;
+        if (k < 3) read_u(stage, k + 1);
+        float p[8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[b][e]);
-    if constexpr (kDense)
-      mt *= a.c;
-    else
-      mt = mt >= 0.f ? mt * top_u : mt == -INFINITY ? mt : 0.f;
-    mt = max32(mt);
-    const bool fire = mt > m_use + kTau;
-    if (__ballot(fire)) {
-      if constexpr (!kDense) {
-        mt = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float4 x = *reinterpret_cast<const float4*>(us + 32 * b + 8 * g + 4 * half);
-            const float u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mt = fmaxf(mt, s[b][4 * g + e] * factor(u[e], s[b][4 * g + e]));
+        for (int e = 0; e < 8; ++e) {
+          const float x = s[b][8 * (k & 1) + e];
+          if constexpr (kDense) {
+            p[e] = __builtin_amdgcn_exp2f(fmaf(x, a.c, neg_m));
+          } else {
+            const float4 y = uf[k & 1][e >> 2];
+            const float u[4] = {y.x, y.y, y.z, y.w};
+            p[e] = __builtin_amdgcn_exp2f(fmaf(x, factor(u[e & 3], x), neg_m));
           }
-        mt = max32(mt);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (kDense) {
+            const v2bf one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+            pw[4 * k + e] = cvt_bf16x2(p[2 * e], p[2 * e + 1]);
+            l_tile = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pw[4 * k + e]), one, l_tile, false);
+          } else {
+            const v2h one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+            pw[4 * k + e] = cvt_f16x2(p[2 * e], p[2 * e + 1]);
+            l_tile = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, pw[4 * k + e]), one, l_tile, false);
+          }
+        }
       }
+    };
+    weights();
+    // (a NaN sum needs no other maximum; m_use is -inf until the row has seen a key, and its weights count for nothing)
+    if (__ballot(l_tile > kMostSum || m_use == -INFINITY) || o_scale != 1.f) {
+      float mt = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float4 x;
+          if constexpr (!kDense) x = *reinterpret_cast<const float4*>(us + 32 * b + 8 * g + 4 * half);
+          const float u[4] = {kDense ? a.c : x.x, kDense ? a.c : x.y, kDense ? a.c : x.z, kDense ? a.c : x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mt = fmaxf(mt, s[b][4 * g + e] * factor(u[e], s[b][4 * g + e]));
+        }
+      mt = max32(mt);
+      const bool fire = max32(l_tile) > kMostSum || m_use == -INFINITY;
       const float m_new = fire ? fmaxf(m_use, mt) : m_use;
       const float alpha = !fire || m_new == m_use ? 1.f : m_use == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_use - m_new);
+      const float beta = alpha * o_scale;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] *= alpha;
+      for (int i = 0; i < 4; ++i) o[i] *= beta;
+      o_scale = 1.f;
       l_run *= alpha;
       m_use = m_new;
       neg_m = m_new == -INFINITY ? kShift : kShift - m_new;
+      read_u(stage, 0);
+      weights();
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int b = k >> 1;
-      if (k < 3) read_u(k + 1);
-      float p[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = s[b][8 * (k & 1) + e];
-        if constexpr (kDense) {
-          p[e] = __builtin_amdgcn_exp2f(fmaf(x, a.c, neg_m));
-        } else {
-          const float4 y = uf[k & 1][e >> 2];
-          const float u[4] = {y.x, y.y, y.z, y.w};
-          p[e] = __builtin_amdgcn_exp2f(fmaf(x, factor(u[e & 3], x), neg_m));
-        }
-      }
-      uint32_t x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (kDense) {
-          const v2bf one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
-          x[e] = cvt_bf16x2(p[2 * e], p[2 * e + 1]);
-          l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, x[e]), one, l_run, false);
-        } else {
-          const v2h one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-          x[e] = cvt_f16x2(p[2 * e], p[2 * e + 1]);
-          l_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, x[e]), one, l_run, false);
-        }
-      }
-      const uint4 pw = make_uint4(x[0], x[1], x[2], x[3]);
-#pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        if constexpr (kDense)
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, vf[k & 1][db]), __builtin_bit_cast(v8bf, pw), o[db], 0, 0, 0);
-        else
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[k & 1][db]), __builtin_bit_cast(v8h, pw), o[db], 0, 0, 0);
-      }
-      if (k < 2) read_v(k + 2);
-    }
-  };
-  // A tile that none of the wave's rows sees: its share of the staging.
-  auto stage_only = [&](int tile) {
-    const int cur = tile & 1;
-    if constexpr (!kDense) check_exponent(tile, cur, max8(reinterpret_cast<const float*>(lds + cur * L::stage + L::u_off) + BKV + 8));
-    Ready nxt;
-    convert(sreg, nxt, std::true_type{});
-    write(cur ^ 1, nxt);
-    load_tile(tile + 2, ahead, sreg);
+    l_run += l_tile;
+    read_v(stage, 0);
+    read_v(stage, 1);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
+  // The waves of a SIMD (w and w + 4) are half a tile apart: while one runs its products the other computes weights, so
+  // neither the matrix cores nor the vector unit waits for the other.  A barrier ends each half; the late waves read V of
+  // tile t - 1 while the early ones stage t + 1, hence three stages.
   if (tile_lo < tile_hi) {
+    const bool late = wave >= kWaves / 2;
     Cursor c = cursor_at(tile_lo);
-    load_tile(tile_lo, c, sreg);
-    if constexpr (!kDense) {  // E from the first tile's largest scale of V
-      float* u = reinterpret_cast<float*>(lds + L::u_off);
-      u[BKV + 8 + wave] = keys_max(finite(sreg.sv) ? sreg.sv : 0.f);
-      __syncthreads();
-      set_exponent(max8(u + BKV + 8));
-      __syncthreads();
-    }
+    if constexpr (SMALL) find_page(tile_lo);
+    load_tile(tile_lo, c, sreg, std::false_type{});
+    if constexpr (!kDense) set_exponent(tile_top(sreg));
     Ready y;
     convert(sreg, y, std::true_type{});
-    write(tile_lo & 1, y);
+    write(st_cur, y);
+    {  // the tile before the first: no weights, and V that they can multiply
+      uint4* dv = reinterpret_cast<uint4*>(lds + st_prev + L::v_off + skey * L::v_pitch + schunk * 32);
+      dv[0] = dv[1] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vf[i >> 2][i & 3] = make_uint4(0, 0, 0, 0);
     c = cursor_next(c, tile_lo + 1);
-    load_tile(tile_lo + 1, c, sreg);
+    if constexpr (SMALL) find_page(tile_lo + 1);
+    load_tile(tile_lo + 1, c, sreg, std::false_type{});
     ahead = cursor_next(c, tile_lo + 2);
+    if constexpr (SMALL) find_page(tile_lo + 2);
     __syncthreads();
     // whole: tiles that every row sees, and the next one too
     const int whole = min(max(lim_min / BKV - 1, tile_lo), tile_hi);
-    for (int tile = tile_lo; tile < whole; ++tile) {
-      body(tile, std::false_type{});
-      ahead = cursor_next(ahead, tile + 3);
+    auto one_page = [&]() __attribute__((always_inline)) { return kDense || SMALL || ahead.cut == BKV; };
+    auto rotate = [&](const Cursor& after) __attribute__((always_inline)) {
+      const int x = st_prev;
+      st_prev = st_cur;
+      st_cur = st_next;
+      st_next = x;
+      ahead = after;
+    };
+    int tile = tile_lo;
+    if (!late) {
+      auto step = [&](auto PARTIAL) __attribute__((always_inline)) {
+        check_exponent(tile, st_cur);
+        const Cursor after = cursor_next(ahead, tile + 3);  // (branches come first: behind them the tile is one block)
+        products(tile, PARTIAL);
+        weigh(tile, st_cur, PARTIAL);
+        rotate(after);
+        __syncthreads();
+        ++tile;
+      };
+      while (tile < tile_hi) {
+        while (tile < whole && one_page()) step(std::false_type{});  // (a loop of its own: O stays in its registers)
+        if (tile < tile_hi) step(std::true_type{});
+      }
+    } else {
+      products(tile, std::true_type{});
+      rotate(cursor_next(ahead, tile + 3));
       __syncthreads();
+      ++tile;
+      auto step = [&](auto PARTIAL) __attribute__((always_inline)) {
+        check_exponent(tile, st_cur);
+        const Cursor after = cursor_next(ahead, tile + 3);
+        weigh(tile - 1, st_prev, PARTIAL);
+        products(tile, PARTIAL);
+        rotate(after);
+        __syncthreads();
+        ++tile;
+      };
+      while (tile < tile_hi) {
+        while (tile < whole && one_page()) step(std::false_type{});
+        if (tile < tile_hi) step(std::true_type{});
+      }
+      weigh(tile - 1, st_prev, std::true_type{});
     }
-    for (int tile = whole; tile < tile_hi; ++tile) {
-      if (tile * BKV >= wave_max)
-        stage_only(tile);
-      else
-        body(tile, std::true_type{});
-      ahead = cursor_next(ahead, tile + 3);
-      __syncthreads();
-    }
+    pv(st_prev);
+    __syncthreads();
   }
 
   // the rows' results: through LDS as bf16 rows (every wave its own; the last barrier has retired the stages), or, with
   // several splits, in fp32 to the workspace
   const float l_tot = sum32(l_run);
-  const float inv = l_tot == 0.f ? 0.f : __builtin_ldexpf(1.0f / l_tot, ev);
+  const float inv = l_tot == 0.f ? 0.f : __builtin_ldexpf(o_scale / l_tot, ev);
   if (splits > 1) {
     if (!row_ok) return;
     const int64_t at = ((static_cast<int64_t>(w) * a.n_kv_heads + head) * a.n_splits + split) * R + 32 * wave + l32;
@@ -618,11 +718,11 @@ int launch_wide(const Args& a, int src, hipStream_t stream) {
   const int64_t items = static_cast<int64_t>(a.n_tiles) * a.n_kv_heads * a.n_splits;
   constexpr int64_t per = kXcds * kRun;
   const dim3 grid(static_cast<uint32_t>((items + per - 1) / per * per));
-  switch (src) {
-    case SRC_E4M3: hipLaunchKernelGGL(attn_wide_kernel<SRC_E4M3>, grid, dim3(kThreads), 0, stream, a); break;
-    case SRC_INT8: hipLaunchKernelGGL(attn_wide_kernel<SRC_INT8>, grid, dim3(kThreads), 0, stream, a); break;
-    default: hipLaunchKernelGGL(attn_wide_kernel<SRC_DENSE>, grid, dim3(kThreads), 0, stream, a); break;
-  }
+  const bool small = a.geom.page_tokens < BKV;
+  void (*kernel)(Args) = attn_wide_kernel<SRC_DENSE, false>;
+  if (src == SRC_E4M3) kernel = small ? attn_wide_kernel<SRC_E4M3, true> : attn_wide_kernel<SRC_E4M3, false>;
+  if (src == SRC_INT8) kernel = small ? attn_wide_kernel<SRC_INT8, true> : attn_wide_kernel<SRC_INT8, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
   return check_launch("wf_attn_batch (many rows)");
 }
 
