@@ -11,6 +11,9 @@
 #include "attn_batch.hpp"
 #include "gemm_core.hpp"
 
+#include <algorithm>
+#include <cmath>
+
 namespace wf {
 namespace attn_batch {
 namespace {
@@ -64,12 +67,30 @@ Plan make_plan(int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_se
   Plan p;
   p.tile_shift = most <= 16 ? 4 : most <= 32 ? 5 : most <= 64 ? 6 : 8;
   p.n_tiles = ((n_rows * group) >> p.tile_shift) + n_seqs;
-  const int64_t wide = p.tile_shift == 8;
   const int64_t full = std::max<int64_t>(1, std::min<int64_t>(p.n_tiles, n_seqs * ((most + (1ll << p.tile_shift) - 1) >> p.tile_shift)));
-  const int64_t units = full * n_kv_heads, want = (wide ? 2 : 4) * cus, least = wide ? 1024 : 256;
-  int64_t keys = (max_kv * units + want - 1) / want;
-  keys = std::max<int64_t>((keys + 127) / 128 * 128, least);
-  p.n_splits = std::max<int64_t>(1, (max_kv + keys - 1) / keys);
+  const int64_t units = full * n_kv_heads;
+  p.n_splits = 1;
+  if (p.tile_shift == 8) {
+    // In times of one 64-key tile of a workgroup (about 2 us, one workgroup to a CU): a piece takes its tiles and a fixed
+    // part of about 4; the rounds of pieces of one sequence (the pieces of several, whose lengths differ, spread over
+    // the CUs with half a piece at the end); partial results of 256 rows are written and read at about 0.03.
+    const double tiles = static_cast<double>((max_kv + 63) / 64);
+    double best = 0;
+    for (int64_t s = 1; s <= 64 && (s == 1 || tiles / s >= 8); ++s) {
+      const double pieces = static_cast<double>(units * s), per = tiles / s;
+      const double rounds = pieces / cus;
+      double cost = n_seqs == 1 ? std::ceil(rounds) * (per + 4) : std::max(rounds, 1.0) * (0.7 * per + 4) + 0.5 * per;
+      if (s > 1) cost += 1.5 + 0.03 * pieces;
+      if (s == 1 || cost < best) {
+        best = cost;
+        p.n_splits = s;
+      }
+    }
+  } else {
+    const int64_t want = 4 * cus;
+    const int64_t keys = std::max<int64_t>(((max_kv * units + want - 1) / want + 127) / 128 * 128, 256);
+    p.n_splits = std::max<int64_t>(1, (max_kv + keys - 1) / keys);
+  }
   p.split_keys = std::max<int64_t>(128, ((max_kv + p.n_splits - 1) / p.n_splits + 127) / 128 * 128);
   p.bytes = p.n_splits == 1 ? 0 : ((p.n_tiles * n_kv_heads * p.n_splits) << p.tile_shift) * (D + 2) * 4;
   return p;

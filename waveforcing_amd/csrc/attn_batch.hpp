@@ -48,6 +48,9 @@ struct Args {
   BatchGeom geom;
 };
 
+// A value that all lanes hold, in a scalar register.
+__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Sequence of row tile w (uniform); n_seqs > 0.
 __device__ inline int tile_seq(const Args& a, int w) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
@@ -75,21 +78,21 @@ struct Tile {
 
 template <bool DENSE>
 __device__ inline bool find_tile(const Args& a, int w, Tile& t) {
-  t.b = tile_seq(a, w);
+  t.b = uniform(tile_seq(a, w));
   if (t.b < 0) return false;
-  t.row0 = a.geom.cu[t.b];
-  const int end = min(a.geom.cu[t.b + 1], a.n_rows);
+  t.row0 = uniform(a.geom.cu[t.b]);
+  const int end = min(uniform(a.geom.cu[t.b + 1]), a.n_rows);
   t.n_new = end - t.row0;
   if (t.row0 < 0 || t.n_new <= 0) return false;
   t.first = (w - ((t.row0 * a.group) >> a.tile_shift) - t.b) << a.tile_shift;
   t.count = t.n_new * a.group;
   if (t.first < 0 || t.first >= t.count) return false;
   if constexpr (DENSE) {
-    t.key0 = min(max(a.cu_kv[t.b], 0), a.n_kv_rows);
-    t.kv_len = min(max(a.cu_kv[t.b + 1], t.key0), a.n_kv_rows) - t.key0;
+    t.key0 = min(max(uniform(a.cu_kv[t.b]), 0), a.n_kv_rows);
+    t.kv_len = min(max(uniform(a.cu_kv[t.b + 1]), t.key0), a.n_kv_rows) - t.key0;
   } else {
     t.key0 = 0;
-    t.kv_len = min(max(a.geom.kv_lens[t.b], 0), kMaxKeys);
+    t.kv_len = min(max(uniform(a.geom.kv_lens[t.b]), 0), kMaxKeys);
   }
   return true;
 }

@@ -49,11 +49,11 @@ struct Lds {
   static constexpr int k_pitch = codes ? D + 16 : 2 * D + 16;
   static constexpr int v_pitch = 2 * D + 64;
   static constexpr int v_off = BKV * k_pitch;
-  static constexpr int u_off = v_off + BKV * v_pitch;         // u [64], then a word of every staging wave: E is too small
-  static constexpr int stage = u_off + (BKV + 8) * 4;
+  static constexpr int u_off = v_off + BKV * v_pitch;         // u [64]
+  static constexpr int stage = u_off + BKV * 4;
   static constexpr int o_pitch = 2 * D + 8;
   static constexpr int out = kWaves * 32 * o_pitch;
-  static constexpr int bytes = 3 * stage + 32;  // three stages, and the waves' largest scales of V
+  static constexpr int bytes = 3 * stage;
   static_assert(bytes >= out, "the results are staged in the same LDS");
 };
 
@@ -89,18 +89,6 @@ __device__ inline uint32_t cvt_f16x2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
 }
 
-// Maximum over the 8 keys (lanes 8 k) that a wave stages, of numbers that are not negative: their bits order as they do.
-__device__ inline uint32_t keys_max(float v) {
-  uint32_t i = f32_bits(v);
-  i = max(i, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(i), static_cast<int>(i), 0x128, 0xF, 0xF, false)));  // lane ^ 8
-  float x = bits_f32(i), y = x;
-  swap16(x, y);
-  i = max(f32_bits(x), f32_bits(y));
-  x = y = bits_f32(i);
-  swap32(x, y);
-  return max(f32_bits(x), f32_bits(y));
-}
-
 __device__ inline bool finite(float v) { return (f32_bits(v) & 0x7f800000u) != 0x7f800000u; }
 
 // SMALL: pages of fewer than 64 positions, where every lane finds its own key's page.
@@ -125,14 +113,14 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   if (i_lin >= n_items) return;
   const int w = a.n_tiles - 1 - i_lin % a.n_tiles;
   const int hs = i_lin / a.n_tiles;
-  const int head = hs % a.n_kv_heads, split = hs / a.n_kv_heads;
+  const int head = hs % a.n_kv_heads, split = a.n_splits - 1 - hs / a.n_kv_heads;  // (what only long caches have first)
   Tile t;
   if (!find_tile<kDense>(a, w, t)) return;
   const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
   const int splits = used_splits(a, lim_max);
   if (split >= splits) return;
   const int k_lo = split * a.split_keys;
-  const int k_hi = split == splits - 1 ? lim_max : k_lo + a.split_keys;
+  const int k_hi = uniform(split == splits - 1 ? lim_max : k_lo + a.split_keys);
   const int tile_lo = k_lo / BKV, tile_hi = (k_hi + BKV - 1) / BKV;
 
   // this wave's rows: the lane's own, and the largest limit
@@ -150,18 +138,28 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   const int skey = tid >> 3, schunk = tid & 7;
   struct Staged {
     u32x4 k0, v0, k1, v1;
-    float sk, sv;
+    float sk, sv;   // the key's scales
+    float sv_lane;  // the scale of V of key `lane` of the tile: every wave sees all 64
   };
   Staged sreg;
-  // Where a tile's keys live (uniform).  Keys before `cut` are rows tok + key of the pool (scales sc + key), `n` of them to
-  // be read; a page boundary inside the tile makes cut < 64, and then every lane finds its own key.
+  // Where a tile's keys live (uniform): the first key's row of K and its scale, those of V at the same distance from
+  // their pool's start.  A page boundary inside the tile makes cut < 64, and then every lane finds its own key.
   struct Cursor {
-    int at, cut, tok, sc, n;
+    int at, cut, n;   // place in the page; keys to its end; keys that may be read (0: no page)
+    const uint8_t* k;
+    const float* sk;
   };
   const int pt = a.geom.page_tokens;
   const int32_t* table = a.geom.tables + static_cast<int64_t>(t.b) * a.geom.ld_table;
+  const int64_t key_bytes = kDense ? a.ldkv * 2 : static_cast<int64_t>(a.n_kv_heads) * D;
+  const int64_t k_to_v = kDense ? reinterpret_cast<const uint8_t*>(a.v_dense) - reinterpret_cast<const uint8_t*>(a.k_dense)
+                                : a.v_codes - a.k_codes;
+  const int64_t sk_to_sv = reinterpret_cast<const uint8_t*>(a.v_scales) - reinterpret_cast<const uint8_t*>(a.k_scales);
   auto cursor_at = [&](int tile) __attribute__((always_inline)) -> Cursor {
-    if constexpr (kDense || SMALL) return Cursor{0, 0, 0, 0, 0};
+    if constexpr (SMALL) return Cursor{};
+    if constexpr (kDense)
+      return Cursor{0, BKV, BKV, reinterpret_cast<const uint8_t*>(a.k_dense + head * D) + (static_cast<int64_t>(t.key0) + tile * BKV) * key_bytes,
+                    nullptr};
     uint32_t lp, at;
     a.geom.page.divmod(static_cast<uint32_t>(tile) * BKV, lp, at);
     const int i = static_cast<int>(lp);
@@ -171,64 +169,61 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     asm volatile("" ::"s"(page));  // awaited here, not among the LDS reads of the tile
     const bool ok = page >= 0 && page < a.geom.pool_pages;
     const int pg = ok ? page : 0, r0 = static_cast<int>(at);
-    return Cursor{r0, min(pt - r0, BKV), pg * pt + r0, (pg * a.n_kv_heads + head) * pt + r0, ok ? BKV : 0};
+    return Cursor{r0, min(pt - r0, BKV), ok ? BKV : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * D,
+                  a.k_scales + ((pg * a.n_kv_heads + head) * pt + r0)};
   };
   auto cursor_next = [&](const Cursor& c, int tile) __attribute__((always_inline)) -> Cursor {
-    if constexpr (kDense || SMALL) return c;
-    if (c.at + BKV >= pt) return cursor_at(tile);
-    return Cursor{c.at + BKV, min(pt - c.at - BKV, BKV), c.tok + BKV, c.sc + BKV, c.n};
+    if constexpr (SMALL) return c;
+    if (!kDense && c.at + BKV >= pt) return cursor_at(tile);
+    return Cursor{c.at + (kDense ? 0 : BKV), kDense ? BKV : min(pt - c.at - BKV, BKV), c.n, c.k + BKV * key_bytes, c.sk + (kDense ? 0 : BKV)};
   };
   Cursor ahead{};
-  const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(kDense ? a.ldkv * 2 : a.n_kv_heads * D) +
-                            (kDense ? 32 : 16) * schunk;  // bytes; rows of a tile stay below 2^31 (checked on the host)
+  const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(key_bytes) +
+                            (kDense ? 32 : 16) * schunk;  // rows of a tile stay below 2^31 bytes (checked on the host)
   constexpr int kWord3 = 0x00020000;  // raw buffer, 32-bit data format
-  // SMALL: the page of this lane's key in the tile that is loaded next (-1: none), asked for a tile ahead
-  int lane_page = -1;
-  auto find_page = [&](int tile) __attribute__((always_inline)) {
-    const int j = tile * BKV + skey;
+  // SMALL: the pages of this lane's keys (skey and lane) in the tile that is loaded next (-1: none), asked for a tile ahead
+  int page_key = -1, page_lane = -1;
+  auto find_page = [&](int j) __attribute__((always_inline)) {
     const int lp = static_cast<int>(a.geom.page.div(static_cast<uint32_t>(j)));
-    lane_page = -1;
-    if (j < k_hi && lp < a.geom.ld_table) lane_page = table[lp];
+    return j < k_hi && lp < a.geom.ld_table ? table[lp] : -1;
+  };
+  auto find_pages = [&](int tile) __attribute__((always_inline)) {
+    page_key = find_page(tile * BKV + skey);
+    page_lane = find_page(tile * BKV + lane);
   };
   // The loads of a tile.  Within one page (ONE) a buffer of the tile's rows that are there reads the others as zero, and
   // a lane's offset never changes.
   auto load_tile = [&](int tile, const Cursor& c, Staged& x, auto ONE) __attribute__((always_inline)) {
-    const int n = min(max(k_hi - tile * BKV, 0), BKV);
-    if constexpr (kDense) {
-      const int64_t first = static_cast<int64_t>(t.key0 + (n ? tile * BKV : 0)) * a.ldkv + head * D;
-      const int bytes = n ? (n - 1) * static_cast<int>(a.ldkv) * 2 + 2 * D : 0;
-      const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.k_dense + first), 0, bytes, kWord3);
-      const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.v_dense + first), 0, bytes, kWord3);
-      x.k0 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row, 0, 0);
-      x.k1 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row + 16, 0, 0);
-      x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
-      x.v1 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row + 16, 0, 0);
-    } else if (decltype(ONE)::value || (!SMALL && c.cut == BKV)) {
+    const int n = uniform(min(max(k_hi - tile * BKV, 0), BKV));
+    if (kDense || decltype(ONE)::value || (!SMALL && c.cut == BKV)) {
       const int m = min(n, c.n);
-      const int64_t first = static_cast<int64_t>(c.tok * a.n_kv_heads + head) * D;
-      const int bytes = m ? ((m - 1) * a.n_kv_heads + 1) * D : 0;
-      const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.k_codes + first), 0, bytes, kWord3);
-      const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.v_codes + first), 0, bytes, kWord3);
-      const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.k_scales + c.sc), 0, 4 * m, kWord3);
-      const auto sv = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.v_scales + c.sc), 0, 4 * m, kWord3);
+      const int bytes = m ? (m - 1) * static_cast<int>(key_bytes) + (kDense ? 2 * D : D) : 0;
+      const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k), 0, bytes, kWord3);
+      const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k + k_to_v), 0, bytes, kWord3);
+      if constexpr (!kDense) {
+        const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(c.sk), 0, 4 * m, kWord3);
+        const auto sv = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(c.sk) + sk_to_sv), 0, 4 * m, kWord3);
+        x.sv_lane = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * lane, 0, 0));
+        x.sk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * skey, 0, 0));
+        x.sv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * skey, 0, 0));
+      }
       x.k0 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row, 0, 0);
+      if constexpr (kDense) x.k1 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row + 16, 0, 0);
       x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
-      x.sk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * skey, 0, 0));
-      x.sv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * skey, 0, 0));
+      if constexpr (kDense) x.v1 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row + 16, 0, 0);
     } else {
-      int page = lane_page;
-      uint32_t lp, at;
-      a.geom.page.divmod(static_cast<uint32_t>(tile * BKV + skey), lp, at);
-      if constexpr (!SMALL) page = skey < n && static_cast<int>(lp) < a.geom.ld_table ? table[lp] : -1;
-      const bool there = page >= 0 && page < a.geom.pool_pages;
-      page = there ? page : 0;
-      const int64_t off = static_cast<int64_t>((page * pt + static_cast<int>(at)) * a.n_kv_heads + head) * D + 16 * schunk;
-      const int sc = (page * a.n_kv_heads + head) * pt + static_cast<int>(at);
+      if constexpr (!SMALL) find_pages(tile);
+      const uint32_t jk = static_cast<uint32_t>(tile * BKV + skey), jl = static_cast<uint32_t>(tile * BKV + lane);
       const u32x4 zero = {0, 0, 0, 0};
-      x.k0 = zero;
-      x.v0 = zero;
-      x.sk = x.sv = 0.f;
-      if (there) {
+      x.k0 = x.v0 = zero;
+      x.sk = x.sv = x.sv_lane = 0.f;
+      if (page_lane >= 0 && page_lane < a.geom.pool_pages)
+        x.sv_lane = a.v_scales[(page_lane * a.n_kv_heads + head) * pt + static_cast<int>(jl - a.geom.page.div(jl) * a.geom.page.d)];
+      if (page_key >= 0 && page_key < a.geom.pool_pages) {
+        const int at = static_cast<int>(jk - a.geom.page.div(jk) * a.geom.page.d);
+        const int64_t off = static_cast<int64_t>((page_key * pt + at) * a.n_kv_heads + head) * D + 16 * schunk;
+        const int sc = (page_key * a.n_kv_heads + head) * pt + at;
         x.k0 = *reinterpret_cast<const u32x4*>(a.k_codes + off);
         x.v0 = *reinterpret_cast<const u32x4*>(a.v_codes + off);
         x.sk = a.k_scales[sc];
@@ -239,6 +234,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 
   int ev = 0;            // E: staged V = V 2^-E
   float sv_lim = 0.f;    // the largest scale of V that E allows: 448 2^7 < 65504
+  // The largest scale of V of a tile (those that are none do not take part), the same in every wave.
+  auto tile_top = [&](float sv_lane) __attribute__((always_inline)) {
+    float v = finite(sv_lane) ? sv_lane : 0.f;
+    for (int off = 32; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
+    return v;
+  };
   auto set_exponent = [&](float top) __attribute__((always_inline)) {  // puts the scale `top` below 2^3
     ev = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top) - 3);
     sv_lim = __builtin_ldexpf(1.f, ev + 7);
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 
   struct Ready {
     uint4 k0, k1, v0, v1;
-    float u, sv;
+    float u;
   };
   // The staged tile as it goes to LDS.  PARTIAL: some row may not see all of it.
   auto convert = [&](Staged x, Ready& y, auto PARTIAL) __attribute__((always_inline)) {
@@ -264,9 +265,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
         for (int e = 0; e < 4; ++e) x.v0[e] = without_nan_codes(x.v0[e]);
         poison = poison || (any >> (lane & 56) & 0xffu);
       }
-      y.sv = poison ? 0.f : x.sv;
       y.u = poison ? bits_f32(0x7fc00000u) : x.sk * a.c;
-      const float f = __builtin_ldexpf(y.sv, -ev);
+      const float f = __builtin_ldexpf(poison ? 0.f : x.sv, -ev);
       const v2h ff = {static_cast<_Float16>(f), static_cast<_Float16>(f)};
       if constexpr (kCodes) {
         y.k0 = make_uint4(x.k0[0], x.k0[1], x.k0[2], x.k0[3]);
@@ -295,7 +295,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     if constexpr (!kDense) {
       float* u = reinterpret_cast<float*>(st + L::u_off);
       u[skey] = y.u;  // (the lanes of one key write the same word)
-      reinterpret_cast<uint32_t*>(u)[BKV + wave] = __ballot(y.sv > sv_lim) ? 1u : 0u;
     }
   };
 
@@ -369,42 +368,17 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   constexpr float kMostSum = kDense ? 256.f : 32768.f;
   float neg_m = kShift;
 
-  float pend = 1.f, o_scale = 1.f;
-  float* top_lds = reinterpret_cast<float*>(lds + 3 * L::stage);
-  // The largest scale of V of a staged tile, over the whole workgroup.
-  auto tile_top = [&](const Staged& x) __attribute__((always_inline)) {
-    reinterpret_cast<uint32_t*>(top_lds)[wave] = keys_max(finite(x.sv) ? x.sv : 0.f);
-    __syncthreads();
-    const uint4 p = *reinterpret_cast<const uint4*>(top_lds), q = *reinterpret_cast<const uint4*>(top_lds + 4);
-    return bits_f32(max(max(max(p.x, p.y), max(p.z, p.w)), max(max(q.x, q.y), max(q.z, q.w))));
-  };
-  // E is too small for the tile of stage `buf`: raise it, note that O is to be rescaled (with the next change of a
-  // maximum: one place that rescales keeps O in its registers), stage the tile's V again.
-  auto raise = [&](int tile, int stage) __attribute__((always_inline)) {
-    Staged x;
-    Ready y;
-    const int page_ahead = lane_page;
-    if constexpr (SMALL) find_page(tile);
-    load_tile(tile, cursor_at(tile), x, std::false_type{});
-    lane_page = page_ahead;
-    const int e_old = ev;
-    set_exponent(tile_top(x));
-    ev = max(ev, e_old);
-    pend *= __builtin_ldexpf(1.f, max(e_old - ev, -200));
-    convert(x, y, std::true_type{});
-    uint4* dv = reinterpret_cast<uint4*>(lds + stage + L::v_off + skey * L::v_pitch + schunk * 32);
-    dv[0] = y.v0;
-    dv[1] = y.v1;
-    __syncthreads();
-  };
-  auto too_small = [&](int stage) __attribute__((always_inline)) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(lds + stage + L::u_off) + BKV;
-    const uint4 x = *reinterpret_cast<const uint4*>(p), y = *reinterpret_cast<const uint4*>(p + 4);
-    return (x.x | x.y | x.z | x.w) | (y.x | y.y | y.z | y.w);
-  };
-  auto check_exponent = [&](int tile, int stage) __attribute__((always_inline)) {
+  // Raising E before tile t + 1 is staged (its scales came with the loads of the last iteration) leaves V of tile t under
+  // the old one: O is rescaled after its product with t, in the next two products(), at the next change of a maximum
+  // (one place that rescales keeps O in its registers).
+  float o_scale = 1.f, pend = 1.f, pend_next = 1.f;
+  auto check_exponent = [&]() __attribute__((always_inline)) {
     if constexpr (!kDense) {
-      if (__builtin_amdgcn_readfirstlane(static_cast<int>(too_small(stage)))) raise(tile, stage);
+      if (__ballot(sreg.sv_lane > sv_lim && finite(sreg.sv_lane))) {
+        const int e_old = ev;
+        set_exponent(tile_top(sreg.sv_lane));
+        pend_next *= __builtin_ldexpf(1.f, max(e_old - ev, -200));
+      }
     }
   };
 
@@ -423,10 +397,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       vf[k & 1][db] = __builtin_bit_cast(uint4, __builtin_shufflevector(read_tr16(p), read_tr16(p + 8 * L::v_pitch), 0, 1, 2, 3, 4, 5, 6, 7));
     }
   };
-  // O^T += V^T P^T of the tile in `stage`; steps 0 and 1 of its V are being read.
-  auto pv = [&](int stage) __attribute__((always_inline)) {
+  // O^T += V^T P^T of the tile in `stage`, two of its four 16-key steps; steps 0 and 1 of its V are being read.
+  auto pv = [&](int stage, int k0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = k0; k < k0 + 2; ++k) {
       const uint4 w = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
@@ -456,7 +430,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     const uint8_t* st = lds + st_cur;
     Ready nxt;
     o_scale *= pend;
-    pend = 1.f;
+    pend = pend_next;
+    pend_next = 1.f;
     __builtin_amdgcn_s_setprio(1);
     auto scores = [&](const auto& kf) __attribute__((always_inline)) {
 #pragma unroll
@@ -478,6 +453,18 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
             s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, kf[b][ks]), qb[ks], s[b], 0, 0, 0);
       }
     };
+    pv(st_prev, 0);
+    convert(sreg, nxt, PARTIAL);
+    if constexpr (!kPartial) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction, two LDS reads, some vector work
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // (K's fragments take the registers that V's first steps leave)
     std::conditional_t<kCodes, v8i, uint4> kf[2][kCodes ? 2 : 8];
 #pragma unroll
     for (int i = 0; i < (kCodes ? 2 : 8); ++i)
@@ -491,21 +478,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
           kf[b][i] = *reinterpret_cast<const uint4*>(st + k_lane + b * 32 * L::k_pitch + i * 32);
         }
       }
-    pv(st_prev);
-    convert(sreg, nxt, PARTIAL);
-    if constexpr (!kPartial) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction, an LDS read or two, some vector work
-        __builtin_amdgcn_sched_group_barrier(0x100, kCodes ? 2 : 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-      }
-    }
+    pv(st_prev, 2);
     __builtin_amdgcn_sched_barrier(0);
     if (!kPartial || tile * BKV < wave_max) scores(kf);
     write(st_next, nxt);
     load_tile(tile + 2, ahead, sreg, One{});
-    if constexpr (SMALL) find_page(tile + 3);
+    if constexpr (SMALL) find_pages(tile + 3);
     read_u(st_cur, 0);
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
@@ -609,9 +587,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   if (tile_lo < tile_hi) {
     const bool late = wave >= kWaves / 2;
     Cursor c = cursor_at(tile_lo);
-    if constexpr (SMALL) find_page(tile_lo);
+    if constexpr (SMALL) find_pages(tile_lo);
     load_tile(tile_lo, c, sreg, std::false_type{});
-    if constexpr (!kDense) set_exponent(tile_top(sreg));
+    if constexpr (!kDense) set_exponent(tile_top(sreg.sv_lane));
     Ready y;
     convert(sreg, y, std::true_type{});
     write(st_cur, y);
@@ -622,10 +600,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) vf[i >> 2][i & 3] = make_uint4(0, 0, 0, 0);
     c = cursor_next(c, tile_lo + 1);
-    if constexpr (SMALL) find_page(tile_lo + 1);
+    if constexpr (SMALL) find_pages(tile_lo + 1);
     load_tile(tile_lo + 1, c, sreg, std::false_type{});
     ahead = cursor_next(c, tile_lo + 2);
-    if constexpr (SMALL) find_page(tile_lo + 2);
+    if constexpr (SMALL) find_pages(tile_lo + 2);
     __syncthreads();
     // whole: tiles that every row sees, and the next one too
     const int whole = min(max(lim_min / BKV - 1, tile_lo), tile_hi);
@@ -640,7 +618,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     int tile = tile_lo;
     if (!late) {
       auto step = [&](auto PARTIAL) __attribute__((always_inline)) {
-        check_exponent(tile, st_cur);
+        check_exponent();
         const Cursor after = cursor_next(ahead, tile + 3);  // (branches come first: behind them the tile is one block)
         products(tile, PARTIAL);
         weigh(tile, st_cur, PARTIAL);
@@ -653,14 +631,15 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
         if (tile < tile_hi) step(std::true_type{});
       }
     } else {
+      check_exponent();
       products(tile, std::true_type{});
       rotate(cursor_next(ahead, tile + 3));
       __syncthreads();
       ++tile;
       auto step = [&](auto PARTIAL) __attribute__((always_inline)) {
-        check_exponent(tile, st_cur);
         const Cursor after = cursor_next(ahead, tile + 3);
         weigh(tile - 1, st_prev, PARTIAL);
+        check_exponent();
         products(tile, PARTIAL);
         rotate(after);
         __syncthreads();
@@ -672,7 +651,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       }
       weigh(tile - 1, st_prev, std::true_type{});
     }
-    pv(st_prev);
+    pv(st_prev, 0);
+    pv(st_prev, 2);
     __syncthreads();
   }
 
