@@ -18,7 +18,8 @@ namespace wf {
 namespace attn_batch {
 namespace {
 
-constexpr int kJoinRows = 16;  // rows of a workgroup, 16 lanes of 8 values each
+constexpr int kJoinRows = 16;    // rows of a workgroup, 16 lanes of 8 values each
+constexpr int kJoinSplits = 64;  // splits at most
 
 // out = sum_s l_s 2^(m_s - m) o_s / sum_s l_s 2^(m_s - m) over the splits s of a row tile that used more than one.
 template <bool DENSE>
@@ -29,23 +30,46 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   const int head = item % a.n_kv_heads, w = item / a.n_kv_heads;
   Tile t;
   if (!find_tile<DENSE>(a, w, t)) return;
-  const int splits = used_splits(a, tile_max(a, t));
+  const int splits = tile_splits(a, tile_max(a, t)).n;
   if (splits < 2) return;
   const int r = part * kJoinRows + (static_cast<int>(threadIdx.x) >> 4), d = 8 * (static_cast<int>(threadIdx.x) & 15);
   if (t.first + r >= t.count) return;
   const int64_t at = static_cast<int64_t>(item) * a.n_splits * R + r;
+  // the splits' maxima and sums: each of the row's 16 lanes reads every 16th, 4 in flight
+  const int l16 = static_cast<int>(threadIdx.x) & 15;
+  float2 ml[kJoinSplits / 16];
   float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, a.part_ml[(at + static_cast<int64_t>(s) * R) * 2]);
-  float sum = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int s = 0; s < splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (at + static_cast<int64_t>(s) * R) * 2);
-    const float g = ml.x == -INFINITY ? 0.f : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
-    const float4* p = reinterpret_cast<const float4*>(a.part_o + (at + static_cast<int64_t>(s) * R) * D + d);
-    const float4 x = p[0], y = p[1];
-    sum += g;
-    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = fmaf(g, v[i], o[i]);
+  for (int i = 0; i < kJoinSplits / 16; ++i) {
+    ml[i] = make_float2(-INFINITY, 0.f);
+    const int s = 16 * i + l16;
+    if (s < splits) ml[i] = *reinterpret_cast<const float2*>(a.part_ml + (at + static_cast<int64_t>(s) * R) * 2);
+  }
+#pragma unroll
+  for (int i = 0; i < kJoinSplits / 16; ++i) top = fmaxf(top, ml[i].x);
+#pragma unroll
+  for (int off = 8; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  float g[kJoinSplits / 16], sum = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < kJoinSplits / 16; ++i) {
+    g[i] = ml[i].x == -INFINITY ? 0.f : ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - top);
+    sum += g[i];
+  }
+#pragma unroll
+  for (int off = 8; off; off >>= 1) sum += __shfl_xor(sum, off);
+  const float* po = a.part_o + at * D + d;
+#pragma unroll
+  for (int i = 0; i < kJoinSplits / 16; ++i) {
+    if (16 * i >= splits) break;
+#pragma unroll 8
+    for (int j = 0; j < min(16, splits - 16 * i); ++j) {
+      const float4* p = reinterpret_cast<const float4*>(po + static_cast<int64_t>(16 * i + j) * R * D);
+      const float4 x = p[0], y = p[1];
+      const float w = __shfl(g[i], (static_cast<int>(threadIdx.x) & 48) + j);
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = fmaf(w, v[e], o[e]);
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   uint32_t qi, gi;
@@ -65,7 +89,7 @@ Plan make_plan(int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_se
   const int64_t group = n_heads / n_kv_heads, cus = gemm::device_cus();
   const int64_t most = max_new * group;
   Plan p;
-  p.tile_shift = most <= 16 ? 4 : most <= 32 ? 5 : most <= 64 ? 6 : 8;
+  p.tile_shift = most <= 16 ? 4 : most <= 64 ? 5 : 8;
   p.n_tiles = ((n_rows * group) >> p.tile_shift) + n_seqs;
   const int64_t full = std::max<int64_t>(1, std::min<int64_t>(p.n_tiles, n_seqs * ((most + (1ll << p.tile_shift) - 1) >> p.tile_shift)));
   const int64_t units = full * n_kv_heads;
@@ -76,7 +100,7 @@ Plan make_plan(int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_se
     // the CUs with half a piece at the end); partial results of 256 rows are written and read at about 0.03.
     const double tiles = static_cast<double>((max_kv + 63) / 64);
     double best = 0;
-    for (int64_t s = 1; s <= 64 && (s == 1 || tiles / s >= 8); ++s) {
+    for (int64_t s = 1; s <= kJoinSplits && (s == 1 || tiles / s >= 8); ++s) {
       const double pieces = static_cast<double>(units * s), per = tiles / s;
       const double rounds = pieces / cus;
       double cost = n_seqs == 1 ? std::ceil(rounds) * (per + 4) : std::max(rounds, 1.0) * (0.7 * per + 4) + 0.5 * per;
@@ -87,9 +111,13 @@ Plan make_plan(int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_se
       }
     }
   } else {
-    const int64_t want = 4 * cus;
-    const int64_t keys = std::max<int64_t>(((max_kv * units + want - 1) / want + 127) / 128 * 128, 256);
-    p.n_splits = std::max<int64_t>(1, (max_kv + keys - 1) / keys);
+    // A piece costs a workgroup about 5 us besides its keys and the join reads its results: two pieces to a CU if the
+    // tiles alone are fewer, of 256 keys at least (12 tiles of 8192 keys: 20 us as 32 pieces each, 121 as one; 128 tiles
+    // of 8192 keys: 64 as 4, 147 as one, 68 as 16).  Where the tiles fill the chip, pieces of some 2048 keys, so that a
+    // few long sequences do not outlast the rest (512 tiles of 1 to 8192 keys: 138 us, 159 as one; where all are as
+    // long, 220 and 214).
+    p.n_splits = std::max((max_kv + 2047) / 2048, std::min(2 * cus / units, (max_kv + 255) / 256));
+    p.n_splits = std::min<int64_t>(std::max<int64_t>(1, p.n_splits), kJoinSplits);
   }
   p.split_keys = std::max<int64_t>(128, ((max_kv + p.n_splits - 1) / p.n_splits + 127) / 128 * 128);
   p.bytes = p.n_splits == 1 ? 0 : ((p.n_tiles * n_kv_heads * p.n_splits) << p.tile_shift) * (D + 2) * 4;

@@ -24,6 +24,8 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
@@ -42,28 +44,16 @@ struct Args {
   int32_t block;
   float c;  // softmax scale * log2(e)
   int32_t tile_shift, n_tiles;
-  int32_t split_keys, n_splits;  // keys of a split (a multiple of 64), splits at most
+  int32_t split_keys, n_splits;  // keys of a split and splits, at most
   float* part_o;                 // [n_tiles][n_kv_heads][n_splits][R][D], each divided by its own sum
   float* part_ml;                // [n_tiles][n_kv_heads][n_splits][R][2]: maximum (log2 units) and sum
   BatchGeom geom;
 };
 
+constexpr int kSplitUnit = 128;  // a split's keys are a multiple of this
+
 // A value that all lanes hold, in a scalar register.
 __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// Sequence of row tile w (uniform); n_seqs > 0.
-__device__ inline int tile_seq(const Args& a, int w) {
-  const int lane = static_cast<int>(threadIdx.x) & 63;
-  int n = 0;
-  for (int base = 0; base < a.geom.n_seqs; base += 64) {
-    const int i = base + lane;
-    const int at = i < a.geom.n_seqs ? ((a.geom.cu[i] * a.group) >> a.tile_shift) + i : 0x7fffffff;
-    const int here = __popcll(__ballot(at <= w));
-    n += here;
-    if (here < 64) break;
-  }
-  return n - 1;
-}
 
 // A workgroup's rows and keys (all uniform).
 struct Tile {
@@ -76,25 +66,52 @@ struct Tile {
   int key0;       // dense: the sequence's first key row
 };
 
+// Sum of the lanes up to this one.
+__device__ inline int prefix_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1 .. 8 within 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to the 16 after, 47 likewise
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the 32 after
+  return x;
+}
+
+// Row tile w of all sequences' tiles, numbered without gaps (so that a grid's surplus workgroups, which hold a place on
+// a CU until they have seen that they have no work, come last).  Every lane reads one sequence's starts and length.
 template <bool DENSE>
 __device__ inline bool find_tile(const Args& a, int w, Tile& t) {
-  t.b = uniform(tile_seq(a, w));
-  if (t.b < 0) return false;
-  t.row0 = uniform(a.geom.cu[t.b]);
-  const int end = min(uniform(a.geom.cu[t.b + 1]), a.n_rows);
-  t.n_new = end - t.row0;
-  if (t.row0 < 0 || t.n_new <= 0) return false;
-  t.first = (w - ((t.row0 * a.group) >> a.tile_shift) - t.b) << a.tile_shift;
-  t.count = t.n_new * a.group;
-  if (t.first < 0 || t.first >= t.count) return false;
-  if constexpr (DENSE) {
-    t.key0 = min(max(uniform(a.cu_kv[t.b]), 0), a.n_kv_rows);
-    t.kv_len = min(max(uniform(a.cu_kv[t.b + 1]), t.key0), a.n_kv_rows) - t.key0;
-  } else {
-    t.key0 = 0;
-    t.kv_len = min(max(uniform(a.geom.kv_lens[t.b]), 0), kMaxKeys);
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  int before = 0;  // tiles of the sequences before this turn's
+  for (int base = 0; base < a.geom.n_seqs; base += 64) {
+    const int i = min(base + lane, a.geom.n_seqs - 1);
+    const int r = a.geom.cu[i];
+    const int n = min(a.geom.cu[i + 1], a.n_rows) - r;
+    const int u = DENSE ? a.cu_kv[i] : a.geom.kv_lens[i], v = DENSE ? a.cu_kv[i + 1] : 0;
+    const bool some = base + lane < a.geom.n_seqs && r >= 0 && n > 0;
+    const int tiles = some ? (n * a.group + (1 << a.tile_shift) - 1) >> a.tile_shift : 0;
+    const int sum = before + prefix_sum(tiles);
+    const uint64_t past = __ballot(some && sum > w);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      t.b = base + at;
+      t.row0 = __builtin_amdgcn_readlane(r, at);
+      t.n_new = __builtin_amdgcn_readlane(n, at);
+      t.first = (w - __builtin_amdgcn_readlane(sum - tiles, at)) << a.tile_shift;
+      t.count = t.n_new * a.group;
+      const int x = __builtin_amdgcn_readlane(u, at), y = __builtin_amdgcn_readlane(v, at);
+      if constexpr (DENSE) {
+        t.key0 = min(max(x, 0), a.n_kv_rows);
+        t.kv_len = min(max(y, t.key0), a.n_kv_rows) - t.key0;
+      } else {
+        t.key0 = 0;
+        t.kv_len = min(max(x, 0), kMaxKeys);
+      }
+      return t.first >= 0 && t.first < t.count;
+    }
+    before = __builtin_amdgcn_readlane(sum, 63);
   }
-  return true;
+  return false;
 }
 
 // Keys that row i of the tile's sequence sees (0 .. lim).
@@ -113,9 +130,15 @@ __device__ inline int tile_max(const Args& a, const Tile& t) {
   return row_limit(a, t, a.group_div.div(last));
 }
 
-// Splits that hold keys of a tile whose rows see up to lim keys; the last one takes what is left.
-__device__ inline int used_splits(const Args& a, int lim) {
-  return lim <= 0 ? 1 : min(a.n_splits, (lim - 1) / a.split_keys + 1);
+// Splits of a tile whose rows see up to lim keys: as many as split_keys asks for, of equal length.
+struct Splits {
+  int n, keys;
+};
+__device__ inline Splits tile_splits(const Args& a, int lim) {
+  if (lim <= a.split_keys || a.n_splits == 1) return Splits{1, max(lim, 0)};
+  const int n = min(a.n_splits, (lim - 1) / a.split_keys + 1);
+  const int keys = ((lim - 1) / n + kSplitUnit) / kSplitUnit * kSplitUnit;
+  return Splits{(lim - 1) / keys + 1, keys};
 }
 
 // Two fp32 -> packed bf16x2, round to nearest even.
@@ -154,6 +177,28 @@ __device__ inline float sum16(float v) {
   float a = v, b = v;
   swap16(a, b);
   return a + b;
+}
+
+// Q as two e4m3 parts under a power of two: q = 2^e (q1 + q2 / 16) with |q| < 2^8 2^e; q1 holds the 4 leading bits of a
+// value, q2 the next 4, exact for a bf16 whose last bit is not below 2^-13 of 2^e.  Exponent of a row from its max|q|:
+__device__ inline int q_exponent(float amax) {
+  return amax > 0.f ? min(max(__builtin_amdgcn_frexp_expf(amax) - 8, -122), 126) : 0;
+}
+// 8 values of a row.
+__device__ inline void split_q(const uint4& x, int e, uint2& q1, uint2& q2) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t c1[2], c2[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float v[4] = {__builtin_ldexpf(bf16_lo_to_f32(w[2 * i]), -e), __builtin_ldexpf(bf16_hi_to_f32(w[2 * i]), -e),
+                        __builtin_ldexpf(bf16_lo_to_f32(w[2 * i + 1]), -e), __builtin_ldexpf(bf16_hi_to_f32(w[2 * i + 1]), -e)};
+    c1[i] = e4m3_pack4_hw(v[0], v[1], v[2], v[3]);
+    float b0, b1, b2, b3;
+    e4m3_unpack4_hw(c1[i], b0, b1, b2, b3);
+    c2[i] = e4m3_pack4_hw((v[0] - b0) * 16.f, (v[1] - b1) * 16.f, (v[2] - b2) * 16.f, (v[3] - b3) * 16.f);
+  }
+  q1 = make_uint2(c1[0], c1[1]);
+  q2 = make_uint2(c2[0], c2[1]);
 }
 
 // True when a byte of w is an e4m3 NaN code; the word with those bytes cleared.

@@ -2,34 +2,44 @@
 // ones, grouped heads).  The cache is read once and little is computed, so HBM bounds it: 264 bytes a key of an 8-bit
 // cache, 512 of a dense one.
 //
-// A workgroup of four waves owns a tile of 16, 32 or 64 rows, one key head and one range of the keys; every wave takes
-// each fourth tile of 32 keys of the range by itself (no barrier in the loop) with the loads of its next tile in
-// flight, and the four results are joined in LDS at the end, those of several ranges by the join kernel.
+// A workgroup owns a tile of 16, 32 or 64 rows, one key head and one range of the keys; every wave takes each W-th tile
+// of 32 keys of the range by itself (no barrier in the loop).  Its loads are one tile ahead: a tile's K leaves its
+// registers with the scores and its V goes to LDS before them, and then the next tile is asked for, so that few
+// registers hold what is in flight and four waves share a SIMD (16 rows).  The waves' results are joined in LDS, those of
+// several ranges by the join kernel.  Calls of few workgroups take more waves to each (W = 8), which saves them the
+// join of ranges.
 //
-// Per 32 keys: K comes straight from memory as the first operand of v_mfma_f32_16x16x32_bf16 (lane (l, g) holds key l,
-// codes 64 i + 16 g .. + 15 of its row; Q, the second operand, is held in the same order), so S^T = K Q^T leaves a lane
-// with one row and the keys 16 b + 4 g + 0..3.  V goes through a wave's own LDS rows, whose transposing reads give the
-// V^T operand of O^T += V^T P^T for the same keys.  The codes of both formats are exact in bf16 (4 and 8 significant
-// bits) and so are the products: the scales are applied in fp32, s_k c to the scores and s_v to the weights, and the
-// weights go in as the sum of two bf16 (16 significant bits; the matrix cores are idle most of the time anyway).
+// Per 32 keys: K comes straight from memory as the first operand of the scores' product S^T = K Q^T, which leaves a lane
+// (l, g) with row l and the keys 16 b + 4 g + 0..3.  e4m3 codes go to v_mfma_scale_f32_16x16x128_f8f6f4 as they are,
+// against Q in two e4m3 parts; int8 codes are exact in bf16 and go to v_mfma_f32_16x16x32_bf16 as dense keys do.  V goes
+// through a wave's own LDS rows, whose transposing reads give the V^T operand of O^T += V^T P^T for the same keys, the
+// codes of both formats exact in bf16.  The scales are applied in fp32, s_k c to the scores and s_v to the weights, and
+// the weights go in as the sum of two bf16 (16 significant bits; the matrix cores are idle most of the time anyway).
 #include "attn_batch.hpp"
 
 namespace wf {
 namespace attn_batch {
 namespace {
 
-constexpr int KT = 32;       // keys of a wave's tile
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kOPitch = D + 4;  // floats of a joined row in LDS
+constexpr int KT = 32;  // keys of a wave's tile
+constexpr int W = 4;    // waves of a workgroup
+constexpr int kQPitch = 2 * D + 16;
 
-template <int SRC>
+template <int SRC, int NB>
 struct Form {
   static constexpr bool dense = SRC == SRC_DENSE;
   static constexpr int row_bytes = dense ? 256 : 128;
   static constexpr int k_loads = 2 * row_bytes / 64;   // 16-byte loads a lane makes of the tile's K (and V)
   static constexpr int v_pitch = dense ? 256 + 32 : 128 + 16;
   static constexpr int wave_lds = KT * v_pitch + 64 * 4;  // V rows, then 32 factors of K and 32 of V
+  static constexpr bool q_lds = NB > 1;                   // Q is read from LDS at every tile (one row block: registers)
+  static constexpr int q_off = W * wave_lds;
+  static constexpr int stage = q_off + (q_lds ? 16 * NB * (kQPitch + 4) : 0);  // and a row's exponent
+  static constexpr int o_slot = 16 * NB * D * 4;          // a wave's results, as they are joined
+  static constexpr int join = W / 2 * o_slot + 2 * W * 16 * NB * 4;
+  static constexpr int lds = stage > join ? stage : join;
+  // waves of a SIMD the registers are allotted for
+  static constexpr int waves = NB == 1 ? 3 : 2;
 };
 
 // 8 codes (2 dwords) as 8 bf16.
@@ -53,6 +63,14 @@ __device__ inline v8bf to_bf16(uint32_t w0, uint32_t w1) {
   return __builtin_bit_cast(v8bf, make_uint4(o[0], o[1], o[2], o[3]));
 }
 
+__device__ inline float absmax8(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(bf16_lo_to_f32(w[i])), fabsf(bf16_hi_to_f32(w[i]))));
+  return m;
+}
+
 // Order the wave's own LDS accesses (the hardware keeps them in order; this keeps the compiler to it).
 __device__ inline void wave_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -61,31 +79,139 @@ __device__ inline void wave_lds_order() {
 }
 
 template <int SRC, int NB>
-__global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
-  using F = Form<SRC>;
+__global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kernel(Args a) {
+  using F = Form<SRC, NB>;
   constexpr bool kDense = F::dense;
   constexpr int R = 16 * NB;
-  constexpr int kStage = kWaves * F::wave_lds;
-  constexpr int kJoin = R * kOPitch * 4 + 2 * kWaves * R * 4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kStage > kJoin ? kStage : kJoin];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[F::lds];
 
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int l16 = lane & 15, g4 = lane >> 4;
-  const int split = static_cast<int>(blockIdx.x) % a.n_splits;
-  const int item = static_cast<int>(blockIdx.x) / a.n_splits;
-  const int head = item % a.n_kv_heads, w = item / a.n_kv_heads;
+  // The splits are the slowest index, so that those which short sequences do not have come last and on every XCD; the
+  // heads are turned from tile to tile and split to split, so that an XCD (every eighth workgroup) reads all of them:
+  // one that read the same 128 of every 1024 bytes would keep only some of its L2 channels busy (64 sequences of up to
+  // 8192 keys over 8 heads: 136 us, 158 with the heads as they come, 182 with the splits fastest).
+  const int items = a.n_tiles * a.n_kv_heads;
+  const int split = static_cast<int>(blockIdx.x) / items, slot = static_cast<int>(blockIdx.x) % items;
+  const int w = slot / a.n_kv_heads, head = (slot + w + (w >> 3) + split) % a.n_kv_heads;
   Tile t;
   if (!find_tile<kDense>(a, w, t)) return;
   const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
-  const int splits = used_splits(a, lim_max);
+  const Splits cut = tile_splits(a, lim_max);
+  const int splits = cut.n;
   if (split >= splits) return;
-  const int k_lo = split * a.split_keys;
-  const int k_hi = split == splits - 1 ? lim_max : k_lo + a.split_keys;
+  const int k_lo = split * cut.keys;
+  const int k_hi = min(lim_max, k_lo + cut.keys);
 
-  // rows: the lane's row of each 16, its query and its limit
-  v8bf qf[NB][4];
+  // One tile in registers: K rows, V rows, the scales of key lane & 31, and which of its keys have no place to be read
+  // from (where every lane finds its own).
+  struct Regs {
+    u32x4 k[F::k_loads], v[F::k_loads];
+    float fk, fv;
+    uint32_t bad;
+  };
+  // Where a tile's keys live: in one page (uniform; `n` of them to be read, the others read as zero), or each on its own.
+  struct Where {
+    bool one;
+    int n;
+    const uint8_t* k;
+    const float* sk;
+  };
+  // Lane & 31's (position, head) row in the pool and its scale; keys past the range or without a page are not there.
+  struct Place {
+    int row, scale;
+    bool there;
+  };
+  const int pt = a.geom.page_tokens;
+  const int64_t key_bytes = kDense ? a.ldkv * 2 : static_cast<int64_t>(a.n_kv_heads) * D;
+  const int64_t k_to_v = kDense ? reinterpret_cast<const uint8_t*>(a.v_dense) - reinterpret_cast<const uint8_t*>(a.k_dense)
+                                : a.v_codes - a.k_codes;
+  const int64_t sk_to_sv = reinterpret_cast<const uint8_t*>(a.v_scales) - reinterpret_cast<const uint8_t*>(a.k_scales);
+  auto where = [&](int t0) __attribute__((always_inline)) -> Where {
+    const int n = uniform(min(max(k_hi - t0, 0), KT));
+    if constexpr (kDense)
+      return Where{true, n, reinterpret_cast<const uint8_t*>(a.k_dense + head * D) + (static_cast<int64_t>(t.key0) + (n ? t0 : 0)) * key_bytes,
+                   nullptr};
+    uint32_t lp, at;
+    a.geom.page.divmod(static_cast<uint32_t>(t0), lp, at);
+    int page = -1;
+    if (n && static_cast<int>(lp) < a.geom.ld_table) page = a.geom.tables[static_cast<int64_t>(t.b) * a.geom.ld_table + lp];
+    page = uniform(page);
+    const bool ok = page >= 0 && page < a.geom.pool_pages;
+    const int pg = ok ? page : 0, r0 = static_cast<int>(at);
+    return Where{r0 + n <= pt, ok ? n : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * D,
+                 a.k_scales + ((pg * a.n_kv_heads + head) * pt + r0)};
+  };
+  auto place = [&](int t0) __attribute__((always_inline)) -> Place {
+    const int j = t0 + (lane & 31);
+    Place p{0, 0, false};
+    int page, at;
+    if (j < k_hi && pool_row(a.geom, t.b, j, page, at))
+      p = Place{(page * pt + at) * a.n_kv_heads + head, (page * a.n_kv_heads + head) * pt + at, true};
+    return p;
+  };
+  // A lane's K bytes of key l16 of each 16: 16 g + 64 i .. + 15; its V bytes: 16 of row lane / C, C lanes to a row
+  constexpr int C = F::row_bytes / 16;
+  const uint32_t k_off = static_cast<uint32_t>(l16) * static_cast<uint32_t>(key_bytes) + 16 * g4;
+  const uint32_t v_off = static_cast<uint32_t>(lane / C) * static_cast<uint32_t>(key_bytes) + 16 * (lane % C);
+  const bool small = !kDense && pt < KT;
+  Place next_place{};  // pages of fewer than 32 positions: the keys' places of the tile after, asked for a tile ahead
+  auto load = [&](int t0, const Where& c, Regs& x) __attribute__((always_inline)) {
+    constexpr int kWord3 = 0x00020000;  // raw buffer, 32-bit data format
+    if (kDense || c.one) {
+      const int bytes = c.n ? (c.n - 1) * static_cast<int>(key_bytes) + F::row_bytes : 0;
+      const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k), 0, bytes, kWord3);
+      const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k + k_to_v), 0, bytes, kWord3);
+      if constexpr (!kDense) {
+        const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(c.sk), 0, 4 * c.n, kWord3);
+        const auto sv = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(c.sk) + sk_to_sv), 0, 4 * c.n, kWord3);
+        x.fk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * (lane & 31), 0, 0));
+        x.fv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * (lane & 31), 0, 0));
+      }
+#pragma unroll
+      for (int i = 0; i < F::k_loads; ++i) {
+        constexpr int per = F::k_loads / 2;
+        x.k[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + static_cast<uint32_t>(i / per * 16 * key_bytes) + i % per * 64, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < F::k_loads; ++i)
+        x.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, v_off + static_cast<uint32_t>(i * (64 / C) * key_bytes), 0, 0);
+      x.bad = 0;
+    } else {
+      const Place p = small ? next_place : place(t0);
+      x.bad = static_cast<uint32_t>(__ballot(!p.there));
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint8_t* kp = a.k_codes + static_cast<int64_t>(__shfl(p.row, 16 * b + l16)) * D + 16 * g4;
+#pragma unroll
+        for (int i = 0; i < F::k_loads / 2; ++i) x.k[F::k_loads / 2 * b + i] = *reinterpret_cast<const u32x4*>(kp + 64 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < F::k_loads; ++i)
+        x.v[i] = *reinterpret_cast<const u32x4*>(a.v_codes + static_cast<int64_t>(__shfl(p.row, 64 / C * i + lane / C)) * D + 16 * (lane % C));
+      x.fk = a.k_scales[p.scale];
+      x.fv = a.v_scales[p.scale];
+    }
+  };
+
+  // the first tile is on its way while Q is made ready
+  int t0 = k_lo + KT * wave;
+  Regs x;
+  Where next{};
+  if (t0 < k_hi) {
+    next = where(t0);
+    if (small) next_place = place(t0);
+    load(t0, next, x);
+    next = where(t0 + W * KT);
+    if (small) next_place = place(t0 + W * KT);
+  }
+
+  // rows: the lane's row of each 16, where its result goes, and its limit
   int lim[NB];
+  int row_at[NB];    // the row of q and out
+  int row_head[NB];  // its head's first element
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int r = t.first + 16 * n + l16;
@@ -93,13 +219,67 @@ __global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
     uint32_t qi, gi;
     a.group_div.divmod(static_cast<uint32_t>(ok ? r : t.first), qi, gi);
     lim[n] = ok ? row_limit(a, t, static_cast<int>(qi)) : 0;
-    const uint16_t* p = a.q + static_cast<int64_t>(t.row0 + static_cast<int>(qi)) * a.ldq + (head * a.group + static_cast<int>(gi)) * D;
+    row_at[n] = t.row0 + static_cast<int>(qi);
+    row_head[n] = (head * a.group + static_cast<int>(gi)) * D;
+  }
+  // Q, the second operand of the scores.  e4m3 keys: q = 2^e (q1 + q2 / 16) as in attn_batch_wide.hip, a lane holding
+  // values 16 g .. + 15 and 64 + 16 g .. + 15 (what its two loads of a key hold).  The others: step s of the product takes
+  // values 64 (s / 2) + 16 g + 8 (s % 2) .. + 7 (dense: 32 s + 8 g .. + 7).
+  constexpr bool kCodes = SRC == SRC_E4M3;
+  auto q_values = [&](int s) { return kDense ? 32 * s + 8 * g4 : 64 * (s >> 1) + 16 * g4 + 8 * (s & 1); };
+  v8bf qf[4];       // one row block's operands
+  v8i qa, qb;       // q1 and q2
+  int q_scale[NB];  // E8M0 scale of q1
+  uint8_t* qbuf = lds + F::q_off;
+  if constexpr (F::q_lds) {
+    int32_t* es = reinterpret_cast<int32_t*>(qbuf + R * kQPitch);
+    for (int c = static_cast<int>(threadIdx.x); c < R * 16; c += 64 * W) {
+      const int r = c >> 4;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (t.first + r < t.count) {
+        uint32_t qi, gi;
+        a.group_div.divmod(static_cast<uint32_t>(t.first + r), qi, gi);
+        v = *reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(t.row0 + static_cast<int>(qi)) * a.ldq +
+                                            (head * a.group + static_cast<int>(gi)) * D + 8 * (c & 15));
+      }
+      if constexpr (kCodes) {
+        float amax = absmax8(v);
+#pragma unroll
+        for (int off = 1; off < 16; off *= 2) amax = fmaxf(amax, __shfl_xor(amax, off));
+        const int e = q_exponent(amax);
+        uint2 c1, c2;
+        split_q(v, e, c1, c2);
+        *reinterpret_cast<uint2*>(qbuf + r * kQPitch + 8 * (c & 15)) = c1;
+        *reinterpret_cast<uint2*>(qbuf + r * kQPitch + D + 8 * (c & 15)) = c2;
+        if ((c & 15) == 0) es[r] = 127 + e;
+      } else {
+        *reinterpret_cast<uint4*>(qbuf + r * kQPitch + 16 * (c & 15)) = v;
+      }
+    }
+    __syncthreads();
+    if constexpr (kCodes) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) q_scale[n] = es[16 * n + l16];
+    }
+  } else {
+    const bool ok = t.first + l16 < t.count;
+    const uint16_t* p = a.q + static_cast<int64_t>(row_at[0]) * a.ldq + row_head[0];
+    uint4 v[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      // step s of the product takes values 64 (s / 2) + 16 g + 8 (s % 2) .. + 7 (dense: 32 s + 8 g .. + 7) of a key's row
-      const int d = kDense ? 32 * s + 8 * g4 : 64 * (s >> 1) + 16 * g4 + 8 * (s & 1);
-      const uint4 v = *reinterpret_cast<const uint4*>(p + d);
-      qf[n][s] = __builtin_bit_cast(v8bf, ok ? v : make_uint4(0, 0, 0, 0));
+      v[s] = *reinterpret_cast<const uint4*>(p + q_values(s));
+      if (!ok) v[s] = make_uint4(0, 0, 0, 0);
+      qf[s] = __builtin_bit_cast(v8bf, v[s]);
+    }
+    if constexpr (kCodes) {
+      const float amax = max16(max32(fmaxf(fmaxf(absmax8(v[0]), absmax8(v[1])), fmaxf(absmax8(v[2]), absmax8(v[3])))));
+      const int e = q_exponent(amax);
+      q_scale[0] = 127 + e;
+      uint2 c1[4], c2[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) split_q(v[s], e, c1[s], c2[s]);
+      qa = __builtin_bit_cast(v8i, c1);
+      qb = __builtin_bit_cast(v8i, c2);
     }
   }
 
@@ -116,81 +296,23 @@ __global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
   uint8_t* vbuf = lds + wave * F::wave_lds;
   float* fbuf = reinterpret_cast<float*>(vbuf + KT * F::v_pitch);
 
-  // one tile in registers: K rows, V rows, factors (lane < 32: s_k of key lane, else s_v of key lane - 32), and which of
-  // its keys have no place to be read from
-  struct Regs {
-    u32x4 k[F::k_loads], v[F::k_loads];
-    float f;
-    uint32_t bad;
-  };
-  // Where the keys of the tile at key t0 live: lane & 31's (position, head) row in the pool (dense: its row of k) and its
-  // scale; keys past the range or without a page are not there.
-  struct Place {
-    int row, scale;
-    bool there;
-  };
-  auto locate = [&](int t0) -> Place {
-    const int j = t0 + (lane & 31);
-    Place p{kDense ? t.key0 : 0, 0, false};
-    if (j >= k_hi) return p;
-    if constexpr (kDense) {
-      p = Place{t.key0 + j, 0, true};
-    } else {
-      int page, at;
-      if (pool_row(a.geom, t.b, j, page, at))
-        p = Place{(page * a.geom.page_tokens + at) * a.n_kv_heads + head, (page * a.n_kv_heads + head) * a.geom.page_tokens + at, true};
-    }
-    return p;
-  };
-  auto load = [&](const Place& p, Regs& x) {
-    x.bad = static_cast<uint32_t>(__ballot(!p.there));
-    const int safe = p.row;
-    if constexpr (kDense) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const uint16_t* kp = a.k_dense + static_cast<int64_t>(__shfl(safe, 16 * b + l16)) * a.ldkv + head * D + 8 * g4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x.k[4 * b + i] = *reinterpret_cast<const u32x4*>(kp + 32 * i);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint16_t* vp = a.v_dense + static_cast<int64_t>(__shfl(safe, 4 * i + (lane >> 4))) * a.ldkv + head * D + 8 * l16;
-        x.v[i] = *reinterpret_cast<const u32x4*>(vp);
-      }
-    } else {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const uint8_t* kp = a.k_codes + static_cast<int64_t>(__shfl(safe, 16 * b + l16)) * D + 16 * g4;
-        x.k[2 * b] = *reinterpret_cast<const u32x4*>(kp);
-        x.k[2 * b + 1] = *reinterpret_cast<const u32x4*>(kp + 64);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* vp = a.v_codes + static_cast<int64_t>(__shfl(safe, 8 * i + (lane >> 3))) * D + 16 * (lane & 7);
-        x.v[i] = *reinterpret_cast<const u32x4*>(vp);
-      }
-      x.f = (lane < 32 ? a.k_scales : a.v_scales)[p.scale];
-    }
-  };
-
-  auto compute = [&](int t0, Regs& x) {
-    if (x.bad) {  // keys past the range or without a page: zero K and V
+  v4f s[NB][2];
+  // V and the factors to LDS, the scores.
+  auto scores = [&](bool masked, Regs& x) __attribute__((always_inline)) {
+    if (!kDense && x.bad) {  // keys past the range or without a page: zero K and V
       const u32x4 zero = {0, 0, 0, 0};
-      constexpr int per = F::k_loads / 2;
 #pragma unroll
       for (int i = 0; i < F::k_loads; ++i) {
-        if (x.bad >> (16 * (i / per) + l16) & 1u) x.k[i] = zero;
-        if (x.bad >> (kDense ? 4 * i + (lane >> 4) : 8 * i + (lane >> 3)) & 1u) x.v[i] = zero;
+        if (x.bad >> (16 * (i / (F::k_loads / 2)) + l16) & 1u) x.k[i] = zero;
+        if (x.bad >> (64 / C * i + lane / C) & 1u) x.v[i] = zero;
       }
-      if (x.bad >> (lane & 31) & 1u) x.f = 0.f;
+      if (x.bad >> (lane & 31) & 1u) x.fk = x.fv = 0.f;
     }
-    const bool masked = t0 + KT > lim_min;
     if constexpr (kDense) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) *reinterpret_cast<u32x4*>(vbuf + (4 * i + (lane >> 4)) * F::v_pitch + 16 * l16) = x.v[i];
     } else {
-      if (lane < 32) x.f *= a.c;
-      fbuf[lane] = x.f;
+      fbuf[lane] = lane < 32 ? x.fk * a.c : x.fv;
       if (SRC == SRC_E4M3 && masked) {
         // A weight of zero does not silence a NaN of V: where some row does not see some key, a NaN code becomes a NaN
         // scale, which only the weights of rows that see the key meet.
@@ -211,24 +333,58 @@ __global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
         *reinterpret_cast<u32x4*>(vbuf + (8 * i + (lane >> 3)) * F::v_pitch + 16 * (lane & 7)) = x.v[i];
     }
     wave_lds_order();
-    v4f s[NB][2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int n = 0; n < NB; ++n) s[n][b] = v4f{0, 0, 0, 0};
+    if constexpr (kCodes) {
+      v8i kf[2];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        v8bf kf;
-        if constexpr (kDense) {
-          kf = __builtin_bit_cast(v8bf, x.k[4 * b + ks]);
-        } else {
-          const u32x4 kk = x.k[2 * b + (ks >> 1)];
-          kf = to_bf16<SRC>(kk[2 * (ks & 1)], kk[2 * (ks & 1) + 1]);
+      for (int b = 0; b < 2; ++b) kf[b] = __builtin_bit_cast(v8i, *reinterpret_cast<u32x4(*)[2]>(&x.k[2 * b]));
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        if constexpr (F::q_lds) {
+          const uint8_t* p = qbuf + (16 * n + l16) * kQPitch + 16 * g4;
+          u32x4 q[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const u32x4*>(p + 64 * i);
+          qa = __builtin_bit_cast(v8i, *reinterpret_cast<u32x4(*)[2]>(&q[0]));
+          qb = __builtin_bit_cast(v8i, *reinterpret_cast<u32x4(*)[2]>(&q[2]));
         }
 #pragma unroll
-        for (int n = 0; n < NB; ++n) s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][ks], s[n][b], 0, 0, 0);
+        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qb, s[n][b], 0, 0, 0, 127, 0, q_scale[n] - 4);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qa, s[n][b], 0, 0, 0, 127, 0, q_scale[n]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      v8bf kf[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if constexpr (kDense) {
+          kf[b] = __builtin_bit_cast(v8bf, x.k[4 * b + ks]);
+        } else {
+          const u32x4 kk = x.k[2 * b + (ks >> 1)];
+          kf[b] = to_bf16<SRC>(kk[2 * (ks & 1)], kk[2 * (ks & 1) + 1]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        v8bf q;
+        if constexpr (F::q_lds)
+          q = __builtin_bit_cast(v8bf, *reinterpret_cast<const uint4*>(qbuf + (16 * n + l16) * kQPitch + 2 * q_values(ks)));
+        else
+          q = qf[ks];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b], q, s[n][b], 0, 0, 0);
       }
     }
+  };
+  v8bf ph[NB], pl[NB];
+  // The weights, as two bf16 parts.
+  auto weigh = [&](int t0, bool masked) __attribute__((always_inline)) {
     float u[8], sv[8];
     if constexpr (!kDense) {
 #pragma unroll
@@ -239,7 +395,6 @@ __global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
         sv[4 * b] = fv.x, sv[4 * b + 1] = fv.y, sv[4 * b + 2] = fv.z, sv[4 * b + 3] = fv.w;
       }
     }
-    v8bf ph[NB], pl[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       float x8[8];
@@ -285,6 +440,9 @@ __global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
       ph[n] = __builtin_bit_cast(v8bf, make_uint4(wh[0], wh[1], wh[2], wh[3]));
       pl[n] = __builtin_bit_cast(v8bf, make_uint4(wl[0], wl[1], wl[2], wl[3]));
     }
+  };
+  // O^T += V^T P^T.
+  auto pv = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v8bf vf;
@@ -301,30 +459,30 @@ __global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
         o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph[n], o[n][i], 0, 0, 0);
         o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[n], o[n][i], 0, 0, 0);
       }
+      if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (reads of two blocks at a time: registers)
     }
     wave_lds_order();
   };
 
-  int t0 = k_lo + KT * wave;
-  if (t0 < k_hi) {
-    Regs cur, nxt;
-    load(locate(t0), cur);
-    Place next = locate(t0 + kWaves * KT);
-    for (; t0 < k_hi; t0 += kWaves * KT) {
-      if (t0 + kWaves * KT < k_hi) {
-        load(next, nxt);
-        next = locate(t0 + 2 * kWaves * KT);
-      }
-      compute(t0, cur);
-      cur = nxt;
+  for (; t0 < k_hi; t0 += W * KT) {
+    const bool masked = t0 + KT > lim_min;
+    scores(masked, x);
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 + W * KT < k_hi) {
+      load(t0 + W * KT, next, x);
+      next = where(t0 + 2 * W * KT);
+      if (small) next_place = place(t0 + 2 * W * KT);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    weigh(t0, masked);
+    pv();
   }
 
-  // join the four waves: their maxima and sums, then the outputs one wave after the other
+  // Join the waves: maxima and sums, then the outputs pairwise (wave i takes in wave i + half), in LDS that no wave
+  // reads any more.
   __syncthreads();
-  float* ob = reinterpret_cast<float*>(lds);
-  float* ms = ob + R * kOPitch;
-  float* ls = ms + kWaves * R;
+  float* ms = reinterpret_cast<float*>(lds + W / 2 * F::o_slot);
+  float* ls = ms + W * R;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     l[n] = sum16(sum32(l[n]));
@@ -334,49 +492,58 @@ __global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
     }
   }
   __syncthreads();
-  float scale[NB];
+  float top[NB], sum[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    float top = -INFINITY;
+    top[n] = -INFINITY;
+    sum[n] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ms[i * R + 16 * n + l16]);
-    scale[n] = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
+    for (int i = 0; i < W; ++i) top[n] = fmaxf(top[n], ms[i * R + 16 * n + l16]);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float mi = ms[i * R + 16 * n + l16];
+      sum[n] += mi == -INFINITY ? 0.f : ls[i * R + 16 * n + l16] * __builtin_amdgcn_exp2f(mi - top[n]);
+    }
+    const float scale = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top[n]);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[n][d] *= scale;
   }
-  for (int i = 0; i < kWaves; ++i) {
-    if (i == wave) {
+#pragma unroll
+  for (int half = W / 2; half >= 1; half /= 2) {
+    // lane's values 4 floats each, lane-linear: conflict-free
+    if (wave >= half && wave < 2 * half) {
+      v4f* p = reinterpret_cast<v4f*>(lds + (wave - half) * F::o_slot) + lane;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          v4f* p = reinterpret_cast<v4f*>(ob + (16 * n + l16) * kOPitch + 16 * d + 4 * g4);
-          const v4f v = o[n][d] * scale[n];
-          *p = i == 0 ? v : *p + v;
-        }
+        for (int d = 0; d < 8; ++d) p[(8 * n + d) * 64] = o[n][d];
     }
     __syncthreads();
+    if (wave < half) {
+      const v4f* p = reinterpret_cast<const v4f*>(lds + wave * F::o_slot) + lane;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[n][d] += p[(8 * n + d) * 64];
+    }
+    if (half > 1) __syncthreads();
   }
-  for (int c = static_cast<int>(threadIdx.x); c < R * 16; c += kThreads) {
-    const int r = c >> 4, d = 8 * (c & 15);
-    if (t.first + r >= t.count) continue;
-    float top = -INFINITY, sum = 0.f;
+  if (wave != 0) return;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ms[i * R + r]);
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) sum += ms[i * R + r] == -INFINITY ? 0.f : ls[i * R + r] * __builtin_amdgcn_exp2f(ms[i * R + r] - top);
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    const float* v = ob + r * kOPitch + d;
+  for (int n = 0; n < NB; ++n) {
+    if (t.first + 16 * n + l16 >= t.count) continue;
+    const float inv = sum[n] == 0.f ? 0.f : 1.0f / sum[n];
     if (splits > 1) {
-      const int64_t at = (static_cast<int64_t>(item) * a.n_splits + split) * R + r;
-      float4* po = reinterpret_cast<float4*>(a.part_o + at * D + d);
-      po[0] = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-      po[1] = make_float4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, sum);
+      const int64_t at = ((static_cast<int64_t>(w) * a.n_kv_heads + head) * a.n_splits + split) * R + 16 * n + l16;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) *reinterpret_cast<v4f*>(a.part_o + at * D + 16 * d + 4 * g4) = o[n][d] * inv;
+      if (g4 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top[n], sum[n]);
     } else {
-      uint32_t qi, gi;
-      a.group_div.divmod(static_cast<uint32_t>(t.first + r), qi, gi);
-      uint16_t* p = a.out + static_cast<int64_t>(t.row0 + static_cast<int>(qi)) * a.ldo + (head * a.group + static_cast<int>(gi)) * D + d;
-      *reinterpret_cast<uint2*>(p) = make_uint2(cvt_bf16x2(v[0] * inv, v[1] * inv), cvt_bf16x2(v[2] * inv, v[3] * inv));
-      *reinterpret_cast<uint2*>(p + 4) = make_uint2(cvt_bf16x2(v[4] * inv, v[5] * inv), cvt_bf16x2(v[6] * inv, v[7] * inv));
+      uint16_t* p = a.out + static_cast<int64_t>(row_at[n]) * a.ldo + row_head[n] + 4 * g4;
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+        *reinterpret_cast<uint2*>(p + 16 * d) =
+            make_uint2(cvt_bf16x2(o[n][d][0] * inv, o[n][d][1] * inv), cvt_bf16x2(o[n][d][2] * inv, o[n][d][3] * inv));
     }
   }
 }
@@ -384,11 +551,10 @@ __global__ __launch_bounds__(kThreads) void attn_few_kernel(Args a) {
 template <int SRC>
 void launch(const Args& a, int row_blocks, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(a.n_tiles) * a.n_kv_heads * a.n_splits);
-  switch (row_blocks) {
-    case 1: hipLaunchKernelGGL((attn_few_kernel<SRC, 1>), grid, dim3(kThreads), 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((attn_few_kernel<SRC, 2>), grid, dim3(kThreads), 0, stream, a); break;
-    default: hipLaunchKernelGGL((attn_few_kernel<SRC, 4>), grid, dim3(kThreads), 0, stream, a); break;
-  }
+  if (row_blocks == 1)
+    hipLaunchKernelGGL((attn_few_kernel<SRC, 1>), grid, dim3(64 * W), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attn_few_kernel<SRC, 2>), grid, dim3(64 * W), 0, stream, a);
 }
 
 }  // namespace

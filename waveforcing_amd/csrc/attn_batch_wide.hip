@@ -32,8 +32,6 @@ namespace {
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef int v8i __attribute__((ext_vector_type(8)));
 
 constexpr int BKV = 64;
 constexpr int kWaves = 8;
@@ -117,10 +115,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   Tile t;
   if (!find_tile<kDense>(a, w, t)) return;
   const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
-  const int splits = used_splits(a, lim_max);
+  const Splits cut = tile_splits(a, lim_max);
+  const int splits = cut.n;
   if (split >= splits) return;
-  const int k_lo = split * a.split_keys;
-  const int k_hi = uniform(split == splits - 1 ? lim_max : k_lo + a.split_keys);
+  const int k_lo = split * cut.keys;
+  const int k_hi = uniform(min(lim_max, k_lo + cut.keys));
   const int tile_lo = k_lo / BKV, tile_hi = (k_hi + BKV - 1) / BKV;
 
   // this wave's rows: the lane's own, and the largest limit
@@ -323,33 +322,15 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
         for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo_to_f32(x[e])), fabsf(bf16_hi_to_f32(x[e]))));
       }
       amax = max32(amax);
-      const int E = __builtin_amdgcn_frexp_expf(amax);  // amax < 2^E
-      // q = 2^e (q1 + q2 / 16), e = E - 8: |q| 2^-e < 256
-      const int e = amax > 0.f ? min(max(E - 8, -122), 126) : 0;
+      const int e = q_exponent(amax);
       q_scale = 127 + e;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        uint32_t c1[8], c2[8];
+        uint2 c1[4], c2[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 x = raw[4 * m + i];
-          const uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float v[4] = {__builtin_ldexpf(bf16_lo_to_f32(y[2 * j]), -e), __builtin_ldexpf(bf16_hi_to_f32(y[2 * j]), -e),
-                                __builtin_ldexpf(bf16_lo_to_f32(y[2 * j + 1]), -e),
-                                __builtin_ldexpf(bf16_hi_to_f32(y[2 * j + 1]), -e)};
-            const uint32_t hi = e4m3_pack4_hw(v[0], v[1], v[2], v[3]);
-            float b0, b1, b2, b3;
-            e4m3_unpack4_hw(hi, b0, b1, b2, b3);
-            c1[2 * i + j] = hi;
-            c2[2 * i + j] = e4m3_pack4_hw((v[0] - b0) * 16.f, (v[1] - b1) * 16.f, (v[2] - b2) * 16.f, (v[3] - b3) * 16.f);
-          }
-        }
-        q1[m] = v8i{static_cast<int>(c1[0]), static_cast<int>(c1[1]), static_cast<int>(c1[2]), static_cast<int>(c1[3]),
-                    static_cast<int>(c1[4]), static_cast<int>(c1[5]), static_cast<int>(c1[6]), static_cast<int>(c1[7])};
-        q2[m] = v8i{static_cast<int>(c2[0]), static_cast<int>(c2[1]), static_cast<int>(c2[2]), static_cast<int>(c2[3]),
-                    static_cast<int>(c2[4]), static_cast<int>(c2[5]), static_cast<int>(c2[6]), static_cast<int>(c2[7])};
+        for (int i = 0; i < 4; ++i) split_q(raw[4 * m + i], e, c1[i], c2[i]);
+        q1[m] = __builtin_bit_cast(v8i, c1);
+        q2[m] = __builtin_bit_cast(v8i, c2);
       }
     }
   }
