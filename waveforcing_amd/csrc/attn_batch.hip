@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   const int head = item % a.n_kv_heads, w = item / a.n_kv_heads;
   Tile t;
   if (!find_tile<DENSE>(a, w, t)) return;
-  const int splits = tile_splits(a, tile_max(a, t)).n;
+  const int splits = used_splits(a, tile_max(a, t));
   if (splits < 2) return;
   const int r = part * kJoinRows + (static_cast<int>(threadIdx.x) >> 4), d = 8 * (static_cast<int>(threadIdx.x) & 15);
   if (t.first + r >= t.count) return;
@@ -103,8 +103,8 @@ Plan make_plan(int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_se
     for (int64_t s = 1; s <= kJoinSplits && (s == 1 || tiles / s >= 8); ++s) {
       const double pieces = static_cast<double>(units * s), per = tiles / s;
       const double rounds = pieces / cus;
-      double cost = n_seqs == 1 ? std::ceil(rounds) * (per + 4) : std::max(rounds, 1.0) * (0.7 * per + 4) + 0.5 * per;
-      if (s > 1) cost += 1.5 + 0.03 * pieces;
+      double cost = n_seqs == 1 ? std::ceil(rounds) * (per + 4) : std::max(rounds, 1.0) * (0.7 * per + 4) + 0.7 * per;
+      if (s > 1) cost += 1.5 + 0.012 * pieces;
       if (s == 1 || cost < best) {
         best = cost;
         p.n_splits = s;

@@ -44,13 +44,11 @@ struct Args {
   int32_t block;
   float c;  // softmax scale * log2(e)
   int32_t tile_shift, n_tiles;
-  int32_t split_keys, n_splits;  // keys of a split and splits, at most
+  int32_t split_keys, n_splits;  // keys of a split (a multiple of 64), splits at most
   float* part_o;                 // [n_tiles][n_kv_heads][n_splits][R][D], each divided by its own sum
   float* part_ml;                // [n_tiles][n_kv_heads][n_splits][R][2]: maximum (log2 units) and sum
   BatchGeom geom;
 };
-
-constexpr int kSplitUnit = 128;  // a split's keys are a multiple of this
 
 // A value that all lanes hold, in a scalar register.
 __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -130,15 +128,9 @@ __device__ inline int tile_max(const Args& a, const Tile& t) {
   return row_limit(a, t, a.group_div.div(last));
 }
 
-// Splits of a tile whose rows see up to lim keys: as many as split_keys asks for, of equal length.
-struct Splits {
-  int n, keys;
-};
-__device__ inline Splits tile_splits(const Args& a, int lim) {
-  if (lim <= a.split_keys || a.n_splits == 1) return Splits{1, max(lim, 0)};
-  const int n = min(a.n_splits, (lim - 1) / a.split_keys + 1);
-  const int keys = ((lim - 1) / n + kSplitUnit) / kSplitUnit * kSplitUnit;
-  return Splits{(lim - 1) / keys + 1, keys};
+// Splits that hold keys of a tile whose rows see up to lim keys.
+__device__ inline int used_splits(const Args& a, int lim) {
+  return min(a.n_splits, max(lim - 1, 0) / a.split_keys + 1);
 }
 
 // Two fp32 -> packed bf16x2, round to nearest even.

@@ -98,11 +98,10 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
   Tile t;
   if (!find_tile<kDense>(a, w, t)) return;
   const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
-  const Splits cut = tile_splits(a, lim_max);
-  const int splits = cut.n;
+  const int splits = used_splits(a, lim_max);
   if (split >= splits) return;
-  const int k_lo = split * cut.keys;
-  const int k_hi = min(lim_max, k_lo + cut.keys);
+  const int k_lo = split * a.split_keys;
+  const int k_hi = split == splits - 1 ? lim_max : k_lo + a.split_keys;
 
   // One tile in registers: K rows, V rows, the scales of key lane & 31, and which of its keys have no place to be read
   // from (where every lane finds its own).

@@ -115,11 +115,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   Tile t;
   if (!find_tile<kDense>(a, w, t)) return;
   const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
-  const Splits cut = tile_splits(a, lim_max);
-  const int splits = cut.n;
+  const int splits = used_splits(a, lim_max);
   if (split >= splits) return;
-  const int k_lo = split * cut.keys;
-  const int k_hi = uniform(min(lim_max, k_lo + cut.keys));
+  const int k_lo = split * a.split_keys;
+  const int k_hi = uniform(split == splits - 1 ? lim_max : k_lo + a.split_keys);
   const int tile_lo = k_lo / BKV, tile_hi = (k_hi + BKV - 1) / BKV;
 
   // this wave's rows: the lane's own, and the largest limit
