@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
   auto load = [&](int t0, const Where& c, Regs& x) __attribute__((always_inline)) {
     constexpr int kWord3 = 0x00020000;  // raw buffer, 32-bit data format
     if (kDense || c.one) {
-      const int bytes = c.n ? (c.n - 1) * static_cast<int>(key_bytes) + F::row_bytes : 0;
+      const int bytes = uniform(c.n ? (c.n - 1) * static_cast<int>(key_bytes) + F::row_bytes : 0);
       const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k), 0, bytes, kWord3);
       const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k + k_to_v), 0, bytes, kWord3);
       if constexpr (!kDense) {
