@@ -6,8 +6,8 @@
 //   lim = kv_len without a block; min(kv_len, (p / block + 1) block) with one, p = kv_len - new + i the row's position.
 //   A row without keys is zero.
 //
-// Two kernels: attn_batch_few.hip for up to 64 (row, head) rows of a sequence per key head, attn_batch_wide.hip for
-// more; long caches are split over workgroups, and the join below puts the splits' results together in their order.
+// Three kernels: attn_batch_few.hip for up to 64 (row, head) rows of a sequence per key head, for more attn_batch_wide.hip
+// over pages and attn_batch_dense.hip over dense keys; long caches are split over workgroups, and the join below puts the splits' results together in their order.
 #include "attn_batch.hpp"
 #include "gemm_core.hpp"
 
@@ -79,30 +79,31 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   *reinterpret_cast<uint2*>(p + 4) = make_uint2(cvt_bf16x2(o[4] * inv, o[5] * inv), cvt_bf16x2(o[6] * inv, o[7] * inv));
 }
 
-// How a call is split: rows of a tile (16, 32 and 64 on the few-rows kernel, 256 on the other), tiles, keys of a split.
+// How a call is split: rows of a tile (16 and 32 on the few-rows kernel, 256 and over dense keys 128 on the others),
+// tiles, keys of a split.
 struct Plan {
   int tile_shift;
   int64_t n_tiles, split_keys, n_splits, bytes;
 };
 
-Plan make_plan(int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_new, int64_t max_kv) {
+Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_new, int64_t max_kv) {
   const int64_t group = n_heads / n_kv_heads, cus = gemm::device_cus();
   const int64_t most = max_new * group;
   Plan p;
-  p.tile_shift = most <= 16 ? 4 : most <= 64 ? 5 : 8;
+  p.tile_shift = most <= 16 ? 4 : most <= 64 ? 5 : dense ? 7 : 8;
   p.n_tiles = ((n_rows * group) >> p.tile_shift) + n_seqs;
   const int64_t full = std::max<int64_t>(1, std::min<int64_t>(p.n_tiles, n_seqs * ((most + (1ll << p.tile_shift) - 1) >> p.tile_shift)));
   const int64_t units = full * n_kv_heads;
   p.n_splits = 1;
-  if (p.tile_shift == 8) {
-    // In times of one 64-key tile of a workgroup (about 2 us, one workgroup to a CU): a piece takes its tiles and a fixed
+  if (p.tile_shift > 5) {
+    // In times of one 64-key tile of a workgroup (about 2 us; one workgroup to a CU, of 128 rows two): a piece takes its tiles and a fixed
     // part of about 4; the rounds of pieces of one sequence (the pieces of several, whose lengths differ, spread over
     // the CUs with half a piece at the end); partial results of 256 rows are written and read at about 0.03.
     const double tiles = static_cast<double>((max_kv + 63) / 64);
     double best = 0;
     for (int64_t s = 1; s <= kJoinSplits && (s == 1 || tiles / s >= 8); ++s) {
       const double pieces = static_cast<double>(units * s), per = tiles / s;
-      const double rounds = pieces / cus;
+      const double rounds = pieces / (dense ? 2 * cus : cus);
       double cost = n_seqs == 1 ? std::ceil(rounds) * (per + 4) : std::max(rounds, 1.0) * (0.7 * per + 4) + 0.7 * per;
       if (s > 1) cost += 1.5 + 0.012 * pieces;
       if (s == 1 || cost < best) {
@@ -154,7 +155,7 @@ int common_args(const char* fn, Args& a, const void* q, int64_t n_rows, int32_t 
 
 int launch(const char* fn, Args& a, int src, int64_t n_seqs, int64_t max_new, int64_t max_kv, void* ws, int64_t ws_bytes,
            hipStream_t stream) {
-  const Plan p = make_plan(a.n_rows, static_cast<int64_t>(a.n_kv_heads) * a.group, a.n_kv_heads, n_seqs, max_new, max_kv);
+  const Plan p = make_plan(src == SRC_DENSE, a.n_rows, static_cast<int64_t>(a.n_kv_heads) * a.group, a.n_kv_heads, n_seqs, max_new, max_kv);
   WF_REQUIRE(product_below({p.n_tiles, a.n_kv_heads, p.n_splits, 16}, 1ll << 31), WF_E_SHAPE,
              "%s: %lld row tiles x %d key heads x %lld splits are too many", fn, (long long)p.n_tiles, a.n_kv_heads,
              (long long)p.n_splits);
@@ -169,7 +170,8 @@ int launch(const char* fn, Args& a, int src, int64_t n_seqs, int64_t max_new, in
   a.n_splits = static_cast<int32_t>(p.n_splits);
   a.part_o = static_cast<float*>(ws);
   a.part_ml = a.part_o + ((p.n_tiles * a.n_kv_heads * p.n_splits) << p.tile_shift) * D;
-  const int st = p.tile_shift == 8 ? launch_wide(a, src, stream) : launch_few(a, src, 1 << (p.tile_shift - 4), stream);
+  const int st = p.tile_shift <= 5 ? launch_few(a, src, 1 << (p.tile_shift - 4), stream)
+                 : src == SRC_DENSE ? launch_dense(a, stream) : launch_wide(a, src, stream);
   if (st || p.n_splits == 1) return st;
   const dim3 grid(static_cast<uint32_t>((p.n_tiles * a.n_kv_heads) << (p.tile_shift - 4)));
   if (src == SRC_DENSE)
@@ -192,7 +194,9 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads, int32_t n_kv_heads,
   WF_REQUIRE(n_rows >= 0 && n_heads > 0 && n_kv_heads > 0 && n_seqs >= 0 && max_new >= 0 && max_kv >= 0, WF_E_INVALID,
              "%s: negative or zero size", fn);
   WF_REQUIRE(n_heads % n_kv_heads == 0, WF_E_SHAPE, "%s: %d heads do not group over %d key heads", fn, n_heads, n_kv_heads);
-  *bytes = wf::attn_batch::make_plan(n_rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv).bytes;
+  *bytes = 0;
+  for (bool dense : {false, true})
+    *bytes = std::max(*bytes, wf::attn_batch::make_plan(dense, n_rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv).bytes);
   return WF_OK;
 }
 

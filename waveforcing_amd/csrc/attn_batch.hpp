@@ -2,9 +2,8 @@
 //
 // The n new rows of a sequence and the G = n_heads / n_kv_heads query heads of a key head make n G rows (i, head) over
 // the same keys; a workgroup takes a tile of R = 2^tile_shift of them for one key head and one range of the keys.
-// Tiles are numbered without knowing the lengths on the host: sequence b's begin at (cu[b] G >> tile_shift) + b, which
-// leaves room for all of them (floor(y) - floor(x) + 1 >= ceil(y - x)), so a launch over
-// (n_rows G >> tile_shift) + n_seqs tiles covers the batch and at most one tile of a sequence stays empty.
+// Tiles are numbered without gaps over the sequences; the host knows the lengths' sum only, and launches
+// (n_rows G >> tile_shift) + n_seqs of them, at least as many as there are (ceil(y) <= floor(y) + 1 for each sequence).
 #pragma once
 
 #include "batch_geom.hpp"
@@ -146,6 +145,13 @@ __device__ inline v2i read_tr8(const uint8_t* addr) {
   return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(addr));
 }
 
+// Order the wave's own LDS accesses (the hardware keeps them in order; this keeps the compiler to it).
+__device__ inline void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // max / sum over lanes l, l ^ 32 and l, l ^ 16.  Inline asm because the compiler reads both results of the swap builtins
 // from one register; the s_nop is the wait state that it puts before them.
 __device__ inline void swap32(float& lo, float& hi) { asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(lo), "+v"(hi)); }
@@ -201,7 +207,8 @@ __device__ inline uint32_t without_nan_codes(uint32_t w) {
 }
 
 int launch_few(const Args& a, int src, int row_blocks, hipStream_t stream);
-int launch_wide(const Args& a, int src, hipStream_t stream);
+int launch_wide(const Args& a, int format, hipStream_t stream);
+int launch_dense(const Args& a, hipStream_t stream);
 
 }  // namespace attn_batch
 }  // namespace wf

@@ -71,13 +71,6 @@ __device__ inline float absmax8(const uint4& v) {
   return m;
 }
 
-// Order the wave's own LDS accesses (the hardware keeps them in order; this keeps the compiler to it).
-__device__ inline void wave_lds_order() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 template <int SRC, int NB>
 __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kernel(Args a) {
   using F = Form<SRC, NB>;

@@ -1,11 +1,11 @@
-// Batched attention, many rows: tiles of 256 (row, head) rows of a sequence over one key head.  Bound by the matrix cores
-// and by the issue of the vector work between their instructions.
+// Batched attention, many rows over pages: tiles of 256 (row, head) rows of a sequence over one key head.  Bound by the
+// matrix cores and by the issue of the vector work between their instructions.
 //
-// Eight waves of 32 rows; keys in tiles of 64 through two LDS stages, staged by all threads (thread t: key t / 8, 16
+// Eight waves of 32 rows; keys in tiles of 64 through three LDS stages, staged by all threads (thread t: key t / 8, 16
 // values t % 8 of its row) one tile ahead of the products, with the loads of the tile after in flight.  S^T = K Q^T on
-// 32x32 products leaves a lane with one row and 32 keys, so a row's maximum is an in-lane maximum and one lane swap, and
-// its weights are directly the second operand of O^T += V^T P^T, whose first operand comes from the staged rows by
-// transposing reads (attn_paged.hip has the layouts).
+// 32x32 products leaves a lane with one row and 32 keys, so a row's sums are in-lane, and its weights are directly the
+// second operand of O^T += V^T P^T, whose first operand comes from the staged rows by transposing reads (attn_paged.hip
+// has the layouts).
 //
 // What is rounded, and where:
 //   e4m3 keys  the codes go to the fp8 matrix cores as they are, Q as the sum of two e4m3 parts under a power-of-two scale
@@ -18,7 +18,6 @@
 //              (a power of two moves no bit of them; values below 2^-29 of the largest lose their last ones).
 //   weights    fp16(64 p), p <= 2^kTau: eight times finer than bf16, down to 2^-31 of the row's largest; the row sum
 //              adds the rounded weights.
-//   dense      K, V, Q and the weights are bf16.
 // A NaN or infinite scale makes the key's score NaN and its V zero, so the rows that see the key become NaN and no
 // others; in tiles that some row does not see whole, so does a NaN code of V.
 #include <utility>
@@ -93,7 +92,6 @@ __device__ inline bool finite(float v) { return (f32_bits(v) & 0x7f800000u) != 0
 template <int SRC, bool SMALL>
 __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   using L = Lds<SRC>;
-  constexpr bool kDense = SRC == SRC_DENSE;
   constexpr bool kCodes = SRC == SRC_E4M3;
   __shared__ __attribute__((aligned(16))) uint8_t lds[L::bytes];
 
@@ -113,7 +111,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   const int hs = i_lin / a.n_tiles;
   const int head = hs % a.n_kv_heads, split = a.n_splits - 1 - hs / a.n_kv_heads;  // (what only long caches have first)
   Tile t;
-  if (!find_tile<kDense>(a, w, t)) return;
+  if (!find_tile<false>(a, w, t)) return;
   const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
   const int splits = used_splits(a, lim_max);
   if (split >= splits) return;
@@ -135,7 +133,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // ---- staging: key skey of the tile, values 16 schunk .. + 15
   const int skey = tid >> 3, schunk = tid & 7;
   struct Staged {
-    u32x4 k0, v0, k1, v1;
+    u32x4 k0, v0;
     float sk, sv;   // the key's scales
     float sv_lane;  // the scale of V of key `lane` of the tile: every wave sees all 64
   };
@@ -149,15 +147,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   };
   const int pt = a.geom.page_tokens;
   const int32_t* table = a.geom.tables + static_cast<int64_t>(t.b) * a.geom.ld_table;
-  const int64_t key_bytes = kDense ? a.ldkv * 2 : static_cast<int64_t>(a.n_kv_heads) * D;
-  const int64_t k_to_v = kDense ? reinterpret_cast<const uint8_t*>(a.v_dense) - reinterpret_cast<const uint8_t*>(a.k_dense)
-                                : a.v_codes - a.k_codes;
+  const int64_t key_bytes = static_cast<int64_t>(a.n_kv_heads) * D;
+  const int64_t k_to_v = a.v_codes - a.k_codes;
   const int64_t sk_to_sv = reinterpret_cast<const uint8_t*>(a.v_scales) - reinterpret_cast<const uint8_t*>(a.k_scales);
   auto cursor_at = [&](int tile) __attribute__((always_inline)) -> Cursor {
     if constexpr (SMALL) return Cursor{};
-    if constexpr (kDense)
-      return Cursor{0, BKV, BKV, reinterpret_cast<const uint8_t*>(a.k_dense + head * D) + (static_cast<int64_t>(t.key0) + tile * BKV) * key_bytes,
-                    nullptr};
     uint32_t lp, at;
     a.geom.page.divmod(static_cast<uint32_t>(tile) * BKV, lp, at);
     const int i = static_cast<int>(lp);
@@ -172,12 +166,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   };
   auto cursor_next = [&](const Cursor& c, int tile) __attribute__((always_inline)) -> Cursor {
     if constexpr (SMALL) return c;
-    if (!kDense && c.at + BKV >= pt) return cursor_at(tile);
-    return Cursor{c.at + (kDense ? 0 : BKV), kDense ? BKV : min(pt - c.at - BKV, BKV), c.n, c.k + BKV * key_bytes, c.sk + (kDense ? 0 : BKV)};
+    if (c.at + BKV >= pt) return cursor_at(tile);
+    return Cursor{c.at + BKV, min(pt - c.at - BKV, BKV), c.n, c.k + BKV * key_bytes, c.sk + BKV};
   };
   Cursor ahead{};
-  const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(key_bytes) +
-                            (kDense ? 32 : 16) * schunk;  // rows of a tile stay below 2^31 bytes (checked on the host)
+  const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(key_bytes) + 16 * schunk;  // rows of a tile stay below 2^31 bytes (checked on the host)
   constexpr int kWord3 = 0x00020000;  // raw buffer, 32-bit data format
   // SMALL: the pages of this lane's keys (skey and lane) in the tile that is loaded next (-1: none), asked for a tile ahead
   int page_key = -1, page_lane = -1;
@@ -193,23 +186,19 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // a lane's offset never changes.
   auto load_tile = [&](int tile, const Cursor& c, Staged& x, auto ONE) __attribute__((always_inline)) {
     const int n = uniform(min(max(k_hi - tile * BKV, 0), BKV));
-    if (kDense || decltype(ONE)::value || (!SMALL && c.cut == BKV)) {
+    if (decltype(ONE)::value || (!SMALL && c.cut == BKV)) {
       const int m = min(n, c.n);
-      const int bytes = m ? (m - 1) * static_cast<int>(key_bytes) + (kDense ? 2 * D : D) : 0;
+      const int bytes = m ? (m - 1) * static_cast<int>(key_bytes) + D : 0;
       const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k), 0, bytes, kWord3);
       const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k + k_to_v), 0, bytes, kWord3);
-      if constexpr (!kDense) {
-        const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(c.sk), 0, 4 * m, kWord3);
-        const auto sv = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(c.sk) + sk_to_sv), 0, 4 * m, kWord3);
-        x.sv_lane = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * lane, 0, 0));
-        x.sk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * skey, 0, 0));
-        x.sv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * skey, 0, 0));
-      }
+      const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(c.sk), 0, 4 * m, kWord3);
+      const auto sv = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(c.sk) + sk_to_sv), 0, 4 * m, kWord3);
+      x.sv_lane = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * lane, 0, 0));
+      x.sk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * skey, 0, 0));
+      x.sv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * skey, 0, 0));
       x.k0 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row, 0, 0);
-      if constexpr (kDense) x.k1 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row + 16, 0, 0);
       x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
-      if constexpr (kDense) x.v1 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row + 16, 0, 0);
     } else {
       if constexpr (!SMALL) find_pages(tile);
       const uint32_t jk = static_cast<uint32_t>(tile * BKV + skey), jl = static_cast<uint32_t>(tile * BKV + lane);
@@ -249,34 +238,27 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   };
   // The staged tile as it goes to LDS.  PARTIAL: some row may not see all of it.
   auto convert = [&](Staged x, Ready& y, auto PARTIAL) __attribute__((always_inline)) {
-    if constexpr (kDense) {
-      y.k0 = make_uint4(x.k0[0], x.k0[1], x.k0[2], x.k0[3]);
-      y.k1 = make_uint4(x.k1[0], x.k1[1], x.k1[2], x.k1[3]);
-      y.v0 = make_uint4(x.v0[0], x.v0[1], x.v0[2], x.v0[3]);
-      y.v1 = make_uint4(x.v1[0], x.v1[1], x.v1[2], x.v1[3]);
-    } else {
-      bool poison = !finite(x.sv);
-      if constexpr (SRC == SRC_E4M3 && decltype(PARTIAL)::value) {
-        const bool nan = has_nan_code(x.v0[0]) || has_nan_code(x.v0[1]) || has_nan_code(x.v0[2]) || has_nan_code(x.v0[3]);
-        const uint64_t any = __ballot(nan);
+    bool poison = !finite(x.sv);
+    if constexpr (SRC == SRC_E4M3 && decltype(PARTIAL)::value) {
+      const bool nan = has_nan_code(x.v0[0]) || has_nan_code(x.v0[1]) || has_nan_code(x.v0[2]) || has_nan_code(x.v0[3]);
+      const uint64_t any = __ballot(nan);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.v0[e] = without_nan_codes(x.v0[e]);
-        poison = poison || (any >> (lane & 56) & 0xffu);
-      }
-      y.u = poison ? bits_f32(0x7fc00000u) : x.sk * a.c;
-      const float f = __builtin_ldexpf(poison ? 0.f : x.sv, -ev);
-      const v2h ff = {static_cast<_Float16>(f), static_cast<_Float16>(f)};
-      if constexpr (kCodes) {
-        y.k0 = make_uint4(x.k0[0], x.k0[1], x.k0[2], x.k0[3]);
-      } else {
-        const uint2 p = i8_bf16(x.k0[0]), q = i8_bf16(x.k0[1]), s = i8_bf16(x.k0[2]), v = i8_bf16(x.k0[3]);
-        y.k0 = make_uint4(p.x, p.y, q.x, q.y);
-        y.k1 = make_uint4(s.x, s.y, v.x, v.y);
-      }
-      const uint2 p = codes_f16<SRC>(x.v0[0]), q = codes_f16<SRC>(x.v0[1]), s = codes_f16<SRC>(x.v0[2]), v = codes_f16<SRC>(x.v0[3]);
-      y.v0 = make_uint4(pk_mul_f16(p.x, ff), pk_mul_f16(p.y, ff), pk_mul_f16(q.x, ff), pk_mul_f16(q.y, ff));
-      y.v1 = make_uint4(pk_mul_f16(s.x, ff), pk_mul_f16(s.y, ff), pk_mul_f16(v.x, ff), pk_mul_f16(v.y, ff));
+      for (int e = 0; e < 4; ++e) x.v0[e] = without_nan_codes(x.v0[e]);
+      poison = poison || (any >> (lane & 56) & 0xffu);
     }
+    y.u = poison ? bits_f32(0x7fc00000u) : x.sk * a.c;
+    const float f = __builtin_ldexpf(poison ? 0.f : x.sv, -ev);
+    const v2h ff = {static_cast<_Float16>(f), static_cast<_Float16>(f)};
+    if constexpr (kCodes) {
+      y.k0 = make_uint4(x.k0[0], x.k0[1], x.k0[2], x.k0[3]);
+    } else {
+      const uint2 p = i8_bf16(x.k0[0]), q = i8_bf16(x.k0[1]), s = i8_bf16(x.k0[2]), v = i8_bf16(x.k0[3]);
+      y.k0 = make_uint4(p.x, p.y, q.x, q.y);
+      y.k1 = make_uint4(s.x, s.y, v.x, v.y);
+    }
+    const uint2 p = codes_f16<SRC>(x.v0[0]), q = codes_f16<SRC>(x.v0[1]), s = codes_f16<SRC>(x.v0[2]), v = codes_f16<SRC>(x.v0[3]);
+    y.v0 = make_uint4(pk_mul_f16(p.x, ff), pk_mul_f16(p.y, ff), pk_mul_f16(q.x, ff), pk_mul_f16(q.y, ff));
+    y.v1 = make_uint4(pk_mul_f16(s.x, ff), pk_mul_f16(s.y, ff), pk_mul_f16(v.x, ff), pk_mul_f16(v.y, ff));
   };
   auto write = [&](int stage, const Ready& y) __attribute__((always_inline)) {
     uint8_t* st = lds + stage;
@@ -290,10 +272,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     }
     dv[0] = y.v0;
     dv[1] = y.v1;
-    if constexpr (!kDense) {
-      float* u = reinterpret_cast<float*>(st + L::u_off);
-      u[skey] = y.u;  // (the lanes of one key write the same word)
-    }
+    float* u = reinterpret_cast<float*>(st + L::u_off);
+    u[skey] = y.u;  // (the lanes of one key write the same word)
   };
 
   // ---- Q, the second operand of the scores, for the whole kernel
@@ -344,8 +324,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   float m_use = -INFINITY;  // the row's maximum in the exponents, log2 units
   float l_run = 0.f;        // this half's row sum
   // Weights are 2^kShift p, and a tile's sum of them (of a lane's 32 keys) at most kMostSum: fp16 ends at 65504.
-  constexpr float kShift = kDense ? 0.f : 6.f;
-  constexpr float kMostSum = kDense ? 256.f : 32768.f;
+  constexpr float kShift = 6.f;
+  constexpr float kMostSum = 32768.f;
   float neg_m = kShift;
 
   // Raising E before tile t + 1 is staged (its scales came with the loads of the last iteration) leaves V of tile t under
@@ -353,12 +333,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // (one place that rescales keeps O in its registers).
   float o_scale = 1.f, pend = 1.f, pend_next = 1.f;
   auto check_exponent = [&]() __attribute__((always_inline)) {
-    if constexpr (!kDense) {
-      if (__ballot(sreg.sv_lane > sv_lim && finite(sreg.sv_lane))) {
-        const int e_old = ev;
-        set_exponent(tile_top(sreg.sv_lane));
-        pend_next *= __builtin_ldexpf(1.f, max(e_old - ev, -200));
-      }
+    if (__ballot(sreg.sv_lane > sv_lim && finite(sreg.sv_lane))) {
+      const int e_old = ev;
+      set_exponent(tile_top(sreg.sv_lane));
+      pend_next *= __builtin_ldexpf(1.f, max(e_old - ev, -200));
     }
   };
 
@@ -384,10 +362,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       const uint4 w = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
-        if constexpr (kDense)
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, vf[k & 1][db]), __builtin_bit_cast(v8bf, w), o[db], 0, 0, 0);
-        else
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[k & 1][db]), __builtin_bit_cast(v8h, w), o[db], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[k & 1][db]), __builtin_bit_cast(v8h, w), o[db], 0, 0, 0);
       }
       if (k < 2) read_v(stage, k + 2);
     }
@@ -398,11 +373,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // wave may see none of t, or the tile to be loaded may span pages; without it the half is one block of instructions.
   float4 uf[2][2];
   auto read_u = [&](int stage, int k) __attribute__((always_inline)) {  // factors of the lane's keys in 16-key step k
-    if constexpr (!kDense) {
-      const float* us = reinterpret_cast<const float*>(lds + stage + L::u_off);
-      uf[k & 1][0] = *reinterpret_cast<const float4*>(us + 16 * k + 4 * half);
-      uf[k & 1][1] = *reinterpret_cast<const float4*>(us + 16 * k + 8 + 4 * half);
-    }
+    const float* us = reinterpret_cast<const float*>(lds + stage + L::u_off);
+    uf[k & 1][0] = *reinterpret_cast<const float4*>(us + 16 * k + 4 * half);
+    uf[k & 1][1] = *reinterpret_cast<const float4*>(us + 16 * k + 8 + 4 * half);
   };
   auto products = [&](int tile, auto PARTIAL) __attribute__((always_inline)) {
     constexpr bool kPartial = decltype(PARTIAL)::value;
@@ -505,25 +478,15 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float x = s[b][8 * (k & 1) + e];
-          if constexpr (kDense) {
-            p[e] = __builtin_amdgcn_exp2f(fmaf(x, a.c, neg_m));
-          } else {
-            const float4 y = uf[k & 1][e >> 2];
-            const float u[4] = {y.x, y.y, y.z, y.w};
-            p[e] = __builtin_amdgcn_exp2f(fmaf(x, factor(u[e & 3], x), neg_m));
-          }
+          const float4 y = uf[k & 1][e >> 2];
+          const float u[4] = {y.x, y.y, y.z, y.w};
+          p[e] = __builtin_amdgcn_exp2f(fmaf(x, factor(u[e & 3], x), neg_m));
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (kDense) {
-            const v2bf one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
-            pw[4 * k + e] = cvt_bf16x2(p[2 * e], p[2 * e + 1]);
-            l_tile = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pw[4 * k + e]), one, l_tile, false);
-          } else {
-            const v2h one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-            pw[4 * k + e] = cvt_f16x2(p[2 * e], p[2 * e + 1]);
-            l_tile = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, pw[4 * k + e]), one, l_tile, false);
-          }
+          const v2h one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+          pw[4 * k + e] = cvt_f16x2(p[2 * e], p[2 * e + 1]);
+          l_tile = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, pw[4 * k + e]), one, l_tile, false);
         }
       }
     };
@@ -535,9 +498,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          float4 x;
-          if constexpr (!kDense) x = *reinterpret_cast<const float4*>(us + 32 * b + 8 * g + 4 * half);
-          const float u[4] = {kDense ? a.c : x.x, kDense ? a.c : x.y, kDense ? a.c : x.z, kDense ? a.c : x.w};
+          const float4 x = *reinterpret_cast<const float4*>(us + 32 * b + 8 * g + 4 * half);
+          const float u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) mt = fmaxf(mt, s[b][4 * g + e] * factor(u[e], s[b][4 * g + e]));
         }
@@ -569,7 +531,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     Cursor c = cursor_at(tile_lo);
     if constexpr (SMALL) find_pages(tile_lo);
     load_tile(tile_lo, c, sreg, std::false_type{});
-    if constexpr (!kDense) set_exponent(tile_top(sreg.sv_lane));
+    set_exponent(tile_top(sreg.sv_lane));
     Ready y;
     convert(sreg, y, std::true_type{});
     write(st_cur, y);
@@ -587,7 +549,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     __syncthreads();
     // whole: tiles that every row sees, and the next one too
     const int whole = min(max(lim_min / BKV - 1, tile_lo), tile_hi);
-    auto one_page = [&]() __attribute__((always_inline)) { return kDense || SMALL || ahead.cut == BKV; };
+    auto one_page = [&]() __attribute__((always_inline)) { return SMALL || ahead.cut == BKV; };
     auto rotate = [&](const Cursor& after) __attribute__((always_inline)) {
       const int x = st_prev;
       st_prev = st_cur;
@@ -674,14 +636,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 
 }  // namespace
 
-int launch_wide(const Args& a, int src, hipStream_t stream) {
+int launch_wide(const Args& a, int format, hipStream_t stream) {
   const int64_t items = static_cast<int64_t>(a.n_tiles) * a.n_kv_heads * a.n_splits;
   constexpr int64_t per = kXcds * kRun;
   const dim3 grid(static_cast<uint32_t>((items + per - 1) / per * per));
   const bool small = a.geom.page_tokens < BKV;
-  void (*kernel)(Args) = attn_wide_kernel<SRC_DENSE, false>;
-  if (src == SRC_E4M3) kernel = small ? attn_wide_kernel<SRC_E4M3, true> : attn_wide_kernel<SRC_E4M3, false>;
-  if (src == SRC_INT8) kernel = small ? attn_wide_kernel<SRC_INT8, true> : attn_wide_kernel<SRC_INT8, false>;
+  void (*kernel)(Args);
+  if (format == WF_KV_E4M3)
+    kernel = small ? attn_wide_kernel<SRC_E4M3, true> : attn_wide_kernel<SRC_E4M3, false>;
+  else
+    kernel = small ? attn_wide_kernel<SRC_INT8, true> : attn_wide_kernel<SRC_INT8, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
   return check_launch("wf_attn_batch (many rows)");
 }
