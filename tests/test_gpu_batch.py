@@ -390,3 +390,196 @@ def test_a_batched_step_as_it_is_used(fmt):
                 check(x[at:at + m], *ob.attend(q[at:at + m], kk, vv, [kv[b] - m + i + 1 for i in range(m)], SCALE))
                 check(y[at:at + m], *ob.attend(x[at:at + m], tk[c:c + text[b]], tv[c:c + text[b]], [text[b]] * m, SCALE))
             at, c = at + m, c + text[b]
+
+
+# ------------------------------------------------- sizes, scales and contents at the kernels' edges
+EDGES = [15, 16, 17, 32, 33, 48, 63, 64, 65, 127, 128, 129, 255, 256, 257]
+
+
+@pytest.mark.parametrize("group", [1, 3])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "dense"])
+def test_row_counts_around_the_tiles(fmt, group):
+    """Sequences whose rows fill, miss and pass a tile by one, with keys that do the same, and idle ones between."""
+    for new in ([n] for n in EDGES if group == 1):
+        run_edges(fmt, group, new, [new[0] + 1])
+    run_edges(fmt, group, EDGES, [n + 64 - n % 64 + i % 3 - 1 for i, n in enumerate(EDGES)])
+    run_edges(fmt, group, [0, 3, 70, 1] * 40, [64 + i % 3 for i in range(160)] if fmt == "dense" else [80 + i % 3 for i in range(160)])
+
+
+def run_edges(fmt, group, new, kv):
+    if fmt == "dense":
+        g = gen(140)
+        batch = CrossBatch(new, kv, DEV)
+        q, k, v = rows(sum(new), 2 * group, g), rows(sum(kv), 2, g), rows(sum(kv), 2, g)
+        out = backend.attn_cross_batch(q, k, v, batch)
+        a = c = 0
+        for i, j in zip(new, kv):
+            check(out[a:a + i], *ob.attend(q[a:a + i], k[c:c + j], v[c:c + j], [j] * i, SCALE))
+            a, c = a + i, c + j
+        return
+    kv = [max(t, n) for t, n in zip(kv, new)]
+    pool, batch, g = make(fmt, 2, 48, kv, new, 141)
+    q = rows(sum(new), 2 * group, g)
+    check_paged(backend.attn_paged_batch(q, batch, block=1), q, pool, batch, fmt, 1)
+
+
+@pytest.mark.parametrize("page", [16, 64, 390])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("new", [4, 150, 300])
+def test_scales_of_v_that_grow_along_the_cache(fmt, new, page):
+    """Scales of V from 2^-40 (and zero) up to 2^30 and back, changing inside and between the tiles: what was summed under
+    a small scale keeps its place when a large one comes, and the other way round."""
+    kv = [new + 700, new + 90]
+    pool, batch, g = make(fmt, 2, page, kv, [new, new], 150)
+    steps = [0, 0, -40, -38, -20, -20, -20, -3, 2, 2, 9, 9, 10, 30, 30, 29, 28, 28, 27, 26, 0, -10, 5, 5, 27, 31]
+    for b, t in enumerate(kv):
+        for p in range(t):
+            e = steps[(p // 37 + 9 * b) % len(steps)]
+            s = 0.0 if p < 20 and b == 0 else 2.0 ** e * 0.013
+            pool.v_scales[batch.pages[b][p // page], :, p % page] = s
+    q = rows(2 * new, 4, g)
+    for block in (0, 1):
+        check_paged(backend.attn_paged_batch(q, batch, block=block), q, pool, batch, fmt, block)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("page", [7, 48, 64, 390])
+@pytest.mark.parametrize("new", [2, 100])
+def test_pages_that_are_none_read_as_zeros(fmt, page, new):
+    """Table entries outside the pool, first, in the middle and last: their keys are zero and take part."""
+    pool, batch, g = make(fmt, 2, page, [1000, 500], [new, new], 160)
+    n = len(batch.pages[0])
+    ks, vs = [], []
+    gone = {0: -1, n // 2: pool.pool_pages, n - 1: 2 ** 30}
+    for i, bad in gone.items():
+        batch.tables[0, i] = bad
+    for which, out in (("k", ks), ("v", vs)):
+        x = cached(pool, batch, fmt, 0, which)
+        for i in gone:
+            x[i * page:(i + 1) * page] = 0
+        out.append(x)
+    q = rows(2 * new, 4, g)
+    out = backend.attn_paged_batch(q, batch, block=1)
+    check(out[:new], *ob.attend(q[:new], ks[0], vs[0], [1000 - new + i + 1 for i in range(new)], SCALE))
+    check(out[new:], *ob.attend(q[new:], cached(pool, batch, fmt, 1, "k"), cached(pool, batch, fmt, 1, "v"),
+                                [500 - new + i + 1 for i in range(new)], SCALE))
+
+
+@pytest.mark.parametrize("new", [1, 9, 140])
+def test_other_sequences_dense_keys_do_not_reach_a_row(new):
+    lens = [63, 65, 130, 1]
+    g = gen(170)
+    batch = CrossBatch([new] * 4, lens, DEV)
+    q, k, v = rows(4 * new, 4, g), rows(sum(lens), 2, g), rows(sum(lens) + 5, 2, g)[:sum(lens)]
+    clean = backend.attn_cross_batch(q, k, v, batch)
+    for bad in (float("nan"), float("inf")):
+        for t in (k, v):
+            save = t.clone()
+            t[63:128] = bad
+            out = backend.attn_cross_batch(q, k, v, batch)
+            for b in (0, 2, 3):
+                same(out[b * new:(b + 1) * new], clean[b * new:(b + 1) * new])
+            assert not bool(torch.isfinite(out[new:2 * new]).any())
+            t.copy_(save)
+
+
+@pytest.mark.parametrize("new", [1, 9, 40, 140])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "dense"])
+def test_queries_that_are_not_finite(fmt, new):
+    """A row of q with a NaN or an infinity is NaN; the others are what they were."""
+    if fmt == "dense":
+        g = gen(180)
+        batch = CrossBatch([new], [200], DEV)
+        k, v = rows(200, 2, g), rows(200, 2, g)
+        attend = lambda q: backend.attn_cross_batch(q, k, v, batch)
+    else:
+        _, batch, g = make(fmt, 2, 64, [200], [new], 181)
+        attend = lambda q: backend.attn_paged_batch(q, batch, block=0)
+    q = rows(new, 4, g)
+    clean = attend(q)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        x = q.clone()
+        x[new // 2, 1, 77] = bad
+        out = attend(x)
+        assert bool(torch.isnan(out[new // 2, 1]).all())
+        out[new // 2, 1] = clean[new // 2, 1]
+        same(out, clean)
+
+
+@pytest.mark.parametrize("new", [1, 20, 140])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "dense"])
+def test_scores_that_rise_and_fall_along_the_keys(fmt, new):
+    """The maximum moves from tile to tile, by little, by much (past what a weight can hold) and back."""
+    rise = [0.0, 0.5, 0.1, 3.0, 3.2, 9.0, 1.0, 30.0, 30.0, 25.0, 60.0, 0.0, 61.0]
+    t = 64 * len(rise) + 11
+    g = gen(190)
+    k = rows(t, 2, g, 0.1)
+    q = rows(new, 4, g, 0.1)
+    q[:, :, 0] = 1.0
+    for i in range(t):
+        k[i, :, 0] = rise[min(i // 64, len(rise) - 1)] / SCALE
+    v = rows(t, 2, g)
+    if fmt == "dense":
+        out = backend.attn_cross_batch(q, k, v, CrossBatch([new], [t], DEV))
+        check(out, *ob.attend(q, k, v, [t] * new, SCALE))
+        return
+    pool, _, _ = make(fmt, 2, 64, [t], [t], 191, spare=0, fill=False)
+    whole = PagedBatch(pool, [list(range(pool.pool_pages))], [t], [t])
+    whole.append(k, v)
+    batch = PagedBatch(pool, whole.pages, [t], [new])
+    check_paged(backend.attn_paged_batch(q, batch, block=1), q, pool, batch, fmt, 1)
+
+
+@pytest.mark.parametrize("new", [3, 150])
+def test_dense_rows_past_32_bit_offsets(new):
+    """q, k, v and out as columns of tensors whose rows are 64 K elements apart: the last sequence's begin past 2^31."""
+    n = 34000                                          # 34000 * 65536 = 2.2e9 elements
+    wide = torch.empty((n, 65536), dtype=torch.bfloat16, device=DEV)
+    cols = lambda c, heads: wide[:, 128 * c:128 * (c + heads)].view(n, heads, 128)
+    q, k, v, out = cols(0, 4), cols(8, 2), cols(12, 2), cols(16, 4)
+    lens = [n - 300, 300]
+    news = [n - new, new]
+    g = gen(200)
+    tail = [slice(n - new, n), slice(n - 300, n)]
+    q[tail[0]] = rows(new, 4, g)
+    for t in (k, v):
+        t[tail[1]] = rows(300, 2, g)
+    batch = CrossBatch([0, new], lens, DEV)
+    batch.cu_q.copy_(torch.tensor([n - new, n - new, n], dtype=torch.int32))   # the first rows are no sequence's
+    batch.n_q = n
+    backend.attn_cross_batch(q, k, v, batch, out=out)
+    check(out[tail[0]], *ob.attend(q[tail[0]], k[tail[1]], v[tail[1]], [300] * new, SCALE))
+
+
+def test_captured_chunks_follow_the_device_lengths():
+    """Many rows over pages and over dense keys, captured once and replayed with other lengths, tables and contents."""
+    pool, batch, g = make("e4m3", 2, 64, [700, 300], [150, 90], 210)
+    cross = CrossBatch([150, 90], [100, 60], DEV)
+    q, k, v = rows(240, 4, g), rows(160, 2, g), rows(160, 2, g)
+
+    def step():
+        x = backend.attn_paged_batch(q, batch, block=1)
+        return x, backend.attn_cross_batch(x, k, v, cross)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for new, kv, text in (([150, 90], [700, 300], [100, 60]), ([240, 0], [500, 1], [1, 0]), ([7, 130], [7, 299], [160, 0])):
+        q.copy_(rows(240, 4, g))
+        batch.cu_new.copy_(torch.tensor([0, new[0], sum(new)], dtype=torch.int32))
+        batch.kv_lens_dev.copy_(torch.tensor(kv, dtype=torch.int32))
+        cross.cu_q.copy_(torch.tensor([0, new[0], sum(new)], dtype=torch.int32))
+        cross.cu_kv.copy_(torch.tensor([0, text[0], sum(text)], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        x, y = (o.clone() for o in outs)
+        eager = PagedBatch(pool, batch.pages, kv, new)
+        check_paged(x[:sum(new)], q[:sum(new)], pool, eager, "e4m3", 1)
+        a = c = 0
+        for i, j in zip(new, text):
+            check(y[a:a + i], *ob.attend(x[a:a + i], k[c:c + j], v[c:c + j], [j] * i, SCALE))
+            a, c = a + i, c + j

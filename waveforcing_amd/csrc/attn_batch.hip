@@ -88,7 +88,7 @@ struct Plan {
 
 Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_new, int64_t max_kv) {
   const int64_t group = n_heads / n_kv_heads, cus = gemm::device_cus();
-  const int64_t most = max_new * group;
+  const int64_t most = std::min(max_new, n_rows) * group;
   Plan p;
   p.tile_shift = most <= 16 ? 4 : most <= 64 ? 5 : dense ? 7 : 8;
   p.n_tiles = ((n_rows * group) >> p.tile_shift) + n_seqs;
@@ -194,6 +194,8 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads, int32_t n_kv_heads,
   WF_REQUIRE(n_rows >= 0 && n_heads > 0 && n_kv_heads > 0 && n_seqs >= 0 && max_new >= 0 && max_kv >= 0, WF_E_INVALID,
              "%s: negative or zero size", fn);
   WF_REQUIRE(n_heads % n_kv_heads == 0, WF_E_SHAPE, "%s: %d heads do not group over %d key heads", fn, n_heads, n_kv_heads);
+  WF_REQUIRE(wf::product_below({n_rows, n_heads}, (1ll << 31) - 65536) && n_seqs < (1ll << 31) && max_kv < (1ll << 31), WF_E_SHAPE,
+             "%s: rows=%lld x heads=%d, %lld sequences or %lld keys reach 2^31", fn, (long long)n_rows, n_heads, (long long)n_seqs, (long long)max_kv);
   *bytes = 0;
   for (bool dense : {false, true})
     *bytes = std::max(*bytes, wf::attn_batch::make_plan(dense, n_rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv).bytes);

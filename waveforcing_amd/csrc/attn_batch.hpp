@@ -182,7 +182,10 @@ __device__ inline float sum16(float v) {
 __device__ inline int q_exponent(float amax) {
   return amax > 0.f ? min(max(__builtin_amdgcn_frexp_expf(amax) - 8, -122), 126) : 0;
 }
-// 8 values of a row.
+// 8 values of a row as split_q takes them: a row that holds an infinity becomes NaN, as its scores are.
+__device__ inline uint4 nan_if_infinite(const uint4& x, float amax) {
+  return amax < INFINITY ? x : make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+}
 __device__ inline void split_q(const uint4& x, int e, uint2& q1, uint2& q2) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
   uint32_t c1[2], c2[2];

@@ -240,7 +240,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
         for (int off = 1; off < 16; off *= 2) amax = fmaxf(amax, __shfl_xor(amax, off));
         const int e = q_exponent(amax);
         uint2 c1, c2;
-        split_q(v, e, c1, c2);
+        split_q(nan_if_infinite(v, amax), e, c1, c2);
         *reinterpret_cast<uint2*>(qbuf + r * kQPitch + 8 * (c & 15)) = c1;
         *reinterpret_cast<uint2*>(qbuf + r * kQPitch + D + 8 * (c & 15)) = c2;
         if ((c & 15) == 0) es[r] = 127 + e;
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
       q_scale[0] = 127 + e;
       uint2 c1[4], c2[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) split_q(v[s], e, c1[s], c2[s]);
+      for (int s = 0; s < 4; ++s) split_q(nan_if_infinite(v[s], amax), e, c1[s], c2[s]);
       qa = __builtin_bit_cast(v8i, c1);
       qb = __builtin_bit_cast(v8i, c2);
     }

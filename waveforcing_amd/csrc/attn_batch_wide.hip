@@ -307,7 +307,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       for (int m = 0; m < 2; ++m) {
         uint2 c1[4], c2[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_q(raw[4 * m + i], e, c1[i], c2[i]);
+        for (int i = 0; i < 4; ++i) split_q(nan_if_infinite(raw[4 * m + i], amax), e, c1[i], c2[i]);
         q1[m] = __builtin_bit_cast(v8i, c1);
         q2[m] = __builtin_bit_cast(v8i, c2);
       }
