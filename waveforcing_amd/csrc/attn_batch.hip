@@ -96,16 +96,18 @@ Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, 
   const int64_t units = full * n_kv_heads;
   p.n_splits = 1;
   if (p.tile_shift > 5) {
-    // In times of one 64-key tile of a workgroup (about 2 us; one workgroup to a CU, of 128 rows two): a piece takes its tiles and a fixed
-    // part of about 4; the rounds of pieces of one sequence (the pieces of several, whose lengths differ, spread over
-    // the CUs with half a piece at the end); partial results of 256 rows are written and read at about 0.03.
+    // In times of one 64-key tile of a workgroup (about 2 us; one workgroup to a CU, of 128 rows two): a piece takes its
+    // tiles and a fixed part of about 4; the rounds of pieces of one sequence (the pieces of several, whose lengths
+    // differ, spread over the CUs, the longest first, with little at the end); partial results of 256 rows are written and
+    // read at about 0.03.  Six sequences of up to 10001 keys, 800 tiles: 412 us whole, 498 in two, 511 in four; 8 over up to
+    // 4001 dense keys, 216 tiles: 77 whole, 55 in three, 58 in eight.
     const double tiles = static_cast<double>((max_kv + 63) / 64);
     double best = 0;
     for (int64_t s = 1; s <= kJoinSplits && (s == 1 || tiles / s >= 8); ++s) {
       const double pieces = static_cast<double>(units * s), per = tiles / s;
       const double rounds = pieces / (dense ? 2 * cus : cus);
-      double cost = n_seqs == 1 ? std::ceil(rounds) * (per + 4) : std::max(rounds, 1.0) * (0.7 * per + 4) + 0.7 * per;
-      if (s > 1) cost += 1.5 + 0.012 * pieces;
+      double cost = n_seqs == 1 ? std::ceil(rounds) * (per + 4) : std::max(rounds, 1.0) * (0.7 * per + 4) + 0.15 * per;
+      if (s > 1) cost += 1.5 + (dense ? 0.015 : 0.03) * pieces;
       if (s == 1 || cost < best) {
         best = cost;
         p.n_splits = s;
