@@ -426,9 +426,14 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads,
  * over the keys j < lim, lim = kv_lens[b] when block == 0, else
  * min(kv_lens[b], (p / block + 1) * block) for the row's position p: every
  * key, causal (block 1), or causal by blocks of `block` positions (a frame,
- * a chunk).  Rows without a key are zero; keys a row does not see do not
- * reach it, whatever they hold.  fp32 scores, softmax and sums; the weights
- * p_j s_v[j] are rounded to bf16 for the second product.  max_new and max_kv
+ * a chunk).  Rows without a key are zero; a row of q that holds a NaN or an
+ * infinity is NaN, and so are the rows that see a key whose scale is none; no
+ * NaN or infinity of a key reaches a row that does not see it.  fp32 scores,
+ * softmax and sums.  Up to 64 (row, head) rows of a sequence per key head the
+ * weights p_j s_v[j] are held in 16 significant bits; with more, p_j in fp16
+ * and V as fp16(V 2^-E), E set by the largest scale of V among the keys that
+ * the row's tile of 256 reads (values below 2^-29 of the largest lose bits).
+ * max_new and max_kv
  * bound the sequences' rows and keys; they choose the split, and results
  * stay right where the device's lengths pass them.  ws: ws_bytes of scratch,
  * 16-byte aligned, at least wf_attn_batch_workspace's.  The attention of
@@ -450,7 +455,8 @@ int wf_attn_paged_batch(const void* q, int64_t n_rows, int32_t n_heads,
 /* The same over dense bf16 keys: sequence b's are the rows cu_kv[b] ..
  * cu_kv[b + 1] of k and v [n_kv_rows][n_kv_heads][128] (row stride ldkv), all
  * of them visible to its query rows cu_q[b] .. cu_q[b + 1].  The text
- * cross-attention with each prompt's own length (naive_rt/rolling_forcing/
+ * cross-attention with each prompt's own length; the weights in 16 significant
+ * bits up to 64 rows, in bf16 with more (naive_rt/rolling_forcing/
  * wan/modules/model.py:165-189). */
 int wf_attn_cross_batch(const void* q, int64_t n_rows, int32_t n_heads,
                         int32_t n_kv_heads, int32_t head_dim, int64_t ldq,

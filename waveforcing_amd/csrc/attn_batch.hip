@@ -21,7 +21,8 @@ namespace {
 constexpr int kJoinRows = 16;    // rows of a workgroup, 16 lanes of 8 values each
 constexpr int kJoinSplits = 64;  // splits at most
 
-// out = sum_s l_s 2^(m_s - m) o_s / sum_s l_s 2^(m_s - m) over the splits s of a row tile that used more than one.
+// out = sum_s l_s 2^(m_s - m) o_s / sum_s l_s 2^(m_s - m) over the splits s of a row tile that used more than one.  Reads
+// the partial results once (few of them: 4-5 us, most of it the launch; the rows' 16 lanes keep 8 loads in flight).
 template <bool DENSE>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
   const int R = 1 << a.tile_shift;

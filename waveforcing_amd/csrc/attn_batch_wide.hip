@@ -7,6 +7,10 @@
 // second operand of O^T += V^T P^T, whose first operand comes from the staged rows by transposing reads (attn_paged.hip
 // has the layouts).
 //
+// 3 x 4680 rows over up to 37440 keys of 12 heads: 2.18 ms, 0.98 PFLOP/s (one sequence at a time, csrc/attn_paged.hip: 1.0
+// PFLOP/s with bf16 keys and weights); a tile takes 2.0 us of a CU, half of it matrix instructions and half the vector work
+// of the weights, which the chip does not overlap further at its power limit.
+//
 // What is rounded, and where:
 //   e4m3 keys  the codes go to the fp8 matrix cores as they are, Q as the sum of two e4m3 parts under a power-of-two scale
 //              of the row: q = 2^e (q1 + q2 / 16), exact where q's last bit is not below 2^-13 of 2^e (|q| < 2^8 2^e);
