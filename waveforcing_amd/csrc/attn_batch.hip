@@ -7,7 +7,8 @@
 //   A row without keys is zero.
 //
 // Three kernels: attn_batch_few.hip for up to 64 (row, head) rows of a sequence per key head, for more attn_batch_wide.hip
-// over pages and attn_batch_dense.hip over dense keys; long caches are split over workgroups, and the join below puts the splits' results together in their order.
+// over pages and attn_batch_dense.hip over dense keys; long caches are split over workgroups, and the join below puts the
+// splits' results together in their order.
 #include "attn_batch.hpp"
 #include "gemm_core.hpp"
 

@@ -10,11 +10,15 @@
 // reads.  The 16-byte chunks of a staged row r are permuted by chunk ^= 4 (r % 4) + r / 4 % 4: the reads of K (16 rows
 // at one chunk) and the transposing reads of V (4 rows at 4 chunks) then meet no bank twice.
 //
-// Rounded to bf16: the weights p, relative to the maximum in use, which is taken anew when a lane's weights of a tile
-// reach 2^20 together (bf16 and fp32 keep their relative precision up to there); the row sum adds the rounded weights.
+// A wave's instructions go out in order, so the vector work is put among the products it does not depend on: the weights of a
+// tile's first 32 keys among the scores of the others, theirs among the first half of P V.  A score that passes the
+// maximum in use by more than 2^20 (bf16 and fp32 keep their relative precision up to there) has O follow a new one.
 //
-// 4 x 4680 rows of 12 heads over 256 keys each: 56 us (71 on 256-row tiles, one workgroup to a CU), of which q and the
-// results take 22 at the copy's rate; 64 more keys take 7 us, 0.98 PFLOP/s.
+// Rounded to bf16: the weights p, relative to the maximum in use; the row sum adds the rounded weights.
+//
+// 4 x 4608 rows of 12 heads over 256 keys each: 50 us (71 on 256-row tiles with one workgroup to a CU, 53 without the order
+// above), of which q and the results take 22 at the copy's rate.  Over 8192 keys 0.90 ms = 1.03 PFLOP/s, and 1.35 with
+// zeros for data: long contexts are bound by the chip's power limit.
 #include "attn_batch.hpp"
 #include "gemm_core.hpp"
 
@@ -33,7 +37,7 @@ constexpr int kRowBytes = 2 * D;
 constexpr int kVOff = BKV * kRowBytes;
 constexpr int kStage = 2 * BKV * kRowBytes;
 constexpr int kOutPitch = kRowBytes + 8;
-constexpr float kMostSum = 1048576.f;  // of a lane's 32 weights of a tile
+constexpr float kMost = 20.f;  // log2 of the largest weight before the maximum is taken anew
 static_assert(kWaves * 32 * kOutPitch <= 2 * kStage, "the results are staged in the same LDS");
 
 // (The parameter is __restrict so that the compiler, which tells the DMA's writes from reads only where an access carries
@@ -119,67 +123,91 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
     __syncthreads();
     if (tile + 1 < tiles) fetch(stage ^ kStage);
     const uint8_t* st = lds + stage;
+    const int n = k_hi - k_lo - tile * BKV;  // keys of the tile, if fewer than 64
+    auto read_k = [&](int b, int i) __attribute__((always_inline)) {
+      return __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(st + (k_at ^ (i << 5)) + b * 32 * kRowBytes));
+    };
+    auto read_vt = [&](int k, int db) __attribute__((always_inline)) {  // V^T operand of 16 keys k, values 32 db ..
+      return __builtin_bit_cast(v8bf, __builtin_shufflevector(read_v(st + (v_at ^ (db << 6)) + 16 * k * kRowBytes),
+                                                              read_v(st + (v_at ^ (db << 6 | 32)) + (16 * k + 8) * kRowBytes),
+                                                              0, 1, 2, 3, 4, 5, 6, 7));
+    };
     v16f s[2];
+    v8bf kf[2][8], vf[4][4];
+    uint32_t pw[16];
+    float l_tile = 0.f;
+    // Weights of the keys 32 b + 8 (e / 4) + 4 half + e % 4, values e of s[b]: two of them.
+    auto weight2 = [&](int b, int e) __attribute__((always_inline)) {
+      const v2bf one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+      uint32_t w2 = cvt_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[b][e], a.c, neg_m)), __builtin_amdgcn_exp2f(fmaf(s[b][e + 1], a.c, neg_m)));
+      l_tile = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w2), one, l_tile, false);
+      asm volatile("" : "+v"(w2), "+v"(l_tile));  // stays here, among the products
+      pw[8 * b + e / 2] = w2;
+    };
+    // Whether the maximum in use serves the scores s[b]; if not, O, the sum and (b = 1) the first half's weights follow
+    // the new one.
+    auto follow = [&](int b) __attribute__((always_inline)) {
+      if (n < BKV) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[b][e] = 32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= n ? -INFINITY : s[b][e];
+      }
+      float mt = s[b][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[b][e]);
+      mt *= a.c;
+      if (__ballot(mt + neg_m > kMost || m_use == -INFINITY)) {
+        mt = max32(mt);
+        const bool fire = mt + neg_m > kMost || m_use == -INFINITY;
+        const float m_new = fire ? fmaxf(m_use, mt) : m_use;
+        const float alpha = !fire || m_new == m_use ? 1.f : m_use == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_use - m_new);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= alpha;
+        l_run *= alpha;
+        m_use = m_new;
+        neg_m = m_new == -INFINITY ? 0.f : -m_new;
+        if (b == 1) {
+          l_tile = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) weight2(0, e);
+        }
+      }
+    };
+    auto pv = [&](int k, int db) __attribute__((always_inline)) {
+      const uint4 p = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
+      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[k][db], __builtin_bit_cast(v8bf, p), o[db], 0, 0, 0);
+    };
 #pragma unroll
     for (int b = 0; b < 2; ++b) s[b] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) kf[0][i] = read_k(0, i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const v4i kf = *reinterpret_cast<const v4i*>(st + (k_at ^ (i << 5)) + b * 32 * kRowBytes);
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, kf), qb[i], s[b], 0, 0, 0);
-      }
-    const int n = k_hi - k_lo - tile * BKV;
-    if (n < BKV) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[b][e] = 32 * b + 8 * (e >> 2) + 4 * half + (e & 3) >= n ? -INFINITY : s[b][e];
+    for (int i = 0; i < 8; ++i) {
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[0][i], qb[i], s[0], 0, 0, 0);
+      kf[1][i] = read_k(1, i);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    // The weights against the maximum so far.  Whether it still serves shows in their sum: a weight past the limit makes
-    // the sum reach it, and then (as before the first key) the exact maximum is taken and the weights are computed again.
-    uint32_t pw[16];
-    float l_tile;
-    auto weights = [&]() __attribute__((always_inline)) {
-      l_tile = 0.f;
+    follow(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const v2bf one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
-        pw[e] = cvt_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[e >> 3][2 * (e & 7)], a.c, neg_m)),
-                           __builtin_amdgcn_exp2f(fmaf(s[e >> 3][2 * (e & 7) + 1], a.c, neg_m)));
-        l_tile = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pw[e]), one, l_tile, false);
-      }
-    };
-    weights();
-    if (__ballot(l_tile > kMostSum || m_use == -INFINITY)) {
-      float mt = -INFINITY;
+    for (int i = 0; i < 8; ++i) {
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[1][i], qb[i], s[1], 0, 0, 0);
+      vf[i >> 2][i & 3] = read_vt(i >> 2, i & 3);
+      weight2(0, 2 * i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    follow(1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[b][e] * a.c);
-      mt = max32(mt);
-      const bool fire = max32(l_tile) > kMostSum || m_use == -INFINITY;
-      const float m_new = fire ? fmaxf(m_use, mt) : m_use;
-      const float alpha = !fire || m_new == m_use ? 1.f : m_use == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_use - m_new);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] *= alpha;
-      l_run *= alpha;
-      m_use = m_new;
-      neg_m = m_new == -INFINITY ? 0.f : -m_new;
-      weights();
+    for (int i = 0; i < 8; ++i) {
+      pv(i >> 2, i & 3);
+      vf[2 + (i >> 2)][i & 3] = read_vt(2 + (i >> 2), i & 3);
+      weight2(1, 2 * i);
+      __builtin_amdgcn_sched_barrier(0);
     }
     l_run += l_tile;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint4 p = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
-#pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        const uint8_t* v0 = st + (v_at ^ (db << 6)) + 16 * k * kRowBytes;
-        const uint8_t* v1 = st + (v_at ^ (db << 6 | 32)) + (16 * k + 8) * kRowBytes;
-        const v8bf vf = __builtin_bit_cast(v8bf, __builtin_shufflevector(read_v(v0), read_v(v1), 0, 1, 2, 3, 4, 5, 6, 7));
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, __builtin_bit_cast(v8bf, p), o[db], 0, 0, 0);
-      }
-    }
+    for (int i = 0; i < 8; ++i) pv(2 + (i >> 2), i & 3);
   }
 
   // the rows' results: through LDS as bf16 rows, every wave its own, or, with several splits, in fp32 to the workspace
