@@ -121,7 +121,10 @@ Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, 
     // of 8192 keys: 64 as 4, 147 as one, 68 as 16).  Where the tiles fill the chip, pieces of some 2048 keys, so that a
     // few long sequences do not outlast the rest (512 tiles of 1 to 8192 keys: 138 us, 159 as one; where all are as
     // long, 220 and 214).
-    p.n_splits = std::max((max_kv + 2047) / 2048, std::min(2 * cus / units, (max_kv + 255) / 256));
+    // (The tiles that there are, where sequences differ: half a tile of each is taken to be empty.)
+    const int64_t some = std::min(n_seqs, n_rows), likely = ((n_rows * group) >> p.tile_shift) + n_seqs / 2;
+    const int64_t tiles = std::max<int64_t>(1, std::min(full, std::max(some, likely))) * n_kv_heads;
+    p.n_splits = std::max((max_kv + 2047) / 2048, std::min(2 * cus / tiles, (max_kv + 255) / 256));
     p.n_splits = std::min<int64_t>(std::max<int64_t>(1, p.n_splits), kJoinSplits);
   }
   p.split_keys = std::max<int64_t>(128, ((max_kv + p.n_splits - 1) / p.n_splits + 127) / 128 * 128);
