@@ -36,7 +36,7 @@ constexpr int kRun = 8;  // neighbouring row tiles that one XCD takes, which rea
 constexpr int kRowBytes = 2 * D;
 constexpr int kVOff = BKV * kRowBytes;
 constexpr int kStage = 2 * BKV * kRowBytes;
-constexpr int kOutPitch = kRowBytes + 8;
+constexpr int kOutPitch = kRowBytes + 16;
 constexpr float kMost = 20.f;  // log2 of the largest weight before the maximum is taken anew
 static_assert(kWaves * 32 * kOutPitch <= 2 * kStage, "the results are staged in the same LDS");
 
@@ -234,14 +234,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
       *reinterpret_cast<uint2*>(ow + l32 * kOutPitch + 64 * db + 16 * g + 8 * half) =
           make_uint2(cvt_bf16x2(o[db][4 * g] * inv, o[db][4 * g + 1] * inv), cvt_bf16x2(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv));
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int row = 2 * i + half;
-    const uint2 v = *reinterpret_cast<const uint2*>(ow + row * kOutPitch + 8 * l32);
+  for (int i = 0; i < 8; ++i) {
+    typedef u32x4 __attribute__((aligned(8))) u32x4_at8;  // (out and its rows are 8-byte aligned)
+    const int row = 4 * i + (lane >> 4);
+    const u32x4 v = *reinterpret_cast<const u32x4*>(ow + row * kOutPitch + 16 * l16);
     if (my_first + row < t.count) {
       uint32_t qj, gj;
       a.group_div.divmod(static_cast<uint32_t>(my_first + row), qj, gj);
-      *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(t.row0 + static_cast<int>(qj)) * a.ldo +
-                                (head * a.group + static_cast<int>(gj)) * D + 4 * l32) = v;
+      *reinterpret_cast<u32x4_at8*>(a.out + static_cast<int64_t>(t.row0 + static_cast<int>(qj)) * a.ldo +
+                                    (head * a.group + static_cast<int>(gj)) * D + 8 * l16) = v;
     }
   }
 }
