@@ -175,3 +175,27 @@ def test_oracle_quantization_is_half_a_step(fmt, half):
     top = x.double().abs().amax(-1, keepdim=True)
     lim = half * top * (1 + 2.0 ** -15) if fmt == "int8" else (half + 2.0 ** -8) * x.double().abs() + s.double()[..., None] * 2.0 ** -10
     assert bool((err <= lim).all())
+
+
+def workspace(*sizes):
+    import ctypes
+
+    n = ctypes.c_int64(-1)
+    _lib.call("wf_attn_batch_workspace", *sizes, ctypes.addressof(n))
+    return n.value
+
+
+def test_workspace_query():
+    """No scratch where nothing is split; a single long sequence takes some, of whole (row, split) records."""
+    assert workspace(0, 8, 8, 0, 0, 0) == 0 and workspace(64, 8, 8, 64, 1, 100) == 0
+    one = workspace(1, 12, 12, 1, 1, 30000)
+    assert one > 0 and one % (130 * 4) == 0
+    for sizes in ((1 << 62, 1, 1, 1, 1, 1), (1 << 20, 1 << 20, 1, 1, 1, 1), (1, 1, 1, 1 << 40, 1, 1), (1, 1, 1, 1, 1, 1 << 40)):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            workspace(*sizes)
+    assert workspace(1, 1, 1, 1, 1 << 62, 1) == 0    # a bound of the rows past the rows is the rows
+    for sizes in ((-1, 1, 1, 1, 1, 1), (1, 0, 1, 1, 1, 1), (1, 1, 1, -1, 1, 1), (1, 1, 1, 1, 1, -1)):
+        with pytest.raises(RuntimeError, match="negative or zero"):
+            workspace(*sizes)
+    with pytest.raises(RuntimeError, match="group"):
+        workspace(1, 3, 2, 1, 1, 1)
