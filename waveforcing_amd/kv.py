@@ -416,18 +416,21 @@ class PagedBatch:
         A batch whose ``new_lens`` are its ``kv_lens`` reads the whole caches.  Given outputs may have more rows
         (left as they are) and a row stride of their own."""
         pool = self.pool
-        outs = []
-        for name, t in (("out_k", out_k), ("out_v", out_v)):
-            if name == "out_v" and not with_v:
-                outs.append(None)
-                continue
+        fresh = None   # a new output, which needs none of the checks of a given one
+
+        def output(name, t):
+            nonlocal fresh
             if t is None:
-                t = torch.empty((self.n_new, pool.n_heads, pool.head_dim), dtype=torch.bfloat16, device=self.device)
+                t = fresh = (torch.empty((self.n_new, pool.n_heads, pool.head_dim), dtype=torch.bfloat16, device=self.device)
+                             if fresh is None else torch.empty_like(fresh))
+                return t, t.data_ptr(), pool.n_heads * pool.head_dim
             at, addr, ld = self._rows(t, name)
             if at is not t:
                 raise ValueError(f"{name} must have dense heads, 16-byte alignment and a row stride that 8 divides")
-            outs.append((t, addr, ld))
-        (k, kp, ld), v = outs
+            return t, addr, ld
+
+        k, kp, ld = output("out_k", out_k)
+        v = output("out_v", out_v) if with_v else None
         if v is not None and v[2] != ld:
             raise ValueError(f"out_k and out_v have different row strides ({ld} and {v[2]})")
         _lib.call_on(self.device, "wf_kv_batch_gather", pool._k_codes_p, pool._v_codes_p, pool._k_scales_p,
