@@ -9,7 +9,7 @@
 //
 // 3 x 4680 rows over up to 37440 keys of 12 heads: 2.18 ms, 0.98 PFLOP/s (one sequence at a time, csrc/attn_paged.hip: 1.0
 // PFLOP/s with bf16 keys and weights); a tile takes 2.0 us of a CU, half of it matrix instructions and half the vector work
-// of the weights, which the chip does not overlap further at its power limit.
+// of the weights (1.06 PFLOP/s on zeros, 0.97 on N(0, 1) data over 18720 keys: instructions first, power close behind).
 //
 // What is rounded, and where:
 //   e4m3 keys  the codes go to the fp8 matrix cores as they are, Q as the sum of two e4m3 parts under a power-of-two scale
