@@ -583,3 +583,19 @@ def test_captured_chunks_follow_the_device_lengths():
         for i, j in zip(new, text):
             check(y[a:a + i], *ob.attend(x[a:a + i], k[c:c + j], v[c:c + j], [j] * i, SCALE))
             a, c = a + i, c + j
+
+
+@pytest.mark.parametrize("new", [1, 20, 140])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "dense"])
+def test_a_scale_of_zero_is_the_mean(fmt, new):
+    """softmax_scale 0 weighs every key a row sees alike, also in tiles that end behind the last one."""
+    if fmt == "dense":
+        g = gen(220)
+        q, k, v = rows(new, 4, g), rows(70, 2, g), rows(70, 2, g)
+        out = backend.attn_cross_batch(q, k, v, CrossBatch([new], [70], DEV), softmax_scale=0.0)
+        check(out, *ob.attend(q, k, v, [70] * new, 0.0))
+        return
+    pool, batch, g = make(fmt, 2, 48, [new + 70], [new], 221)
+    q = rows(new, 4, g)
+    for block in (0, 1):
+        check_paged(backend.attn_paged_batch(q, batch, block=block, softmax_scale=0.0), q, pool, batch, fmt, block, scale=0.0)

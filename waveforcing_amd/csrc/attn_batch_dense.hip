@@ -117,6 +117,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
   float neg_m = 0.f;
   float l_run = 0.f;        // this half's row sum
 
+  const float c = fmaxf(a.c, 1.2e-38f);  // not zero, so that a hidden key's -inf stays one
   int stage = 0;
   for (int tile = 0; tile < tiles; ++tile, stage ^= kStage) {
     gemm::wait_counts<0, 15>();  // this wave's part of the tile is there; behind the barrier all of it, and nobody reads the other stage
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
     // Weights of the keys 32 b + 8 (e / 4) + 4 half + e % 4, values e of s[b]: two of them.
     auto weight2 = [&](int b, int e) __attribute__((always_inline)) {
       const v2bf one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
-      uint32_t w2 = cvt_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[b][e], a.c, neg_m)), __builtin_amdgcn_exp2f(fmaf(s[b][e + 1], a.c, neg_m)));
+      uint32_t w2 = cvt_bf16x2(__builtin_amdgcn_exp2f(fmaf(s[b][e], c, neg_m)), __builtin_amdgcn_exp2f(fmaf(s[b][e + 1], c, neg_m)));
       l_tile = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w2), one, l_tile, false);
       asm volatile("" : "+v"(w2), "+v"(l_tile));  // stays here, among the products
       pw[8 * b + e / 2] = w2;
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
       float mt = s[b][0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[b][e]);
-      mt *= a.c;
+      mt *= c;
       if (__ballot(mt + neg_m > kMost || m_use == -INFINITY)) {
         mt = max32(mt);
         const bool fire = mt + neg_m > kMost || m_use == -INFINITY;
