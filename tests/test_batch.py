@@ -199,3 +199,13 @@ def test_workspace_query():
             workspace(*sizes)
     with pytest.raises(RuntimeError, match="group"):
         workspace(1, 3, 2, 1, 1, 1)
+
+
+def test_one_long_sequence_does_not_split_the_many_short_ones_finely():
+    """The pieces of a sequence shrink in number as the other sequences' surplus ones grow."""
+    record = 16 * 130 * 4 * 8                          # a split of a tile of 16 rows of each of 8 key heads
+    pieces = [workspace(n, 40, 8, n, 1, 131072) // record // (n * 5 // 16 + n) for n in (1, 64, 256, 1024)]
+    assert pieces == sorted(pieces, reverse=True) and pieces[0] == 64 and 1 < pieces[-1] <= 8
+    with pytest.raises(RuntimeError, match="too many"):   # a grid of 2^32 threads
+        _lib.call("wf_attn_cross_batch", 16, 1 << 19, 512, 512, 128, 512 * 128, 16, 16, 1, 512 * 128, 16, 16, 1 << 19, 1, 1,
+                  1.0, 16, 512 * 128, 16, 1 << 40, None)

@@ -120,11 +120,14 @@ Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, 
     // tiles alone are fewer, of 256 keys at least (12 tiles of 8192 keys: 20 us as 32 pieces each, 121 as one; 128 tiles
     // of 8192 keys: 64 as 4, 147 as one, 68 as 16).  Where the tiles fill the chip, pieces of some 2048 keys, so that a
     // few long sequences do not outlast the rest (512 tiles of 1 to 8192 keys: 138 us, 159 as one; where all are as
-    // long, 220 and 214).
+    // long, 220 and 214).  One long sequence among many short ones has each of them send as many workgroups that find
+    // nothing to do, at some 3 ns each, against 12 ns for a key of the longest piece: at most the square root of 4 max_kv /
+    // tiles pieces (256 sequences of 512 keys, one of 131072, 8 heads: 318 us as 16 pieces, 541 as 64, 484 as 4).
     // (The tiles that there are, where sequences differ: half a tile of each is taken to be empty.)
     const int64_t some = std::min(n_seqs, n_rows), likely = ((n_rows * group) >> p.tile_shift) + n_seqs / 2;
     const int64_t tiles = std::max<int64_t>(1, std::min(full, std::max(some, likely))) * n_kv_heads;
-    p.n_splits = std::max((max_kv + 2047) / 2048, std::min(2 * cus / tiles, (max_kv + 255) / 256));
+    const int64_t even = std::llround(std::sqrt(4.0 * static_cast<double>(max_kv) / static_cast<double>(tiles)));
+    p.n_splits = std::max(std::min((max_kv + 2047) / 2048, even), std::min(2 * cus / tiles, (max_kv + 255) / 256));
     p.n_splits = std::min<int64_t>(std::max<int64_t>(1, p.n_splits), kJoinSplits);
   }
   p.split_keys = std::max<int64_t>(128, ((max_kv + p.n_splits - 1) / p.n_splits + 127) / 128 * 128);
@@ -163,7 +166,9 @@ int common_args(const char* fn, Args& a, const void* q, int64_t n_rows, int32_t 
 int launch(const char* fn, Args& a, int src, int64_t n_seqs, int64_t max_new, int64_t max_kv, void* ws, int64_t ws_bytes,
            hipStream_t stream) {
   const Plan p = make_plan(src == SRC_DENSE, a.n_rows, static_cast<int64_t>(a.n_kv_heads) * a.group, a.n_kv_heads, n_seqs, max_new, max_kv);
-  WF_REQUIRE(product_below({p.n_tiles, a.n_kv_heads, p.n_splits, 16}, 1ll << 31), WF_E_SHAPE,
+  // (a grid holds fewer than 2^32 threads: 512 or fewer of each item, rounded up to 64 items; 16 x 256 where rows are joined)
+  WF_REQUIRE(product_below({p.n_tiles + 64, a.n_kv_heads, p.n_splits, 512}, 1ll << 32) &&
+                 (p.n_splits == 1 || product_below({p.n_tiles, a.n_kv_heads, 16 * 256}, 1ll << 32)), WF_E_SHAPE,
              "%s: %lld row tiles x %d key heads x %lld splits are too many", fn, (long long)p.n_tiles, a.n_kv_heads,
              (long long)p.n_splits);
   WF_REQUIRE(a.ldkv < (1 << 23) && a.n_kv_heads < (1 << 16), WF_E_SHAPE, "%s: key rows of %lld elements or %d heads", fn,
