@@ -430,9 +430,9 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads,
  * infinity is NaN, and so are the rows that see a key whose scale is none; no
  * NaN or infinity of a key reaches a row that does not see it.  fp32 scores,
  * softmax and sums.  Up to 64 (row, head) rows of a sequence per key head the
- * weights p_j s_v[j] are held in 16 significant bits; with more, p_j in fp16
- * and V as fp16(V 2^-E), E set by the largest scale of V among the keys that
- * the row's tile of 256 reads (values below 2^-29 of the largest lose bits).
+ * weights p_j s_v[j] are held in 16 significant bits; with more, in 11 (fp16:
+ * those below 2^-20 of the largest that the row sees lose bits, and so do all
+ * where the scales of V are below 2^-100).
  * max_new and max_kv
  * bound the sequences' rows and keys; they choose the split, and results
  * stay right where the device's lengths pass them.  ws: ws_bytes of scratch,

@@ -58,10 +58,11 @@ def attend(q, k, v, limits, scale):
     2^10 tiles' roundings).  The quotient of two sums doubles e.  The result is rounded to bf16 once: 2^-8.
 
     Two absolute terms come with fp16 (many rows), whose numbers are 2^-24 apart below 2^-14, half a step 2^-25.  A
-    weight is held as 64 times its ratio to a maximum that the row's largest weight reaches, so it is off by at most
-    2^-25 / 64 = 2^-31 of that largest weight: together 2^-31 w_max sum_j |v_j| over the seen keys.  A value is held
-    as V 2^-E with 2^E at most a quarter of the largest scale of V, which is at most max|V| / 127: it is off by at most
-    2^-25 2^E <= 2^-27 max|V| / 127 < 2^-33 max|V|, and so is their weighted mean.
+    weight times its key's scale of V is held as 64 times its ratio to the largest such product M that the row has
+    seen, or more, so it is off by at most 2^-25 / 64 = 2^-31 of M, and multiplies an exact code.  For keys whose scale
+    is not below that of M's key these errors are together at most 2^-31 w_max sum_j |v_j| over the seen keys.  Of a key
+    of smaller scale the error is at most 2^-31 M |code| <= 2^-31 w_max max|V|, of either sign; 2^-33 max|V| is allowed
+    for the mean of them, which a quarter of such a key reaches at the worst and hundreds of ordinary ones do not.
     """
     q, k, v = q.double(), k.double(), v.double()
     n, heads, _ = q.shape

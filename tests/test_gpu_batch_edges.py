@@ -1,0 +1,90 @@
+"""Batched attention where values, lengths and bounds are far from the ordinary: the contract's edges, on the GPU, against
+64 bits (oracle/batch.py)."""
+
+import pytest
+import torch
+
+from oracle import batch as ob
+from test_gpu_batch import DEV, SCALE, cached, check, make, rows, same
+from waveforcing_amd import backend
+from waveforcing_amd.kv import PagedBatch
+
+pytestmark = pytest.mark.gpu
+
+
+def attend_quietly(q, k, v, loud, limits):
+    """The exact output, and the bound that it has without the loud keys' values: their weights are below 2^-100 here, so
+    neither they nor their roundings reach a result."""
+    ref, _ = ob.attend(q, k, v, limits, SCALE)
+    quiet = v.clone()
+    quiet[loud] = 0
+    return ref, ob.attend(q, k, quiet, limits, SCALE)[1]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("ratio", [18, 22, 26, 40, 70])
+@pytest.mark.parametrize("new", [9, 100, 300])
+def test_quiet_values_among_loud_ones_keep_their_bits(fmt, ratio, new):
+    """Rows whose weight is on keys with V 2^ratio below that of other keys of the same tile."""
+    t = new + 150
+    pool, batch, g = make(fmt, 2, 48, [t], [new], 300)
+    at = torch.arange(t, device=DEV)
+    loud = at % 5 == 3
+    page = torch.tensor(batch.pages[0], device=DEV)[at // 48]
+    k = rows(t, 2, g, 0.1)
+    k[:, :, 0] = torch.where(loud, -400.0, 400.0)[:, None].bfloat16()   # scores of both kinds 2^150 apart in weight
+    pool.k_codes[page, at % 48], pool.k_scales[page, :, at % 48] = ob.quantize(k, fmt)
+    pool.v_scales[page, :, at % 48] *= torch.where(loud, 2.0 ** 14, 2.0 ** (14 - ratio))[:, None]
+    q = rows(new, 4, g, 0.1)
+    q[:, :, 0] = 1.5
+    k, v = (cached(pool, batch, fmt, 0, name) for name in "kv")
+    for block in (0, 1):
+        limits = [ob.limit(t - new + i, t, block) for i in range(new)]
+        check(backend.attn_paged_batch(q, batch, block=block), *attend_quietly(q, k, v, loud, limits))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("new", [9, 100, 300])
+def test_hidden_values_do_not_move_a_bit(fmt, new):
+    """Finite values behind a row's limit, 2^10 to 2^100 above those it sees."""
+    pool, batch, g = make(fmt, 2, 64, [new + 37], [new], 310)
+    q = rows(new, 4, g)
+    clean = backend.attn_paged_batch(q, batch, block=1)
+    p = new + 36
+    page, at = batch.pages[0][p // 64], p % 64
+    for e in (10, 30, 100):
+        pool.v_scales[page, :, at] = 2.0 ** e
+        pool.k_scales[page, :, at] = 2.0
+        out = backend.attn_paged_batch(q, batch, block=1)
+        same(out[:-1], clean[:-1])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("new", [9, 100])
+@pytest.mark.parametrize("scale", [1e-8, 2.0 ** -60, 2.0 ** 40])
+def test_values_behind_a_tile_of_zeros(fmt, new, scale):
+    """The first keys' pages are none (zero K and V); the others' scales of V are small, or large."""
+    t = 128 + new + 20
+    pool, batch, g = make(fmt, 2, 64, [t], [new], 320)
+    batch.tables[0, :2] = -1
+    pool.v_scales.copy_(scale * (1 + torch.rand(pool.v_scales.shape, generator=g, device=DEV)).bfloat16())
+    q = rows(new, 4, g)
+    k, v = (cached(pool, batch, fmt, 0, name) for name in "kv")
+    k[:128], v[:128] = 0, 0
+    limits = [t - new + i + 1 for i in range(new)]
+    check(backend.attn_paged_batch(q, batch, block=1), *ob.attend(q, k, v, limits, SCALE))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("new, t", [(9, 300), (100, 300), (100, 9001)])
+@pytest.mark.parametrize("first, then", [(-75, 60), (60, -75), (-70, 100), (0, -126)])
+def test_keys_of_any_scale_count_alike(fmt, new, t, first, then):
+    """Equal scores: every seen key counts once, whatever its scale of V, and a negative one turns its value's sign."""
+    pool, batch, g = make(fmt, 2, 64, [t], [new], 380)
+    at = torch.arange(t, device=DEV)
+    page = torch.tensor(batch.pages[0], device=DEV)[at // 64]
+    e = torch.where(at < t // 2, 2.0 ** first, 2.0 ** then) * torch.where(at % 7 == 2, -0.01, 0.01)
+    pool.v_scales[page, :, at % 64] = e[:, None]
+    q = torch.zeros((new, 4, 128), dtype=torch.bfloat16, device=DEV)
+    k, v = (cached(pool, batch, fmt, 0, name) for name in "kv")
+    check(backend.attn_paged_batch(q, batch, block=1), *ob.attend(q, k, v, [t - new + i + 1 for i in range(new)], SCALE))

@@ -54,7 +54,8 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   float g[kJoinSplits / 16], sum = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < kJoinSplits / 16; ++i) {
-    g[i] = ml[i].x == -INFINITY ? 0.f : ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - top);
+    const float e = __builtin_amdgcn_exp2f(0.5f * (ml[i].x - top));  // (twice: a sum may be large where its maximum is far below)
+    g[i] = ml[i].x == -INFINITY ? 0.f : ml[i].y * e * e;
     sum += g[i];
   }
 #pragma unroll

@@ -17,13 +17,14 @@
 //              the product is that of the codes with Q in fp32, and s_k c multiplies the score in fp32.  Staging K costs
 //              no conversion and half the LDS.
 //   int8 keys  the codes are exact in bf16, as Q is.
-//   V          fp16(code s_v 2^-E), 11 significant bits, E a power of two of the workgroup's keys so far: staged values
-//              stay below 2^16, and a tile whose scales pass the limit raises E first, rescales O and is staged again
-//              (a power of two moves no bit of them; values below 2^-29 of the largest lose their last ones).
-//   weights    fp16(64 p), p <= 2^kTau: eight times finer than bf16, down to 2^-31 of the row's largest; the row sum
-//              adds the rounded weights.
-// A NaN or infinite scale makes the key's score NaN and its V zero, so the rows that see the key become NaN and no
-// others; in tiles that some row does not see whole, so does a NaN code of V.
+//   V          the codes are exact in fp16.
+//   weights    fp16(p s_v), the product in fp32: 11 significant bits, eight times finer than bf16.  p is relative to a reference
+//              of the row, set by the p s_v of the keys that it sees: the largest so far is between 2^6 and 2^15, so bits are
+//              lost below 2^-20 of it, 2^-31 of it at most.  (The scale in V instead, under an exponent that the tile shares,
+//              saves an instruction a score, but there a key that a row does not see, or gives no weight, takes the bits of
+//              those that it does.)  The row sum adds the p in fp32.
+// A NaN or infinite scale of V makes the key's score NaN and its weight of V zero, so the rows that see the key become NaN
+// and no others; in tiles that some row does not see whole, so does a NaN code of V.
 #include <utility>
 
 #include "attn_batch.hpp"
@@ -41,6 +42,12 @@ constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int R = 32 * kWaves;
 constexpr int kXcds = 8;
+// A row's weights p are relative to a reference, set so that the largest p s_v it had seen was 2^kShift; they may grow by
+// 2^kGrow before a new one is taken (fp16 ends at 2^16).  A scale of V below 2^kFloor counts as that in the reference, so
+// that the p stay below 2^(kShift + kGrow - kFloor) and their sums in fp32.
+constexpr float kShift = 6.f, kGrow = 9.f, kFloor = -80.f;
+constexpr _Float16 kMost = 32768.f;
+constexpr float kMostSum = 0x1p95f;
 constexpr int kRun = 2;  // neighbouring row tiles that one XCD takes, which read the same keys (1: 0.7 % slower, 4: 2.5 %)
 static_assert(kThreads == BKV * 8, "one thread per key and 16 values of its row");
 
@@ -50,31 +57,29 @@ struct Lds {
   static constexpr int k_pitch = codes ? D + 16 : 2 * D + 16;
   static constexpr int v_pitch = 2 * D + 64;
   static constexpr int v_off = BKV * k_pitch;
-  static constexpr int u_off = v_off + BKV * v_pitch;         // u [64]
-  static constexpr int stage = u_off + BKV * 4;
+  static constexpr int u_off = v_off + BKV * v_pitch;         // factor of the scores u [64], scale of V [64]
+  static constexpr int stage = u_off + 2 * BKV * 4;
   static constexpr int o_pitch = 2 * D + 8;
   static constexpr int out = kWaves * 32 * o_pitch;
   static constexpr int bytes = 3 * stage;
   static_assert(bytes >= out, "the results are staged in the same LDS");
 };
 
-__device__ inline uint32_t pk_mul_f16(uint32_t a, v2h f) {
-  return __builtin_bit_cast(uint32_t, static_cast<v2h>(__builtin_bit_cast(v2h, a) * f));
-}
-
-// 4 codes as 4 fp16 (exact).
+// 4 codes as 4 fp16 (exact), negated if `neg`.
 template <int SRC>
-__device__ inline uint2 codes_f16(uint32_t w) {
+__device__ inline uint2 codes_f16(uint32_t w, bool neg) {
   if constexpr (SRC == SRC_E4M3) {
+    w ^= neg ? 0x80808080u : 0u;
     return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)));
   } else {
     // code + 128 as the last byte of 1024 + it, less 1152
     const uint32_t x = w ^ 0x80808080u;
-    const v2h k = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    const _Float16 s1 = static_cast<_Float16>(neg ? -1.0f : 1.0f), k1 = static_cast<_Float16>(neg ? 1152.0f : -1152.0f);
+    const v2h s = {s1, s1}, k = {k1, k1};
     const uint32_t lo = __builtin_amdgcn_perm(x, 0x64646464u, 0x00050004u), hi = __builtin_amdgcn_perm(x, 0x64646464u, 0x00070006u);
-    return make_uint2(__builtin_bit_cast(uint32_t, static_cast<v2h>(__builtin_bit_cast(v2h, lo) + k)),
-                      __builtin_bit_cast(uint32_t, static_cast<v2h>(__builtin_bit_cast(v2h, hi) + k)));
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2h, lo), s, k)),
+                      __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2h, hi), s, k)));
   }
 }
 
@@ -137,8 +142,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   const int skey = tid >> 3, schunk = tid & 7;
   struct Staged {
     u32x4 k0, v0;
-    float sk, sv;   // the key's scales
-    float sv_lane;  // the scale of V of key `lane` of the tile: every wave sees all 64
+    float sk, sv;  // the key's scales
   };
   Staged sreg;
   // Where a tile's keys live (uniform): the first key's row of K and its scale, those of V at the same distance from
@@ -175,15 +179,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   Cursor ahead{};
   const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(key_bytes) + 16 * schunk;  // rows of a tile stay below 2^31 bytes (checked on the host)
   constexpr int kWord3 = 0x00020000;  // raw buffer, 32-bit data format
-  // SMALL: the pages of this lane's keys (skey and lane) in the tile that is loaded next (-1: none), asked for a tile ahead
-  int page_key = -1, page_lane = -1;
-  auto find_page = [&](int j) __attribute__((always_inline)) {
-    const int lp = static_cast<int>(a.geom.page.div(static_cast<uint32_t>(j)));
-    return j < k_hi && lp < a.geom.ld_table ? table[lp] : -1;
-  };
-  auto find_pages = [&](int tile) __attribute__((always_inline)) {
-    page_key = find_page(tile * BKV + skey);
-    page_lane = find_page(tile * BKV + lane);
+  // SMALL: the page of this lane's key in the tile that is loaded next (-1: none), asked for a tile ahead
+  int page_key = -1;
+  auto find_page = [&](int tile) __attribute__((always_inline)) {
+    const int j = tile * BKV + skey, lp = static_cast<int>(a.geom.page.div(static_cast<uint32_t>(j)));
+    page_key = j < k_hi && lp < a.geom.ld_table ? table[lp] : -1;
   };
   // The loads of a tile.  Within one page (ONE) a buffer of the tile's rows that are there reads the others as zero, and
   // a lane's offset never changes.
@@ -197,19 +197,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(c.sk), 0, 4 * m, kWord3);
       const auto sv = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(c.sk) + sk_to_sv), 0, 4 * m, kWord3);
-      x.sv_lane = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * lane, 0, 0));
       x.sk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * skey, 0, 0));
       x.sv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * skey, 0, 0));
       x.k0 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row, 0, 0);
       x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
     } else {
-      if constexpr (!SMALL) find_pages(tile);
-      const uint32_t jk = static_cast<uint32_t>(tile * BKV + skey), jl = static_cast<uint32_t>(tile * BKV + lane);
+      if constexpr (!SMALL) find_page(tile);
+      const uint32_t jk = static_cast<uint32_t>(tile * BKV + skey);
       const u32x4 zero = {0, 0, 0, 0};
       x.k0 = x.v0 = zero;
-      x.sk = x.sv = x.sv_lane = 0.f;
-      if (page_lane >= 0 && page_lane < a.geom.pool_pages)
-        x.sv_lane = a.v_scales[(page_lane * a.n_kv_heads + head) * pt + static_cast<int>(jl - a.geom.page.div(jl) * a.geom.page.d)];
+      x.sk = x.sv = 0.f;
       if (page_key >= 0 && page_key < a.geom.pool_pages) {
         const int at = static_cast<int>(jk - a.geom.page.div(jk) * a.geom.page.d);
         const int64_t off = static_cast<int64_t>((page_key * pt + at) * a.n_kv_heads + head) * D + 16 * schunk;
@@ -222,26 +219,13 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     }
   };
 
-  int ev = 0;            // E: staged V = V 2^-E
-  float sv_lim = 0.f;    // the largest scale of V that E allows: 448 2^7 < 65504
-  // The largest scale of V of a tile (those that are none do not take part), the same in every wave.
-  auto tile_top = [&](float sv_lane) __attribute__((always_inline)) {
-    float v = finite(sv_lane) ? sv_lane : 0.f;
-    for (int off = 32; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
-    return v;
-  };
-  auto set_exponent = [&](float top) __attribute__((always_inline)) {  // puts the scale `top` below 2^3
-    ev = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top) - 3);
-    sv_lim = __builtin_ldexpf(1.f, ev + 7);
-  };
-
   struct Ready {
     uint4 k0, k1, v0, v1;
-    float u;
+    float u, sv;
   };
   // The staged tile as it goes to LDS.  PARTIAL: some row may not see all of it.
   auto convert = [&](Staged x, Ready& y, auto PARTIAL) __attribute__((always_inline)) {
-    bool poison = !finite(x.sv);
+    bool poison = !finite(x.sv);  // the score is NaN for the rows that see the key, the weight of V zero for the others
     if constexpr (SRC == SRC_E4M3 && decltype(PARTIAL)::value) {
       const bool nan = has_nan_code(x.v0[0]) || has_nan_code(x.v0[1]) || has_nan_code(x.v0[2]) || has_nan_code(x.v0[3]);
       const uint64_t any = __ballot(nan);
@@ -250,8 +234,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       poison = poison || (any >> (lane & 56) & 0xffu);
     }
     y.u = poison ? bits_f32(0x7fc00000u) : x.sk * a.c;
-    const float f = __builtin_ldexpf(poison ? 0.f : x.sv, -ev);
-    const v2h ff = {static_cast<_Float16>(f), static_cast<_Float16>(f)};
+    y.sv = poison ? 0.f : fabsf(x.sv);
+    const bool neg = x.sv < 0.f;
     if constexpr (kCodes) {
       y.k0 = make_uint4(x.k0[0], x.k0[1], x.k0[2], x.k0[3]);
     } else {
@@ -259,9 +243,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       y.k0 = make_uint4(p.x, p.y, q.x, q.y);
       y.k1 = make_uint4(s.x, s.y, v.x, v.y);
     }
-    const uint2 p = codes_f16<SRC>(x.v0[0]), q = codes_f16<SRC>(x.v0[1]), s = codes_f16<SRC>(x.v0[2]), v = codes_f16<SRC>(x.v0[3]);
-    y.v0 = make_uint4(pk_mul_f16(p.x, ff), pk_mul_f16(p.y, ff), pk_mul_f16(q.x, ff), pk_mul_f16(q.y, ff));
-    y.v1 = make_uint4(pk_mul_f16(s.x, ff), pk_mul_f16(s.y, ff), pk_mul_f16(v.x, ff), pk_mul_f16(v.y, ff));
+    const uint2 p = codes_f16<SRC>(x.v0[0], neg), q = codes_f16<SRC>(x.v0[1], neg), s = codes_f16<SRC>(x.v0[2], neg), v = codes_f16<SRC>(x.v0[3], neg);
+    y.v0 = make_uint4(p.x, p.y, q.x, q.y);
+    y.v1 = make_uint4(s.x, s.y, v.x, v.y);
   };
   auto write = [&](int stage, const Ready& y) __attribute__((always_inline)) {
     uint8_t* st = lds + stage;
@@ -276,7 +260,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     dv[0] = y.v0;
     dv[1] = y.v1;
     float* u = reinterpret_cast<float*>(st + L::u_off);
-    u[skey] = y.u;  // (the lanes of one key write the same word)
+    u[skey] = y.u;  // (the lanes of one key write the same words)
+    u[BKV + skey] = y.sv;
   };
 
   // ---- Q, the second operand of the scores, for the whole kernel
@@ -326,22 +311,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   for (int i = 0; i < 4; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   float m_use = -INFINITY;  // the row's maximum in the exponents, log2 units
   float l_run = 0.f;        // this half's row sum
-  // Weights are 2^kShift p, and a tile's sum of them (of a lane's 32 keys) at most kMostSum: fp16 ends at 65504.
-  constexpr float kShift = 6.f;
-  constexpr float kMostSum = 32768.f;
   float neg_m = kShift;
-
-  // Raising E before tile t + 1 is staged (its scales came with the loads of the last iteration) leaves V of tile t under
-  // the old one: O is rescaled after its product with t, in the next two products(), at the next change of a maximum
-  // (one place that rescales keeps O in its registers).
-  float o_scale = 1.f, pend = 1.f, pend_next = 1.f;
-  auto check_exponent = [&]() __attribute__((always_inline)) {
-    if (__ballot(sreg.sv_lane > sv_lim && finite(sreg.sv_lane))) {
-      const int e_old = ev;
-      set_exponent(tile_top(sreg.sv_lane));
-      pend_next *= __builtin_ldexpf(1.f, max(e_old - ev, -200));
-    }
-  };
 
   // Stages (bytes in LDS) of the tiles t - 1, t and t + 1.
   int st_prev = 0, st_cur = L::stage, st_next = 2 * L::stage;
@@ -374,20 +344,17 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // The matrix half of tile t: O += the tile before (steps 0 and 1 of its V have been asked for), the scores of t, and
   // among the products the staging of tile t + 1 and the loads of t + 2.  PARTIAL: some row may not see all of t + 1, the
   // wave may see none of t, or the tile to be loaded may span pages; without it the half is one block of instructions.
-  float4 uf[2][2];
-  auto read_u = [&](int stage, int k) __attribute__((always_inline)) {  // factors of the lane's keys in 16-key step k
-    const float* us = reinterpret_cast<const float*>(lds + stage + L::u_off);
-    uf[k & 1][0] = *reinterpret_cast<const float4*>(us + 16 * k + 4 * half);
-    uf[k & 1][1] = *reinterpret_cast<const float4*>(us + 16 * k + 8 + 4 * half);
+  float4 uf[2], sf[2];
+  auto read_u = [&](int stage, int j) __attribute__((always_inline)) {  // factors and scales of V of the keys 8 j + 4 half + 0 .. 3
+    const float* us = reinterpret_cast<const float*>(lds + stage + L::u_off) + 8 * j + 4 * half;
+    uf[j & 1] = *reinterpret_cast<const float4*>(us);
+    sf[j & 1] = *reinterpret_cast<const float4*>(us + BKV);
   };
   auto products = [&](int tile, auto PARTIAL) __attribute__((always_inline)) {
     constexpr bool kPartial = decltype(PARTIAL)::value;
     using One = std::bool_constant<!kPartial && !SMALL>;
     const uint8_t* st = lds + st_cur;
     Ready nxt;
-    o_scale *= pend;
-    pend = pend_next;
-    pend_next = 1.f;
     __builtin_amdgcn_s_setprio(1);
     auto scores = [&](const auto& kf) __attribute__((always_inline)) {
 #pragma unroll
@@ -439,7 +406,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     if (!kPartial || tile * BKV < wave_max) scores(kf);
     write(st_next, nxt);
     load_tile(tile + 2, ahead, sreg, One{});
-    if constexpr (SMALL) find_pages(tile + 3);
+    if constexpr (SMALL) find_page(tile + 3);
     read_u(st_cur, 0);
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
@@ -467,54 +434,56 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       if constexpr (kPartial) return x == -INFINITY ? 1.f : u;
       return u;
     };
-    // The weights against the maximum so far.  Whether it still serves shows in their sum: a weight past the limit makes
-    // the sum reach it, and then (as before a row's first key) the exact maximum is taken and the weights are computed
-    // again.  So no tile pays for a maximum that does not change.
+    // The weights against the row's reference so far.  Whether it still serves shows in the largest of the fp16 weights (and in
+    // the sum, where scales are near zero); if not, and before a row's first key, the exact maximum is taken and the
+    // weights are computed again.  So no tile pays for an exact maximum that does not change.
     float l_tile;
+    v2h top;
     auto weights = [&]() __attribute__((always_inline)) {
       l_tile = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int b = k >> 1;
-        if (k < 3) read_u(stage, k + 1);
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = s[b][8 * (k & 1) + e];
-          const float4 y = uf[k & 1][e >> 2];
-          const float u[4] = {y.x, y.y, y.z, y.w};
-          p[e] = __builtin_amdgcn_exp2f(fmaf(x, factor(u[e & 3], x), neg_m));
-        }
+      for (int j = 0; j < 8; ++j) {
+        if (j < 7) read_u(stage, j + 1);
+        const float u[4] = {uf[j & 1].x, uf[j & 1].y, uf[j & 1].z, uf[j & 1].w};
+        const float sv[4] = {sf[j & 1].x, sf[j & 1].y, sf[j & 1].z, sf[j & 1].w};
+        float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const v2h one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-          pw[4 * k + e] = cvt_f16x2(p[2 * e], p[2 * e + 1]);
-          l_tile = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, pw[4 * k + e]), one, l_tile, false);
+          const float x = s[j >> 2][4 * (j & 3) + e];
+          p[e] = __builtin_amdgcn_exp2f(fmaf(x, factor(u[e], x), neg_m));
+          l_tile += p[e];
+          p[e] *= sv[e];
         }
+        pw[2 * j] = cvt_f16x2(p[0], p[1]);
+        pw[2 * j + 1] = cvt_f16x2(p[2], p[3]);
+        const v2h lo = __builtin_bit_cast(v2h, pw[2 * j]), hi = __builtin_bit_cast(v2h, pw[2 * j + 1]);
+        top = j ? __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, lo), hi) : __builtin_elementwise_maximum(lo, hi);
       }
     };
     weights();
-    // (a NaN sum needs no other maximum; m_use is -inf until the row has seen a key, and its weights count for nothing)
-    if (__ballot(l_tile > kMostSum || m_use == -INFINITY) || o_scale != 1.f) {
+    // (NaN needs no other reference; m_use is -inf until the row has seen a key, and its weights count for nothing)
+    if (__ballot(top[0] > kMost || top[1] > kMost || l_tile > kMostSum || m_use == -INFINITY)) {
       float mt = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 x = *reinterpret_cast<const float4*>(us + 32 * b + 8 * g + 4 * half);
-          const float u[4] = {x.x, x.y, x.z, x.w};
+          const float4 z = *reinterpret_cast<const float4*>(us + BKV + 32 * b + 8 * g + 4 * half);
+          const float u[4] = {x.x, x.y, x.z, x.w}, sv[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mt = fmaxf(mt, s[b][4 * g + e] * factor(u[e], s[b][4 * g + e]));
+          for (int e = 0; e < 4; ++e)
+            mt = fmaxf(mt, fmaf(s[b][4 * g + e], factor(u[e], s[b][4 * g + e]), fmaxf(__builtin_amdgcn_logf(sv[e]), kFloor)));
+          __builtin_amdgcn_sched_barrier(0);
         }
       mt = max32(mt);
-      const bool fire = max32(l_tile) > kMostSum || m_use == -INFINITY;
+      const bool fire = m_use == -INFINITY || mt - m_use > kGrow;
       const float m_new = fire ? fmaxf(m_use, mt) : m_use;
-      const float alpha = !fire || m_new == m_use ? 1.f : m_use == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_use - m_new);
-      const float beta = alpha * o_scale;
+      // (in two steps: a sum of small scales' p may be large, and still count where the step as one is below 2^-126)
+      const float alpha = m_new == m_use ? 1.f : m_use == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (m_use - m_new));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] *= beta;
-      o_scale = 1.f;
-      l_run *= alpha;
+      for (int i = 0; i < 4; ++i) o[i] *= alpha * alpha;
+      l_run = l_run * alpha * alpha;
       m_use = m_new;
       neg_m = m_new == -INFINITY ? kShift : kShift - m_new;
       read_u(stage, 0);
@@ -532,9 +501,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   if (tile_lo < tile_hi) {
     const bool late = wave >= kWaves / 2;
     Cursor c = cursor_at(tile_lo);
-    if constexpr (SMALL) find_pages(tile_lo);
+    if constexpr (SMALL) find_page(tile_lo);
     load_tile(tile_lo, c, sreg, std::false_type{});
-    set_exponent(tile_top(sreg.sv_lane));
     Ready y;
     convert(sreg, y, std::true_type{});
     write(st_cur, y);
@@ -545,10 +513,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) vf[i >> 2][i & 3] = make_uint4(0, 0, 0, 0);
     c = cursor_next(c, tile_lo + 1);
-    if constexpr (SMALL) find_pages(tile_lo + 1);
+    if constexpr (SMALL) find_page(tile_lo + 1);
     load_tile(tile_lo + 1, c, sreg, std::false_type{});
     ahead = cursor_next(c, tile_lo + 2);
-    if constexpr (SMALL) find_pages(tile_lo + 2);
+    if constexpr (SMALL) find_page(tile_lo + 2);
     __syncthreads();
     // whole: tiles that every row sees, and the next one too
     const int whole = min(max(lim_min / BKV - 1, tile_lo), tile_hi);
@@ -563,7 +531,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     int tile = tile_lo;
     if (!late) {
       auto step = [&](auto PARTIAL) __attribute__((always_inline)) {
-        check_exponent();
         const Cursor after = cursor_next(ahead, tile + 3);  // (branches come first: behind them the tile is one block)
         products(tile, PARTIAL);
         weigh(tile, st_cur, PARTIAL);
@@ -576,7 +543,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
         if (tile < tile_hi) step(std::true_type{});
       }
     } else {
-      check_exponent();
       products(tile, std::true_type{});
       rotate(cursor_next(ahead, tile + 3));
       __syncthreads();
@@ -584,7 +550,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       auto step = [&](auto PARTIAL) __attribute__((always_inline)) {
         const Cursor after = cursor_next(ahead, tile + 3);
         weigh(tile - 1, st_prev, PARTIAL);
-        check_exponent();
         products(tile, PARTIAL);
         rotate(after);
         __syncthreads();
@@ -604,7 +569,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // the rows' results: through LDS as bf16 rows (every wave its own; the last barrier has retired the stages), or, with
   // several splits, in fp32 to the workspace
   const float l_tot = sum32(l_run);
-  const float inv = l_tot == 0.f ? 0.f : __builtin_ldexpf(o_scale / l_tot, ev);
+  const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;
   if (splits > 1) {
     if (!row_ok) return;
     const int64_t at = ((static_cast<int64_t>(w) * a.n_kv_heads + head) * a.n_splits + split) * R + 32 * wave + l32;
