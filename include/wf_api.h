@@ -427,15 +427,14 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads,
  * min(kv_lens[b], (p / block + 1) * block) for the row's position p: every
  * key, causal (block 1), or causal by blocks of `block` positions (a frame,
  * a chunk).  Rows without a key are zero; a row of q that holds a NaN or an
- * infinity is NaN, and so are the rows that see a key whose scale is none; no
- * NaN or infinity of a key reaches a row that does not see it.  fp32 scores,
- * softmax and sums.  Up to 64 (row, head) rows of a sequence per key head the
- * weights p_j s_v[j] are held in 16 significant bits; with more, in 11 (fp16:
- * those below 2^-20 of the largest that the row sees lose bits, and so do all
- * where the scales of V are below 2^-100).
- * max_new and max_kv
- * bound the sequences' rows and keys; they choose the split, and results
- * stay right where the device's lengths pass them.  ws: ws_bytes of scratch,
+ * infinity is NaN, and so are the rows that see a key with a scale of K or V
+ * that is NaN or infinite; no NaN or infinity of a key reaches a row that does
+ * not see it.  fp32 scores, softmax and sums.  Up to 64 (row, head) rows of a
+ * sequence per key head the weights p_j s_v[j] are held in 16 significant
+ * bits; with more, in 11 (fp16: those below 2^-20 of the largest that the row
+ * sees lose bits, and so do all where the scales of V are below 2^-100).
+ * max_new and max_kv bound the sequences' rows and keys; they choose the
+ * split, and results stay right where the device's lengths pass them.  ws: ws_bytes of scratch,
  * 16-byte aligned, at least wf_attn_batch_workspace's.  The attention of
  * wf_attn_paged_fp8 for a batch (wave_rt/runtime/backend.py:141-148), with
  * the block-causal mask of naive_rt/rolling_forcing/wan/modules/

@@ -5,9 +5,9 @@ import pytest
 import torch
 
 from oracle import batch as ob
-from test_gpu_batch import DEV, SCALE, cached, check, make, rows, same
+from test_gpu_batch import DEV, SCALE, cached, check, gen, make, rows, same
 from waveforcing_amd import backend
-from waveforcing_amd.kv import PagedBatch
+from waveforcing_amd.kv import CrossBatch
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,64 @@ def test_keys_of_any_scale_count_alike(fmt, new, t, first, then):
     q = torch.zeros((new, 4, 128), dtype=torch.bfloat16, device=DEV)
     k, v = (cached(pool, batch, fmt, 0, name) for name in "kv")
     check(backend.attn_paged_batch(q, batch, block=1), *ob.attend(q, k, v, [t - new + i + 1 for i in range(new)], SCALE))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf")])
+@pytest.mark.parametrize("new", [1, 20, 140])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "dense"])
+def test_infinite_queries_over_one_key(fmt, new, bad):
+    """A row of q that holds an infinity is NaN, also where its every score is -inf."""
+    g = gen(330)
+    k = torch.zeros((new, 2, 128), dtype=torch.bfloat16, device=DEV)
+    k[:, :, 3] = 1.0
+    v, q = rows(new, 2, g), rows(new, 4, g)
+    if fmt == "dense":
+        batch = CrossBatch([new], [1], DEV)
+        attend = lambda x: backend.attn_cross_batch(x, k[:1], v[:1], batch)
+    else:
+        pool, batch, _ = make(fmt, 2, 64, [new], [new], 331)
+        batch.append(k, v)
+        attend = lambda x: backend.attn_paged_batch(x, batch, block=1)
+    clean = attend(q)
+    for i in {0, new // 2, new - 1}:
+        x = q.clone()
+        x[i, 1, 3] = bad
+        out = attend(x)
+        assert bool(torch.isnan(out[i, 1]).all())
+        out[i, 1] = clean[i, 1]
+        same(out, clean)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("new", [1, 20, 140])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_a_scale_that_is_not_finite_makes_the_rows_that_see_it_nan(fmt, new, bad, which):
+    """Whatever the sign of the score that an infinite scale of K gives; the rows before it keep their bits."""
+    pool, batch, g = make(fmt, 2, 64, [new + 90], [new], 340)
+    q = rows(new, 4, g)
+    clean = backend.attn_paged_batch(q, batch, block=1)
+    for p in (new + 89, 90 + new // 2, 5):
+        scales = getattr(pool, which + "_scales")
+        page, at = batch.pages[0][p // 64], p % 64
+        save = scales[page, :, at].clone()
+        scales[page, :, at] = bad
+        out = backend.attn_paged_batch(q, batch, block=1)
+        sees = torch.arange(90, 90 + new, device=DEV) >= p
+        assert bool(torch.isnan(out[sees]).all())
+        same(out[~sees], clean[~sees])
+        scales[page, :, at] = save
+
+
+@pytest.mark.parametrize("new", [1, 140])
+def test_dense_scores_of_minus_infinity(new):
+    """exp(-inf) is 0 where another key is finite, and a row all of whose scores are -inf has no mean."""
+    g = gen(350)
+    q, k, v = rows(new, 4, g).abs() + 0.1, rows(70, 2, g), rows(70, 2, g)
+    batch = CrossBatch([new], [70], DEV)
+    k[3, :, 9] = -float("inf")
+    keep = [i for i in range(70) if i != 3]
+    out = backend.attn_cross_batch(q, k, v, batch)
+    check(out, *ob.attend(q, k[keep], v[keep], [69] * new, SCALE))
+    k[:, :, 9] = -float("inf")
+    assert bool(torch.isnan(backend.attn_cross_batch(q, k, v, batch)).all())

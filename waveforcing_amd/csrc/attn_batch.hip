@@ -74,9 +74,9 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
       for (int e = 0; e < 8; ++e) o[e] = fmaf(w, v[e], o[e]);
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   uint32_t qi, gi;
   a.group_div.divmod(static_cast<uint32_t>(t.first + r), qi, gi);
+  const float inv = row_inverse(sum, row_limit(a, t, static_cast<int>(qi)));
   uint16_t* p = a.out + static_cast<int64_t>(t.row0 + static_cast<int>(qi)) * a.ldo + (head * a.group + static_cast<int>(gi)) * D + d;
   *reinterpret_cast<uint2*>(p) = make_uint2(cvt_bf16x2(o[0] * inv, o[1] * inv), cvt_bf16x2(o[2] * inv, o[3] * inv));
   *reinterpret_cast<uint2*>(p + 4) = make_uint2(cvt_bf16x2(o[4] * inv, o[5] * inv), cvt_bf16x2(o[6] * inv, o[7] * inv));

@@ -132,6 +132,12 @@ __device__ inline int used_splits(const Args& a, int lim) {
   return min(a.n_splits, max(lim - 1, 0) / a.split_keys + 1);
 }
 
+// 1 / sum of a row's weights.  A row that sees keys and whose weights are all zero has scores of -inf only (an infinite q, or
+// dense keys that are): there is no mean of them, and it is NaN.
+__device__ inline float row_inverse(float sum, int lim) {
+  return sum != 0.f ? 1.0f / sum : lim > 0 ? bits_f32(0x7fc00000u) : 0.f;
+}
+
 // Two fp32 -> packed bf16x2, round to nearest even.
 __device__ inline uint32_t cvt_bf16x2(float lo, float hi) { return pack_bf16x2_hw(lo, hi); }
 

@@ -213,7 +213,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
 
   // the rows' results: through LDS as bf16 rows, every wave its own, or, with several splits, in fp32 to the workspace
   const float l_tot = sum32(l_run);
-  const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;
+  const float inv = row_inverse(l_tot, splits > 1 ? 0 : t.kv_len);  // (of several splits the join sees whether all are empty)
   if (splits > 1) {
     if (!row_ok) return;
     const int64_t at = ((static_cast<int64_t>(w) * a.n_kv_heads + head) * a.n_splits + split) * R + 32 * wave + l32;

@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
 #pragma unroll
       for (int i = 0; i < 8; ++i) *reinterpret_cast<u32x4*>(vbuf + (4 * i + (lane >> 4)) * F::v_pitch + 16 * l16) = x.v[i];
     } else {
-      fbuf[lane] = lane < 32 ? x.fk * a.c : x.fv;
+      fbuf[lane] = lane < 32 ? fmaf(x.fk, 0.f, x.fk * a.c) : x.fv;  // (an infinite scale of K: NaN, whatever the score's sign)
       if (SRC == SRC_E4M3 && masked) {
         // A weight of zero does not silence a NaN of V: where some row does not see some key, a NaN code becomes a NaN
         // scale, which only the weights of rows that see the key meet.
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     if (t.first + 16 * n + l16 >= t.count) continue;
-    const float inv = sum[n] == 0.f ? 0.f : 1.0f / sum[n];
+    const float inv = row_inverse(sum[n], splits > 1 ? 0 : lim[n]);  // (of several splits the join sees whether all are empty)
     if (splits > 1) {
       const int64_t at = ((static_cast<int64_t>(w) * a.n_kv_heads + head) * a.n_splits + split) * R + 16 * n + l16;
 #pragma unroll

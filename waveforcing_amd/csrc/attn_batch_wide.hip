@@ -23,8 +23,8 @@
 //              lost below 2^-20 of it, 2^-31 of it at most.  (The scale in V instead, under an exponent that the tile shares,
 //              saves an instruction a score, but there a key that a row does not see, or gives no weight, takes the bits of
 //              those that it does.)  The row sum adds the p in fp32.
-// A NaN or infinite scale of V makes the key's score NaN and its weight of V zero, so the rows that see the key become NaN
-// and no others; in tiles that some row does not see whole, so does a NaN code of V.
+// A NaN or infinite scale makes the key's score NaN and its weight of V zero, so the rows that see the key become NaN and
+// no others; in tiles that some row does not see whole, so does a NaN code of V.
 #include <utility>
 
 #include "attn_batch.hpp"
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   };
   // The staged tile as it goes to LDS.  PARTIAL: some row may not see all of it.
   auto convert = [&](Staged x, Ready& y, auto PARTIAL) __attribute__((always_inline)) {
-    bool poison = !finite(x.sv);  // the score is NaN for the rows that see the key, the weight of V zero for the others
+    bool poison = !finite(x.sv) || !finite(x.sk);  // the score is NaN for the rows that see the key, the weight of V zero for the others
     if constexpr (SRC == SRC_E4M3 && decltype(PARTIAL)::value) {
       const bool nan = has_nan_code(x.v0[0]) || has_nan_code(x.v0[1]) || has_nan_code(x.v0[2]) || has_nan_code(x.v0[3]);
       const uint64_t any = __ballot(nan);
@@ -569,7 +569,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // the rows' results: through LDS as bf16 rows (every wave its own; the last barrier has retired the stages), or, with
   // several splits, in fp32 to the workspace
   const float l_tot = sum32(l_run);
-  const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;
+  const float inv = row_inverse(l_tot, splits > 1 ? 0 : lim);  // (of several splits the join sees whether all are empty)
   if (splits > 1) {
     if (!row_ok) return;
     const int64_t at = ((static_cast<int64_t>(w) * a.n_kv_heads + head) * a.n_splits + split) * R + 32 * wave + l32;
