@@ -149,3 +149,25 @@ def test_dense_scores_of_minus_infinity(new):
     check(out, *ob.attend(q, k[keep], v[keep], [69] * new, SCALE))
     k[:, :, 9] = -float("inf")
     assert bool(torch.isnan(backend.attn_cross_batch(q, k, v, batch)).all())
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("new", [6, 150])
+def test_rows_past_the_tensors_keep_the_others_in_place(fmt, new):
+    """Device lengths that pass the tensors' rows: append, read-back and attention place the rows that there are alike."""
+    pool, batch, g = make(fmt, 2, 48, [40, 2 * new + 100], [3, new], 360)
+    batch.cu_new[2] = 3 + 2 * new                      # twice the rows of q, k and v
+    k, v, q = rows(3 + new, 2, g), rows(3 + new, 2, g), rows(3 + new, 4, g)
+    batch.append(k, v)
+    gk, gv = batch.gather()
+    for x, y in ((k, gk), (v, gv)):
+        same(y, ob.values(*ob.quantize(x, fmt), fmt).float().bfloat16())
+    first = 100                                        # position of the second sequence's first row
+    page = torch.tensor(batch.pages[1], device=DEV)[torch.arange(first, first + new, device=DEV) // 48]
+    at = torch.arange(first, first + new, device=DEV) % 48
+    same(pool.k_codes[page, at], ob.quantize(k[3:], fmt)[0])
+    for block in (1, 16):
+        out = backend.attn_paged_batch(q, batch, block=block)
+        t = 2 * new + 100
+        check(out[3:], *ob.attend(q[3:], cached(pool, batch, fmt, 1, "k"), cached(pool, batch, fmt, 1, "v"),
+                                  [ob.limit(first + i, t, block) for i in range(new)], SCALE))

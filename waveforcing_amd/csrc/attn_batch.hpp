@@ -56,7 +56,8 @@ __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v);
 struct Tile {
   int b;          // sequence
   int row0;       // its first row in q
-  int n_new;      // its rows
+  int n_new;      // its rows that are in q
+  int pos0;       // position of its first row (the rows of cu count, also those past q's last)
   int first;      // the tile's first (i, head) row of the sequence
   int count;      // (i, head) rows of the sequence
   int kv_len;
@@ -83,7 +84,8 @@ __device__ inline bool find_tile(const Args& a, int w, Tile& t) {
   for (int base = 0; base < a.geom.n_seqs; base += 64) {
     const int i = min(base + lane, a.geom.n_seqs - 1);
     const int r = a.geom.cu[i];
-    const int n = min(a.geom.cu[i + 1], a.n_rows) - r;
+    const int end = a.geom.cu[i + 1];
+    const int n = min(end, a.n_rows) - r;
     const int u = DENSE ? a.cu_kv[i] : a.geom.kv_lens[i], v = DENSE ? a.cu_kv[i + 1] : 0;
     const bool some = base + lane < a.geom.n_seqs && r >= 0 && n > 0;
     const int tiles = some ? (n * a.group + (1 << a.tile_shift) - 1) >> a.tile_shift : 0;
@@ -103,6 +105,7 @@ __device__ inline bool find_tile(const Args& a, int w, Tile& t) {
       } else {
         t.key0 = 0;
         t.kv_len = min(max(x, 0), kMaxKeys);
+        t.pos0 = t.kv_len - (__builtin_amdgcn_readlane(end, at) - t.row0);
       }
       return t.first >= 0 && t.first < t.count;
     }
@@ -114,7 +117,7 @@ __device__ inline bool find_tile(const Args& a, int w, Tile& t) {
 // Keys that row i of the tile's sequence sees (0 .. lim).
 __device__ inline int row_limit(const Args& a, const Tile& t, int i) {
   if (a.block == 0) return t.kv_len;
-  const int p = t.kv_len - t.n_new + i;
+  const int p = t.pos0 + i;
   if (p < 0) return 0;
   const int64_t end = (static_cast<int64_t>(p / a.block) + 1) * a.block;
   return static_cast<int>(min(static_cast<int64_t>(t.kv_len), end));
