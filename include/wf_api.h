@@ -363,10 +363,10 @@ int wf_attn_dense_bf16(const void* q, int64_t lq, int32_t n_heads,
  *
  * Several generation streams in one launch.  Sequence b (b < n_seqs) owns the
  * rows cu_new[b] .. cu_new[b + 1] of the ragged row tensors (cu_new int32
- * [n_seqs + 1], cu_new[0] = 0, not decreasing; rows from cu_new[n_seqs] on
- * are padding and are left as they are; rows that cu_new counts past n_rows
- * are not there, and keep their positions).  kv_lens[b] (int32) positions are
- * in its cache, those of its rows last: row i of the sequence stands at
+ * [n_seqs + 1], not decreasing; rows from cu_new[n_seqs] on, and before
+ * cu_new[0], are padding and are left as they are; rows that cu_new counts
+ * past n_rows are not there, and keep their positions).  kv_lens[b] (int32)
+ * positions are in its cache, those of its rows last: row i of the sequence stands at
  * position kv_lens[b] - (cu_new[b + 1] - cu_new[b]) + i.  Position p lives in
  * physical page tables[b][p / page_tokens] (int32 [n_seqs][ld_table]), row
  * p % page_tokens, of pools laid out as for wf_fp8_kv_pack with n_kv_heads

@@ -171,3 +171,21 @@ def test_rows_past_the_tensors_keep_the_others_in_place(fmt, new):
         t = 2 * new + 100
         check(out[3:], *ob.attend(q[3:], cached(pool, batch, fmt, 1, "k"), cached(pool, batch, fmt, 1, "v"),
                                   [ob.limit(first + i, t, block) for i in range(new)], SCALE))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_rows_before_the_first_sequence_are_nobodys(fmt):
+    """A first start behind row 0: the rows before it are neither cached (where older positions lie) nor read back."""
+    pool, batch, g = make(fmt, 2, 16, [30], [8], 370)
+    codes, scales = pool.k_codes.clone(), pool.k_scales.clone()
+    batch.cu_new[0] = 5
+    k = rows(8, 2, g)
+    batch.append(k, k)
+    for p in range(27):                                # 27 .. 29 are the three rows'
+        page, at = batch.pages[0][p // 16], p % 16
+        same(pool.k_codes[page, at], codes[page, at])
+        same(pool.k_scales[page, :, at], scales[page, :, at])
+    out = torch.full((8, 2, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    batch.gather(with_v=False, out_k=out)
+    assert bool((out[:5] == 7).all())
+    same(out[5:], ob.values(*ob.quantize(k[5:], fmt), fmt).float().bfloat16())

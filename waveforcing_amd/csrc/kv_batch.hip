@@ -46,7 +46,7 @@ __device__ inline bool place(const KvBatchArgs& a, uint32_t blk, int& row, int& 
   row = static_cast<int>(t);
   head = static_cast<int>(h);
   const int b = seq_of_group8(a.geom, row);
-  if (row >= a.n_rows || b >= a.geom.n_seqs) return false;
+  if (row >= a.n_rows || b >= a.geom.n_seqs || row < a.geom.cu[b]) return false;  // (rows before the first start are nobody's)
   int page, at;
   if (!pool_row(a.geom, b, a.geom.kv_lens[b] - a.geom.cu[b + 1] + row, page, at)) return false;
   code_row = (static_cast<int64_t>(page) * a.geom.page_tokens + at) * a.n_heads + head;
