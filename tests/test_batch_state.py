@@ -1,0 +1,33 @@
+"""Batched sequences, host side: what a batch keeps over refused calls and new lengths (no GPU)."""
+
+import pytest
+
+from waveforcing_amd.kv import Fp8PagePool, PagedBatch
+
+
+def pool(cls=Fp8PagePool):
+    return cls(6, 2, 128, 16, "cpu")
+
+
+def state(b):
+    return (b.kv_lens, b.new_lens, b.n_new, b.max_new, b.max_kv, b.cu_new.tolist(), b.kv_lens_dev.tolist(),
+            b.tables.tolist())
+
+
+@pytest.mark.parametrize("kv, new, most, error", [
+    ([20, 9], [9, 1], 4, ValueError),                       # a bound below the lengths
+    ([20, 9], [9], None, ValueError),                       # one length short
+    ([33, 9], [9, 1], None, RuntimeError),                  # past the pages
+    ([20, 9], [21, 1], None, ValueError),                   # more new rows than positions
+    ([20, -1], [9, 1], None, ValueError),
+    ([20, 9], [9, (1 << 31) - 1024], None, ValueError),
+    ([20, "x"], [9, 1], None, ValueError),
+])
+def test_refused_lengths_leave_the_batch_as_it_was(kv, new, most, error):
+    b = PagedBatch(pool(), [[4, 1], [3]], [5, 7], [1, 2], max_kv=40)
+    before = state(b)
+    with pytest.raises(error):
+        b.set_lens(kv, new, max_kv=most)
+    assert state(b) == before
+    b.set_lens([20, 9], [9, 1], max_kv=32)
+    assert state(b) == ([20, 9], [9, 1], 10, 9, 32, [0, 9, 10], [20, 9], [[4, 1], [3, -1]])

@@ -328,7 +328,8 @@ class PagedBatch:
         self.n_seqs = len(self.pages)
         self.device = pool.k_codes.device
         wide = max((len(p) for p in self.pages), default=0)
-        self._check_lens(kv_lens, [1] * self.n_seqs if new_lens is None else new_lens)
+        lens = self._checked_lens(kv_lens, [1] * self.n_seqs if new_lens is None else new_lens, max_kv)
+        self._take_lens(*lens)
         n = self.n_seqs
         flat = [*_starts(self.new_lens), *self.kv_lens]
         for ids in self.pages:
@@ -340,9 +341,8 @@ class PagedBatch:
         self._lens_dev = dev[:2 * n + 1]
         self._geom = (self.cu_new.data_ptr(), self.kv_lens_dev.data_ptr(), n, self.tables.data_ptr() if wide else None,
                       wide)
-        self._set_bounds(max_kv)
 
-    def _check_lens(self, kv_lens, new_lens) -> None:
+    def _checked_lens(self, kv_lens, new_lens, max_kv):
         kv, new = _int32_list(kv_lens, "kv_lens"), _int32_list(new_lens, "new_lens")
         if not len(kv) == len(new) == self.n_seqs:
             raise ValueError(f"{self.n_seqs} page lists, {len(kv)} kv_lens and {len(new)} new_lens")
@@ -351,26 +351,25 @@ class PagedBatch:
                 raise ValueError(f"sequence {b}: {n} new rows among {t} cached positions")
             if t > len(ids) * self.pool.page_tokens:
                 raise RuntimeError(f"page table of {len(ids)} pages cannot hold {t} tokens (sequence {b})")
-        self.kv_lens, self.new_lens = kv, new
-        self.n_new = sum(new)
-        if self.n_new >= _MOST:
-            raise ValueError(f"{self.n_new} new rows")
-        self._writable = False
-
-    def _set_bounds(self, max_kv) -> None:
-        longest = max(self.kv_lens, default=0)
+        if sum(new) >= _MOST:
+            raise ValueError(f"{sum(new)} new rows")
+        longest = max(kv, default=0)
         if max_kv is not None and max_kv < longest:
             raise ValueError(f"max_kv={max_kv} is below a sequence's {longest} positions")
-        self.max_kv = longest if max_kv is None else int(max_kv)
-        self.max_new = max(self.new_lens, default=0)
+        return kv, new, longest if max_kv is None else int(max_kv)
+
+    def _take_lens(self, kv: list[int], new: list[int], max_kv: int) -> None:
+        self.kv_lens, self.new_lens, self.max_kv = kv, new, max_kv
+        self.n_new, self.max_new = sum(new), max(new, default=0)
+        self._writable = False
         self._ws: dict = {}
 
     def set_lens(self, kv_lens: Sequence[int], new_lens: Sequence[int] | None = None, max_kv: int | None = None) -> None:
         """The lengths of the next step (``new_lens``: as they are by default); one copy to the device, ordered on the
-        current stream."""
-        self._check_lens(kv_lens, self.new_lens if new_lens is None else new_lens)
-        self._set_bounds(max_kv)
-        self._lens_dev.copy_(torch.tensor([*_starts(self.new_lens), *self.kv_lens], dtype=torch.int32))
+        current stream.  A refused call leaves the batch as it was."""
+        lens = self._checked_lens(kv_lens, self.new_lens if new_lens is None else new_lens, max_kv)
+        self._lens_dev.copy_(torch.tensor([*_starts(lens[1]), *lens[0]], dtype=torch.int32))
+        self._take_lens(*lens)
 
     def _check_written_pages(self) -> None:
         """Every page that a new row is written to belongs to one place of one sequence."""
