@@ -31,3 +31,21 @@ def test_refused_lengths_leave_the_batch_as_it_was(kv, new, most, error):
     assert state(b) == before
     b.set_lens([20, 9], [9, 1], max_kv=32)
     assert state(b) == ([20, 9], [9, 1], 10, 9, 32, [0, 9, 10], [20, 9], [[4, 1], [3, -1]])
+
+
+def test_a_given_bound_stays():
+    b = PagedBatch(pool(), [[4, 1], [3]], [5, 7], max_kv=32)
+    b.set_lens([6, 8])
+    assert b.max_kv == 32
+    b.set_lens([7, 9], max_kv=20)
+    assert b.max_kv == 20
+    b.set_lens([25, 9])                                     # past the bound
+    assert b.max_kv == 25
+    b.set_lens([8, 10])
+    assert b.max_kv == 20
+    b = PagedBatch(pool(), [[4, 1], [3]], [5, 7])           # none given: the longest
+    b.set_lens([9, 8])
+    assert b.max_kv == 9
+    b.set_lens([1, 8])
+    assert b.max_kv == 8
+    assert PagedBatch(pool(), [], []).max_kv == 0

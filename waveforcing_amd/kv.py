@@ -314,7 +314,8 @@ class PagedBatch:
     The kernels read the lengths and tables on the device: ``cu_new`` int32 [n + 1], ``kv_lens_dev`` int32 [n],
     ``tables`` int32 [n, pages].  A captured graph replays with what they hold then (:meth:`set_lens`, or the
     caller's own kernels); ``max_kv`` (default: the longest of ``kv_lens``) should bound the lengths it will see,
-    since it chooses how long caches are split.
+    since it chooses how long caches are split.  A given bound stays until another is given;
+    longer lengths raise it while they last.
     """
 
     def __init__(self, pool: Fp8PagePool, pages: Sequence[Sequence[int]], kv_lens: Sequence[int],
@@ -327,6 +328,7 @@ class PagedBatch:
                     raise RuntimeError(f"page id {i} outside pool of {pool.pool_pages} pages")
         self.n_seqs = len(self.pages)
         self.device = pool.k_codes.device
+        self._bound = 0   # max_kv as given
         wide = max((len(p) for p in self.pages), default=0)
         lens = self._checked_lens(kv_lens, [1] * self.n_seqs if new_lens is None else new_lens, max_kv)
         self._take_lens(*lens)
@@ -356,10 +358,11 @@ class PagedBatch:
         longest = max(kv, default=0)
         if max_kv is not None and max_kv < longest:
             raise ValueError(f"max_kv={max_kv} is below a sequence's {longest} positions")
-        return kv, new, longest if max_kv is None else int(max_kv)
+        return kv, new, self._bound if max_kv is None else int(max_kv)
 
-    def _take_lens(self, kv: list[int], new: list[int], max_kv: int) -> None:
-        self.kv_lens, self.new_lens, self.max_kv = kv, new, max_kv
+    def _take_lens(self, kv: list[int], new: list[int], bound: int) -> None:
+        self.kv_lens, self.new_lens, self._bound = kv, new, bound
+        self.max_kv = max(bound, *kv) if kv else bound
         self.n_new, self.max_new = sum(new), max(new, default=0)
         self._writable = False
         self._ws: dict = {}
