@@ -2,7 +2,7 @@
 
 import pytest
 
-from waveforcing_amd.kv import Fp8PagePool, PagedBatch
+from waveforcing_amd.kv import Fp8PagePool, Int8PagePool, PagedBatch
 
 
 def pool(cls=Fp8PagePool):
@@ -49,3 +49,12 @@ def test_a_given_bound_stays():
     b.set_lens([1, 8])
     assert b.max_kv == 8
     assert PagedBatch(pool(), [], []).max_kv == 0
+
+
+def test_a_view_reads_pages_in_their_own_format():
+    for cls, other in ((Fp8PagePool, Int8PagePool), (Int8PagePool, Fp8PagePool)):
+        p = pool(cls)
+        view = cls.view_of(p, 2, 3)
+        assert (view.format, view.pool_pages) == (p.format, 3) and view.k_codes.data_ptr() == p.k_codes[2].data_ptr()
+        with pytest.raises(TypeError, match="another code format"):
+            other.view_of(p, 2, 3)

@@ -130,6 +130,8 @@ class Fp8PagePool:
     def view_of(cls, base: "Fp8PagePool", first_page: int, n_pages: int) -> "Fp8PagePool":
         """Pages [first_page, first_page + n_pages) of ``base`` as a pool of their own (shared storage,
         page ids relative to first_page)."""
+        if base.format != cls.format:
+            raise TypeError(f"{cls.__name__} cannot view the pages of {type(base).__name__}: another code format")
         if first_page < 0 or n_pages < 1 or first_page + n_pages > base.pool_pages:
             raise ValueError(f"pages [{first_page}, {first_page + n_pages}) outside a pool of {base.pool_pages}")
         self = cls.__new__(cls)
