@@ -1,7 +1,10 @@
 """Batched sequences, host side: what a batch keeps over refused calls and new lengths (no GPU)."""
 
+import ctypes
+
 import pytest
 
+from waveforcing_amd import _lib
 from waveforcing_amd.kv import Fp8PagePool, Int8PagePool, PagedBatch
 
 
@@ -58,3 +61,19 @@ def test_a_view_reads_pages_in_their_own_format():
         assert (view.format, view.pool_pages) == (p.format, 3) and view.k_codes.data_ptr() == p.k_codes[2].data_ptr()
         with pytest.raises(TypeError, match="another code format"):
             other.view_of(p, 2, 3)
+
+
+def workspace(*sizes):
+    n = ctypes.c_int64(-1)
+    _lib.call("wf_attn_batch_workspace", *sizes, ctypes.addressof(n))
+    return n.value
+
+
+def test_workspace_of_sizes_that_no_call_takes_is_refused():
+    """Sizes whose product passes 64 bits: refused as the attention refuses them, not wrapped around."""
+    most = (1 << 31) - 1
+    for sizes in ((1, 1 << 30, 1 << 30, most, 1, most), (1, 1 << 20, 1 << 20, 1 << 20, 1, 1 << 30),
+                  (1 << 15, 1 << 15, 1 << 15, 1 << 19, 1, most)):
+        with pytest.raises(RuntimeError, match="too many"):
+            workspace(*sizes)
+    assert workspace(0, most, most, most, 1, most) == 0     # no rows: a call that returns at once

@@ -87,6 +87,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
 struct Plan {
   int tile_shift;
   int64_t n_tiles, split_keys, n_splits, bytes;
+  bool fits;  // the grids; bytes hold nothing otherwise
 };
 
 Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_seqs, int64_t max_new, int64_t max_kv) {
@@ -132,7 +133,10 @@ Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, 
     p.n_splits = std::min<int64_t>(std::max<int64_t>(1, p.n_splits), kJoinSplits);
   }
   p.split_keys = std::max<int64_t>(128, ((max_kv + p.n_splits - 1) / p.n_splits + 127) / 128 * 128);
-  p.bytes = p.n_splits == 1 ? 0 : ((p.n_tiles * n_kv_heads * p.n_splits) << p.tile_shift) * (D + 2) * 4;
+  // (a grid holds fewer than 2^32 threads: 512 or fewer of each item, rounded up to 64 items; 16 x 256 where rows are joined)
+  p.fits = product_below({p.n_tiles + 64, n_kv_heads, p.n_splits, 512}, 1ll << 32) &&
+           (p.n_splits == 1 || product_below({p.n_tiles, n_kv_heads, 16 * 256}, 1ll << 32));
+  p.bytes = p.n_splits == 1 || !p.fits ? 0 : ((p.n_tiles * n_kv_heads * p.n_splits) << p.tile_shift) * (D + 2) * 4;
   return p;
 }
 
@@ -167,10 +171,7 @@ int common_args(const char* fn, Args& a, const void* q, int64_t n_rows, int32_t 
 int launch(const char* fn, Args& a, int src, int64_t n_seqs, int64_t max_new, int64_t max_kv, void* ws, int64_t ws_bytes,
            hipStream_t stream) {
   const Plan p = make_plan(src == SRC_DENSE, a.n_rows, static_cast<int64_t>(a.n_kv_heads) * a.group, a.n_kv_heads, n_seqs, max_new, max_kv);
-  // (a grid holds fewer than 2^32 threads: 512 or fewer of each item, rounded up to 64 items; 16 x 256 where rows are joined)
-  WF_REQUIRE(product_below({p.n_tiles + 64, a.n_kv_heads, p.n_splits, 512}, 1ll << 32) &&
-                 (p.n_splits == 1 || product_below({p.n_tiles, a.n_kv_heads, 16 * 256}, 1ll << 32)), WF_E_SHAPE,
-             "%s: %lld row tiles x %d key heads x %lld splits are too many", fn, (long long)p.n_tiles, a.n_kv_heads,
+  WF_REQUIRE(p.fits, WF_E_SHAPE, "%s: %lld row tiles x %d key heads x %lld splits are too many", fn, (long long)p.n_tiles, a.n_kv_heads,
              (long long)p.n_splits);
   WF_REQUIRE(a.ldkv < (1 << 23) && a.n_kv_heads < (1 << 16), WF_E_SHAPE, "%s: key rows of %lld elements or %d heads", fn,
              (long long)a.ldkv, a.n_kv_heads);
@@ -210,8 +211,14 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads, int32_t n_kv_heads,
   WF_REQUIRE(wf::product_below({n_rows, n_heads}, (1ll << 31) - 65536) && n_seqs < (1ll << 31) && max_kv < (1ll << 31), WF_E_SHAPE,
              "%s: rows=%lld x heads=%d, %lld sequences or %lld keys reach 2^31", fn, (long long)n_rows, n_heads, (long long)n_seqs, (long long)max_kv);
   *bytes = 0;
-  for (bool dense : {false, true})
-    *bytes = std::max(*bytes, wf::attn_batch::make_plan(dense, n_rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv).bytes);
+  bool fits = false;  // one of the two attentions takes them
+  for (bool dense : {false, true}) {
+    const auto p = wf::attn_batch::make_plan(dense, n_rows, n_heads, n_kv_heads, n_seqs, max_new, max_kv);
+    fits = fits || p.fits;
+    *bytes = std::max(*bytes, p.bytes);
+  }
+  WF_REQUIRE(n_rows == 0 || n_seqs == 0 || fits, WF_E_SHAPE, "%s: %lld rows of %lld sequences x %d heads are too many", fn,
+             (long long)n_rows, (long long)n_seqs, n_heads);
   return WF_OK;
 }
 
