@@ -77,3 +77,10 @@ def test_workspace_of_sizes_that_no_call_takes_is_refused():
         with pytest.raises(RuntimeError, match="too many"):
             workspace(*sizes)
     assert workspace(0, most, most, most, 1, most) == 0     # no rows: a call that returns at once
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 2.9e38, float("inf")])
+def test_a_scale_that_overflows_in_base_2_is_refused(scale):
+    args = (16, 4, 4, 2, 128, 512, 32, 48, 8, 256, 64, 80, 1, 4, 8, scale, 96, 512, None, 0, None)
+    with pytest.raises(RuntimeError, match="softmax_scale"):
+        _lib.call("wf_attn_cross_batch", *args)

@@ -147,8 +147,9 @@ int common_args(const char* fn, Args& a, const void* q, int64_t n_rows, int32_t 
                 int64_t ldq, float softmax_scale, void* out, int64_t ldo) {
   WF_REQUIRE(n_heads > 0 && n_heads % n_kv_heads == 0, WF_E_SHAPE, "%s: %d heads do not group over %d key heads", fn,
              n_heads, n_kv_heads);
-  WF_REQUIRE(softmax_scale >= 0.f && softmax_scale < 3.0e38f, WF_E_INVALID,
-             "%s: softmax_scale=%g must be finite and non-negative", fn, static_cast<double>(softmax_scale));
+  WF_REQUIRE(softmax_scale >= 0.f && std::isfinite(softmax_scale * kLog2e), WF_E_INVALID,
+             "%s: softmax_scale=%g must not be negative, and finite as a factor of base-2 exponents too", fn,
+             static_cast<double>(softmax_scale));
   const int64_t hd = static_cast<int64_t>(n_heads) * D;
   WF_REQUIRE(ldq >= hd && ldo >= hd, WF_E_INVALID, "%s: ldq/ldo smaller than n_heads*head_dim", fn);
   WF_REQUIRE(product_below({n_rows, n_heads}, (1ll << 31) - 65536), WF_E_SHAPE, "%s: rows=%lld x heads=%d reaches 2^31", fn,
