@@ -466,6 +466,39 @@ int wf_attn_cross_batch(const void* q, int64_t n_rows, int32_t n_heads,
                         int64_t max_kv, float softmax_scale, void* out,
                         int64_t ldo, void* ws, int64_t ws_bytes, void* stream);
 
+/* The last three into new outputs: rows before n_rows that no sequence owns
+ * when the work runs (wf_kv_batch_gather_fresh: that have no position) are
+ * zeroed instead of left as they are. */
+int wf_kv_batch_gather_fresh(const uint8_t* k_codes, const uint8_t* v_codes,
+                             const float* k_scales, const float* v_scales,
+                             int64_t pool_pages, int32_t format,
+                             int32_t page_tokens, const int32_t* cu_new,
+                             const int32_t* kv_lens, int64_t n_seqs,
+                             const int32_t* tables, int64_t ld_table,
+                             int64_t n_rows, int32_t n_kv_heads,
+                             int32_t head_dim, void* k_out, void* v_out,
+                             int64_t ld_out, void* stream);
+int wf_attn_paged_batch_fresh(const void* q, int64_t n_rows, int32_t n_heads,
+                              int32_t n_kv_heads, int32_t head_dim,
+                              int64_t ldq, int32_t format,
+                              const uint8_t* k_codes, const uint8_t* v_codes,
+                              const float* k_scales, const float* v_scales,
+                              int64_t pool_pages, int32_t page_tokens,
+                              const int32_t* cu_new, const int32_t* kv_lens,
+                              int64_t n_seqs, const int32_t* tables,
+                              int64_t ld_table, int64_t max_new,
+                              int64_t max_kv, int32_t block,
+                              float softmax_scale, void* out, int64_t ldo,
+                              void* ws, int64_t ws_bytes, void* stream);
+int wf_attn_cross_batch_fresh(const void* q, int64_t n_rows, int32_t n_heads,
+                              int32_t n_kv_heads, int32_t head_dim,
+                              int64_t ldq, const void* k, const void* v,
+                              int64_t n_kv_rows, int64_t ldkv,
+                              const int32_t* cu_q, const int32_t* cu_kv,
+                              int64_t n_seqs, int64_t max_q, int64_t max_kv,
+                              float softmax_scale, void* out, int64_t ldo,
+                              void* ws, int64_t ws_bytes, void* stream);
+
 /* ------------------------------------------------- block row-wise stages */
 
 /* y = LayerNorm(x) (fp32 statistics, optional bf16 affine w/b, rounded to

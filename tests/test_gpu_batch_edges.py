@@ -6,8 +6,8 @@ import torch
 
 from oracle import batch as ob
 from test_gpu_batch import DEV, SCALE, cached, check, gen, make, rows, same
-from waveforcing_amd import backend
-from waveforcing_amd.kv import CrossBatch
+from waveforcing_amd import _lib, backend
+from waveforcing_amd.kv import CrossBatch, Fp8PagePool, PagedBatch
 
 pytestmark = pytest.mark.gpu
 
@@ -189,3 +189,83 @@ def test_rows_before_the_first_sequence_are_nobodys(fmt):
     batch.gather(with_v=False, out_k=out)
     assert bool((out[:5] == 7).all())
     same(out[5:], ob.values(*ob.quantize(k[5:], fmt), fmt).float().bfloat16())
+
+
+def spoil(*shapes):
+    """Leaves NaN in the memory that the next new tensors of these shapes take."""
+    held = [torch.full(s, float("nan"), dtype=torch.bfloat16, device=DEV) for s in shapes]
+    del held
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "dense"])
+@pytest.mark.parametrize("new, hkv", [(1, 2), (9, 2), (40, 3), (700, 1)])
+def test_rows_that_the_device_leaves_out_are_zero_in_a_new_output(fmt, new, hkv):
+    """Starts on the device that own fewer rows than the tensors have, before, between (none) and behind the sequences."""
+    n, heads = 3 * new, 2 * hkv
+    g = gen(390)
+    q = rows(n + 2, heads, g)                          # two rows behind the batch's
+    if fmt == "dense":
+        batch = CrossBatch([new] * 3, [50, 0, 33], DEV)
+        k, v = rows(83, hkv, g), rows(83, hkv, g)
+        starts, attend = batch.cu_q, lambda **kw: backend.attn_cross_batch(q, k, v, batch, **kw)
+    else:
+        pool, batch, _ = make(fmt, hkv, 48, [new + 60, new, new + 300], [new] * 3, 391)
+        starts, attend = batch.cu_new, lambda **kw: backend.attn_paged_batch(q, batch, block=1, **kw)
+    whole = attend()
+    assert bool((whole[n:] == 0).all()) and bool((whole[:new] != 0).any())
+    for first, last in ((0, n), (0, n - 1), (0, new), (1, n), (new // 2, new), (0, 0), (n, n)):
+        starts.copy_(torch.tensor([first, max(first, min(new, last)), max(first, min(2 * new, last)), last], dtype=torch.int32))
+        owned = torch.arange(n + 2, device=DEV)
+        owned = (owned >= first) & (owned < last)
+        spoil((n + 2, heads, 128))
+        out = attend()
+        assert bool(torch.isfinite(out).all()) and bool((out[~owned] == 0).all())
+        given = torch.full_like(out, 7.0)
+        same(attend(out=given)[owned], out[owned])
+        assert bool((given[~owned] == 7).all())
+        if fmt != "dense":
+            spoil((n, hkv, 128), (n, hkv, 128))
+            gk, gv = batch.gather()
+            assert bool((gk[~owned[:n]] == 0).all()) and bool((gv[~owned[:n]] == 0).all())
+            half = torch.full_like(gk, 7.0)
+            spoil((n, hkv, 128))
+            _, other = batch.gather(out_k=half)
+            same(other, gv)
+            assert bool((half[~owned[:n]] == 7).all())
+            same(half[owned[:n]], gk[owned[:n]])
+
+
+@pytest.mark.parametrize("new", [8, 200])
+def test_replays_with_fewer_rows_hold_none_of_the_rows_before(new):
+    pool, batch, g = make("int8", 2, 64, [new + 300, new + 10], [new, new], 400)
+    cross = CrossBatch([new, new], [70, 20], DEV)
+    q, k, v = rows(2 * new, 4, g), rows(90, 2, g), rows(90, 2, g)
+
+    def step():
+        x = backend.attn_paged_batch(q, batch, block=1)
+        return (x, backend.attn_cross_batch(q, k, v, cross), *batch.gather())
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for a, b in ((new, new), (new, 1), (2, 0), (0, 5), (new, new)):
+        for t in (batch.cu_new, cross.cu_q):
+            t.copy_(torch.tensor([0, a, a + b], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for x, y in zip(outs, want):
+            assert bool((x[a + b:] == 0).all())
+            same(x, y)
+
+
+def test_a_new_output_without_sequences_is_refused_at_the_entry():
+    x = torch.zeros((4, 2, 128), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="rows without a sequence"):
+        _lib.call("wf_attn_cross_batch_fresh", x.data_ptr(), 4, 2, 2, 128, 256, x.data_ptr(), x.data_ptr(), 4, 256, None, None, 0, 4,
+                  4, 1.0, x.data_ptr(), 256, None, 0, None)
+    assert PagedBatch(Fp8PagePool(1, 2, 128, 16, DEV), [], []).gather()[0].shape == (0, 2, 128)

@@ -145,6 +145,9 @@ GEMM_GELU_TANH = 1
 LINEAR_GELU_INPUT = 2
 FP8_TENSOR_WEIGHT = 0
 FP8_TENSOR_ACT = 1
+for _name in ("wf_kv_batch_gather", "wf_attn_paged_batch", "wf_attn_cross_batch"):
+    SIGNATURES[_name + "_fresh"] = SIGNATURES[_name]
+
 FP8_AMAX_PARTIALS = 1024
 BF16_SILU_IN = 1
 BF16_SILU_OUT = 2

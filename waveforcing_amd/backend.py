@@ -157,7 +157,7 @@ def attn_paged_batch(q: torch.Tensor, batch: PagedBatch, block: int = 0, softmax
     position (``block`` 0), those up to its own (1: causal), or those up to the end of its block of ``block``
     positions (a frame's or a chunk's tokens: the block-causal mask).  The rows' own K/V are read from the
     cache (:meth:`PagedBatch.append` first).  A row that sees nothing is zero; rows behind the batch's are left
-    as they are in ``out`` (zero in a new output).  For one call geometry the results are the same bits on
+    as they are in ``out``; in a new output they are zero, and so are those that the device's starts leave out.  For one call geometry the results are the same bits on
     every run; how long caches are split, and with it the order of the sums, goes by the batch's sizes.
     """
     if not isinstance(batch, PagedBatch):
@@ -172,7 +172,7 @@ def attn_paged_batch(q: torch.Tensor, batch: PagedBatch, block: int = 0, softmax
     n = batch.workspace_bytes(H)
     ws = torch.empty((n,), dtype=torch.uint8, device=batch.device) if n else None
     cu, lens, n_seqs, tables, wide = batch._geom
-    _lib.call_on(batch.device, "wf_attn_paged_batch", q.data_ptr(), batch.n_new, H, pool.n_heads, 128, ldq, pool.format,
+    _lib.call_on(batch.device, "wf_attn_paged_batch" if out is not None else "wf_attn_paged_batch_fresh", q.data_ptr(), batch.n_new, H, pool.n_heads, 128, ldq, pool.format,
                  pool._k_codes_p, pool._v_codes_p, pool._k_scales_p, pool._v_scales_p, pool.pool_pages, pool.page_tokens,
                  cu, lens, n_seqs, tables, wide, batch.max_new, batch.max_kv, block,
                  128 ** -0.5 if softmax_scale is None else float(softmax_scale), o.data_ptr(), ldo, _lib.ptr(ws), n)
@@ -185,7 +185,8 @@ def attn_cross_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: C
     cross-attention of several streams, each with its prompt's own length.
 
     q [rows, heads, 128]; k, v [encoder rows, key heads, 128], all bf16, the sequences' rows one after the other
-    as ``batch`` counts them; key heads group over ``heads``.  A sequence without encoder rows gets zeros.
+    as ``batch`` counts them; key heads group over ``heads``.  A sequence without encoder rows gets zeros; rows that no
+    sequence owns are left as they are in ``out`` and zero in a new output.
     """
     if not isinstance(batch, CrossBatch):
         raise TypeError("attn_cross_batch takes a CrossBatch")
@@ -212,7 +213,7 @@ def attn_cross_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: C
     cu_q, cu_kv, n_seqs, max_q, max_kv = batch._geom
     n = batch.workspace_bytes(H, hkv)
     ws = torch.empty((n,), dtype=torch.uint8, device=batch.device) if n else None
-    _lib.call_on(batch.device, "wf_attn_cross_batch", q.data_ptr(), batch.n_q, H, hkv, 128, ldq, k.data_ptr(), v.data_ptr(),
+    _lib.call_on(batch.device, "wf_attn_cross_batch" if out is not None else "wf_attn_cross_batch_fresh", q.data_ptr(), batch.n_q, H, hkv, 128, ldq, k.data_ptr(), v.data_ptr(),
                  batch.n_kv, k.stride(0) if rows > 1 else hkv * D, cu_q, cu_kv, n_seqs, max_q, max_kv,
                  128 ** -0.5 if softmax_scale is None else float(softmax_scale), o.data_ptr(), ldo, _lib.ptr(ws), n)
     return o

@@ -133,8 +133,8 @@ Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, 
     p.n_splits = std::min<int64_t>(std::max<int64_t>(1, p.n_splits), kJoinSplits);
   }
   p.split_keys = std::max<int64_t>(128, ((max_kv + p.n_splits - 1) / p.n_splits + 127) / 128 * 128);
-  // (a grid holds fewer than 2^32 threads: 512 or fewer of each item, rounded up to 64 items; 16 x 256 where rows are joined)
-  p.fits = product_below({p.n_tiles + 64, n_kv_heads, p.n_splits, 512}, 1ll << 32) &&
+  // (a grid holds fewer than 2^32 threads: 512 or fewer of each item, rounded up to 64 items, and kClearers more; 16 x 256 where rows are joined)
+  p.fits = product_below({p.n_tiles + 64 + kClearers, n_kv_heads, p.n_splits, 512}, 1ll << 32) &&
            (p.n_splits == 1 || product_below({p.n_tiles, n_kv_heads, 16 * 256}, 1ll << 32));
   p.bytes = p.n_splits == 1 || !p.fits ? 0 : ((p.n_tiles * n_kv_heads * p.n_splits) << p.tile_shift) * (D + 2) * 4;
   return p;
@@ -170,7 +170,7 @@ int common_args(const char* fn, Args& a, const void* q, int64_t n_rows, int32_t 
 }
 
 int launch(const char* fn, Args& a, int src, int64_t n_seqs, int64_t max_new, int64_t max_kv, void* ws, int64_t ws_bytes,
-           hipStream_t stream) {
+           bool fresh, hipStream_t stream) {
   const Plan p = make_plan(src == SRC_DENSE, a.n_rows, static_cast<int64_t>(a.n_kv_heads) * a.group, a.n_kv_heads, n_seqs, max_new, max_kv);
   WF_REQUIRE(p.fits, WF_E_SHAPE, "%s: %lld row tiles x %d key heads x %lld splits are too many", fn, (long long)p.n_tiles, a.n_kv_heads,
              (long long)p.n_splits);
@@ -185,8 +185,8 @@ int launch(const char* fn, Args& a, int src, int64_t n_seqs, int64_t max_new, in
   a.n_splits = static_cast<int32_t>(p.n_splits);
   a.part_o = static_cast<float*>(ws);
   a.part_ml = a.part_o + ((p.n_tiles * a.n_kv_heads * p.n_splits) << p.tile_shift) * D;
-  const int st = p.tile_shift <= 5 ? launch_few(a, src, 1 << (p.tile_shift - 4), stream)
-                 : src == SRC_DENSE ? launch_dense(a, stream) : launch_wide(a, src, stream);
+  const int st = p.tile_shift <= 5 ? launch_few(a, src, 1 << (p.tile_shift - 4), fresh, stream)
+                 : src == SRC_DENSE ? launch_dense(a, fresh, stream) : launch_wide(a, src, fresh, stream);
   if (st || p.n_splits == 1) return st;
   const dim3 grid(static_cast<uint32_t>((p.n_tiles * a.n_kv_heads) << (p.tile_shift - 4)));
   if (src == SRC_DENSE)
@@ -194,6 +194,56 @@ int launch(const char* fn, Args& a, int src, int64_t n_seqs, int64_t max_new, in
   else
     hipLaunchKernelGGL(join_kernel<false>, grid, dim3(256), 0, stream, a);
   return check_launch(fn);
+}
+
+int paged_batch(const char* fn, bool fresh, const void* q, int64_t n_rows, int32_t n_heads, int32_t n_kv_heads,
+                int32_t head_dim, int64_t ldq, int32_t format, const uint8_t* k_codes, const uint8_t* v_codes,
+                const float* k_scales, const float* v_scales, int64_t pool_pages, int32_t page_tokens,
+                const int32_t* cu_new, const int32_t* kv_lens, int64_t n_seqs, const int32_t* tables, int64_t ld_table,
+                int64_t max_new, int64_t max_kv, int32_t block, float softmax_scale, void* out, int64_t ldo, void* ws,
+                int64_t ws_bytes, void* stream) {
+  if (int st = check_batch(fn, n_rows, n_kv_heads, head_dim, cu_new, kv_lens, n_seqs)) return st;
+  if (int st = check_pool(fn, format, n_kv_heads, page_tokens, pool_pages, tables, ld_table)) return st;
+  WF_REQUIRE(n_rows == 0 || n_seqs == 0 || pool_pages > 0, WF_E_INVALID, "%s: an empty pool", fn);
+  WF_REQUIRE(block >= 0, WF_E_INVALID, "%s: block=%d must not be negative", fn, block);
+  WF_REQUIRE(max_new >= 0 && max_kv >= 0 && max_kv < (1ll << 31), WF_E_INVALID, "%s: bad bound of the lengths", fn);
+  Args a;
+  if (int st = common_args(fn, a, q, n_rows, n_heads, n_kv_heads, ldq, softmax_scale, out, ldo)) return st;
+  WF_REQUIRE(!fresh || n_rows == 0 || n_seqs > 0, WF_E_INVALID, "%s: rows without a sequence", fn);
+  if (n_rows == 0 || n_seqs == 0) return WF_OK;
+  WF_REQUIRE(q && out && k_codes && v_codes && k_scales && v_scales, WF_E_INVALID, "%s: null pointer", fn);
+  WF_REQUIRE(aligned(k_codes, 16) && aligned(v_codes, 16), WF_E_ALIGN, "%s: code pools must be 16-byte aligned", fn);
+  a.k_codes = k_codes;
+  a.v_codes = v_codes;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.block = block;
+  a.geom = make_batch_geom(cu_new, kv_lens, n_seqs, tables, ld_table, page_tokens, pool_pages);
+  return launch(fn, a, format, n_seqs, max_new, max_kv, ws, ws_bytes, fresh, as_stream(stream));
+}
+
+int cross_batch(const char* fn, bool fresh, const void* q, int64_t n_rows, int32_t n_heads, int32_t n_kv_heads,
+                int32_t head_dim, int64_t ldq, const void* k, const void* v, int64_t n_kv_rows, int64_t ldkv,
+                const int32_t* cu_q, const int32_t* cu_kv, int64_t n_seqs, int64_t max_q, int64_t max_kv,
+                float softmax_scale, void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
+  if (int st = check_batch(fn, n_rows, n_kv_heads, head_dim, cu_q, cu_kv, n_seqs)) return st;
+  WF_REQUIRE(max_q >= 0 && max_kv >= 0 && max_kv < (1ll << 31), WF_E_INVALID, "%s: bad bound of the lengths", fn);
+  WF_REQUIRE(n_kv_rows >= 0 && n_kv_rows < kMaxKeys, WF_E_SHAPE, "%s: %lld key rows", fn, (long long)n_kv_rows);
+  WF_REQUIRE(ldkv >= static_cast<int64_t>(n_kv_heads) * head_dim && ldkv % 8 == 0, WF_E_INVALID,
+             "%s: ldkv=%lld must be >= n_kv_heads*head_dim and a multiple of 8", fn, (long long)ldkv);
+  Args a;
+  if (int st = common_args(fn, a, q, n_rows, n_heads, n_kv_heads, ldq, softmax_scale, out, ldo)) return st;
+  WF_REQUIRE(!fresh || n_rows == 0 || n_seqs > 0, WF_E_INVALID, "%s: rows without a sequence", fn);
+  if (n_rows == 0 || n_seqs == 0) return WF_OK;
+  WF_REQUIRE(q && out && (n_kv_rows == 0 || (k && v)), WF_E_INVALID, "%s: null pointer", fn);
+  WF_REQUIRE(aligned(k, 16) && aligned(v, 16), WF_E_ALIGN, "%s: k and v must be 16-byte aligned", fn);
+  a.k_dense = static_cast<const uint16_t*>(k);
+  a.v_dense = static_cast<const uint16_t*>(v);
+  a.ldkv = ldkv;
+  a.n_kv_rows = static_cast<int32_t>(n_kv_rows);
+  a.cu_kv = cu_kv;
+  a.geom = make_batch_geom(cu_q, cu_kv, n_seqs, nullptr, 0, 1, 0);
+  return launch(fn, a, SRC_DENSE, n_seqs, max_q, max_kv, ws, ws_bytes, fresh, as_stream(stream));
 }
 
 }  // namespace
@@ -229,48 +279,40 @@ int wf_attn_paged_batch(const void* q, int64_t n_rows, int32_t n_heads, int32_t 
                         const int32_t* kv_lens, int64_t n_seqs, const int32_t* tables, int64_t ld_table, int64_t max_new,
                         int64_t max_kv, int32_t block, float softmax_scale, void* out, int64_t ldo, void* ws,
                         int64_t ws_bytes, void* stream) {
-  static const char* fn = "wf_attn_paged_batch";
-  if (int st = wf::check_batch(fn, n_rows, n_kv_heads, head_dim, cu_new, kv_lens, n_seqs)) return st;
-  if (int st = wf::check_pool(fn, format, n_kv_heads, page_tokens, pool_pages, tables, ld_table)) return st;
-  WF_REQUIRE(n_rows == 0 || n_seqs == 0 || pool_pages > 0, WF_E_INVALID, "%s: an empty pool", fn);
-  WF_REQUIRE(block >= 0, WF_E_INVALID, "%s: block=%d must not be negative", fn, block);
-  WF_REQUIRE(max_new >= 0 && max_kv >= 0 && max_kv < (1ll << 31), WF_E_INVALID, "%s: bad bound of the lengths", fn);
-  wf::attn_batch::Args a;
-  if (int st = wf::attn_batch::common_args(fn, a, q, n_rows, n_heads, n_kv_heads, ldq, softmax_scale, out, ldo)) return st;
-  if (n_rows == 0 || n_seqs == 0) return WF_OK;
-  WF_REQUIRE(q && out && k_codes && v_codes && k_scales && v_scales, WF_E_INVALID, "%s: null pointer", fn);
-  WF_REQUIRE(wf::attn_batch::aligned(k_codes, 16) && wf::attn_batch::aligned(v_codes, 16), WF_E_ALIGN, "%s: code pools must be 16-byte aligned", fn);
-  a.k_codes = k_codes;
-  a.v_codes = v_codes;
-  a.k_scales = k_scales;
-  a.v_scales = v_scales;
-  a.block = block;
-  a.geom = wf::make_batch_geom(cu_new, kv_lens, n_seqs, tables, ld_table, page_tokens, pool_pages);
-  return wf::attn_batch::launch(fn, a, format, n_seqs, max_new, max_kv, ws, ws_bytes, wf::as_stream(stream));
+  return wf::attn_batch::paged_batch("wf_attn_paged_batch", false, q, n_rows, n_heads, n_kv_heads, head_dim, ldq,
+                                     format, k_codes, v_codes, k_scales, v_scales, pool_pages, page_tokens, cu_new,
+                                     kv_lens, n_seqs, tables, ld_table, max_new, max_kv, block, softmax_scale, out, ldo,
+                                     ws, ws_bytes, stream);
+}
+
+int wf_attn_paged_batch_fresh(const void* q, int64_t n_rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                              int64_t ldq, int32_t format, const uint8_t* k_codes, const uint8_t* v_codes,
+                              const float* k_scales, const float* v_scales, int64_t pool_pages, int32_t page_tokens,
+                              const int32_t* cu_new, const int32_t* kv_lens, int64_t n_seqs, const int32_t* tables,
+                              int64_t ld_table, int64_t max_new, int64_t max_kv, int32_t block, float softmax_scale,
+                              void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
+  return wf::attn_batch::paged_batch("wf_attn_paged_batch_fresh", true, q, n_rows, n_heads, n_kv_heads, head_dim, ldq,
+                                     format, k_codes, v_codes, k_scales, v_scales, pool_pages, page_tokens, cu_new,
+                                     kv_lens, n_seqs, tables, ld_table, max_new, max_kv, block, softmax_scale, out, ldo,
+                                     ws, ws_bytes, stream);
 }
 
 int wf_attn_cross_batch(const void* q, int64_t n_rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t ldq,
                         const void* k, const void* v, int64_t n_kv_rows, int64_t ldkv, const int32_t* cu_q,
                         const int32_t* cu_kv, int64_t n_seqs, int64_t max_q, int64_t max_kv, float softmax_scale,
                         void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
-  static const char* fn = "wf_attn_cross_batch";
-  if (int st = wf::check_batch(fn, n_rows, n_kv_heads, head_dim, cu_q, cu_kv, n_seqs)) return st;
-  WF_REQUIRE(max_q >= 0 && max_kv >= 0 && max_kv < (1ll << 31), WF_E_INVALID, "%s: bad bound of the lengths", fn);
-  WF_REQUIRE(n_kv_rows >= 0 && n_kv_rows < wf::attn_batch::kMaxKeys, WF_E_SHAPE, "%s: %lld key rows", fn, (long long)n_kv_rows);
-  WF_REQUIRE(ldkv >= static_cast<int64_t>(n_kv_heads) * head_dim && ldkv % 8 == 0, WF_E_INVALID,
-             "%s: ldkv=%lld must be >= n_kv_heads*head_dim and a multiple of 8", fn, (long long)ldkv);
-  wf::attn_batch::Args a;
-  if (int st = wf::attn_batch::common_args(fn, a, q, n_rows, n_heads, n_kv_heads, ldq, softmax_scale, out, ldo)) return st;
-  if (n_rows == 0 || n_seqs == 0) return WF_OK;
-  WF_REQUIRE(q && out && (n_kv_rows == 0 || (k && v)), WF_E_INVALID, "%s: null pointer", fn);
-  WF_REQUIRE(wf::attn_batch::aligned(k, 16) && wf::attn_batch::aligned(v, 16), WF_E_ALIGN, "%s: k and v must be 16-byte aligned", fn);
-  a.k_dense = static_cast<const uint16_t*>(k);
-  a.v_dense = static_cast<const uint16_t*>(v);
-  a.ldkv = ldkv;
-  a.n_kv_rows = static_cast<int32_t>(n_kv_rows);
-  a.cu_kv = cu_kv;
-  a.geom = wf::make_batch_geom(cu_q, cu_kv, n_seqs, nullptr, 0, 1, 0);
-  return wf::attn_batch::launch(fn, a, wf::attn_batch::SRC_DENSE, n_seqs, max_q, max_kv, ws, ws_bytes, wf::as_stream(stream));
+  return wf::attn_batch::cross_batch("wf_attn_cross_batch", false, q, n_rows, n_heads, n_kv_heads, head_dim, ldq, k, v,
+                                     n_kv_rows, ldkv, cu_q, cu_kv, n_seqs, max_q, max_kv, softmax_scale, out, ldo, ws,
+                                     ws_bytes, stream);
+}
+
+int wf_attn_cross_batch_fresh(const void* q, int64_t n_rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                              int64_t ldq, const void* k, const void* v, int64_t n_kv_rows, int64_t ldkv,
+                              const int32_t* cu_q, const int32_t* cu_kv, int64_t n_seqs, int64_t max_q, int64_t max_kv,
+                              float softmax_scale, void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
+  return wf::attn_batch::cross_batch("wf_attn_cross_batch_fresh", true, q, n_rows, n_heads, n_kv_heads, head_dim, ldq,
+                                     k, v, n_kv_rows, ldkv, cu_q, cu_kv, n_seqs, max_q, max_kv, softmax_scale, out, ldo,
+                                     ws, ws_bytes, stream);
 }
 
 }  // extern "C"

@@ -41,6 +41,7 @@ struct Args {
   int32_t n_rows, n_kv_heads, group;
   FastDiv group_div;
   int32_t block;
+  uint32_t clear_from;  // workgroups from this one on zero the rows of out that no sequence owns
   float c;  // softmax scale * log2(e)
   int32_t tile_shift, n_tiles;
   int32_t split_keys, n_splits;  // keys of a split (a multiple of 64), splits at most
@@ -112,6 +113,19 @@ __device__ inline bool find_tile(const Args& a, int w, Tile& t) {
     before = __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
+}
+
+// Rows that no sequence owns, before the first start and from the last one on, are zeroed in a fresh output by kClearers
+// workgroups of their own behind the grid's others.
+constexpr int kClearers = 128;
+template <int THREADS>
+__device__ inline void clear_rest(const Args& a) {
+  const int before = min(max(a.geom.cu[0], 0), a.n_rows), from = min(max(a.geom.cu[a.geom.n_seqs], before), a.n_rows);
+  const int n = before + a.n_rows - from, width = a.n_kv_heads * a.group * D;
+  for (int i = static_cast<int>(blockIdx.x - a.clear_from); i < n; i += kClearers) {
+    uint16_t* p = a.out + static_cast<int64_t>(i < before ? i : i - before + from) * a.ldo;
+    for (int c = 4 * static_cast<int>(threadIdx.x); c < width; c += 4 * THREADS) *reinterpret_cast<uint2*>(p + c) = make_uint2(0, 0);
+  }
 }
 
 // Keys that row i of the tile's sequence sees (0 .. lim).
@@ -218,9 +232,10 @@ __device__ inline uint32_t without_nan_codes(uint32_t w) {
   return w & ~(n * 0xffu);
 }
 
-int launch_few(const Args& a, int src, int row_blocks, hipStream_t stream);
-int launch_wide(const Args& a, int format, hipStream_t stream);
-int launch_dense(const Args& a, hipStream_t stream);
+// (a by value: each sets clear_from)
+int launch_few(Args a, int src, int row_blocks, bool fresh, hipStream_t stream);
+int launch_wide(Args a, int format, bool fresh, hipStream_t stream);
+int launch_dense(Args a, bool fresh, hipStream_t stream);
 
 }  // namespace attn_batch
 }  // namespace wf

@@ -46,6 +46,7 @@ __device__ inline v4s read_v(const uint8_t* __restrict p) { return read_tr16(p);
 
 __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+  if (blockIdx.x >= a.clear_from) return clear_rest<64 * kWaves>(a);
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int l32 = lane & 31, half = lane >> 5, l16 = lane & 15;
@@ -54,11 +55,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
   const int n_items = a.n_tiles * a.n_kv_heads * a.n_splits;
   const int xcd = static_cast<int>(blockIdx.x) % kXcds, slot = static_cast<int>(blockIdx.x) / kXcds;
   const int i_lin = ((slot / kRun) * kXcds + xcd) * kRun + slot % kRun;
-  if (i_lin >= n_items) return;
   const int w = i_lin % a.n_tiles, hs = i_lin / a.n_tiles;
   const int head = hs % a.n_kv_heads, split = hs / a.n_kv_heads;
   Tile t;
-  if (!find_tile<true>(a, w, t)) return;
+  if (i_lin >= n_items || !find_tile<true>(a, w, t)) return;
   const int splits = used_splits(a, t.kv_len);
   if (split >= splits) return;
   const int k_lo = split * a.split_keys;
@@ -250,10 +250,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dense_kernel(Args a) {
 
 }  // namespace
 
-int launch_dense(const Args& a, hipStream_t stream) {
+int launch_dense(Args a, bool fresh, hipStream_t stream) {
   const int64_t items = static_cast<int64_t>(a.n_tiles) * a.n_kv_heads * a.n_splits;
   constexpr int64_t per = kXcds * kRun;
-  hipLaunchKernelGGL(attn_dense_kernel, dim3(static_cast<uint32_t>((items + per - 1) / per * per)), dim3(64 * kWaves), 0, stream, a);
+  a.clear_from = static_cast<uint32_t>((items + per - 1) / per * per);
+  const dim3 grid(a.clear_from + (fresh ? kClearers : 0));
+  hipLaunchKernelGGL(attn_dense_kernel, grid, dim3(64 * kWaves), 0, stream, a);
   return check_launch("wf_attn_batch (many rows, dense keys)");
 }
 

@@ -83,6 +83,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
   constexpr int R = 16 * NB;
   __shared__ __attribute__((aligned(16))) uint8_t lds[F::lds];
 
+  if (blockIdx.x >= a.clear_from) return clear_rest<64 * W>(a);
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int l16 = lane & 15, g4 = lane >> 4;
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     uint32_t lp, at;
     a.geom.page.divmod(static_cast<uint32_t>(t0), lp, at);
     int page = -1;
-    if (n && static_cast<int>(lp) < a.geom.ld_table) page = a.geom.tables[static_cast<int64_t>(t.b) * a.geom.ld_table + lp];
+    if (n && static_cast<int>(lp) < a.geom.ld_table) page = uniform_page(a.geom.tables, static_cast<int64_t>(t.b) * a.geom.ld_table + lp);
     page = uniform(page);
     const bool ok = page >= 0 && page < a.geom.pool_pages;
     const int pg = ok ? page : 0, r0 = static_cast<int>(at);
@@ -546,8 +547,9 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
 }
 
 template <int SRC>
-void launch(const Args& a, int row_blocks, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(a.n_tiles) * a.n_kv_heads * a.n_splits);
+void launch(Args& a, int row_blocks, bool fresh, hipStream_t stream) {
+  a.clear_from = static_cast<uint32_t>(a.n_tiles) * a.n_kv_heads * a.n_splits;
+  const dim3 grid(a.clear_from + (fresh ? kClearers : 0));
   if (row_blocks == 1)
     hipLaunchKernelGGL((attn_few_kernel<SRC, 1>), grid, dim3(64 * W), 0, stream, a);
   else
@@ -556,11 +558,11 @@ void launch(const Args& a, int row_blocks, hipStream_t stream) {
 
 }  // namespace
 
-int launch_few(const Args& a, int src, int row_blocks, hipStream_t stream) {
+int launch_few(Args a, int src, int row_blocks, bool fresh, hipStream_t stream) {
   switch (src) {
-    case SRC_E4M3: launch<SRC_E4M3>(a, row_blocks, stream); break;
-    case SRC_INT8: launch<SRC_INT8>(a, row_blocks, stream); break;
-    default: launch<SRC_DENSE>(a, row_blocks, stream); break;
+    case SRC_E4M3: launch<SRC_E4M3>(a, row_blocks, fresh, stream); break;
+    case SRC_INT8: launch<SRC_INT8>(a, row_blocks, fresh, stream); break;
+    default: launch<SRC_DENSE>(a, row_blocks, fresh, stream); break;
   }
   return check_launch("wf_attn_batch (few rows)");
 }

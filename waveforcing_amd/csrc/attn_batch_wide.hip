@@ -104,6 +104,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   constexpr bool kCodes = SRC == SRC_E4M3;
   __shared__ __attribute__((aligned(16))) uint8_t lds[L::bytes];
 
+  if (blockIdx.x >= a.clear_from) return clear_rest<kThreads>(a);
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -117,9 +118,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   const int i_run = (slot / kRun) * kXcds + xcd;
   const int head = i_run % a.n_kv_heads, rs = i_run / a.n_kv_heads;
   const int w = a.n_tiles - 1 - (rs % runs) * kRun - slot % kRun, split = a.n_splits - 1 - rs / runs;
-  if (w < 0 || split < 0) return;
   Tile t;
-  if (!find_tile<false>(a, w, t)) return;
+  if (w < 0 || split < 0 || !find_tile<false>(a, w, t)) return;
   const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
   const int splits = used_splits(a, lim_max);
   if (split >= splits) return;
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     a.geom.page.divmod(static_cast<uint32_t>(tile) * BKV, lp, at);
     const int i = static_cast<int>(lp);
     int page = -1;
-    if (i < a.geom.ld_table) page = table[i];
+    if (i < a.geom.ld_table) page = uniform_page(table, i);
     page = __builtin_amdgcn_readfirstlane(page);
     asm volatile("" ::"s"(page));  // awaited here, not among the LDS reads of the tile
     const bool ok = page >= 0 && page < a.geom.pool_pages;
@@ -604,10 +604,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 
 }  // namespace
 
-int launch_wide(const Args& a, int format, hipStream_t stream) {
+int launch_wide(Args a, int format, bool fresh, hipStream_t stream) {
   const int64_t items = static_cast<int64_t>((a.n_tiles + kRun - 1) / kRun * kRun) * a.n_kv_heads * a.n_splits;
   constexpr int64_t per = kXcds * kRun;
-  const dim3 grid(static_cast<uint32_t>((items + per - 1) / per * per));
+  a.clear_from = static_cast<uint32_t>((items + per - 1) / per * per);
+  const dim3 grid(a.clear_from + (fresh ? kClearers : 0));
   const bool small = a.geom.page_tokens < BKV;
   void (*kernel)(Args);
   if (format == WF_KV_E4M3)

@@ -35,6 +35,7 @@ struct KvBatchArgs {
   int32_t n_rows;
   uint32_t n_blocks;  // of K
   uint32_t n_items;   // of K and V
+  int32_t fresh;      // gather: rows without a position are zeroed
   FastDiv heads;
   BatchGeom geom;
 };
@@ -46,7 +47,7 @@ __device__ inline bool place(const KvBatchArgs& a, uint32_t blk, int& row, int& 
   row = static_cast<int>(t);
   head = static_cast<int>(h);
   const int b = seq_of_group8(a.geom, row);
-  if (row >= a.n_rows || b >= a.geom.n_seqs || row < a.geom.cu[b]) return false;  // (rows before the first start are nobody's)
+  if (row >= a.n_rows || b >= a.geom.n_seqs || row < a.geom.cu[0]) return false;  // (rows before the first start are nobody's)
   int page, at;
   if (!pool_row(a.geom, b, a.geom.kv_lens[b] - a.geom.cu[b + 1] + row, page, at)) return false;
   code_row = (static_cast<int64_t>(page) * a.geom.page_tokens + at) * a.n_heads + head;
@@ -139,15 +140,20 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvBatchArgs a) {
   if (!item(a, blk, which)) return;
   int row, head;
   int64_t code_row = 0, scale_at = 0;
-  if (!place(a, blk, row, head, code_row, scale_at)) return;
+  const bool ok = place(a, blk, row, head, code_row, scale_at);
+  if (!ok && (!a.fresh || row >= a.n_rows)) return;
   const uint32_t lane8 = threadIdx.x & 7u;
+  uint4* p = reinterpret_cast<uint4*>(a.dst[which] + static_cast<int64_t>(row) * a.ld + head * kHeadDim) + lane8 * 2;
+  if (!ok) {
+    p[0] = p[1] = make_uint4(0, 0, 0, 0);
+    return;
+  }
   const uint4 c = reinterpret_cast<const uint4*>(a.codes[which] + code_row * kHeadDim)[lane8];
   const float s = a.scales[which][scale_at];
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
   uint2 o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = FMT == WF_KV_INT8 ? dequant4_i8(w[i], s) : dequant4(w[i], s);
-  uint4* p = reinterpret_cast<uint4*>(a.dst[which] + static_cast<int64_t>(row) * a.ld + head * kHeadDim) + lane8 * 2;
   p[0] = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
   p[1] = make_uint4(o[2].x, o[2].y, o[3].x, o[3].y);
 }
@@ -155,7 +161,7 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvBatchArgs a) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Checks and launch of both directions; k, v: the dense rows (const-cast for append, which only reads them).
-int kv_batch(const char* fn, bool write, void* k, void* v, int64_t n_rows, int32_t n_heads, int32_t head_dim, int64_t ld,
+int kv_batch(const char* fn, bool write, bool fresh, void* k, void* v, int64_t n_rows, int32_t n_heads, int32_t head_dim, int64_t ld,
              int32_t format, const int32_t* cu, const int32_t* kv_lens, int64_t n_seqs, const int32_t* tables,
              int64_t ld_table, int32_t page_tokens, uint8_t* k_codes, uint8_t* v_codes, float* k_scales,
              float* v_scales, int64_t pool_pages, void* stream) {
@@ -163,6 +169,7 @@ int kv_batch(const char* fn, bool write, void* k, void* v, int64_t n_rows, int32
   if (int st = check_pool(fn, format, n_heads, page_tokens, pool_pages, tables, ld_table)) return st;
   WF_REQUIRE(product_below({n_rows, n_heads}, (1ll << 31) - kRowsPerBlock), WF_E_SHAPE, "%s: rows=%lld x heads=%d reaches 2^31",
              fn, (long long)n_rows, n_heads);
+  WF_REQUIRE(!fresh || n_rows == 0 || n_seqs > 0, WF_E_INVALID, "%s: rows without a sequence", fn);
   if (n_rows == 0 || n_seqs == 0) return WF_OK;
   WF_REQUIRE(k && k_codes && k_scales, WF_E_INVALID, "%s: null K pointer", fn);
   WF_REQUIRE(!v || (v_codes && v_scales), WF_E_INVALID, "%s: V given without V pool", fn);
@@ -184,6 +191,7 @@ int kv_batch(const char* fn, bool write, void* k, void* v, int64_t n_rows, int32
   a.n_rows = static_cast<int32_t>(n_rows);
   a.n_blocks = static_cast<uint32_t>((n_rows * n_heads + kRowsPerBlock - 1) / kRowsPerBlock);
   a.n_items = v ? 2 * a.n_blocks : a.n_blocks;
+  a.fresh = fresh;
   a.heads = FastDiv(static_cast<uint32_t>(n_heads));
   a.geom = make_batch_geom(cu, kv_lens, n_seqs, tables, ld_table, page_tokens, pool_pages);
   const dim3 grid((a.n_items + kXcds - 1) / kXcds * kXcds);
@@ -202,7 +210,7 @@ int wf_kv_batch_append(const void* k, const void* v, int64_t n_rows, int32_t n_k
                        int32_t format, const int32_t* cu_new, const int32_t* kv_lens, int64_t n_seqs,
                        const int32_t* tables, int64_t ld_table, int32_t page_tokens, uint8_t* k_codes,
                        uint8_t* v_codes, float* k_scales, float* v_scales, int64_t pool_pages, void* stream) {
-  return wf::kv_batch("wf_kv_batch_append", true, const_cast<void*>(k), const_cast<void*>(v), n_rows, n_kv_heads,
+  return wf::kv_batch("wf_kv_batch_append", true, false, const_cast<void*>(k), const_cast<void*>(v), n_rows, n_kv_heads,
                       head_dim, ld_kv, format, cu_new, kv_lens, n_seqs, tables, ld_table, page_tokens, k_codes, v_codes,
                       k_scales, v_scales, pool_pages, stream);
 }
@@ -211,7 +219,18 @@ int wf_kv_batch_gather(const uint8_t* k_codes, const uint8_t* v_codes, const flo
                        int64_t pool_pages, int32_t format, int32_t page_tokens, const int32_t* cu_new,
                        const int32_t* kv_lens, int64_t n_seqs, const int32_t* tables, int64_t ld_table, int64_t n_rows,
                        int32_t n_kv_heads, int32_t head_dim, void* k_out, void* v_out, int64_t ld_out, void* stream) {
-  return wf::kv_batch("wf_kv_batch_gather", false, k_out, v_out, n_rows, n_kv_heads, head_dim, ld_out, format, cu_new,
+  return wf::kv_batch("wf_kv_batch_gather", false, false, k_out, v_out, n_rows, n_kv_heads, head_dim, ld_out, format, cu_new,
+                      kv_lens, n_seqs, tables, ld_table, page_tokens, const_cast<uint8_t*>(k_codes),
+                      const_cast<uint8_t*>(v_codes), const_cast<float*>(k_scales), const_cast<float*>(v_scales),
+                      pool_pages, stream);
+}
+
+int wf_kv_batch_gather_fresh(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_scales,
+                             const float* v_scales, int64_t pool_pages, int32_t format, int32_t page_tokens,
+                             const int32_t* cu_new, const int32_t* kv_lens, int64_t n_seqs, const int32_t* tables,
+                             int64_t ld_table, int64_t n_rows, int32_t n_kv_heads, int32_t head_dim,
+                             void* k_out, void* v_out, int64_t ld_out, void* stream) {
+  return wf::kv_batch("wf_kv_batch_gather_fresh", false, true, k_out, v_out, n_rows, n_kv_heads, head_dim, ld_out, format, cu_new,
                       kv_lens, n_seqs, tables, ld_table, page_tokens, const_cast<uint8_t*>(k_codes),
                       const_cast<uint8_t*>(v_codes), const_cast<float*>(k_scales), const_cast<float*>(v_scales),
                       pool_pages, stream);

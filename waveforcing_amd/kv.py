@@ -418,15 +418,17 @@ class PagedBatch:
     def gather(self, with_v: bool = True, out_k: torch.Tensor | None = None, out_v: torch.Tensor | None = None):
         """The new rows' positions read back as bf16 [rows, heads, 128] (wf_kv_batch_gather): what is cached there.
         A batch whose ``new_lens`` are its ``kv_lens`` reads the whole caches.  Given outputs may have more rows
-        (left as they are) and a row stride of their own."""
+        (left as they are) and a row stride of their own.  Rows that have no position on the device are left as they
+        are in a given output and zero in a new one."""
         pool = self.pool
         fresh = None   # a new output, which needs none of the checks of a given one
+        new = out_k is None and (out_v is None or not with_v)   # new outputs only: the kernel zeroes what it does not write
 
         def output(name, t):
             nonlocal fresh
             if t is None:
-                t = fresh = (torch.empty((self.n_new, pool.n_heads, pool.head_dim), dtype=torch.bfloat16, device=self.device)
-                             if fresh is None else torch.empty_like(fresh))
+                t = fresh = (torch.empty_like(fresh) if fresh is not None else (torch.empty if new else torch.zeros)(
+                    (self.n_new, pool.n_heads, pool.head_dim), dtype=torch.bfloat16, device=self.device))
                 return t, t.data_ptr(), pool.n_heads * pool.head_dim
             at, addr, ld = self._rows(t, name)
             if at is not t:
@@ -437,7 +439,7 @@ class PagedBatch:
         v = output("out_v", out_v) if with_v else None
         if v is not None and v[2] != ld:
             raise ValueError(f"out_k and out_v have different row strides ({ld} and {v[2]})")
-        _lib.call_on(self.device, "wf_kv_batch_gather", pool._k_codes_p, pool._v_codes_p, pool._k_scales_p,
+        _lib.call_on(self.device, "wf_kv_batch_gather_fresh" if new else "wf_kv_batch_gather", pool._k_codes_p, pool._v_codes_p, pool._k_scales_p,
                      pool._v_scales_p, pool.pool_pages, pool.format, pool.page_tokens, *self._geom, self.n_new,
                      pool.n_heads, pool.head_dim, kp, None if v is None else v[1], ld)
         return k if v is None else (k, v[0])
