@@ -374,8 +374,9 @@ int wf_attn_dense_bf16(const void* q, int64_t lq, int32_t n_heads,
  * [0, pool_pages) is not written, and read as above (gather: the row is left
  * as it is; attention: zero K and V).  cu_new, kv_lens and tables are read on
  * the device when the work runs, so a captured graph follows their contents.
- * head_dim is 128; a pool has fewer than 2^31 (position, head) rows and may
- * have any size in bytes; page_tokens >= 1.
+ * head_dim is 128, key heads are fewer than 2^16 and heads than 2^24; a pool
+ * has fewer than 2^31 (position, head) rows and may have any size in bytes;
+ * page_tokens >= 1.
  *
  * Formats of a page:
  *   WF_KV_E4M3  wf_fp8_kv_pack's codes and scales;

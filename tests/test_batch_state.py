@@ -84,3 +84,16 @@ def test_a_scale_that_overflows_in_base_2_is_refused(scale):
     args = (16, 4, 4, 2, 128, 512, 32, 48, 8, 256, 64, 80, 1, 4, 8, scale, 96, 512, None, 0, None)
     with pytest.raises(RuntimeError, match="softmax_scale"):
         _lib.call("wf_attn_cross_batch", *args)
+
+
+@pytest.mark.parametrize("heads", [1 << 16, 1 << 24, 1 << 25])
+def test_rows_of_heads_past_32_bit_offsets_are_refused(heads):
+    """Elements are placed in a row by 32-bit numbers; the entry points take fewer heads than would pass them."""
+    ld = 128 * heads
+    with pytest.raises(RuntimeError, match="2\\^16 or more"):
+        _lib.call("wf_kv_batch_append", 16, 32, 1, heads, 128, ld, 0, 48, 64, 1, 80, 1, 1, 96, 112, 128, 144, 1, None)
+    with pytest.raises(RuntimeError, match="2\\^16 or more"):
+        _lib.call("wf_kv_batch_gather", 96, 112, 128, 144, 1, 0, 1, 48, 64, 1, 80, 1, 1, heads, 128, 16, 32, ld, None)
+    if heads >= 1 << 24:
+        with pytest.raises(RuntimeError, match="2\\^24 or more"):
+            _lib.call("wf_attn_cross_batch", 16, 1, heads, 1, 128, ld, 32, 48, 8, 256, 64, 80, 1, 1, 8, 0.1, 96, ld, None, 0, None)

@@ -147,6 +147,7 @@ int common_args(const char* fn, Args& a, const void* q, int64_t n_rows, int32_t 
                 int64_t ldq, float softmax_scale, void* out, int64_t ldo) {
   WF_REQUIRE(n_heads > 0 && n_heads % n_kv_heads == 0, WF_E_SHAPE, "%s: %d heads do not group over %d key heads", fn,
              n_heads, n_kv_heads);
+  WF_REQUIRE(n_heads < (1 << 24), WF_E_SHAPE, "%s: %d heads, 2^24 or more", fn, n_heads);  // (as check_batch's)
   WF_REQUIRE(softmax_scale >= 0.f && std::isfinite(softmax_scale * kLog2e), WF_E_INVALID,
              "%s: softmax_scale=%g must not be negative, and finite as a factor of base-2 exponents too", fn,
              static_cast<double>(softmax_scale));
@@ -174,8 +175,7 @@ int launch(const char* fn, Args& a, int src, int64_t n_seqs, int64_t max_new, in
   const Plan p = make_plan(src == SRC_DENSE, a.n_rows, static_cast<int64_t>(a.n_kv_heads) * a.group, a.n_kv_heads, n_seqs, max_new, max_kv);
   WF_REQUIRE(p.fits, WF_E_SHAPE, "%s: %lld row tiles x %d key heads x %lld splits are too many", fn, (long long)p.n_tiles, a.n_kv_heads,
              (long long)p.n_splits);
-  WF_REQUIRE(a.ldkv < (1 << 23) && a.n_kv_heads < (1 << 16), WF_E_SHAPE, "%s: key rows of %lld elements or %d heads", fn,
-             (long long)a.ldkv, a.n_kv_heads);
+  WF_REQUIRE(a.ldkv < (1 << 23), WF_E_SHAPE, "%s: key rows of %lld elements", fn, (long long)a.ldkv);
   WF_REQUIRE(ws_bytes >= p.bytes && (p.bytes == 0 || ws), WF_E_INVALID, "%s: a workspace of %lld bytes where %lld are needed", fn,
              (long long)ws_bytes, (long long)p.bytes);
   WF_REQUIRE(aligned(ws, 16), WF_E_ALIGN, "%s: the workspace must be 16-byte aligned", fn);

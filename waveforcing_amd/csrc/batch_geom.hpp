@@ -72,6 +72,8 @@ inline int check_batch(const char* fn, int64_t n_rows, int32_t n_kv_heads, int32
              "%s: negative or zero size (rows=%lld kv_heads=%d seqs=%lld)", fn, (long long)n_rows, n_kv_heads,
              (long long)n_seqs);
   WF_REQUIRE(head_dim == 128, WF_E_SHAPE, "%s: head_dim=%d unsupported (must be 128)", fn, head_dim);
+  // (an element's place in its row is counted in 32 bits)
+  WF_REQUIRE(n_kv_heads < (1 << 16), WF_E_SHAPE, "%s: %d key heads, 2^16 or more", fn, n_kv_heads);
   WF_REQUIRE(n_seqs < (1ll << 20), WF_E_SHAPE, "%s: more than 2^20 sequences", fn);
   WF_REQUIRE(n_seqs == 0 || n_rows == 0 || (cu && kv_lens), WF_E_INVALID, "%s: null row starts or lengths", fn);
   return WF_OK;
