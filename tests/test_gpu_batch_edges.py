@@ -269,3 +269,28 @@ def test_a_new_output_without_sequences_is_refused_at_the_entry():
         _lib.call("wf_attn_cross_batch_fresh", x.data_ptr(), 4, 2, 2, 128, 256, x.data_ptr(), x.data_ptr(), 4, 256, None, None, 0, 4,
                   4, 1.0, x.data_ptr(), 256, None, 0, None)
     assert PagedBatch(Fp8PagePool(1, 2, 128, 16, DEV), [], []).gather()[0].shape == (0, 2, 128)
+
+
+@pytest.mark.parametrize("new", [2, 100])
+@pytest.mark.parametrize("shift", [1, 4])
+def test_dense_rows_at_any_address(new, shift):
+    """Contiguous rows that begin in the middle of a 16-byte word are copied, not refused."""
+    g = gen(410)
+
+    def at_shift(x):
+        flat = torch.empty(x.numel() + shift, dtype=x.dtype, device=DEV)
+        y = flat[shift:].view(x.shape)
+        y.copy_(x)
+        assert y.data_ptr() % 16 and y.is_contiguous()
+        return y
+
+    pool, batch, _ = make("int8", 2, 16, [new + 30], [new], 411)
+    other, same_pages, _ = make("int8", 2, 16, [new + 30], [new], 411)
+    q, k, v = rows(new, 4, g), rows(new, 2, g), rows(new, 2, g)
+    batch.append(k, v)
+    same_pages.append(at_shift(k), at_shift(v))
+    same(pool.k_codes, other.k_codes)
+    same(pool.v_scales, other.v_scales)
+    same(backend.attn_paged_batch(at_shift(q), batch, block=1), backend.attn_paged_batch(q, batch, block=1))
+    cross = CrossBatch([new], [new], DEV)
+    same(backend.attn_cross_batch(at_shift(q), at_shift(k), v, cross), backend.attn_cross_batch(q, k, v, cross))

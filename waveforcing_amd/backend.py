@@ -28,7 +28,7 @@ from typing import Callable
 import torch
 
 from . import _lib
-from .kv import CrossBatch, PagedBatch, PagedKV
+from .kv import CrossBatch, PagedBatch, PagedKV, dense
 
 ATTENTION_BACKENDS = ("torch_sdpa", "fa_custom", "sa", "fa", "fa2", "hip_fp8", "hip_fp8_qk", "hip_fp8_qkpv")
 
@@ -137,7 +137,7 @@ def _batch_rows(q: torch.Tensor, out: torch.Tensor | None, rows: int, device):
     if N < rows:
         raise ValueError(f"q has {N} rows, the batch {rows}")
     if q.stride(2) != 1 or q.stride(1) != D or q.data_ptr() % 16 or q.stride(0) % 8 or (N > 1 and q.stride(0) < H * D):
-        q = q.contiguous()
+        q = dense(q)
     if out is None:
         out = torch.empty((N, H, D), dtype=torch.bfloat16, device=device)
         if N > rows:
@@ -202,14 +202,14 @@ def attn_cross_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: C
     if not hkv or H % hkv or not H:
         raise ValueError(f"{H} query heads do not group over {hkv} key heads")
 
-    def dense(t):
+    def rows_of(t):
         if t.stride(2) != 1 or t.stride(1) != D or t.stride(0) % 8 or t.data_ptr() % 16 or (rows > 1 and t.stride(0) < hkv * D):
-            t = t.contiguous()
+            t = dense(t)
         return t
 
-    k, v = dense(k), dense(v)
+    k, v = rows_of(k), rows_of(v)
     if rows > 1 and k.stride(0) != v.stride(0):
-        k, v = k.contiguous(), v.contiguous()
+        k, v = dense(k), dense(v)
     cu_q, cu_kv, n_seqs, max_q, max_kv = batch._geom
     n = batch.workspace_bytes(H, hkv)
     ws = torch.empty((n,), dtype=torch.uint8, device=batch.device) if n else None

@@ -53,6 +53,12 @@ class PageTable:
         return len(self.host)
 
 
+def dense(x: torch.Tensor) -> torch.Tensor:
+    """x contiguous and 16-byte aligned, as the kernels read it; a copy if it is not."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
 def _as_thd(x: torch.Tensor, name: str):
     """Accept [T, H, D] or the reference's [1, T, H, D] views (paged.py:207-208) and return
     (tensor, address, (T, H, D), token stride) of the data the kernels read.
@@ -75,7 +81,7 @@ def _as_thd(x: torch.Tensor, name: str):
     s0, s1, s2 = strides
     addr = x.data_ptr()
     if s2 != 1 or s1 != D or s0 % 8 or addr % 16 or (T > 1 and s0 < H * D):
-        x = x.reshape(T, H, D).contiguous()
+        x = dense(x.reshape(T, H, D))
         addr, s0 = x.data_ptr(), H * D
     return x, addr, (T, H, D), (s0 if T > 1 else H * D)
 
@@ -409,7 +415,7 @@ class PagedBatch:
         if v is not None:
             vt, vp, vld = self._rows(v, "v")
             if vld != ld:   # one row stride serves K and V
-                kt, vt = kt.reshape(-1, pool.n_heads, 128).contiguous(), vt.reshape(-1, pool.n_heads, 128).contiguous()
+                kt, vt = dense(kt.reshape(-1, pool.n_heads, 128)), dense(vt.reshape(-1, pool.n_heads, 128))
                 kp, vp, ld = kt.data_ptr(), vt.data_ptr(), pool.n_heads * 128
         _lib.call_on(self.device, "wf_kv_batch_append", kp, vp, self.n_new, pool.n_heads, pool.head_dim, ld, pool.format,
                      *self._geom, pool.page_tokens, pool._k_codes_p, pool._v_codes_p, pool._k_scales_p,
