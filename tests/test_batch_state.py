@@ -3,9 +3,10 @@
 import ctypes
 
 import pytest
+import torch
 
-from waveforcing_amd import _lib
-from waveforcing_amd.kv import Fp8PagePool, Int8PagePool, PagedBatch
+from waveforcing_amd import _lib, backend
+from waveforcing_amd.kv import CrossBatch, Fp8PagePool, Int8PagePool, PagedBatch
 
 
 def pool(cls=Fp8PagePool):
@@ -97,3 +98,13 @@ def test_rows_of_heads_past_32_bit_offsets_are_refused(heads):
     if heads >= 1 << 24:
         with pytest.raises(RuntimeError, match="2\\^24 or more"):
             _lib.call("wf_attn_cross_batch", 16, 1, heads, 1, 128, ld, 32, 48, 8, 256, 64, 80, 1, 1, 8, 0.1, 96, ld, None, 0, None)
+
+
+def test_tensors_on_the_cpu_are_refused_by_name():
+    b, c = PagedBatch(pool(), [[0]], [5], [3]), CrossBatch([3], [3], "cpu")
+    x = torch.zeros((3, 2, 128), dtype=torch.bfloat16)
+    for name, run in (("wf_kv_batch_append", lambda: b.append(x, x)), ("wf_kv_batch_gather", lambda: b.gather()),
+                      ("wf_attn_paged_batch", lambda: backend.attn_paged_batch(x, b)),
+                      ("wf_attn_cross_batch", lambda: backend.attn_cross_batch(x, x, x, c))):
+        with pytest.raises(ValueError, match=f"{name}.*on cpu"):
+            run()

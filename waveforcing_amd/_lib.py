@@ -220,6 +220,8 @@ def call_on(device, name: str, *args) -> None:
     with that device current."""
     import torch
 
+    if device.index is None:   # the CPU
+        raise ValueError(f"{name}: the tensors are on {device}; the kernels run on a GPU")
     if torch._C._cuda_getDevice() == device.index:
         call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
