@@ -431,16 +431,17 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads,
  * a chunk).  Rows without a key are zero; a row of q that holds a NaN or an
  * infinity is NaN, and so are the rows that see a key with a scale of K or V
  * that is NaN or infinite; no NaN or infinity of a key reaches a row that does
- * not see it.  fp32 scores, softmax and sums.  Up to 64 (row, head) rows of a
+ * not see it.  softmax_scale is not negative.  fp32 scores (of e4m3 keys from
+ * q held to 2^-13 of its row's largest value), softmax and sums.  Up to 64 (row, head) rows of a
  * sequence per key head the weights p_j s_v[j] are held in 16 significant
  * bits; with more, in 11 (fp16: those below 2^-20 of the largest that the row
  * sees lose bits, and so do all where the scales of V are below 2^-100).
  * max_new and max_kv bound the sequences' rows and keys; they choose the
- * split, and results stay right where the device's lengths pass them.  ws: ws_bytes of scratch,
- * 16-byte aligned, at least wf_attn_batch_workspace's.  The attention of
- * wf_attn_paged_fp8 for a batch (wave_rt/runtime/backend.py:141-148), with
- * the block-causal mask of naive_rt/rolling_forcing/wan/modules/
- * causal_model.py as an argument. */
+ * split, and with it the order of the sums, and results stay right where the
+ * device's lengths pass them.  ws: ws_bytes of scratch, 16-byte aligned, at
+ * least wf_attn_batch_workspace's.  The attention of wf_attn_paged_fp8 for a
+ * batch (wave_rt/runtime/backend.py:141-148), with the block-causal mask of
+ * naive_rt/rolling_forcing/wan/modules/causal_model.py as an argument. */
 int wf_attn_paged_batch(const void* q, int64_t n_rows, int32_t n_heads,
                         int32_t n_kv_heads, int32_t head_dim, int64_t ldq,
                         int32_t format, const uint8_t* k_codes,
@@ -457,7 +458,8 @@ int wf_attn_paged_batch(const void* q, int64_t n_rows, int32_t n_heads,
  * cu_kv[b + 1] of k and v [n_kv_rows][n_kv_heads][128] (row stride ldkv), all
  * of them visible to its query rows cu_q[b] .. cu_q[b + 1].  The text
  * cross-attention with each prompt's own length; the weights in 16 significant
- * bits up to 64 rows, in bf16 with more (naive_rt/rolling_forcing/
+ * bits up to 64 rows, in bf16 with more; a row of q that holds a NaN or an
+ * infinity is NaN (naive_rt/rolling_forcing/
  * wan/modules/model.py:165-189). */
 int wf_attn_cross_batch(const void* q, int64_t n_rows, int32_t n_heads,
                         int32_t n_kv_heads, int32_t head_dim, int64_t ldq,

@@ -103,8 +103,8 @@ Plan make_plan(bool dense, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads, 
     // In times of one 64-key tile of a workgroup (about 2 us; one workgroup to a CU, of 128 rows two): a piece takes its
     // tiles and a fixed part of about 4; the rounds of pieces of one sequence (the pieces of several, whose lengths
     // differ, spread over the CUs, the longest first, with little at the end); partial results of 256 rows are written and
-    // read at about 0.03.  Six sequences of up to 10001 keys, 800 tiles: 412 us whole, 498 in two, 511 in four; 8 over up to
-    // 4001 dense keys, 216 tiles: 77 whole, 55 in three, 58 in eight.
+    // read at about 0.03.  Six sequences of up to 10001 keys, 800 tiles: 388 us whole, 466 in two, 494 in four; 8 over up to
+    // 4001 dense keys, 216 tiles: 69 whole, 50 in three, 57 in eight.
     const double tiles = static_cast<double>((max_kv + 63) / 64);
     double best = 0;
     for (int64_t s = 1; s <= kJoinSplits && (s == 1 || tiles / s >= 8); ++s) {

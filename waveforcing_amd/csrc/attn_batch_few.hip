@@ -17,9 +17,9 @@
 // codes of both formats exact in bf16.  The scales are applied in fp32, s_k c to the scores and s_v to the weights, and
 // the weights go in as the sum of two bf16 (16 significant bits; the matrix cores are idle most of the time anyway).
 //
-// Measured: 64 single tokens of 40 heads over 8 key heads and 8192 keys each 214-223 us (4.9-5.2 TB/s), 256 over 2048 206 us
-// (5.4), 12 over 37440 of 12 heads 260 us (5.5).  With 17 to 64 rows the vector work bounds it: 48 sequences of 25 rows
-// over 8192 keys 186 us (4.5), of 60 rows 320 us.
+// Measured: 64 single tokens of 40 heads over 8 key heads and 8192 keys each 219-224 us (4.9-5.1 TB/s), 256 over 2048 208 us
+// (5.3), 12 over 37440 of 12 heads 272 us (5.2).  With 17 to 64 rows the vector work bounds it: 48 sequences of 25 rows
+// over 8192 keys of 8 heads 189 us (4.4), of 60 rows 322 us.
 #include "attn_batch.hpp"
 
 namespace wf {

@@ -7,9 +7,10 @@
 // second operand of O^T += V^T P^T, whose first operand comes from the staged rows by transposing reads (attn_paged.hip
 // has the layouts).
 //
-// 3 x 4680 rows over up to 37440 keys of 12 heads: 2.18 ms, 0.98 PFLOP/s (one sequence at a time, csrc/attn_paged.hip: 1.0
-// PFLOP/s with bf16 keys and weights); a tile takes 2.0 us of a CU, half of it matrix instructions and half the vector work
-// of the weights (1.06 PFLOP/s on zeros, 0.97 on N(0, 1) data over 18720 keys: instructions first, power close behind).
+// 3 x 4680 rows over up to 37440 keys of 12 heads: 2.17-2.23 ms, 0.97 PFLOP/s (one sequence at a time, csrc/attn_paged.hip: 1.0
+// PFLOP/s with bf16 keys and weights).  Of the cycles in which a CU has work (85 % of the kernel's) the matrix cores are busy
+// 51 % and the vector unit issues 59 %, the matrix instructions' own 5 % among them.  Over 18720 keys 1.10 PFLOP/s on
+// zeros and 0.98 on N(0, 1) data, int8 0.97 and 0.88: instructions first, power close behind.
 //
 // What is rounded, and where:
 //   e4m3 keys  the codes go to the fp8 matrix cores as they are, Q as the sum of two e4m3 parts under a power-of-two scale
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 
   // Item: runs of kRun neighbouring row tiles go to the XCDs in turn (workgroups are dealt to them round-robin), the
   // heads of a run one after the other.  The last tiles of a sequence, whose causal rows see most, come first in every
-  // head, so that little is left at the end (two clips of 7 frames: 737 us, 818 with a head after the other).
+  // head, so that little is left at the end (two clips of 7 frames: 10 % less time than with a head after the other).
   const int runs = (a.n_tiles + kRun - 1) / kRun;
   const int xcd = static_cast<int>(blockIdx.x) % kXcds, slot = static_cast<int>(blockIdx.x) / kXcds;
   const int i_run = (slot / kRun) * kXcds + xcd;

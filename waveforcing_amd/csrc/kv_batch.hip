@@ -13,7 +13,7 @@
 // maximum that gives a also tells a row that holds one: it is stored as scale NaN and zero codes, and reads back as NaN
 // whole in both formats, instead of as a finite row of a scale that its other values set.
 //
-// Four chunks of 4680 rows of 12 heads: append 39-41 us (4.3-4.5 TB/s of 174 MB), gather 29 us (5.9); 64 single rows 4 us
+// Four chunks of 4680 rows of 12 heads: append 40-41 us (4.3 TB/s of 174 MB), gather 30 us (5.8); 64 single rows 4 us
 // each, the launch.
 #include "batch_geom.hpp"
 #include "kv_row.hpp"
