@@ -469,9 +469,10 @@ int wf_attn_cross_batch(const void* q, int64_t n_rows, int32_t n_heads,
                         int64_t max_kv, float softmax_scale, void* out,
                         int64_t ldo, void* ws, int64_t ws_bytes, void* stream);
 
-/* The last three into new outputs: rows before n_rows that no sequence owns
- * when the work runs (wf_kv_batch_gather_fresh: that have no position) are
- * zeroed instead of left as they are. */
+/* wf_kv_batch_gather, wf_attn_paged_batch and wf_attn_cross_batch into new
+ * outputs: rows before n_rows that no sequence owns when the work runs
+ * (wf_kv_batch_gather_fresh: that have no position) are zeroed instead of left
+ * as they are.  Rows need a sequence (n_seqs > 0). */
 int wf_kv_batch_gather_fresh(const uint8_t* k_codes, const uint8_t* v_codes,
                              const float* k_scales, const float* v_scales,
                              int64_t pool_pages, int32_t format,
