@@ -274,6 +274,61 @@ int wf_fp8_linear_pertensor(const void* x, int64_t m, int64_t k, int64_t ldx,
                             uint8_t* ws_codes, float* ws_scale,
                             float* ws_partials, void* stream);
 
+/* ------------------------------------------------- MXFP4: 4-bit rows
+ *
+ * Microscaled 4-bit floating point: blocks of 32 consecutive values, e2m1
+ * codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) under a power of
+ * two.  Per block, with a = max|x|:
+ *   s    = the smallest power of two with a < 7 s, at least 2^-125 and at
+ *          most 2^125; scale byte E with s = 2^(E - 127) (E8M0)
+ *   code = the nearest e2m1 number to x / s, an even code on a tie, at most 6
+ * (no value is off by more than half the step of its binade).  A block that
+ * holds a NaN or an infinity is E = 255 with zero codes, and reads back as NaN.
+ *
+ * Layout of rows x [rows][k], k % 32 == 0:
+ *   codes  u8 [rows][k / 2], the even value of a pair in the low half
+ *   scales u8 [ceil(k / 128)][rows4][4], rows4 = rows rounded up to 4: byte
+ *          b of (g, r) is that of values 128 g + 32 b .. + 31 of row r, 0
+ *          where the row has no such values or there is no row
+ * The 4-bit counterpart of the reference's W8A8 linear (wave_rt/runtime/
+ * fp8.py:21-61); it has no 4-bit form itself.
+ */
+
+/* Rows of bf16 x (row stride ldx) into codes and scales, as activations (rows
+ * = tokens) or weights (rows = output channels).  x, codes and scales 16-byte
+ * aligned, ldx % 8 == 0. */
+int wf_mxfp4_quant(const void* x, int64_t rows, int64_t k, int64_t ldx,
+                   uint8_t* codes, uint8_t* scales, void* stream);
+
+/* The values of codes and scales as bf16 [rows][k] (row stride ldo, a multiple
+ * of 8), exact for scale bytes 2 .. 252; 255 reads as NaN. */
+int wf_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales,
+                     int64_t rows, int64_t k, void* out, int64_t ldo,
+                     void* stream);
+
+#define WF_MXFP4_FUSED_ROWS 16
+
+/* y[m][n] = bf16(act(sum_k a[m,k] w[n,k] + bias[n])) of two MXFP4 operands
+ * (rows of a, rows of w), fp32 sums; bias bf16 [n] or NULL; act GELU(tanh)
+ * with flags & WF_GEMM_GELU_TANH, in fp32 (rounded once).  A scale byte of
+ * 255 makes its row of a (of w: its column of y) NaN.  k % 32 == 0; n, ldy %
+ * 4 == 0; codes and scales 16-byte, y and bias 8-byte aligned; codes of an
+ * operand fewer than 2^31 bytes.  The order of the sums goes by the sizes. */
+int wf_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scales,
+                  const uint8_t* w, const uint8_t* w_scales, int64_t m,
+                  int64_t n, int64_t k, const void* bias, void* y,
+                  int64_t ldy, int32_t flags, void* stream);
+
+/* wf_mxfp4_quant of bf16 x [m][k] (row stride ldx) followed by wf_gemm_mxfp4,
+ * with the same results bit for bit.  Up to WF_MXFP4_FUSED_ROWS rows are
+ * quantized inside the product's kernel and need no workspace; above,
+ * ws_codes and ws_scales hold the quantized rows (sizes as the layout's). */
+int wf_mxfp4_linear(const void* x, int64_t m, int64_t k, int64_t ldx,
+                    const uint8_t* w, const uint8_t* w_scales,
+                    const void* bias, int64_t n, void* y, int64_t ldy,
+                    int32_t flags, uint8_t* ws_codes, uint8_t* ws_scales,
+                    void* stream);
+
 /* ------------------------------------------------ FP8 KV, per tensor
  *
  * The reference's per-tensor FP8 KV exchange (_all_gather_fp8,

@@ -91,6 +91,15 @@ SIGNATURES: dict[str, list] = {
         _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
         _c_void_p, _c_void_p, _c_void_p, _c_void_p,
     ],
+    "wf_mxfp4_quant": [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p],
+    "wf_mxfp4_dequant": [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p],
+    "wf_gemm_mxfp4": [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i32, _c_void_p,
+    ],
+    "wf_mxfp4_linear": [
+        _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _c_void_p,
+        _c_void_p,
+    ],
     "wf_attn_paged_fp8": [
         _c_void_p, _i64, _i32, _i32, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
         _i64, _i32, _c_void_p, _i64, _i64, _f32, _c_void_p, _i64, _c_void_p,
@@ -154,6 +163,7 @@ BF16_SILU_OUT = 2
 BF16_GELU_OUT = 4
 KV_E4M3 = 0
 KV_INT8 = 1
+MXFP4_FUSED_ROWS = 16
 W8A8_STATIC_MAX_CODES = 64 << 20
 W8A8_STATIC_MAX_ROWS = 65536
 

@@ -24,4 +24,7 @@ int launch_gemm_fp8_pertensor(const uint8_t* a, const uint8_t* w, int64_t M, int
 int launch_fp8_quant_pertensor(const void* x, int64_t rows, int64_t k, int64_t ldx, int mode, uint8_t* codes,
                                float* scale, float* partials, hipStream_t stream);
 
+int launch_mxfp4_quant(const void* x, int64_t rows, int64_t k, int64_t ldx, uint8_t* codes, uint8_t* scales,
+                       hipStream_t stream);
+
 }  // namespace wf

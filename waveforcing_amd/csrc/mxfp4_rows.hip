@@ -1,0 +1,125 @@
+// Rows of bf16 into MXFP4 codes and scales (weights once, activations at every call), and back.  Both stream through HBM:
+// 2 bytes a value on one side, 17/32 on the other.
+//
+// Layout: codes [rows][k / 2]; scales [ceil(k / 128)][rows4][4], rows4 = rows rounded up to 4: byte b of (g, r) belongs to
+// the values 128 g + 32 b .. + 31 of row r (0 where the row has none).  So the scales of the K range that a matrix
+// instruction or an LDS stage takes from neighbouring rows are contiguous, one word a row.
+//
+// A wave takes 4 rows x 512 values: one 16-byte load a lane and row, a block in 4 lanes, whose maximum is two DPP steps; a
+// lane's 8 codes are one word, and the 4 rows' scale words leave as 16 bytes of one lane in 16.
+#include "launchers.hpp"
+#include "mxfp4_codec.hpp"
+
+namespace wf {
+namespace {
+
+constexpr int kRows = 4;        // of a wave
+constexpr int kChunk = 512;     // values of a row that a wave takes
+constexpr int kWaves = 4;
+
+template <int CTRL>
+__device__ inline uint32_t dpp(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
+}
+
+__global__ __launch_bounds__(64 * kWaves) void mxfp4_quant_kernel(const uint16_t* x, int rows, int k, int64_t ldx, uint8_t* codes,
+                                                                  uint8_t* scales, int rows4) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int row0 = (static_cast<int>(blockIdx.x) * kWaves + (static_cast<int>(threadIdx.x) >> 6)) * kRows;
+  if (row0 >= rows) return;
+  const int at = static_cast<int>(blockIdx.y) * kChunk + 8 * lane;  // (k % 32 == 0: a block is there or not, whole)
+  uint4 v[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    v[r] = make_uint4(0, 0, 0, 0);
+    if (row0 + r < rows && at < k) v[r] = *reinterpret_cast<const uint4*>(x + (row0 + r) * ldx + at);
+  }
+  uint32_t word[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const uint32_t w[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+    uint32_t top = mx::max_half(mx::max_bits2(mx::max_bits2(w[0], w[1]), mx::max_bits2(w[2], w[3])));
+    top = max(top, dpp<0xB1>(top));  // quad_perm [1,0,3,2], [2,3,0,1]
+    top = max(top, dpp<0x4E>(top));
+    const int e = mx::scale_byte(top);
+    uint32_t c = mx::encode8(w, mx::scale_of(e));
+    if (e == mx::kNanE) c = 0;
+    const bool there = row0 + r < rows && at < k;
+    if (there) *reinterpret_cast<uint32_t*>(codes + static_cast<int64_t>(row0 + r) * (k >> 1) + (at >> 1)) = c;
+    // the four blocks' bytes of 16 lanes as one word
+    uint32_t s = there ? static_cast<uint32_t>(e) << (8 * ((lane >> 2) & 3)) : 0u;
+    s |= dpp<0x124>(s);  // row_ror:4, 8
+    s |= dpp<0x128>(s);
+    word[r] = s;
+  }
+  const int g = static_cast<int>(blockIdx.y) * (kChunk / 128) + (lane >> 4);
+  if ((lane & 15) == 0 && at < k)
+    *reinterpret_cast<uint4*>(scales + (static_cast<int64_t>(g) * rows4 + row0) * 4) = make_uint4(word[0], word[1], word[2], word[3]);
+}
+
+__global__ __launch_bounds__(64 * kWaves) void mxfp4_dequant_kernel(const uint8_t* codes, const uint8_t* scales, int rows, int k,
+                                                                    int rows4, uint16_t* out, int64_t ldo) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int row0 = (static_cast<int>(blockIdx.x) * kWaves + (static_cast<int>(threadIdx.x) >> 6)) * kRows;
+  const int at = static_cast<int>(blockIdx.y) * kChunk + 8 * lane;
+  if (row0 >= rows || at >= k) return;
+  const int g = at / 128;
+  const uint4 s = *reinterpret_cast<const uint4*>(scales + (static_cast<int64_t>(g) * rows4 + row0) * 4);
+  const uint32_t word[kRows] = {s.x, s.y, s.z, s.w};
+  uint32_t c[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r)
+    c[r] = row0 + r < rows ? *reinterpret_cast<const uint32_t*>(codes + static_cast<int64_t>(row0 + r) * (k >> 1) + (at >> 1)) : 0u;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r)
+    if (row0 + r < rows)
+      *reinterpret_cast<uint4*>(out + (row0 + r) * ldo + at) = mx::decode8(c[r], mx::scale_of((word[r] >> (8 * ((lane >> 2) & 3))) & 0xffu));
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Checks that both directions share.
+int check_rows(const char* fn, const void* dense, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, int64_t ld) {
+  WF_REQUIRE(rows >= 0 && k >= 0 && ld >= k, WF_E_INVALID, "%s: bad sizes rows=%lld k=%lld row stride=%lld", fn, (long long)rows,
+             (long long)k, (long long)ld);
+  WF_REQUIRE(k % mx::kBlock == 0, WF_E_SHAPE, "%s: k=%lld must be a multiple of 32", fn, (long long)k);
+  // (a grid holds fewer than 2^32 threads, 16 for a row; chunks of a row are its y, at most 65535)
+  WF_REQUIRE(rows < (1ll << 28) - 64 && k <= 65535ll * kChunk, WF_E_SHAPE, "%s: rows=%lld or k=%lld too large", fn, (long long)rows, (long long)k);
+  if (rows == 0 || k == 0) return WF_OK;
+  WF_REQUIRE(dense && codes && scales, WF_E_INVALID, "%s: null pointer", fn);
+  WF_REQUIRE(aligned(dense, 16) && ld % 8 == 0 && aligned(codes, 16) && aligned(scales, 16), WF_E_ALIGN,
+             "%s: rows, codes and scales must be 16-byte aligned, the row stride a multiple of 8", fn);
+  return WF_OK;
+}
+
+dim3 rows_grid(int64_t rows, int64_t k) {
+  return dim3(static_cast<uint32_t>((rows + kRows * kWaves - 1) / (kRows * kWaves)), static_cast<uint32_t>((k + kChunk - 1) / kChunk));
+}
+
+}  // namespace
+
+int launch_mxfp4_quant(const void* x, int64_t rows, int64_t k, int64_t ldx, uint8_t* codes, uint8_t* scales, hipStream_t stream) {
+  hipLaunchKernelGGL(mxfp4_quant_kernel, rows_grid(rows, k), dim3(64 * kWaves), 0, stream, static_cast<const uint16_t*>(x),
+                     static_cast<int>(rows), static_cast<int>(k), ldx, codes, scales, static_cast<int>((rows + 3) / 4 * 4));
+  return check_launch("wf_mxfp4_quant");
+}
+
+}  // namespace wf
+
+extern "C" {
+
+int wf_mxfp4_quant(const void* x, int64_t rows, int64_t k, int64_t ldx, uint8_t* codes, uint8_t* scales, void* stream) {
+  if (int st = wf::check_rows("wf_mxfp4_quant", x, codes, scales, rows, k, ldx)) return st;
+  if (rows == 0 || k == 0) return WF_OK;
+  return wf::launch_mxfp4_quant(x, rows, k, ldx, codes, scales, wf::as_stream(stream));
+}
+
+int wf_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t ldo, void* stream) {
+  if (int st = wf::check_rows("wf_mxfp4_dequant", out, codes, scales, rows, k, ldo)) return st;
+  if (rows == 0 || k == 0) return WF_OK;
+  hipLaunchKernelGGL(wf::mxfp4_dequant_kernel, wf::rows_grid(rows, k), dim3(64 * wf::kWaves), 0, wf::as_stream(stream), codes, scales,
+                     static_cast<int>(rows), static_cast<int>(k), static_cast<int>((rows + 3) / 4 * 4), static_cast<uint16_t*>(out), ldo);
+  return wf::check_launch("wf_mxfp4_dequant");
+}
+
+}  // extern "C"
