@@ -437,11 +437,18 @@ int wf_attn_dense_bf16(const void* q, int64_t lq, int32_t n_heads,
  *   WF_KV_E4M3  wf_fp8_kv_pack's codes and scales;
  *   WF_KV_INT8  s = max(max|x| / 127, 1e-8), code = clamp(rint(x / s), -127,
  *               127) (fp32; wf_act_quant_i8's arithmetic per (token, head)),
- *               the codes as signed bytes.
+ *               the codes as signed bytes;
+ *   WF_KV_MXFP4 wf_mxfp4_quant's codes and scale bytes of the row's four
+ *               blocks: codes u8 [pool_pages][page_tokens][n_kv_heads][64],
+ *               and in the place of the fp32 scale of (page, head, row) its
+ *               4 bytes (the pointers to scales point to those).  A byte of
+ *               255, and 253 and 254, which append never writes, make the
+ *               key one with a NaN scale.
  * ------------------------------------------------------------------- */
 
 #define WF_KV_E4M3 0
 #define WF_KV_INT8 1
+#define WF_KV_MXFP4 4
 
 /* Quantize the rows of K and V (bf16 [n_rows][n_kv_heads][128], row stride
  * ld_kv; V may be NULL with its pools) into their positions' pages.  A row

@@ -151,3 +151,36 @@ def test_scale_byte_from_the_bits_is_the_definition():
     block = torch.zeros((len(x), 32), dtype=torch.bfloat16)
     block[:, 0] = x
     assert torch.equal(om.quantize(block)[1][:, 0].long(), byte)
+
+
+# -------------------------------------------------------------------- pages
+def test_page_pools():
+    from waveforcing_amd.kv import Fp8PagePool, Int8PagePool, Mxfp4PagePool
+
+    pool = Mxfp4PagePool(3, 2, 128, 16, "cpu")
+    assert pool.k_codes.shape == (3, 16, 2, 64) and pool.v_scales.shape == (3, 2, 16, 4) and pool.v_scales.dtype == torch.uint8
+    assert pool.nbytes == Mxfp4PagePool.bytes_for(3, 2, 128, 16)
+    for call in (pool.pack, pool.unpack, pool.pack_k_norm_rope):
+        with pytest.raises(TypeError, match="MXFP4 pages"):
+            call()
+    for other in (Fp8PagePool, Int8PagePool):
+        with pytest.raises(TypeError, match="another code format"):
+            other.view_of(pool, 0, 1)
+        with pytest.raises(TypeError, match="another code format"):
+            Mxfp4PagePool.view_of(other(3, 2, 128, 16, "cpu"), 0, 1)
+    assert Mxfp4PagePool.view_of(pool, 1, 2).k_scales.data_ptr() == pool.k_scales[1].data_ptr()
+
+
+def test_one_sequence_attention_refuses_the_pages():
+    from waveforcing_amd import backend
+    from waveforcing_amd.kv import Mxfp4PagePool, PagedKV
+
+    pool = Mxfp4PagePool(3, 2, 128, 64, "cpu")
+    with pytest.raises(Exception, match="e4m3"):
+        backend.attn_paged_fp8(torch.zeros((1, 2, 128), dtype=torch.bfloat16), PagedKV(pool, pool.page_table([0]), 1))
+
+
+def test_unknown_formats_are_refused():
+    for fmt in (-1, 2, 3, 5):
+        with pytest.raises(RuntimeError, match="unknown cache format"):
+            _lib.call("wf_kv_batch_append", 16, 16, 1, 2, 128, 256, fmt, 16, 16, 1, 16, 1, 16, 16, 16, 16, 16, 4, None)

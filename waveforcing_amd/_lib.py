@@ -163,6 +163,7 @@ BF16_SILU_OUT = 2
 BF16_GELU_OUT = 4
 KV_E4M3 = 0
 KV_INT8 = 1
+KV_MXFP4 = 4
 MXFP4_FUSED_ROWS = 16
 W8A8_STATIC_MAX_CODES = 64 << 20
 W8A8_STATIC_MAX_ROWS = 65536

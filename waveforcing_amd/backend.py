@@ -81,7 +81,7 @@ def attn_paged_fp8(q: torch.Tensor, k: PagedKV, v: PagedKV | None = None, causal
     Lq, H, D = q3.shape
     pool = k.pool
     if pool.format != _lib.KV_E4M3:
-        raise TypeError("hip_fp8 attention reads e4m3 pages; int8 pages are attended through attn_paged_batch")
+        raise TypeError("hip_fp8 attention reads e4m3 pages; int8 and MXFP4 pages are attended through attn_paged_batch")
     if H != pool.n_heads or D != pool.head_dim:
         raise ValueError(f"q heads/dim ({H}, {D}) differ from the pool ({pool.n_heads}, {pool.head_dim})")
     if q3.stride(2) != 1 or q3.stride(1) != D or q3.data_ptr() % 16 or q3.stride(0) % 8:

@@ -8,6 +8,7 @@
 
 #include "batch_geom.hpp"
 #include "fp8_codec.hpp"
+#include "mxfp4_codec.hpp"
 #include "wf_common.hpp"
 
 namespace wf {
@@ -17,7 +18,7 @@ constexpr int D = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxKeys = 0x7fffffff - 1024;  // of a sequence: the tiles that are loaded ahead stay below 2^31
 constexpr float kTau = 8.0f;  // lazy rescale: a row's maximum in its exponents is raised when exceeded by more than this
-enum { SRC_E4M3 = WF_KV_E4M3, SRC_INT8 = WF_KV_INT8, SRC_DENSE = 2 };
+enum { SRC_E4M3 = WF_KV_E4M3, SRC_INT8 = WF_KV_INT8, SRC_MXFP4 = WF_KV_MXFP4, SRC_DENSE = 2 };
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -33,7 +34,7 @@ struct Args {
   uint16_t* out;
   int64_t ldq, ldo;
   const uint8_t *k_codes, *v_codes;
-  const float *k_scales, *v_scales;
+  const float *k_scales, *v_scales;  // MXFP4: 4 bytes in each one's place
   const uint16_t *k_dense, *v_dense;
   const int32_t* cu_kv;  // dense: [n_seqs + 1]
   int64_t ldkv;
@@ -223,6 +224,13 @@ __device__ inline void split_q(const uint4& x, int e, uint2& q1, uint2& q2) {
   }
   q1 = make_uint2(c1[0], c1[1]);
   q2 = make_uint2(c2[0], c2[1]);
+}
+
+// MXFP4 pages: a scale byte that stands for NaN (255; 253 and 254, which nothing writes, would pass bf16's range).
+constexpr int kMxNan = mx::kMaxE + 1;
+// True when a byte of w is one.
+__device__ inline bool has_nan_scale(uint32_t w) {
+  return (w & 0xffu) >= kMxNan || (w >> 8 & 0xffu) >= kMxNan || (w >> 16 & 0xffu) >= kMxNan || (w >> 24) >= kMxNan;
 }
 
 // True when a byte of w is an e4m3 NaN code; the word with those bytes cleared.

@@ -32,10 +32,11 @@ constexpr int kQPitch = 2 * D + 16;
 
 template <int SRC, int NB>
 struct Form {
-  static constexpr bool dense = SRC == SRC_DENSE;
-  static constexpr int row_bytes = dense ? 256 : 128;
+  static constexpr bool dense = SRC == SRC_DENSE, mx = SRC == SRC_MXFP4;
+  static constexpr int row_bytes = dense ? 256 : mx ? 64 : 128;
   static constexpr int k_loads = 2 * row_bytes / 64;   // 16-byte loads a lane makes of the tile's K (and V)
-  static constexpr int v_pitch = dense ? 256 + 32 : 128 + 16;
+  static constexpr bool v_bf16 = dense || mx;          // V in LDS (else its codes)
+  static constexpr int v_pitch = v_bf16 ? 256 + 32 : 128 + 16;
   static constexpr int wave_lds = KT * v_pitch + 64 * 4;  // V rows, then 32 factors of K and 32 of V
   static constexpr bool q_lds = NB > 1;                   // Q is read from LDS at every tile (one row block: registers)
   static constexpr int q_off = W * wave_lds;
@@ -79,7 +80,8 @@ __device__ inline float absmax8(const uint4& v) {
 template <int SRC, int NB>
 __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kernel(Args a) {
   using F = Form<SRC, NB>;
-  constexpr bool kDense = F::dense;
+  constexpr bool kDense = F::dense, kMx = F::mx;
+  constexpr bool kScaled = !kDense && !kMx;  // one fp32 scale a key, applied to scores and weights
   constexpr int R = 16 * NB;
   __shared__ __attribute__((aligned(16))) uint8_t lds[F::lds];
 
@@ -107,6 +109,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
   struct Regs {
     u32x4 k[F::k_loads], v[F::k_loads];
     float fk, fv;
+    int ek[2], ev[2];  // MXFP4: the scale bytes of the lane's blocks
     uint32_t bad;
   };
   // Where a tile's keys live: in one page (uniform; `n` of them to be read, the others read as zero), or each on its own.
@@ -122,7 +125,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     bool there;
   };
   const int pt = a.geom.page_tokens;
-  const int64_t key_bytes = kDense ? a.ldkv * 2 : static_cast<int64_t>(a.n_kv_heads) * D;
+  const int64_t key_bytes = kDense ? a.ldkv * 2 : static_cast<int64_t>(a.n_kv_heads) * F::row_bytes;
   const int64_t k_to_v = kDense ? reinterpret_cast<const uint8_t*>(a.v_dense) - reinterpret_cast<const uint8_t*>(a.k_dense)
                                 : a.v_codes - a.k_codes;
   const int64_t sk_to_sv = reinterpret_cast<const uint8_t*>(a.v_scales) - reinterpret_cast<const uint8_t*>(a.k_scales);
@@ -138,7 +141,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     page = uniform(page);
     const bool ok = page >= 0 && page < a.geom.pool_pages;
     const int pg = ok ? page : 0, r0 = static_cast<int>(at);
-    return Where{r0 + n <= pt, ok ? n : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * D,
+    return Where{r0 + n <= pt, ok ? n : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * F::row_bytes,
                  a.k_scales + ((pg * a.n_kv_heads + head) * pt + r0)};
   };
   auto place = [&](int t0) __attribute__((always_inline)) -> Place {
@@ -165,8 +168,16 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
         const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(c.sk), 0, 4 * c.n, kWord3);
         const auto sv = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(c.sk) + sk_to_sv), 0, 4 * c.n, kWord3);
-        x.fk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * (lane & 31), 0, 0));
-        x.fv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * (lane & 31), 0, 0));
+        if constexpr (kMx) {  // block g of K's key 16 i + l16; block lane % 4 of V's key 16 i + lane / 4
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            x.ek[i] = __builtin_amdgcn_raw_buffer_load_b8(sk, 64 * i + 4 * l16 + g4, 0, 0);
+            x.ev[i] = __builtin_amdgcn_raw_buffer_load_b8(sv, 64 * i + lane, 0, 0);
+          }
+        } else {
+          x.fk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * (lane & 31), 0, 0));
+          x.fv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * (lane & 31), 0, 0));
+        }
       }
 #pragma unroll
       for (int i = 0; i < F::k_loads; ++i) {
@@ -182,15 +193,23 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
       x.bad = static_cast<uint32_t>(__ballot(!p.there));
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const uint8_t* kp = a.k_codes + static_cast<int64_t>(__shfl(p.row, 16 * b + l16)) * D + 16 * g4;
+        const uint8_t* kp = a.k_codes + static_cast<int64_t>(__shfl(p.row, 16 * b + l16)) * F::row_bytes + 16 * g4;
 #pragma unroll
         for (int i = 0; i < F::k_loads / 2; ++i) x.k[F::k_loads / 2 * b + i] = *reinterpret_cast<const u32x4*>(kp + 64 * i);
       }
 #pragma unroll
       for (int i = 0; i < F::k_loads; ++i)
-        x.v[i] = *reinterpret_cast<const u32x4*>(a.v_codes + static_cast<int64_t>(__shfl(p.row, 64 / C * i + lane / C)) * D + 16 * (lane % C));
-      x.fk = a.k_scales[p.scale];
-      x.fv = a.v_scales[p.scale];
+        x.v[i] = *reinterpret_cast<const u32x4*>(a.v_codes + static_cast<int64_t>(__shfl(p.row, 64 / C * i + lane / C)) * F::row_bytes + 16 * (lane % C));
+      if constexpr (kMx) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x.ek[i] = reinterpret_cast<const uint8_t*>(a.k_scales + __shfl(p.scale, 16 * i + l16))[g4];
+          x.ev[i] = reinterpret_cast<const uint8_t*>(a.v_scales + __shfl(p.scale, 16 * i + (lane >> 2)))[lane & 3];
+        }
+      } else {
+        x.fk = a.k_scales[p.scale];
+        x.fv = a.v_scales[p.scale];
+      }
     }
   };
 
@@ -220,11 +239,12 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     row_at[n] = t.row0 + static_cast<int>(qi);
     row_head[n] = (head * a.group + static_cast<int>(gi)) * D;
   }
-  // Q, the second operand of the scores.  e4m3 keys: q = 2^e (q1 + q2 / 16) as in attn_batch_wide.hip, a lane holding
+  // Q, the second operand of the scores.  e4m3 and MXFP4 keys: q = 2^e (q1 + q2 / 16) as in attn_batch_wide.hip, a lane holding
   // values 16 g .. + 15 and 64 + 16 g .. + 15 (what its two loads of a key hold).  The others: step s of the product takes
   // values 64 (s / 2) + 16 g + 8 (s % 2) .. + 7 (dense: 32 s + 8 g .. + 7).
-  constexpr bool kCodes = SRC == SRC_E4M3;
+  constexpr bool kCodes = SRC == SRC_E4M3 || kMx;  // K's codes go to the matrix cores as they are
   auto q_values = [&](int s) { return kDense ? 32 * s + 8 * g4 : 64 * (s >> 1) + 16 * g4 + 8 * (s & 1); };
+  constexpr int kFormat = kMx ? 4 : 0;  // of K's codes: e2m1, e4m3
   v8bf qf[4];       // one row block's operands
   v8i qa, qb;       // q1 and q2
   int q_scale[NB];  // E8M0 scale of q1
@@ -303,10 +323,32 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
       for (int i = 0; i < F::k_loads; ++i) {
         if (x.bad >> (16 * (i / (F::k_loads / 2)) + l16) & 1u) x.k[i] = zero;
         if (x.bad >> (64 / C * i + lane / C) & 1u) x.v[i] = zero;
+        if constexpr (kMx) {
+          if (x.bad >> (16 * i + l16) & 1u) x.ek[i] = 127;
+          if (x.bad >> (16 * i + (lane >> 2)) & 1u) x.ev[i] = 127;
+        }
       }
       if (x.bad >> (lane & 31) & 1u) x.fk = x.fv = 0.f;
     }
-    if constexpr (kDense) {
+    if constexpr (kMx) {
+      // A NaN scale of V, which a weight of zero would not silence, becomes one of K: the score of the key is NaN, and is
+      // hidden from the rows that do not see it.
+      if (__ballot(max(max(x.ek[0], x.ek[1]), max(x.ev[0], x.ev[1])) >= kMxNan)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint64_t v_nan = __ballot(x.ev[i] >= kMxNan);
+          if (x.ek[i] >= kMxNan || (v_nan >> (4 * l16) & 15u)) x.ek[i] = mx::kNanE;
+          if (x.ev[i] >= kMxNan) x.ev[i] = 127;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float s = mx::scale_of(x.ev[i]);
+        uint4* p = reinterpret_cast<uint4*>(vbuf + (16 * i + (lane >> 2)) * F::v_pitch + 64 * (lane & 3));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = mx::decode8(x.v[i][e], s);
+      }
+    } else if constexpr (kDense) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) *reinterpret_cast<u32x4*>(vbuf + (4 * i + (lane >> 4)) * F::v_pitch + 16 * l16) = x.v[i];
     } else {
@@ -338,7 +380,14 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     if constexpr (kCodes) {
       v8i kf[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) kf[b] = __builtin_bit_cast(v8i, *reinterpret_cast<u32x4(*)[2]>(&x.k[2 * b]));
+      for (int b = 0; b < 2; ++b) {
+        if constexpr (kMx) {
+          const v4i c = __builtin_bit_cast(v4i, x.k[b]);
+          kf[b] = __builtin_shufflevector(c, c, 0, 1, 2, 3, -1, -1, -1, -1);
+        } else {
+          kf[b] = __builtin_bit_cast(v8i, *reinterpret_cast<u32x4(*)[2]>(&x.k[2 * b]));
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         if constexpr (F::q_lds) {
@@ -350,9 +399,9 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
           qb = __builtin_bit_cast(v8i, *reinterpret_cast<u32x4(*)[2]>(&q[2]));
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qb, s[n][b], 0, 0, 0, 127, 0, q_scale[n] - 4);
+        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qb, s[n][b], kFormat, 0, 0, kMx ? x.ek[b] : 127, 0, q_scale[n] - 4);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qa, s[n][b], 0, 0, 0, 127, 0, q_scale[n]);
+        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qa, s[n][b], kFormat, 0, 0, kMx ? x.ek[b] : 127, 0, q_scale[n]);
       }
       return;
     }
@@ -384,7 +433,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
   // The weights, as two bf16 parts.
   auto weigh = [&](int t0, bool masked) __attribute__((always_inline)) {
     float u[8], sv[8];
-    if constexpr (!kDense) {
+    if constexpr (kScaled) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const float4 fu = *reinterpret_cast<const float4*>(fbuf + 16 * b + 4 * g4);
@@ -397,7 +446,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     for (int n = 0; n < NB; ++n) {
       float x8[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x8[e] = s[n][e >> 2][e & 3] * (kDense ? a.c : u[e]);
+      for (int e = 0; e < 8; ++e) x8[e] = s[n][e >> 2][e & 3] * (kScaled ? u[e] : a.c);
       if (masked) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -421,7 +470,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
         const float p = __builtin_amdgcn_exp2f(x8[e] + neg);
         l[n] += p;
         float wgt = p;
-        if constexpr (!kDense) {
+        if constexpr (kScaled) {
           wgt = p * sv[e];
           if (masked && x8[e] == -INFINITY) wgt = 0.f;
         }
@@ -444,7 +493,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v8bf vf;
-      if constexpr (kDense) {
+      if constexpr (F::v_bf16) {
         const uint8_t* p = vbuf + (4 * g4 + (l16 >> 2)) * F::v_pitch + (16 * i + 4 * (l16 & 3)) * 2;
         vf = __builtin_bit_cast(v8bf, __builtin_shufflevector(read_tr16(p), read_tr16(p + 16 * F::v_pitch), 0, 1, 2, 3, 4, 5, 6, 7));
       } else {
@@ -561,6 +610,7 @@ void launch(Args& a, int row_blocks, bool fresh, hipStream_t stream) {
 int launch_few(Args a, int src, int row_blocks, bool fresh, hipStream_t stream) {
   switch (src) {
     case SRC_E4M3: launch<SRC_E4M3>(a, row_blocks, fresh, stream); break;
+    case SRC_MXFP4: launch<SRC_MXFP4>(a, row_blocks, fresh, stream); break;
     case SRC_INT8: launch<SRC_INT8>(a, row_blocks, fresh, stream); break;
     default: launch<SRC_DENSE>(a, row_blocks, fresh, stream); break;
   }

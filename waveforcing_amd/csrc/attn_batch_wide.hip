@@ -49,16 +49,19 @@ constexpr int kXcds = 8;
 constexpr float kShift = 6.f, kGrow = 9.f, kFloor = -80.f;
 constexpr _Float16 kMost = 32768.f;
 constexpr float kMostSum = 0x1p95f;
+constexpr float kMostMx = 0x1p20f;  // of bf16 weights, whose bits do not go by their size: the sum of a tile's
 constexpr int kRun = 2;  // neighbouring row tiles that one XCD takes, which read the same keys (1: 0.7 % slower, 4: 2.5 %)
 static_assert(kThreads == BKV * 8, "one thread per key and 16 values of its row");
 
 template <int SRC>
 struct Lds {
-  static constexpr bool codes = SRC == SRC_E4M3;              // K as codes
-  static constexpr int k_pitch = codes ? D + 16 : 2 * D + 16;
+  static constexpr bool mx = SRC == SRC_MXFP4;
+  static constexpr bool codes = SRC == SRC_E4M3 || mx;        // K as codes
+  static constexpr int row_bytes = mx ? D / 2 : D;            // of codes in a page
+  static constexpr int k_pitch = codes ? row_bytes + 16 : 2 * D + 16;
   static constexpr int v_pitch = 2 * D + 64;
   static constexpr int v_off = BKV * k_pitch;
-  static constexpr int u_off = v_off + BKV * v_pitch;         // factor of the scores u [64], scale of V [64]
+  static constexpr int u_off = v_off + BKV * v_pitch;         // factor of the scores u [64] (MXFP4: scale bytes of K), scale of V [64]
   static constexpr int stage = u_off + 2 * BKV * 4;
   static constexpr int o_pitch = 2 * D + 8;
   static constexpr int out = kWaves * 32 * o_pitch;
@@ -102,7 +105,7 @@ __device__ inline bool finite(float v) { return (f32_bits(v) & 0x7f800000u) != 0
 template <int SRC, bool SMALL>
 __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   using L = Lds<SRC>;
-  constexpr bool kCodes = SRC == SRC_E4M3;
+  constexpr bool kCodes = L::codes, kMx = L::mx;
   __shared__ __attribute__((aligned(16))) uint8_t lds[L::bytes];
 
   if (blockIdx.x >= a.clear_from) return clear_rest<kThreads>(a);
@@ -141,9 +144,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 
   // ---- staging: key skey of the tile, values 16 schunk .. + 15
   const int skey = tid >> 3, schunk = tid & 7;
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
   struct Staged {
-    u32x4 k0, v0;
-    float sk, sv;  // the key's scales
+    std::conditional_t<kMx, u32x2, u32x4> k0, v0;
+    float sk, sv;  // the key's scales (MXFP4: their bytes)
   };
   Staged sreg;
   // Where a tile's keys live (uniform): the first key's row of K and its scale, those of V at the same distance from
@@ -155,7 +159,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   };
   const int pt = a.geom.page_tokens;
   const int32_t* table = a.geom.tables + static_cast<int64_t>(t.b) * a.geom.ld_table;
-  const int64_t key_bytes = static_cast<int64_t>(a.n_kv_heads) * D;
+  const int64_t key_bytes = static_cast<int64_t>(a.n_kv_heads) * L::row_bytes;
   const int64_t k_to_v = a.v_codes - a.k_codes;
   const int64_t sk_to_sv = reinterpret_cast<const uint8_t*>(a.v_scales) - reinterpret_cast<const uint8_t*>(a.k_scales);
   auto cursor_at = [&](int tile) __attribute__((always_inline)) -> Cursor {
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     asm volatile("" ::"s"(page));  // awaited here, not among the LDS reads of the tile
     const bool ok = page >= 0 && page < a.geom.pool_pages;
     const int pg = ok ? page : 0, r0 = static_cast<int>(at);
-    return Cursor{r0, min(pt - r0, BKV), ok ? BKV : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * D,
+    return Cursor{r0, min(pt - r0, BKV), ok ? BKV : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * L::row_bytes,
                   a.k_scales + ((pg * a.n_kv_heads + head) * pt + r0)};
   };
   auto cursor_next = [&](const Cursor& c, int tile) __attribute__((always_inline)) -> Cursor {
@@ -178,7 +182,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     return Cursor{c.at + BKV, min(pt - c.at - BKV, BKV), c.n, c.k + BKV * key_bytes, c.sk + BKV};
   };
   Cursor ahead{};
-  const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(key_bytes) + 16 * schunk;  // rows of a tile stay below 2^31 bytes (checked on the host)
+  const uint32_t lane_row = static_cast<uint32_t>(skey) * static_cast<uint32_t>(key_bytes) + L::row_bytes / 8 * schunk;  // rows of a tile stay below 2^31 bytes (checked on the host)
   constexpr int kWord3 = 0x00020000;  // raw buffer, 32-bit data format
   // SMALL: the page of this lane's key in the tile that is loaded next (-1: none), asked for a tile ahead
   int page_key = -1;
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     const int n = uniform(min(max(k_hi - tile * BKV, 0), BKV));
     if (decltype(ONE)::value || (!SMALL && c.cut == BKV)) {
       const int m = min(n, c.n);
-      const int bytes = m ? (m - 1) * static_cast<int>(key_bytes) + D : 0;
+      const int bytes = m ? (m - 1) * static_cast<int>(key_bytes) + L::row_bytes : 0;
       const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k), 0, bytes, kWord3);
       const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(c.k + k_to_v), 0, bytes, kWord3);
       const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(c.sk), 0, 4 * m, kWord3);
@@ -200,20 +204,25 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
           const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(c.sk) + sk_to_sv), 0, 4 * m, kWord3);
       x.sk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * skey, 0, 0));
       x.sv = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sv, 4 * skey, 0, 0));
-      x.k0 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row, 0, 0);
-      x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
+      if constexpr (kMx) {
+        x.k0 = __builtin_amdgcn_raw_buffer_load_b64(rk, lane_row, 0, 0);
+        x.v0 = __builtin_amdgcn_raw_buffer_load_b64(rv, lane_row, 0, 0);
+      } else {
+        x.k0 = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_row, 0, 0);
+        x.v0 = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_row, 0, 0);
+      }
     } else {
       if constexpr (!SMALL) find_page(tile);
       const uint32_t jk = static_cast<uint32_t>(tile * BKV + skey);
-      const u32x4 zero = {0, 0, 0, 0};
-      x.k0 = x.v0 = zero;
+      typedef decltype(x.k0) codes_t;
+      x.k0 = x.v0 = codes_t{};
       x.sk = x.sv = 0.f;
       if (page_key >= 0 && page_key < a.geom.pool_pages) {
         const int at = static_cast<int>(jk - a.geom.page.div(jk) * a.geom.page.d);
-        const int64_t off = static_cast<int64_t>((page_key * pt + at) * a.n_kv_heads + head) * D + 16 * schunk;
+        const int64_t off = static_cast<int64_t>((page_key * pt + at) * a.n_kv_heads + head) * L::row_bytes + L::row_bytes / 8 * schunk;
         const int sc = (page_key * a.n_kv_heads + head) * pt + at;
-        x.k0 = *reinterpret_cast<const u32x4*>(a.k_codes + off);
-        x.v0 = *reinterpret_cast<const u32x4*>(a.v_codes + off);
+        x.k0 = *reinterpret_cast<const codes_t*>(a.k_codes + off);
+        x.v0 = *reinterpret_cast<const codes_t*>(a.v_codes + off);
         x.sk = a.k_scales[sc];
         x.sv = a.v_scales[sc];
       }
@@ -226,6 +235,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   };
   // The staged tile as it goes to LDS.  PARTIAL: some row may not see all of it.
   auto convert = [&](Staged x, Ready& y, auto PARTIAL) __attribute__((always_inline)) {
+    if constexpr (kMx) {
+      // a NaN scale of K or V: that of all of K's blocks, so the score of the key is NaN for the rows that see it
+      const uint32_t ek = f32_bits(x.sk), ev = f32_bits(x.sv);
+      const bool poison = has_nan_scale(ek) || has_nan_scale(ev);
+      const float s = mx::scale_of(poison ? 127 : (ev >> (8 * (schunk >> 1))) & 0xffu);
+      y.u = bits_f32(poison ? ~0u : ek);
+      y.k0 = make_uint4(x.k0[0], x.k0[1], 0, 0);
+      y.v0 = mx::decode8(x.v0[0], s);
+      y.v1 = mx::decode8(x.v0[1], s);
+    } else {
     bool poison = !finite(x.sv) || !finite(x.sk);  // the score is NaN for the rows that see the key, the weight of V zero for the others
     if constexpr (SRC == SRC_E4M3 && decltype(PARTIAL)::value) {
       const bool nan = has_nan_code(x.v0[0]) || has_nan_code(x.v0[1]) || has_nan_code(x.v0[2]) || has_nan_code(x.v0[3]);
@@ -247,11 +266,14 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     const uint2 p = codes_f16<SRC>(x.v0[0], neg), q = codes_f16<SRC>(x.v0[1], neg), s = codes_f16<SRC>(x.v0[2], neg), v = codes_f16<SRC>(x.v0[3], neg);
     y.v0 = make_uint4(p.x, p.y, q.x, q.y);
     y.v1 = make_uint4(s.x, s.y, v.x, v.y);
+    }
   };
   auto write = [&](int stage, const Ready& y) __attribute__((always_inline)) {
     uint8_t* st = lds + stage;
     uint4* dv = reinterpret_cast<uint4*>(st + L::v_off + skey * L::v_pitch + schunk * 32);
-    if constexpr (kCodes) {
+    if constexpr (kMx) {
+      *reinterpret_cast<uint2*>(st + skey * L::k_pitch + schunk * 8) = make_uint2(y.k0.x, y.k0.y);
+    } else if constexpr (kCodes) {
       *reinterpret_cast<uint4*>(st + skey * L::k_pitch + schunk * 16) = y.k0;
     } else {
       uint4* dk = reinterpret_cast<uint4*>(st + skey * L::k_pitch + schunk * 32);
@@ -262,7 +284,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     dv[1] = y.v1;
     float* u = reinterpret_cast<float*>(st + L::u_off);
     u[skey] = y.u;  // (the lanes of one key write the same words)
-    u[BKV + skey] = y.sv;
+    if constexpr (!kMx) u[BKV + skey] = y.sv;
   };
 
   // ---- Q, the second operand of the scores, for the whole kernel
@@ -274,8 +296,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     uint4 raw[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      // e4m3: values 64 (i / 4) + 32 half + 8 (i % 4) .. + 7; else 16 i + 8 half .. + 7
-      raw[i] = *reinterpret_cast<const uint4*>(qp + (kCodes ? 64 * (i >> 2) + 32 * half + 8 * (i & 3) : 16 * i + 8 * half));
+      // e4m3: values 64 (i / 4) + 32 half + 8 (i % 4) .. + 7; MXFP4, where the lanes of K hold 32 values in a row and the fp8
+      // operand's first and last 16 bytes belong to different blocks: 64 (i / 4) + 32 (i / 2 % 2) + 16 half + 8 (i % 2) .. + 7;
+      // else 16 i + 8 half .. + 7
+      raw[i] = *reinterpret_cast<const uint4*>(qp + (kMx ? 64 * (i >> 2) + 32 * ((i >> 1) & 1) + 16 * half + 8 * (i & 1) : kCodes ? 64 * (i >> 2) + 32 * half + 8 * (i & 3) : 16 * i + 8 * half));
       if (!row_ok) raw[i] = make_uint4(0, 0, 0, 0);
     }
     if constexpr (!kCodes) {
@@ -304,7 +328,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   }
 
   // Per-lane LDS offsets: K fragment of key block b, step s; V^T operand of d block db, 16-key step, read 0 / 1
-  const int k_lane = kCodes ? l32 * L::k_pitch + half * 32 : l32 * L::k_pitch + half * 16;
+  const int k_lane = kCodes ? l32 * L::k_pitch + half * (kMx ? 16 : 32) : l32 * L::k_pitch + half * 16;
   const int v_lane = L::v_off + (4 * half + ((lane & 15) >> 2)) * L::v_pitch + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
 
   v16f o[4];
@@ -312,7 +336,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   for (int i = 0; i < 4; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
   float m_use = -INFINITY;  // the row's maximum in the exponents, log2 units
   float l_run = 0.f;        // this half's row sum
-  float neg_m = kShift;
+  float neg_m = kMx ? 0.f : kShift;
 
   // Stages (bytes in LDS) of the tiles t - 1, t and t + 1.
   int st_prev = 0, st_cur = L::stage, st_next = 2 * L::stage;
@@ -336,7 +360,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       const uint4 w = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[k & 1][db]), __builtin_bit_cast(v8h, w), o[db], 0, 0, 0);
+        if constexpr (kMx)
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, vf[k & 1][db]), __builtin_bit_cast(v8bf, w), o[db], 0, 0, 0);
+        else
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[k & 1][db]), __builtin_bit_cast(v8h, w), o[db], 0, 0, 0);
       }
       if (k < 2) read_v(stage, k + 2);
     }
@@ -346,7 +373,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // among the products the staging of tile t + 1 and the loads of t + 2.  PARTIAL: some row may not see all of t + 1, the
   // wave may see none of t, or the tile to be loaded may span pages; without it the half is one block of instructions.
   float4 uf[2], sf[2];
-  auto read_u = [&](int stage, int j) __attribute__((always_inline)) {  // factors and scales of V of the keys 8 j + 4 half + 0 .. 3
+  int ke[2];  // MXFP4: the scale bytes of key l32 of each 32, from the lane's first one on
+  auto read_u = [&](int stage, int j) __attribute__((always_inline)) {
+    if constexpr (kMx) return;  // factors and scales of V of the keys 8 j + 4 half + 0 .. 3
     const float* us = reinterpret_cast<const float*>(lds + stage + L::u_off) + 8 * j + 4 * half;
     uf[j & 1] = *reinterpret_cast<const float4*>(us);
     sf[j & 1] = *reinterpret_cast<const float4*>(us + BKV);
@@ -364,10 +393,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int m = i >> 2, b = i & 1;
-          if (i & 2)
+          if constexpr (kMx) {
+            const v8i& q = i & 2 ? q1[m] : q2[m];
+            const int e = i & 2 ? q_scale : q_scale - 4;
+            s[b] = m ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q, s[b], 4, 0, 2, ke[b], 0, e)
+                     : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q, s[b], 4, 0, 0, ke[b], 0, e);
+          } else if (i & 2) {
             s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q1[m], s[b], 0, 0, 0, 127, 0, q_scale);
-          else
+          } else {
             s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q2[m], s[b], 0, 0, 0, 127, 0, q_scale - 4);
+          }
         }
       } else {
 #pragma unroll
@@ -394,7 +429,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     for (int i = 0; i < (kCodes ? 2 : 8); ++i)
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        if constexpr (kCodes) {
+        if constexpr (kMx) {
+          const v4i c = *reinterpret_cast<const v4i*>(st + k_lane + b * 32 * L::k_pitch + 32 * i);
+          kf[b][i] = __builtin_shufflevector(c, c, 0, 1, 2, 3, -1, -1, -1, -1);
+          if (i == 0) ke[b] = static_cast<int>(*reinterpret_cast<const uint32_t*>(st + L::u_off + 4 * (32 * b + l32)) >> (8 * half));
+        } else if constexpr (kCodes) {
           const uint8_t* p = st + k_lane + b * 32 * L::k_pitch + 64 * i;
           const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 16);
           kf[b][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -442,6 +481,17 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     v2h top;
     auto weights = [&]() __attribute__((always_inline)) {
       l_tile = 0.f;
+      if constexpr (kMx) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float x = s[j >> 3][2 * (j & 7)], z = s[j >> 3][2 * (j & 7) + 1];
+          const float p = __builtin_amdgcn_exp2f(fmaf(x, factor(a.c, x), neg_m)), q = __builtin_amdgcn_exp2f(fmaf(z, factor(a.c, z), neg_m));
+          l_tile += p;
+          l_tile += q;
+          pw[j] = cvt_bf16x2(p, q);
+        }
+        return;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (j < 7) read_u(stage, j + 1);
@@ -463,8 +513,20 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     };
     weights();
     // (NaN needs no other reference; m_use is -inf until the row has seen a key, and its weights count for nothing)
-    if (__ballot(top[0] > kMost || top[1] > kMost || l_tile > kMostSum || m_use == -INFINITY)) {
+    auto moves = [&]() __attribute__((always_inline)) {
+      if constexpr (kMx)
+        return l_tile > kMostMx || m_use == -INFINITY;
+      else
+        return top[0] > kMost || top[1] > kMost || l_tile > kMostSum || m_use == -INFINITY;
+    };
+    if (__ballot(moves())) {
       float mt = -INFINITY;
+      if constexpr (kMx) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[b][e] * factor(a.c, s[b][e]));
+      } else {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -477,6 +539,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
             mt = fmaxf(mt, fmaf(s[b][4 * g + e], factor(u[e], s[b][4 * g + e]), fmaxf(__builtin_amdgcn_logf(sv[e]), kFloor)));
           __builtin_amdgcn_sched_barrier(0);
         }
+      }
       mt = max32(mt);
       const bool fire = m_use == -INFINITY || mt - m_use > kGrow;
       const float m_new = fire ? fmaxf(m_use, mt) : m_use;
@@ -486,7 +549,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       for (int i = 0; i < 4; ++i) o[i] *= alpha * alpha;
       l_run = l_run * alpha * alpha;
       m_use = m_new;
-      neg_m = m_new == -INFINITY ? kShift : kShift - m_new;
+      neg_m = m_new == -INFINITY ? (kMx ? 0.f : kShift) : (kMx ? 0.f : kShift) - m_new;
       read_u(stage, 0);
       weights();
     }
@@ -614,6 +677,8 @@ int launch_wide(Args a, int format, bool fresh, hipStream_t stream) {
   void (*kernel)(Args);
   if (format == WF_KV_E4M3)
     kernel = small ? attn_wide_kernel<SRC_E4M3, true> : attn_wide_kernel<SRC_E4M3, false>;
+  else if (format == WF_KV_MXFP4)
+    kernel = small ? attn_wide_kernel<SRC_MXFP4, true> : attn_wide_kernel<SRC_MXFP4, false>;
   else
     kernel = small ? attn_wide_kernel<SRC_INT8, true> : attn_wide_kernel<SRC_INT8, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);

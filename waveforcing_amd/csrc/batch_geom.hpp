@@ -81,7 +81,7 @@ inline int check_batch(const char* fn, int64_t n_rows, int32_t n_kv_heads, int32
 
 inline int check_pool(const char* fn, int32_t format, int32_t n_kv_heads, int32_t page_tokens, int64_t pool_pages,
                       const int32_t* tables, int64_t ld_table) {
-  WF_REQUIRE(format == WF_KV_E4M3 || format == WF_KV_INT8, WF_E_INVALID, "%s: unknown cache format %d", fn, format);
+  WF_REQUIRE(format == WF_KV_E4M3 || format == WF_KV_INT8 || format == WF_KV_MXFP4, WF_E_INVALID, "%s: unknown cache format %d", fn, format);
   WF_REQUIRE(page_tokens > 0 && pool_pages >= 0 && ld_table >= 0, WF_E_INVALID,
              "%s: negative or zero size (page_tokens=%d pool_pages=%lld ld_table=%lld)", fn, page_tokens,
              (long long)pool_pages, (long long)ld_table);

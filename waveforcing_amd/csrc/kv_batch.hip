@@ -11,12 +11,16 @@
 //   int8: s = max(a / 127, 1e-8), code = clamp(rint(x / s), -127, 127), fp32 (rows.hpp's quant_i8).
 // The magnitudes of bf16 numbers order as their bits do, and those of infinities and NaN come last, so the integer
 // maximum that gives a also tells a row that holds one: it is stored as scale NaN and zero codes, and reads back as NaN
-// whole in both formats, instead of as a finite row of a scale that its other values set.
+// whole in every format, instead of as a finite row of a scale that its other values set.
+//
+// MXFP4 rows: 64 bytes of codes and 4 scale bytes, in the place of the fp32 scale.  A block of 32 values is two lanes' (one DPP
+// step), a lane's 16 codes are 8 bytes, and the four blocks' bytes meet in two more steps.
 //
 // Four chunks of 4680 rows of 12 heads: append 40-41 us (4.3 TB/s of 174 MB), gather 30 us (5.8); 64 single rows 4 us
 // each, the launch.
 #include "batch_geom.hpp"
 #include "kv_row.hpp"
+#include "mxfp4_codec.hpp"
 #include "rows.hpp"
 
 namespace wf {
@@ -74,6 +78,12 @@ __device__ inline uint32_t group8_umax(uint32_t v) {
   return max(v, static_cast<uint32_t>(o));
 }
 
+// OR of v over pairs of lanes of an aligned group of 8 (each pair holding one value).
+__device__ inline uint32_t group8_or_pairs(uint32_t v) {
+  v |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4E, 0xF, 0xF, false));
+  return v | static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xF, 0xF, false));
+}
+
 template <int FMT>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvBatchArgs a) {
   uint32_t blk;
@@ -93,6 +103,18 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvBatchArgs a) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+  if constexpr (FMT == WF_KV_MXFP4) {
+    const uint32_t block = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xF, 0xF, false)));
+    const bool nan = group8_umax(top) >= 0x7f80u;
+    const int e = mx::scale_byte(block);
+    const float s = mx::scale_of(e);
+    const uint32_t bytes = nan ? ~0u : group8_or_pairs(static_cast<uint32_t>(e) << (8 * (lane8 >> 1)));
+    if (!ok) return;
+    const uint2 c = nan ? make_uint2(0, 0) : make_uint2(mx::encode8(w, s), mx::encode8(w + 4, s));
+    reinterpret_cast<uint2*>(a.codes[which] + code_row * (kHeadDim / 2))[lane8] = c;
+    if (lane8 == 0) reinterpret_cast<uint32_t*>(a.scales[which])[scale_at] = bytes;
+    return;
+  }
   top = group8_umax(top);
   if (!ok) return;
   const float amax = bf16_bits_to_f32(static_cast<uint16_t>(top));
@@ -148,6 +170,14 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvBatchArgs a) {
     p[0] = p[1] = make_uint4(0, 0, 0, 0);
     return;
   }
+  if constexpr (FMT == WF_KV_MXFP4) {
+    const uint2 c = reinterpret_cast<const uint2*>(a.codes[which] + code_row * (kHeadDim / 2))[lane8];
+    const uint32_t bytes = reinterpret_cast<const uint32_t*>(a.scales[which])[scale_at];
+    const float s = mx::scale_of((bytes >> (8 * (lane8 >> 1))) & 0xffu);
+    p[0] = mx::decode8(c.x, s);
+    p[1] = mx::decode8(c.y, s);
+    return;
+  }
   const uint4 c = reinterpret_cast<const uint4*>(a.codes[which] + code_row * kHeadDim)[lane8];
   const float s = a.scales[which][scale_at];
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
@@ -195,8 +225,13 @@ int kv_batch(const char* fn, bool write, bool fresh, void* k, void* v, int64_t n
   a.heads = FastDiv(static_cast<uint32_t>(n_heads));
   a.geom = make_batch_geom(cu, kv_lens, n_seqs, tables, ld_table, page_tokens, pool_pages);
   const dim3 grid((a.n_items + kXcds - 1) / kXcds * kXcds);
-  void (*kernel)(KvBatchArgs) = write ? (format == WF_KV_INT8 ? kv_append_kernel<WF_KV_INT8> : kv_append_kernel<WF_KV_E4M3>)
-                                      : (format == WF_KV_INT8 ? kv_gather_kernel<WF_KV_INT8> : kv_gather_kernel<WF_KV_E4M3>);
+  void (*kernel)(KvBatchArgs);
+  if (format == WF_KV_MXFP4)
+    kernel = write ? kv_append_kernel<WF_KV_MXFP4> : kv_gather_kernel<WF_KV_MXFP4>;
+  else if (format == WF_KV_INT8)
+    kernel = write ? kv_append_kernel<WF_KV_INT8> : kv_gather_kernel<WF_KV_INT8>;
+  else
+    kernel = write ? kv_append_kernel<WF_KV_E4M3> : kv_gather_kernel<WF_KV_E4M3>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, as_stream(stream), a);
   return check_launch(fn);
 }

@@ -103,6 +103,8 @@ class Fp8PagePool:
     """K and V page pools in HBM with pack / gather-dequant through the HIP kernels."""
 
     format = _lib.KV_E4M3
+    row_bytes = 128                        # codes of a (token, head)
+    scale_type, scale_dims = torch.float32, ()   # a (token, head)'s scales
 
     def __init__(
         self,
@@ -119,12 +121,12 @@ class Fp8PagePool:
         self.head_dim = head_dim
         self.page_tokens = page_tokens
         self.device = torch.device(device)
-        shape_c = (pool_pages, page_tokens, n_heads, head_dim)
-        shape_s = (pool_pages, n_heads, page_tokens)
+        shape_c = (pool_pages, page_tokens, n_heads, self.row_bytes)
+        shape_s = (pool_pages, n_heads, page_tokens, *self.scale_dims)
         self.k_codes = torch.zeros(shape_c, dtype=torch.uint8, device=self.device)
         self.v_codes = torch.zeros(shape_c, dtype=torch.uint8, device=self.device)
-        self.k_scales = torch.zeros(shape_s, dtype=torch.float32, device=self.device)
-        self.v_scales = torch.zeros(shape_s, dtype=torch.float32, device=self.device)
+        self.k_scales = torch.zeros(shape_s, dtype=self.scale_type, device=self.device)
+        self.v_scales = torch.zeros(shape_s, dtype=self.scale_type, device=self.device)
         self._cache_ptrs()
 
     def _cache_ptrs(self) -> None:
@@ -291,6 +293,32 @@ class Int8PagePool(Fp8PagePool):
 
     def _one_sequence(self, *args, **kwargs):
         raise TypeError("int8 pages are written and read through PagedBatch (append, gather)")
+
+    pack = pack_k_norm_rope = unpack = _one_sequence
+
+
+class Mxfp4PagePool(Int8PagePool):
+    """The pools with microscaled 4-bit codes (MXFP4): 64 bytes of codes (two to a byte, the even value low) and 4 scale bytes
+    (E8M0, one for every 32 values) per (token, head), 68 bytes where the 8-bit pools take 132; quantized as by
+    ``mxfp4.quant_mxfp4``:
+
+        codes  uint8 [pool_pages, page_tokens, H, 64]
+        scales uint8 [pool_pages, H, page_tokens, 4]
+
+    A value is off by up to a sixth of itself (half a step of e2m1) where 8-bit codes keep 4 to 8 bits.  Written, read and
+    attended through :class:`PagedBatch`."""
+
+    format = _lib.KV_MXFP4
+    row_bytes = 64
+    scale_type, scale_dims = torch.uint8, (4,)
+
+    @staticmethod
+    def bytes_for(pool_pages: int, n_heads: int, head_dim: int, page_tokens: int) -> int:
+        """Device bytes of a pool (K and V codes + scales)."""
+        return 2 * pool_pages * page_tokens * n_heads * (head_dim // 2 + 4)
+
+    def _one_sequence(self, *args, **kwargs):
+        raise TypeError("MXFP4 pages are written and read through PagedBatch (append, gather)")
 
     pack = pack_k_norm_rope = unpack = _one_sequence
 
