@@ -285,11 +285,15 @@ int wf_fp8_linear_pertensor(const void* x, int64_t m, int64_t k, int64_t ldx,
  * (no value is off by more than half the step of its binade).  A block that
  * holds a NaN or an infinity is E = 255 with zero codes, and reads back as NaN.
  *
- * Layout of rows x [rows][k], k % 32 == 0:
- *   codes  u8 [rows][k / 2], the even value of a pair in the low half
- *   scales u8 [ceil(k / 128)][rows4][4], rows4 = rows rounded up to 4: byte
- *          b of (g, r) is that of values 128 g + 32 b .. + 31 of row r, 0
- *          where the row has no such values or there is no row
+ * Layout of rows x [rows][k], k % 32 == 0, in panels of 16 rows by 128
+ * values, P = ceil(rows / 16), G = ceil(k / 128):
+ *   codes  u8 [P][G][4][16][16]: byte j of (p, g, b, r) holds the values
+ *          128 g + 32 b + 2 j (low half) and the one after it (high half) of
+ *          row 16 p + r
+ *   scales u8 [P][G][16][4]: byte b of (p, g, r) is the scale byte of the
+ *          values 128 g + 32 b .. + 31 of row 16 p + r
+ * both zero where there is no such row or value (waveforcing_amd.mxfp4
+ * converts to and from rows of codes and rows of scales).
  * The 4-bit counterpart of the reference's W8A8 linear (wave_rt/runtime/
  * fp8.py:21-61); it has no 4-bit form itself.
  */
@@ -313,7 +317,7 @@ int wf_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales,
  * with flags & WF_GEMM_GELU_TANH, in fp32 (rounded once).  A scale byte of
  * 255 makes its row of a (of w: its column of y) NaN.  k % 32 == 0; n, ldy %
  * 4 == 0; codes and scales 16-byte, y and bias 8-byte aligned; codes of an
- * operand fewer than 2^31 bytes.  The order of the sums goes by the sizes. */
+ * operand fewer than 2^31 bytes.  Reads whole panels.  The order of the sums goes by the sizes. */
 int wf_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scales,
                   const uint8_t* w, const uint8_t* w_scales, int64_t m,
                   int64_t n, int64_t k, const void* bias, void* y,

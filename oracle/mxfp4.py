@@ -44,13 +44,19 @@ def unpack(b: torch.Tensor) -> torch.Tensor:
     return torch.stack((b & 15, b >> 4), -1).flatten(-2)
 
 
-def scale_layout(scales: torch.Tensor) -> torch.Tensor:
-    """Scale bytes [rows, k / 32] as [ceil(k / 128)][rows4][4]."""
+def panels(codes: torch.Tensor, scales: torch.Tensor):
+    """Code bytes [rows, k / 2] and scale bytes [rows, k / 32] as panels of 16 rows by 128 values (include/wf_api.h)."""
     rows, n = scales.shape
-    out = torch.zeros((-(-n // 4), -(-rows // 4) * 4, 4), dtype=torch.uint8, device=scales.device)
-    for b in range(n):
-        out[b // 4, :rows, b % 4] = scales[:, b]
-    return out
+    P, G = -(-rows // 16), -(-n // 4)
+    c = torch.zeros((P, G, 4, 16, 16), dtype=torch.uint8, device=codes.device)
+    s = torch.zeros((P, G, 16, 4), dtype=torch.uint8, device=codes.device)
+    for p in range(P):
+        m = min(16, rows - 16 * p)
+        at = slice(16 * p, 16 * p + m)
+        for i in range(n):
+            c[p, i // 4, i % 4, :m] = codes[at, 16 * i:16 * i + 16]
+            s[p, i // 4, :m, i % 4] = scales[at, i]
+    return c, s
 
 
 def gelu(y: torch.Tensor) -> torch.Tensor:

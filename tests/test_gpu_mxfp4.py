@@ -48,16 +48,19 @@ def test_rows_and_back(m, k):
     x[0] = 0
     x[m - 1, k - 1] = float("nan")
     x[m // 2, 3] = float("-inf")
-    codes, scales = mxfp4.quant_mxfp4(x)
+    q = mxfp4.quant_mxfp4(x)
     c, s = om.quantize(x)
-    same(codes, om.pack(c))
-    same(scales, om.scale_layout(s))
+    for got, want in zip(q, om.panels(om.pack(c), s)):
+        same(got, want)
+    assert q[2:] == (m, k)
+    for got, want in zip(mxfp4.to_rows(q), (om.pack(c), s)):
+        same(got, want)
     out = torch.full((m, k + 16), 7.0, dtype=torch.bfloat16, device=DEV)
-    mxfp4.dequant_mxfp4(codes, scales, out=out[:, 8:8 + k])
+    mxfp4.dequant_mxfp4(*q, out=out[:, 8:8 + k])
     assert bool((out[:, :8] == 7).all()) and bool((out[:, 8 + k:] == 7).all())
     want = om.values(c, s).float().bfloat16()
     torch.testing.assert_close(out[:, 8:8 + k], want, rtol=0, atol=0, equal_nan=True)
-    torch.testing.assert_close(mxfp4.dequant_mxfp4(codes, scales), want, rtol=0, atol=0, equal_nan=True)
+    torch.testing.assert_close(mxfp4.dequant_mxfp4(*q), want, rtol=0, atol=0, equal_nan=True)
 
 
 def test_every_bf16_under_every_neighbouring_maximum():
@@ -67,16 +70,16 @@ def test_every_bf16_under_every_neighbouring_maximum():
     for i, f in enumerate((0, 1, 1.75, 3.49, 100)):
         block[:, 32 * i + 9] = x
         block[:, 32 * i + 20] = (x.float() * -f).bfloat16()
-    codes, scales = mxfp4.quant_mxfp4(block)
+    codes, scales = mxfp4.to_rows(mxfp4.quant_mxfp4(block))
     c, s = om.quantize(block)
-    same(scales, om.scale_layout(s))
+    same(scales, s)
     same(codes, om.pack(c))
 
 
 def test_every_code_and_scale_byte_reads_back():
     codes = torch.arange(256, dtype=torch.int64, device=DEV).to(torch.uint8)[:, None].expand(256, 16 * 256).contiguous()
     s = torch.arange(256, dtype=torch.int64, device=DEV).to(torch.uint8)[None].expand(256, 256).contiguous()
-    got = mxfp4.dequant_mxfp4(codes, mxfp4.scales_from_rows(s))
+    got = mxfp4.dequant_mxfp4(*mxfp4.from_rows(codes, s))
     want = om.values(om.unpack(codes), s).float().bfloat16()
     torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
 
@@ -87,8 +90,8 @@ def test_unaligned_and_transposed_rows_are_copied_and_empty_ones_pass():
     same(mxfp4.quant_mxfp4(x)[0], mxfp4.quant_mxfp4(x.clone())[0])
     t = rows(64, 40, g).t()
     same(mxfp4.quant_mxfp4(t)[0], mxfp4.quant_mxfp4(t.contiguous())[0])
-    codes, scales = mxfp4.quant_mxfp4(x[:0])
-    assert codes.shape == (0, 1040) and mxfp4.dequant_mxfp4(codes, scales).shape == (0, 2080)
+    empty = mxfp4.quant_mxfp4(x[:0])
+    assert empty.codes.shape == (0, 17, 4, 16, 16) and mxfp4.dequant_mxfp4(*empty).shape == (0, 2080)
 
 
 # --------------------------------------------------------------- products
@@ -106,12 +109,13 @@ def test_linear_at_every_row_count(k, n):
         y, none = linear(x)
         assert none is None
         check(y, *om.product(exact(x), exact(w), bias, gelu))
-        same(y, mxfp4.gemm_mxfp4(*mxfp4.quant_mxfp4(x), linear.w_codes, linear.w_scales, linear.bias, gelu))
+        same(y, mxfp4.gemm_mxfp4(mxfp4.quant_mxfp4(x), linear.weight_rows, linear.bias, gelu))
         same(y, linear(x)[0])
 
 
 @pytest.mark.parametrize("m, k, n", [(1, 1536, 4608), (16, 5120, 13824), (3, 13824, 5120), (40, 8960, 1536), (64, 5120, 5120),
-                                     (390, 1536, 8960), (1560, 1536, 1536), (1100, 1568, 8196), (4680, 1536, 4608), (2000, 5120, 5120)])
+                                     (390, 1536, 8960), (1560, 1536, 1536), (1100, 1568, 8196), (4680, 1536, 4608), (2000, 5120, 5120),
+                                     (4680, 1536, 8960), (1560, 5120, 13824), (4680, 5120, 5120), (4681, 2592, 5124), (2570, 800, 7172)])
 def test_linear_at_the_presets_sizes(m, k, n):
     g = gen(m + k + n)
     x, w, b = rows(m, k, g), rows(n, k, g, 0.02), rows(1, n, g)[0].contiguous()
@@ -135,7 +139,7 @@ def test_strides_shapes_and_given_outputs(m):
     q = mxfp4.quant_mxfp4(x)
     for lo in (4, 8):                        # rows of 8-byte and of 16-byte alignment
         out.fill_(7.0)
-        got = mxfp4.gemm_mxfp4(*q, linear.w_codes, linear.w_scales, out=out[1:m + 1, lo:lo + n])
+        got = mxfp4.gemm_mxfp4(q, linear.weight_rows, out=out[1:m + 1, lo:lo + n])
         same(got, y)
         out[1:m + 1, lo:lo + n] = 7
         assert bool((out == 7).all())
@@ -169,6 +173,22 @@ def test_ranges_of_the_scales(m):
     x = (x.float() * torch.tensor([2.0 ** -130, 2.0 ** -60, 1.0, 2.0 ** 60], device=DEV)[e][:, None]).bfloat16()
     w[:, 128:] = (w[:, 128:].float() * 2.0 ** -40).bfloat16()
     check(mxfp4.WaveMxfp4Linear(w, None)(x)[0], *om.product(exact(x), exact(w)))
+
+
+@pytest.mark.parametrize("m", [2, 30, 200])
+def test_padding_rows_of_panels_reach_nothing(m):
+    """Whatever stands in a panel's rows and values past the last: NaN scales and codes of other rows."""
+    g = gen(m)
+    k, n = 416, 36                           # 14 values blocks of 16, 4 rows of the last panel
+    x, w = rows(m, k, g), rows(n, k, g, 0.05)
+    a, b = mxfp4.quant_mxfp4(x), mxfp4.quant_mxfp4(w)
+    want = mxfp4.gemm_mxfp4(a, b)
+    for q in (a, b):
+        last = q.rows - 16 * (q.codes.shape[0] - 1)
+        q.codes[-1, :, :, last:] = 0x77
+        q.scales[-1, :, last:] = 255
+    same(mxfp4.gemm_mxfp4(a, b), want)
+    same(mxfp4.dequant_mxfp4(*a), exact(x).float().bfloat16())
 
 
 def test_captured_linear_replays_and_two_streams():

@@ -38,17 +38,22 @@ def test_oracle_ties_signs_and_nonfinite_blocks():
     assert scales.tolist() == [[255]] and not codes.any() and torch.isnan(om.values(codes, scales)).all()
 
 
-def test_scale_layout_round_trip():
+def test_panels_round_trip():
     g = torch.Generator().manual_seed(1)
-    for rows, blocks in ((1, 1), (3, 5), (4, 4), (9, 12), (130, 7)):
+    for rows, blocks in ((1, 1), (3, 5), (16, 4), (17, 12), (130, 7), (0, 3)):
+        c = torch.randint(0, 256, (rows, 16 * blocks), generator=g, dtype=torch.int64).to(torch.uint8)
         s = torch.randint(0, 256, (rows, blocks), generator=g, dtype=torch.int64).to(torch.uint8)
-        laid = mxfp4.scales_from_rows(s)
-        assert torch.equal(laid, om.scale_layout(s))
-        assert torch.equal(mxfp4.scales_to_rows(laid, rows, 32 * blocks), s)
-    with pytest.raises(ValueError, match="have shape"):
-        mxfp4.scales_to_rows(laid, 4, 224)
-    with pytest.raises(ValueError, match="expected uint8"):
-        mxfp4.scales_from_rows(s.float())
+        q = mxfp4.from_rows(c, s)
+        want = om.panels(c, s)
+        assert torch.equal(q.codes, want[0]) and torch.equal(q.scales, want[1]) and q[2:] == (rows, 32 * blocks)
+        back = mxfp4.to_rows(q)
+        assert torch.equal(back[0], c) and torch.equal(back[1], s)
+    for c, s in ((torch.zeros((2, 16)), torch.zeros((2, 1))), (torch.zeros(16, dtype=torch.uint8), torch.zeros((1, 1), dtype=torch.uint8))):
+        with pytest.raises(ValueError, match="expected uint8"):
+            mxfp4.from_rows(c, s)
+    for shape_c, shape_s in (((2, 16), (2, 2)), ((2, 24), (2, 1)), ((2, 16), (3, 1))):
+        with pytest.raises(ValueError, match="do not go with"):
+            mxfp4.from_rows(torch.zeros(shape_c, dtype=torch.uint8), torch.zeros(shape_s, dtype=torch.uint8))
 
 
 def test_python_refusals():
@@ -58,33 +63,38 @@ def test_python_refusals():
             mxfp4.quant_mxfp4(bad)
     with pytest.raises(ValueError, match="on a GPU"):
         mxfp4.quant_mxfp4(bf)
-    codes, scales = torch.zeros((4, 32), dtype=torch.uint8), torch.zeros((1, 4, 4), dtype=torch.uint8)
+    q = mxfp4.from_rows(torch.zeros((4, 32), dtype=torch.uint8), torch.zeros((4, 2), dtype=torch.uint8))
     with pytest.raises(ValueError, match="on a GPU"):
-        mxfp4.dequant_mxfp4(codes, scales)
-    with pytest.raises(ValueError, match="the codes must be"):
-        mxfp4.dequant_mxfp4(codes[:, :8], scales)
-    with pytest.raises(ValueError, match="the scales must be"):
-        mxfp4.dequant_mxfp4(codes, scales[:, :3])
-    with pytest.raises(ValueError, match="out must be bf16"):
-        mxfp4.dequant_mxfp4(codes, scales, out=torch.zeros((4, 64)))
+        mxfp4.dequant_mxfp4(*q)
+    for bad, text in ((q._replace(rows=17), "q's codes must be"), (q._replace(k=160), "q's codes must be"), (q._replace(k=48), "not a multiple"),
+                      (q._replace(rows=-1), "-1 rows"), (q._replace(scales=q.scales[:, :, :8]), "q's scales must be"),
+                      (q._replace(codes=q.codes.float()), "q's codes must be"),
+                      (q._replace(codes=torch.zeros(1025, dtype=torch.uint8)[1:].view(1, 1, 4, 16, 16)), "16-byte aligned")):
+        with pytest.raises(ValueError, match=text):
+            mxfp4.dequant_mxfp4(*bad)
+    for out in (torch.zeros((4, 64)), bf[:, :32], torch.zeros((4, 68), dtype=torch.bfloat16)[:, :64], bf.t()):
+        with pytest.raises(ValueError, match="out must be bf16"):
+            mxfp4.dequant_mxfp4(*q, out=out)
+    wide = mxfp4.from_rows(torch.zeros((4, 64), dtype=torch.uint8), torch.zeros((4, 4), dtype=torch.uint8))
     with pytest.raises(ValueError, match="a has rows of 64 values"):
-        mxfp4.gemm_mxfp4(codes, scales, torch.zeros((4, 64), dtype=torch.uint8), scales)
+        mxfp4.gemm_mxfp4(q, wide)
     with pytest.raises(ValueError, match="bias must be"):
-        mxfp4.gemm_mxfp4(codes, scales, codes, scales, bias=torch.zeros(4))
+        mxfp4.gemm_mxfp4(q, q, bias=torch.zeros(4))
+    with pytest.raises(ValueError, match="on a GPU"):
+        mxfp4.gemm_mxfp4(q, q)
     with pytest.raises(ValueError, match="move the weight to a GPU"):
         mxfp4.WaveMxfp4Linear(bf, None)
-    for shape in ((6, 32), (0, 0)):
+    for n, k in ((6, 32), (4, 0)):
         with pytest.raises(ValueError, match="unsupported linear shape"):
-            mxfp4.WaveMxfp4Linear.from_codes(torch.zeros((shape[0], shape[1]), dtype=torch.uint8),
-                                             torch.zeros((-(-shape[1] // 64), -(-shape[0] // 4) * 4, 4), dtype=torch.uint8))
-    linear = mxfp4.WaveMxfp4Linear.from_codes(codes, torch.zeros((4, 2), dtype=torch.uint8), torch.zeros(4))
-    assert linear.w_scales.shape == (1, 4, 4) and linear.bias.dtype == torch.bfloat16 and linear.in_features == 64
+            mxfp4.WaveMxfp4Linear.from_quantized(mxfp4.from_rows(torch.zeros((n, k // 2), dtype=torch.uint8), torch.zeros((n, k // 32), dtype=torch.uint8)))
+    linear = mxfp4.WaveMxfp4Linear.from_quantized(q, torch.zeros(4))
+    assert linear.bias.dtype == torch.bfloat16 and linear.in_features == 64 and linear.weight_rows == q
     with pytest.raises(ValueError, match="input width 32"):
         linear(torch.zeros((1, 32), dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="on a GPU"):
         linear(bf)
     with pytest.raises(ValueError, match="bias has shape"):
-        mxfp4.WaveMxfp4Linear.from_codes(codes, scales, torch.zeros(5))
+        mxfp4.WaveMxfp4Linear.from_quantized(q, torch.zeros(5))
 
 
 def test_swap_refuses_what_the_others_refuse():
@@ -116,7 +126,7 @@ def test_quant_refusals(args, text):
     (dict(n=6), "multiples of 4"), (dict(ldy=10), "multiples of 4"), (dict(a=None), "null pointer"), (dict(w=None), "null pointer"),
     (dict(y=None), "null pointer"), (dict(w_scales=None), "null pointer"), (dict(w=24), "aligned"), (dict(a=24), "aligned"),
     (dict(y=4), "aligned"), (dict(bias=4), "aligned"), (dict(flags=2), "unknown flags"), (dict(m=1 << 27, k=64), "2 GiB"),
-    (dict(n=1 << 27, ldy=1 << 27, k=64), "2 GiB"), (dict(m=1 << 25, n=1 << 25, ldy=1 << 25, k=32), "too large"),
+    (dict(n=1 << 27, ldy=1 << 27, k=64), "2 GiB"), (dict(m=1 << 24, n=1 << 24, ldy=1 << 24, k=32), "too large"),
 ])
 def test_product_refusals(change, text):
     d = dict(a=16, a_scales=16, w=16, w_scales=16, m=20, n=8, k=32, bias=None, y=16, ldy=8, flags=0)

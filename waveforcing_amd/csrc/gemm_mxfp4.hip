@@ -2,18 +2,18 @@
 // (mxfp4_rows.hip has the layouts), sums and epilogue in fp32, rounded once.  The scaled matrix instruction takes codes and
 // scales as they are: v_mfma_scale_f32_32x32x64_f8f6f4 at twice the fp8 rate, products of its sums exact to 2^-24 of sum|a w|.
 //
-// Many rows (gemm_mxfp4_kernel): the tiles and the K loop of the 8-bit products (gemm_w8a8.hip), whose 128 bytes of a row
-// are here 256 values: operands by DMA into XOR-swizzled LDS rows, three stages (the 256-row tile: two), a step of four
-// sub-steps, the next sub-step's fragments read and a later step's DMAs issued between the matrix instructions.  A step's
-// scales, two words a row (each of 128 values), come with its stage; a lane holds 32 consecutive values of one row in each
-// operand, so the byte it needs is 2 s + (its half) of the word: one shift a word, and the instruction's byte select.
+// Many rows (gemm_mxfp4_kernel): the K loop of the 8-bit products (gemm_w8a8.hip), whose 128 bytes of a row are here 256
+// values: operands by DMA into LDS, three stages (the 256-row tile: two), a step of four sub-steps, the next sub-step's
+// fragments read and a later step's DMAs issued between the matrix instructions.  A panel (16 rows x 128 values, 1 KB in the
+// order of the lanes) is one DMA, and 16 lanes' fragments are 256 bytes in a row: no swizzle, and every place in LDS is a
+// constant from the lane's first.  The scales, a word a row and panel, come with their stage; the byte a lane needs is
+// 2 s + (its half) of the word: one shift a word, and the instruction's byte select.
 //
-// Few rows (gemm_mxfp4_few_kernel): up to 64 rows, bound by reading the weight once.  A workgroup takes 16 or 32 columns and
-// all rows; its waves split K and go without barriers, operands straight from memory in the layout of the 16x16x128
-// instruction (16 bytes of a row a lane), and add up in LDS in the order of the waves.  Up to 16 rows the activations are
-// quantized in the same kernel: a lane's operand is one whole block, so the maximum, the scale and the codes need no other
-// lane.
+// Few rows (gemm_mxfp4_few_kernel): bound by reading the weight once.  A workgroup takes 16 or 32 columns and all rows; its
+// waves split K and go without barriers, operands straight from memory, and add up in LDS in the order of the waves.  Up to
+// WF_MXFP4_FUSED_ROWS rows the activations are quantized in the same kernel.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_core.hpp"
 #include "launchers.hpp"
@@ -26,6 +26,11 @@ using namespace gemm;
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
+// A part of the output that one tile covers: rows [m0, m1), columns [n0, n1), from m0 and n0 on in whole tiles.
+struct Rect {
+  int m0, m1, n0, n1;
+};
+
 struct MxArgs {
   const uint16_t* x;  // few rows: bf16 rows (stride ldx) quantized by the kernel, or null
   int64_t ldx;
@@ -36,6 +41,8 @@ struct MxArgs {
   int64_t ldy;
   int gelu;
   int vec16;  // y and ldy allow 16-byte row stores
+  Rect rect[4];  // of the first tile: 0, 1; of the second: 2, 3
+  int count[4];  // their tiles
 };
 
 __device__ inline v8i widen(const v4i& v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
@@ -52,78 +59,76 @@ struct MxTile {
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
   static constexpr int NBA = BM / 8 / NW, NBB = BN / 8 / NW;       // 1 KB DMA blocks of codes per wave and step
-  static constexpr int NSA = (BM + 127) / 128, NSB = (BN + 127) / 128;  // 1 KB DMA blocks of scales per step
+  static constexpr int NSA = (BM + 127) / 128, NSB = (BN + 127) / 128;  // 1 KB DMA blocks of scales per step (64 rows: half used)
   static constexpr int B_OFF = BM * BK, SA_OFF = B_OFF + BN * BK, SB_OFF = SA_OFF + NSA * 1024;
   static constexpr int STAGE = SB_OFF + NSB * 1024;
   static constexpr int WCOLS = BN / WN, WPITCH = WCOLS * 2 + 16;
   static constexpr int EPI = BN * 4;                               // the bias as fp32
   static constexpr int LDS = ST * STAGE + EPI;
-  static_assert(NBA * 8 * NW == BM && NBB * 8 * NW == BN && NSA + NSB <= NW, "DMA blocks");
+  static_assert(NBA * 8 * NW == BM && NBB * 8 * NW == BN && NSA + NSB <= NW && NW % 2 == 0, "DMA blocks");
   static_assert(NW * 2 * 32 * WPITCH <= ST * STAGE, "wave staging fits the stages");
   static_assert(LDS <= 160 * 1024, "LDS of one workgroup");
 };
 using TileBig = MxTile<256, 256, 2, 4, 2>;
 using TileStd = MxTile<128, 256, 2, 4, 3>;
 using TileMid = MxTile<128, 128, 2, 4, 3>;
+using TileHalf = MxTile<64, 128, 2, 2, 3>;
 using TileSmall = MxTile<64, 64, 2, 2, 3>;
 
 constexpr int SUB = 4;       // sub-steps of a step, 64 values each
+constexpr uint32_t kFar = 0x7ffffff0u;
 
+// Tile t of rect r.
 template <typename T>
-__global__ __launch_bounds__(T::THREADS, 1) void gemm_mxfp4_kernel(MxArgs p) {
+__device__ __attribute__((always_inline)) inline void mx_tile(const MxArgs& p, const Rect& r, int t, uint8_t* lds) {
   constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN, NW = T::NW, MI = T::MI, NI = T::NI, ST = T::ST;
   constexpr int NBA = T::NBA, NDMA = T::NBA + T::NBB, STAGE = T::STAGE, NS = T::NSA + T::NSB;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
   float* const epi = reinterpret_cast<float*>(lds + ST * STAGE);
 
-  // tiles: an XCD's workgroups (blockIdx % 8) are a contiguous range, walked in bands of GROUP_M tile rows
-  const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
-  const int n_tiles = tiles_m * tiles_n, per_xcd = (n_tiles + NUM_XCD - 1) / NUM_XCD;
-  const int t = static_cast<int>(blockIdx.x % NUM_XCD) * per_xcd + static_cast<int>(blockIdx.x) / NUM_XCD;
-  if (t >= n_tiles || static_cast<int>(blockIdx.x) / NUM_XCD >= per_xcd) return;
+  // in bands of GROUP_M tile rows
+  const int tiles_m = (r.m1 - r.m0 + BM - 1) / BM, tiles_n = (r.n1 - r.n0 + BN - 1) / BN;
   const int per_group = GROUP_M * tiles_n;
   const int first_m = (t / per_group) * GROUP_M;
   const int band = min(tiles_m - first_m, GROUP_M);
-  const int m0 = (first_m + (t % per_group) % band) * BM, n0 = ((t % per_group) / band) * BN;
+  const int m0 = r.m0 + (first_m + (t % per_group) % band) * BM, n0 = r.n0 + ((t % per_group) / band) * BN;
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int l32 = lane & 31, half = lane >> 5;
 
-  const int row_bytes = p.K >> 1, groups = (p.K + 127) / 128, M4 = (p.M + 3) & ~3, N4 = (p.N + 3) & ~3;
-  const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a), 0, p.M * row_bytes, kBufferRsrcWord3);
-  const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.w), 0, p.N * row_bytes, kBufferRsrcWord3);
-  // DMA block j of this wave: rows (j NW + wave) 8 .. + 7 of A (j < NBA) or W; 16-byte chunk c of row r lands at c ^ (r / 2 % 8).
-  // The blocks' rows differ by 8 NW, so a lane has one chunk and one offset for each operand.
-  static_assert(NW % 2 == 0, "the blocks of a wave share the swizzle");
-  const int drow = wave * 8 + (lane >> 3), dcol = 16 * ((lane & 7) ^ ((drow >> 1) & 7));
-  const int doff_a = (m0 + drow) * row_bytes + dcol, doff_w = (n0 + drow) * row_bytes + dcol;
-  // scales: wave i brings 1 KB (i % (NSA + NSB); the same bytes twice cost less than a branch in the loop) of the step's
-  // [2 groups][BM] words of A, then of W's; words past the last group read as zero, those of rows past the last belong to
-  // outputs that are not stored
+  const int groups = (p.K + 127) / 128, pa = (p.M + 15) / 16, pw = (p.N + 15) / 16;  // panels
+  const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a), 0, pa * groups * 1024, kBufferRsrcWord3);
+  const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.w), 0, pw * groups * 1024, kBufferRsrcWord3);
+
+  // DMA block j of this wave: panel (j NW + wave) / 2 of the tile's rows, the step's first or second 128 values (wave % 2).
+  // Panels past the last row are past the buffer's end and read as zero.
+  const uint32_t doff_a = static_cast<uint32_t>(((m0 / 16 + wave / 2) * groups + (wave & 1)) * 1024 + 16 * lane);
+  const uint32_t doff_w = static_cast<uint32_t>(((n0 / 16 + wave / 2) * groups + (wave & 1)) * 1024 + 16 * lane);
+  // scales: wave i brings 1 KB (i % (NSA + NSB); the same bytes twice cost less than a branch in the loop), 128 bytes a panel
   const int sblk = wave % NS;
   const bool s_is_a = sblk < T::NSA;
-  const int srow4 = s_is_a ? M4 : N4;
-  const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(s_is_a ? p.a_scales : p.w_scales), 0, groups * srow4 * 4, kBufferRsrcWord3);
+  const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(s_is_a ? p.a_scales : p.w_scales), 0,
+                                                    (s_is_a ? pa : pw) * groups * 64, kBufferRsrcWord3);
   const int sdst = T::SA_OFF + sblk * 1024;
-  int soff = kOutOfRange - groups * srow4 * 4;  // (what it grows by over the steps)
-  {
-    const int word = ((s_is_a ? sblk : sblk - T::NSA) * 64 + lane) * 4, b = s_is_a ? BM : BN, g = word / b;
-    if (g < 2) soff = (g * srow4 + (s_is_a ? m0 : n0) + word % b) * 4;
-  }
+  const int spanel = (s_is_a ? sblk : sblk - T::NSA) * 8 + (lane >> 3), sgroup = (lane >> 2) & 1;
+  // Offsets are unsigned: kFar more is out of every buffer's range.  (In scalar registers where they are uniform, not a vector
+  // register for each block; and no branch in the loop.)
+  const bool s_in = spanel < (s_is_a ? BM : BN) / 16;
+  const uint32_t soff = s_in ? static_cast<uint32_t>((((s_is_a ? m0 : n0) / 16 + spanel) * groups) * 64 + 16 * (lane & 7)) : kFar;
+  const uint32_t s_second = s_in && sgroup ? kFar : 0u;  // the words of the second 128 values
   auto dma = [&](auto J, int step, int stage) __attribute__((always_inline)) {
     constexpr int j = decltype(J)::value;
-    const int k0 = step * BK;
+    // (a last step of 128 values: nothing in the place of the second 128, not the next panel's first)
     if constexpr (j == NDMA) {
-      dma16(rs, lds + stage * STAGE + sdst, soff + __builtin_amdgcn_readfirstlane(step * 2 * srow4 * 4));
+      const uint32_t half_step = __builtin_amdgcn_readfirstlane(2 * step + 1 < groups ? 0 : -1);
+      dma16(rs, lds + stage * STAGE + sdst, static_cast<int>(soff + static_cast<uint32_t>(step) * 128u + (half_step & s_second)));
     } else {
-      // (the uniform part in a scalar register, not a vector register for each block)
-      const int by = __builtin_amdgcn_readfirstlane((j < NBA ? j : j - NBA) * NW * 8 * row_bytes + k0);
-      const int off = k0 + dcol < row_bytes ? (j < NBA ? doff_a : doff_w) + by : kOutOfRange;
+      const uint32_t at = static_cast<uint32_t>((j < NBA ? j : j - NBA) * (NW / 2) * groups * 1024 + step * 2048);
+      const uint32_t by = __builtin_amdgcn_readfirstlane(2 * step + (wave & 1) < groups ? at : kFar);
       if constexpr (j < NBA)
-        dma16(ra, lds + stage * STAGE + (j * NW + wave) * 1024, off);
+        dma16(ra, lds + stage * STAGE + (j * NW + wave) * 1024, static_cast<int>(doff_a + by));
       else
-        dma16(rw, lds + stage * STAGE + T::B_OFF + ((j - NBA) * NW + wave) * 1024, off);
+        dma16(rw, lds + stage * STAGE + T::B_OFF + ((j - NBA) * NW + wave) * 1024, static_cast<int>(doff_w + by));
     }
   };
 
@@ -131,13 +136,12 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mxfp4_kernel(MxArgs p) {
   for (int c = static_cast<int>(threadIdx.x); c < BN; c += T::THREADS)
     epi[c] = p.bias && n0 + c < p.N ? bf16_bits_to_f32(p.bias[n0 + c]) : 0.f;
 
-  // Fragments: sub-step s of a lane's row is its chunk 2 s + half; the rows one lane reads differ by multiples of 32
-  const int x = (l32 >> 1) & 7;
-  const int lane_a = (wm * (BM / WM) + l32) * BK, lane_b = T::B_OFF + (wn * (BN / WN) + l32) * BK;
-  const int lane_sa = T::SA_OFF + (wm * (BM / WM) + l32) * 4, lane_sb = T::SB_OFF + (wn * (BN / WN) + l32) * 4;
-  int koff[SUB];
-#pragma unroll
-  for (int s = 0; s < SUB; ++s) koff[s] = 16 * ((2 * s + half) ^ x);
+  // Fragments: a lane's 32 values of sub-step s are block 2 (s % 2) + half of its row in the panel of the step's first (s < 2)
+  // or second 128 values
+  const int lane_a = (wm * (BM / WM) / 16 + (l32 >> 4)) * 2048 + half * 256 + (l32 & 15) * 16;
+  const int lane_b = T::B_OFF + (wn * (BN / WN) / 16 + (l32 >> 4)) * 2048 + half * 256 + (l32 & 15) * 16;
+  const int lane_sa = T::SA_OFF + (wm * (BM / WM) / 16 + (l32 >> 4)) * 128 + (l32 & 15) * 4;
+  const int lane_sb = T::SB_OFF + (wn * (BN / WN) / 16 + (l32 >> 4)) * 128 + (l32 & 15) * 4;
 
   v16f acc[NI][MI];
 #pragma unroll
@@ -154,13 +158,13 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mxfp4_kernel(MxArgs p) {
     constexpr int o = decltype(O)::value, s = decltype(S)::value;
     const uint8_t* st = lds + stage * STAGE;
     if constexpr (o < MI)
-      fa[s & 1][o] = *reinterpret_cast<const v4i*>(st + lane_a + koff[s] + o * 32 * BK);
+      fa[s & 1][o] = *reinterpret_cast<const v4i*>(st + lane_a + (s >> 1) * 1024 + (s & 1) * 512 + o * 4096);
     else if constexpr (o < NFR)
-      fw[s & 1][o - MI] = *reinterpret_cast<const v4i*>(st + lane_b + koff[s] + (o - MI) * 32 * BK);
+      fw[s & 1][o - MI] = *reinterpret_cast<const v4i*>(st + lane_b + (s >> 1) * 1024 + (s & 1) * 512 + (o - MI) * 4096);
     else if constexpr (o < NFR + MI)
-      sa[s >> 1][o - NFR] = *reinterpret_cast<const int*>(st + lane_sa + (s >> 1) * BM * 4 + (o - NFR) * 128);
+      sa[s >> 1][o - NFR] = *reinterpret_cast<const int*>(st + lane_sa + (s >> 1) * 64 + (o - NFR) * 256);
     else
-      sw[s >> 1][o - NFR - MI] = *reinterpret_cast<const int*>(st + lane_sb + (s >> 1) * BN * 4 + (o - NFR - MI) * 128);
+      sw[s >> 1][o - NFR - MI] = *reinterpret_cast<const int*>(st + lane_sb + (s >> 1) * 64 + (o - NFR - MI) * 256);
   };
   // The products of sub-step S and, spread between them, the reads of sub-step (S + 1) % 4 from rstage (RD) and the DMAs
   // of slot SLOT (of SUB; two stages: all in slot 0) of step dstep into dstage (DM).
@@ -198,7 +202,7 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mxfp4_kernel(MxArgs p) {
   };
 
   // Stages 0 and 1; only stage 0 is waited for here (a wave's DMAs land in order).
-  const int nk = (row_bytes + BK - 1) / BK;
+  const int nk = (groups + 1) / 2;
   static_for<NDMA + 1>([&](auto J) { dma(J, 0, 0); });
   if (nk > 1) static_for<NDMA + 1>([&](auto J) { dma(J, 1, 1); });
   if (nk == 1)
@@ -304,122 +308,187 @@ __global__ __launch_bounds__(T::THREADS, 1) void gemm_mxfp4_kernel(MxArgs p) {
   }
 }
 
+// The tiles of T1, then those of T2 (the output's rest), in one launch: a CU takes its next tile as soon as it is done with one.
+// An XCD's workgroups (blockIdx % 8) take a contiguous range of each rect's tiles.
+template <typename T1, typename T2>
+__global__ __launch_bounds__(T1::THREADS, 1) void gemm_mxfp4_kernel(MxArgs p) {
+  static_assert(T1::THREADS == T2::THREADS, "one launch");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[T1::LDS > T2::LDS ? T1::LDS : T2::LDS];
+  int w = static_cast<int>(blockIdx.x), at = 0, t = 0;
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int per_xcd = (p.count[i] + NUM_XCD - 1) / NUM_XCD, padded = per_xcd * NUM_XCD;
+    if (!found && w < padded) {
+      found = true;
+      at = i;
+      t = w % NUM_XCD * per_xcd + w / NUM_XCD;
+    }
+    w -= padded;
+  }
+  const Rect r{at == 0 ? p.rect[0].m0 : at == 1 ? p.rect[1].m0 : at == 2 ? p.rect[2].m0 : p.rect[3].m0,
+               at == 0 ? p.rect[0].m1 : at == 1 ? p.rect[1].m1 : at == 2 ? p.rect[2].m1 : p.rect[3].m1,
+               at == 0 ? p.rect[0].n0 : at == 1 ? p.rect[1].n0 : at == 2 ? p.rect[2].n0 : p.rect[3].n0,
+               at == 0 ? p.rect[0].n1 : at == 1 ? p.rect[1].n1 : at == 2 ? p.rect[2].n1 : p.rect[3].n1};
+  const int count = at == 0 ? p.count[0] : at == 1 ? p.count[1] : at == 2 ? p.count[2] : p.count[3];
+  if (t >= count) return;
+  if constexpr (std::is_same<T1, T2>::value)
+    mx_tile<T1>(p, r, t, lds);
+  else if (at < 2)
+    mx_tile<T1>(p, r, t, lds);
+  else
+    mx_tile<T2>(p, r, t, lds);
+}
+
 // ---------------------------------------------------------------- few rows
+// Order the wave's own LDS accesses (the hardware keeps them in order; this keeps the compiler to it).
+__device__ inline void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 constexpr int kFewRows = 64, kFusedRows = WF_MXFP4_FUSED_ROWS;
 
-// NB blocks of 16 rows, NC of 16 columns, W waves that share K in turns of 128 values; QUANT: the rows are bf16.
-template <int NB, int NC, int W, bool QUANT>
-__global__ __launch_bounds__(64 * W) void gemm_mxfp4_few_kernel(MxArgs p) {
+constexpr int kRun = 2;
+constexpr int kXPitch = 80;  // LDS bytes of a quantized row's 128 values (16 rows' 16-byte reads touch every bank alike)
+
+// NB blocks of 16 rows, NC of 16 columns, W waves that share K in turns of 128 values, DEEP turns of a wave in flight; XR: the
+// rows are bf16, up to 4 XR of them (0: they are codes).  OCC: waves of a SIMD that the registers are allotted for.
+template <int NB, int NC, int W, int DEEP, int OCC, int XR>
+__global__ __launch_bounds__(64 * W, OCC) void gemm_mxfp4_few_kernel(MxArgs p) {
+  constexpr bool QUANT = XR > 0;
   static_assert(!QUANT || NB == 1, "rows quantized in the kernel: one block");
-  __shared__ __attribute__((aligned(16))) v4f part[W > 1 ? W - 1 : 1][NB * NC][64];
+  constexpr int kPart = (W - 1) * NB * NC * 64 * 16, kX = QUANT ? W * 16 * (kXPitch + 4) : 0;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kPart > kX ? kPart : kX];
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int l16 = lane & 15, g4 = lane >> 4;
   const int n0 = static_cast<int>(blockIdx.x) * 16 * NC;
-  const int row_bytes = p.K >> 1, steps = (p.K + 127) / 128, M4 = (p.M + 3) & ~3, N4 = (p.N + 3) & ~3;
-  const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.w), 0, p.N * row_bytes, kBufferRsrcWord3);
-  const auto rsw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.w_scales), 0, steps * N4 * 4, kBufferRsrcWord3);
-  const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a), 0, QUANT ? 0 : p.M * row_bytes, kBufferRsrcWord3);
-  const auto rsa = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a_scales), 0, QUANT ? 0 : steps * M4 * 4, kBufferRsrcWord3);
+  const int steps = (p.K + 127) / 128, pa = (p.M + 15) / 16, pw = (p.N + 15) / 16;  // panels
+  const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.w), 0, pw * steps * 1024, kBufferRsrcWord3);
+  const auto rsw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.w_scales), 0, pw * steps * 64, kBufferRsrcWord3);
+  // rows past the last are out of the buffer's range and read as zero
+  const auto ra = QUANT ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p.x), 0, static_cast<int>(((p.M - 1) * p.ldx + p.K) * 2), kBufferRsrcWord3)
+                        : __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a), 0, pa * steps * 1024, kBufferRsrcWord3);
+  const auto rsa = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a_scales), 0, QUANT ? 0 : pa * steps * 64, kBufferRsrcWord3);
+  const int xrow = static_cast<int>(p.ldx) * 2;
+  uint8_t* const xbuf = lds + wave * 16 * (kXPitch + 4);
 
   v4f acc[NB][NC];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[b][c] = v4f{0, 0, 0, 0};
-  // a lane's 32 values of a step: those from 128 s + 32 g4 on, of column n0 + 16 c + l16 and row 16 b + l16
+  // A lane's operands of a step are 32 values, from 128 s + 32 g4 on, of column n0 + 16 c + l16 and row 16 b + l16.  bf16 rows
+  // are loaded as 256 bytes of 4 rows at a time, quantized by four lanes a block, and change lanes through LDS.
   struct Regs {
-    u32x4 w[NC], a[QUANT ? 4 : NB];
+    u32x4 w[NC], a[QUANT ? XR : NB];
     int sw[NC], sa[NB];
   };
-  const bool row_ok = l16 < p.M;
-  const uint16_t* xrow = QUANT ? p.x + static_cast<int64_t>(row_ok ? l16 : 0) * p.ldx + 32 * g4 : nullptr;
-  auto load = [&](int s, Regs& r) __attribute__((always_inline)) {
-    const bool there = 128 * s + 32 * g4 < p.K;  // (K % 32 == 0; also false past the last step)
+  const int first = n0 / 16 * steps;  // panel
+  auto load = [&](int step, Regs& r) __attribute__((always_inline)) {
+    const int s = __builtin_amdgcn_readfirstlane(step);  // (in scalar registers, no vector register for each load's place)
+    const bool there = s < steps;
+    if constexpr (QUANT) {
+      const int at = 128 * s + 8 * l16;
+#pragma unroll
+      for (int i = 0; i < XR; ++i) r.a[i] = __builtin_amdgcn_raw_buffer_load_b128(ra, at < p.K ? (4 * i + g4) * xrow + 2 * at : kOutOfRange, 0, 0);
+    }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int n = n0 + 16 * c + l16;
-      r.w[c] = __builtin_amdgcn_raw_buffer_load_b128(rw, there ? n * row_bytes + 64 * s + 16 * g4 : kOutOfRange, 0, 0);
-      r.sw[c] = __builtin_amdgcn_raw_buffer_load_b8(rsw, there && n < p.N ? (s * N4 + n) * 4 + g4 : kOutOfRange, 0, 0);
+      const int panel = first + c * steps + s;
+      r.w[c] = __builtin_amdgcn_raw_buffer_load_b128(rw, (there ? panel * 1024 : kOutOfRange - 1024) + 16 * lane, 0, 0);
+      r.sw[c] = __builtin_amdgcn_raw_buffer_load_b32(rsw, (there ? panel * 64 : kOutOfRange - 64) + 4 * l16, 0, 0);
     }
-    if constexpr (QUANT) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r.a[i] = u32x4{0, 0, 0, 0};
-        if (row_ok && there) r.a[i] = *reinterpret_cast<const u32x4*>(xrow + 128 * s + 8 * i);
-      }
-    } else {
+    if constexpr (!QUANT) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const int m = 16 * b + l16;
-        r.a[b] = __builtin_amdgcn_raw_buffer_load_b128(ra, there ? m * row_bytes + 64 * s + 16 * g4 : kOutOfRange, 0, 0);
-        r.sa[b] = __builtin_amdgcn_raw_buffer_load_b8(rsa, there && m < p.M ? (s * M4 + m) * 4 + g4 : kOutOfRange, 0, 0);
+        const int panel = b * steps + s;
+        r.a[b] = __builtin_amdgcn_raw_buffer_load_b128(ra, (there ? panel * 1024 : kOutOfRange - 1024) + 16 * lane, 0, 0);
+        r.sa[b] = __builtin_amdgcn_raw_buffer_load_b32(rsa, (there ? panel * 64 : kOutOfRange - 64) + 4 * l16, 0, 0);
       }
     }
   };
   auto product = [&](Regs& r) __attribute__((always_inline)) {
     v4i a[NB];
     if constexpr (QUANT) {
-      uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = mx::max_bits2(top, mx::max_bits2(mx::max_bits2(r.a[i][0], r.a[i][1]), mx::max_bits2(r.a[i][2], r.a[i][3])));
-      const int e = mx::scale_byte(mx::max_half(top));
-      const float s = mx::scale_of(e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < XR; ++i) {  // (what LDS holds of other rows belongs to sums that are not stored)
         const uint32_t w[4] = {r.a[i][0], r.a[i][1], r.a[i][2], r.a[i][3]};
-        a[0][i] = static_cast<int>(mx::encode8(w, s));  // (whatever the codes, a scale byte of 255 makes the sum NaN)
+        uint32_t top = mx::max_half(mx::max_bits2(mx::max_bits2(w[0], w[1]), mx::max_bits2(w[2], w[3])));
+        top = max(top, mx::dpp_u32<0xB1>(top));
+        top = max(top, mx::dpp_u32<0x4E>(top));
+        const int e = mx::scale_byte(top);
+        const int row = 4 * i + g4;  // (whatever the codes, a scale byte of 255 makes the sum NaN)
+        *reinterpret_cast<uint32_t*>(xbuf + row * kXPitch + 4 * l16) = mx::encode8(w, mx::scale_of(e));
+        xbuf[16 * kXPitch + 4 * row + (l16 >> 2)] = static_cast<uint8_t>(e);  // (the block's four lanes the same: no branch)
       }
-      r.sa[0] = e;
+      wave_order();
+      a[0] = *reinterpret_cast<const v4i*>(xbuf + l16 * kXPitch + 16 * g4);
+      r.sa[0] = xbuf[16 * kXPitch + 4 * l16 + g4];
+      wave_order();
     } else {
 #pragma unroll
       for (int b = 0; b < NB; ++b) a[b] = __builtin_bit_cast(v4i, r.a[b]);
     }
+    // (a lane's own byte of the row's word; loads of single bytes are no cheaper than of 16)
+    int sw[NC], sa[NB];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) sw[c] = static_cast<int>(static_cast<uint32_t>(r.sw[c]) >> (8 * g4));
+#pragma unroll
+    for (int b = 0; b < NB; ++b) sa[b] = QUANT ? r.sa[b] : static_cast<int>(static_cast<uint32_t>(r.sa[b]) >> (8 * g4));
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         acc[b][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(__builtin_bit_cast(v4i, r.w[c])), widen(a[b]), acc[b][c], 4, 4, 0,
-                                                                     r.sw[c] & 0xff, 0, r.sa[b] & 0xff);
+                                                                     sw[c], 0, sa[b]);
   };
-  constexpr int DEEP = NB == 4 ? 2 : 4;  // steps whose loads are in flight
+  // the wave's i-th turn: runs of kRun neighbouring steps, whose scales share a cache line
+  auto step_of = [&](int i) __attribute__((always_inline)) { return (i / kRun * W + wave) * kRun + i % kRun; };
+  static_assert(DEEP % kRun == 0, "whole runs in flight");
   Regs r[DEEP];
 #pragma unroll
-  for (int d = 0; d < DEEP; ++d) load(wave + W * d, r[d]);
-  for (int s = wave; s < steps; s += W * DEEP) {
+  for (int d = 0; d < DEEP; ++d) load(step_of(d), r[d]);
+  // (the bias of the columns that wave 0 stores, asked for before the sums)
+  uint2 bias[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int n = n0 + 16 * c + 4 * g4;
+    bias[c] = make_uint2(0, 0);
+    if (wave == 0 && p.bias && n < p.N) bias[c] = *reinterpret_cast<const uint2*>(p.bias + n);
+  }
+  for (int i = 0; step_of(i) < steps; i += DEEP) {
 #pragma unroll
     for (int d = 0; d < DEEP; ++d) {
       product(r[d]);
-      load(s + W * (DEEP + d), r[d]);
+      __builtin_amdgcn_sched_barrier(0);  // (the loads take the registers that the product leaves)
+      load(step_of(i + DEEP + d), r[d]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
-  if constexpr (W > 1) {
-    if (wave) {
+  if constexpr (QUANT) __syncthreads();  // the sums take the place of the rows
+  v4f* const part = reinterpret_cast<v4f*>(lds) + lane;
+  if (wave) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) part[wave - 1][b * NC + c][lane] = acc[b][c];
-    }
-    __syncthreads();
-    if (wave) return;
+      for (int c = 0; c < NC; ++c) part[((wave - 1) * NB * NC + b * NC + c) * 64] = acc[b][c];
   }
+  __syncthreads();
+  if (wave) return;
   // wave 0 adds the others' sums, in their order, and stores
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       v4f v = acc[b][c];
-      if constexpr (W > 1) {
 #pragma unroll
-        for (int i = 0; i < W - 1; ++i) v += part[i][b * NC + c][lane];
-      }
+      for (int i = 0; i < W - 1; ++i) v += part[(i * NB * NC + b * NC + c) * 64];
       const int m = 16 * b + l16, n = n0 + 16 * c + 4 * g4;  // rows of the first operand, 4 to a lane: columns of y
       if (m >= p.M || n >= p.N) continue;
-      if (p.bias) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p.bias + n);
-        v[0] += bf16_lo_to_f32(w.x), v[1] += bf16_hi_to_f32(w.x), v[2] += bf16_lo_to_f32(w.y), v[3] += bf16_hi_to_f32(w.y);
-      }
+      v[0] += bf16_lo_to_f32(bias[c].x), v[1] += bf16_hi_to_f32(bias[c].x), v[2] += bf16_lo_to_f32(bias[c].y), v[3] += bf16_hi_to_f32(bias[c].y);
       if (p.gelu) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = gelu_tanh(v[e]);
@@ -428,50 +497,126 @@ __global__ __launch_bounds__(64 * W) void gemm_mxfp4_few_kernel(MxArgs p) {
     }
 }
 
-template <int NB, int NC, bool QUANT>
-void launch_few_waves(const MxArgs& p, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>((p.N + 16 * NC - 1) / (16 * NC)));
-  if (p.K <= 128 * 8)
-    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<NB, NC, 4, QUANT>), grid, dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<NB, NC, 8, QUANT>), grid, dim3(512), 0, stream, p);
-}
+constexpr int kDeep = 2;  // (3 or 4 turns in flight: 5-25 % slower at one row, even at 64)
 
-template <int NB, bool QUANT>
+// Columns and waves of a workgroup.  Enough columns that the rows are not read too often, enough waves that the weight is on
+// its way everywhere: some 6 waves to a CU.  16 x 5120 -> 13824 in columns of 16, 32, 64: 10.5, 9.9, 9.6 us (its product alone);
+// 1 x 13824 -> 5120 12.5, 10.3, 15.0; 1 x 1536 -> 1536 2.9, 3.3, 4.2; in 4, 8, 16 waves 1 x 5120 -> 13824 9.1, 9.4, 10.3,
+// 13824 -> 5120 (columns of 16) 14.4, 10.4, 11.7.
+template <int NB, int XR>
 void launch_few(const MxArgs& p, hipStream_t stream) {
-  if (p.N >= 32 * device_cus())
-    launch_few_waves<NB, 2, QUANT>(p, stream);
+  auto go = [&](auto C, auto WAVES) {
+    constexpr int NC = decltype(C)::value, W = decltype(WAVES)::value;
+    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<NB, NC, W, kDeep, 4, XR>), dim3(static_cast<uint32_t>((p.N + 16 * NC - 1) / (16 * NC))),
+                       dim3(64 * W), 0, stream, p);
+  };
+  const int cus = device_cus();
+  if (p.N >= 32 * cus)
+    if constexpr (XR == 4)  // (the rows are quantized anew by every workgroup: 16 x 5120 -> 13824 12.9 us in columns of 32, 11.5 of 64)
+      go(ic<4>{}, ic<8>{});
+    else
+      go(ic<2>{}, ic<4>{});
+  else if (p.N >= 20 * cus)
+    go(ic<2>{}, ic<8>{});
   else
-    launch_few_waves<NB, 1, QUANT>(p, stream);
+    go(ic<1>{}, ic<8>{});
 }
 
-template <typename T>
-void launch_tile(const MxArgs& p, hipStream_t stream) {
-  const int64_t tiles = static_cast<int64_t>((p.M + T::BM - 1) / T::BM) * ((p.N + T::BN - 1) / T::BN);
-  hipLaunchKernelGGL((gemm_mxfp4_kernel<T>), dim3(static_cast<uint32_t>((tiles + NUM_XCD - 1) / NUM_XCD * NUM_XCD)), dim3(T::THREADS), 0,
-                     stream, p);
+int64_t tiles_of(const Rect& r, int bm, int bn) {
+  return static_cast<int64_t>((r.m1 - r.m0 + bm - 1) / bm) * ((r.n1 - r.n0 + bn - 1) / bn);
+}
+
+template <typename T1, typename T2>
+void launch_tiles(MxArgs p, hipStream_t stream) {
+  int64_t grid = 0;
+  for (int i = 0; i < 4; ++i) {
+    p.count[i] = static_cast<int>(i < 2 ? tiles_of(p.rect[i], T1::BM, T1::BN) : tiles_of(p.rect[i], T2::BM, T2::BN));
+    grid += (p.count[i] + NUM_XCD - 1) / NUM_XCD * NUM_XCD;
+  }
+  hipLaunchKernelGGL((gemm_mxfp4_kernel<T1, T2>), dim3(static_cast<uint32_t>(grid)), dim3(T1::THREADS), 0, stream, p);
+}
+
+// What a tile costs, in us: `fixed` and `step` for each 256 values of K, with the chip's CUs all busy; `step2` where two share a
+// CU.  Single launches of 64 .. 4680 rows at K = 1536, 5120, 13824 (6, 20, 54 steps) measured, a round of tiles on all CUs: 256 x
+// 256 15, 38, 90 us; 128 x 256 9, 24, 57; 128 x 128 6.3, 16.7, 33; 64 x 128 4.5, 11.5, 26 (two to a CU 6, 17.5, 45); 64 x 64
+// 3.5, 8.6, 20.5 (two: 5, 12.6, 31).
+struct TileCost {
+  int bm, bn;
+  double fixed, step, step2;
+};
+constexpr TileCost kCost[] = {{256, 256, 5., 1.6, 0.}, {128, 256, 3., 1.02, 0.}, {128, 128, 2.5, 0.62, 0.}, {64, 128, 2., 0.46, 0.82}, {64, 64, 1.5, 0.37, 0.56}};
+
+double round_cost(const TileCost& c, int64_t tiles, int64_t steps, int64_t cus) {
+  const int64_t rounds = (tiles + cus - 1) / cus;
+  const double one = c.fixed + c.step * static_cast<double>(steps);
+  if (c.step2 == 0.) return static_cast<double>(rounds) * one;
+  return static_cast<double>(rounds / 2) * (c.fixed + c.step2 * static_cast<double>(steps)) + static_cast<double>(rounds % 2) * one;
+}
+
+// The cheapest by these figures: one tile for the whole output, or whole rounds of 256 x 256 tiles (whole tile rows, then a
+// part of the next) and 128 x 256 or 128 x 128 ones over the rest, so that no round is mostly idle.  4680 x 13824 -> 5120, 380
+// large tiles on 256 CUs: 180 us in them alone, 173 in 740 of 128 x 256.
+void launch_many(MxArgs p, hipStream_t stream) {
+  const int64_t cus = device_cus(), steps = (p.K + 255) / 256;
+  const Rect all{0, p.M, 0, p.N}, none{0, 0, 0, 0};
+  int best = 0, rest = 0;
+  int64_t big = 0;  // large tiles of a mixed plan
+  double cost = 0.;
+  for (int i = 0; i < 5; ++i) {
+    const double c = round_cost(kCost[i], tiles_of(all, kCost[i].bm, kCost[i].bn), steps, cus);
+    if (i == 0 || c < cost) {
+      cost = c;
+      best = i;
+    }
+  }
+  const int64_t tn = (p.N + 255) / 256, n_big = tiles_of(all, 256, 256);
+  Rect mixed[4] = {none, none, none, none};
+  for (int64_t n = cus; n < n_big; n += cus) {
+    const int row = static_cast<int>(n / tn) * 256, col = static_cast<int>(n % tn) * 256, next = std::min(row + 256, p.M);
+    const Rect r[4] = {{0, row, 0, p.N}, col ? Rect{row, next, 0, col} : none, col ? Rect{row, next, col, p.N} : none,
+                       {col ? next : row, p.M, 0, p.N}};
+    for (int i = 1; i <= 2; ++i) {
+      const double c = static_cast<double>(n / cus) * (kCost[0].fixed + kCost[0].step * static_cast<double>(steps)) +
+                       round_cost(kCost[i], tiles_of(r[2], kCost[i].bm, kCost[i].bn) + tiles_of(r[3], kCost[i].bm, kCost[i].bn), steps, cus);
+      if (c < cost) {
+        cost = c;
+        big = n;
+        rest = i;
+        std::copy(r, r + 4, mixed);
+      }
+    }
+  }
+  std::fill(p.rect, p.rect + 4, none);
+  p.rect[0] = all;
+  if (big) {
+    std::copy(mixed, mixed + 4, p.rect);
+    return rest == 1 ? launch_tiles<TileBig, TileStd>(p, stream) : launch_tiles<TileBig, TileMid>(p, stream);
+  }
+  switch (best) {
+    case 0: return launch_tiles<TileBig, TileStd>(p, stream);
+    case 1: return launch_tiles<TileStd, TileStd>(p, stream);
+    case 2: return launch_tiles<TileMid, TileMid>(p, stream);
+    case 3: return launch_tiles<TileHalf, TileHalf>(p, stream);
+    default: return launch_tiles<TileSmall, TileSmall>(p, stream);
+  }
 }
 
 int launch_gemm(const MxArgs& p, hipStream_t stream) {
   if (p.x) {
-    launch_few<1, true>(p, stream);
-  } else if (p.M <= 16) {
-    launch_few<1, false>(p, stream);
-  } else if (p.M <= 32) {
-    launch_few<2, false>(p, stream);
-  } else if (p.M <= kFewRows) {
-    launch_few<4, false>(p, stream);
-  } else {
-    auto tiles = [&](int bm, int bn) { return static_cast<int64_t>((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-    const int64_t cus = device_cus();
-    if (tiles(256, 256) >= cus)
-      launch_tile<TileBig>(p, stream);
-    else if (tiles(128, 256) >= cus)
-      launch_tile<TileStd>(p, stream);
-    else if (tiles(128, 128) >= cus)
-      launch_tile<TileMid>(p, stream);
+    if (p.M <= 4)
+      launch_few<1, 1>(p, stream);
+    else if (p.M <= 8)
+      launch_few<1, 2>(p, stream);
     else
-      launch_tile<TileSmall>(p, stream);
+      launch_few<1, 4>(p, stream);
+  } else if (p.M <= 16) {
+    launch_few<1, 0>(p, stream);
+  } else if (p.M <= 32) {
+    launch_few<2, 0>(p, stream);
+  } else if (p.M <= kFewRows) {
+    launch_few<4, 0>(p, stream);
+  } else {
+    launch_many(p, stream);
   }
   return check_launch("wf_gemm_mxfp4");
 }
@@ -481,8 +626,8 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 // Checks and arguments that both entry points share.
 int make_args(const char* fn, MxArgs& p, int64_t m, int64_t n, int64_t k, const uint8_t* w, const uint8_t* w_scales, const void* bias,
               void* y, int64_t ldy, int32_t flags) {
-  WF_REQUIRE(m < (1ll << 31) - 512 && n < (1ll << 31) - 512 && k < (1ll << 31) && product_below({m + 512, k / 2}, (1ll << 31) - 64) &&
-                 product_below({n + 512, k / 2}, (1ll << 31) - 64),
+  WF_REQUIRE(m < (1ll << 31) - 512 && n < (1ll << 31) - 512 && k < (1ll << 31) && product_below({m + 512, k / 2 + 64}, (1ll << 31) - 4096) &&
+                 product_below({n + 512, k / 2 + 64}, (1ll << 31) - 4096),
              WF_E_SHAPE, "%s: operands of 2 GiB or more are not supported", fn);
   // (a grid holds fewer than 2^32 threads; outputs of so many tiles are on the largest)
   WF_REQUIRE(product_below({m / 256 + 1, n / 256 + 1, 512}, 1ll << 32), WF_E_SHAPE, "%s: m=%lld x n=%lld is too large", fn, (long long)m,
@@ -538,6 +683,7 @@ int wf_mxfp4_linear(const void* x, int64_t m, int64_t k, int64_t ldx, const uint
   WF_REQUIRE(x, WF_E_INVALID, "%s: null pointer", fn);
   WF_REQUIRE(wf::aligned(x, 16) && ldx % 8 == 0, WF_E_ALIGN, "%s: x must be 16-byte aligned with ldx %% 8 == 0", fn);
   if (m <= wf::kFusedRows) {
+    WF_REQUIRE(ldx < (1 << 26), WF_E_SHAPE, "%s: a row stride of %lld elements", fn, (long long)ldx);  // (offsets of 16 rows in 32 bits)
     p.x = static_cast<const uint16_t*>(x);
     p.ldx = ldx;
   } else {

@@ -39,6 +39,12 @@ __device__ inline uint32_t max_bits2(uint32_t a, uint32_t b) {
 }
 __device__ inline uint32_t max_half(uint32_t a) { return max(a & 0xffffu, a >> 16); }
 
+// v of the lane that a DPP control names.
+template <int CTRL>
+__device__ inline uint32_t dpp_u32(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
+}
+
 // 8 bf16 (four words) as 8 codes under s (v_cvt_scalef32_pk_fp4_bf16: nearest, ties to even, saturated at 6; equal to the
 // definition for every finite bf16).
 __device__ inline uint32_t encode8(const uint32_t* w, float s) {

@@ -6,12 +6,14 @@ and a linear's weight is read in half the bytes of an 8-bit one.  The 4-bit coun
 ``waveforcing_amd.fp8`` (wave_rt/runtime/fp8.py:21-61; the reference has no 4-bit form), with the same interfaces:
 ``WaveMxfp4Linear.forward(x) -> (y, None)`` and an in-place module swap over ``transformer.blocks``.
 
-Scales are laid out for the kernels: uint8 ``[ceil(k / 128), rows4, 4]`` with ``rows4`` the rows rounded up to 4, byte b of
-(g, r) belonging to values ``128 g + 32 b .. + 31`` of row r.  :func:`scales_to_rows` and :func:`scales_from_rows` convert
-to and from one row of ``k / 32`` bytes for every row, the layout in which MX checkpoints hold them.
+Quantized rows are laid out for the kernels, in panels of 16 rows by 128 values that a wave's matrix instruction takes as they
+lie in memory (:class:`Mxfp4Rows`); :func:`to_rows` and :func:`from_rows` convert to and from codes and scales row by row, as MX
+checkpoints hold them.
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 import torch.nn as nn
@@ -23,8 +25,22 @@ from .kv import dense
 BLOCK = 32
 
 
-def _scales_shape(rows: int, k: int) -> tuple[int, int, int]:
-    return -(-k // 128), -(-rows // 4) * 4, 4
+class Mxfp4Rows(NamedTuple):
+    """``rows`` quantized rows of ``k`` values, as :func:`quant_mxfp4` returns them; P = ceil(rows / 16), G = ceil(k / 128).
+
+    codes uint8 [P, G, 4, 16, 16]: byte j of (p, g, b, r) holds the values 128 g + 32 b + 2 j (low half) and the next (high
+    half) of row 16 p + r; scales uint8 [P, G, 16, 4]: byte b of (p, g, r) is the E8M0 byte of the values 128 g + 32 b .. + 31
+    of that row.  Both are zero where there is no such row or value."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    k: int
+
+
+def _shapes(rows: int, k: int) -> tuple[tuple, tuple]:
+    p, g = -(-rows // 16), -(-k // 128)
+    return (p, g, 4, 16, 16), (p, g, 16, 4)
 
 
 def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
@@ -34,7 +50,7 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     if x.shape[1] % BLOCK:
         raise ValueError(f"{name} has rows of {x.shape[1]} values: not a multiple of {BLOCK}")
     rows, k = x.shape
-    if rows and k and (x.stride(1) != 1 or x.data_ptr() % 16 or (rows > 1 and (x.stride(0) % 8 or x.stride(0) < k))):
+    if rows and k and (x.stride(1) != 1 or x.data_ptr() % 16 or (rows > 1 and (x.stride(0) % 8 or not k <= x.stride(0) < 1 << 26))):
         x = dense(x)
     return x
 
@@ -43,18 +59,19 @@ def _ld(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _operand(codes: torch.Tensor, scales: torch.Tensor, name: str) -> tuple[int, int]:
-    """(rows, k) of codes and scales as :func:`quant_mxfp4` returns them."""
-    if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.shape[1] % 16:
-        raise ValueError(f"{name} codes must be contiguous uint8 [rows, k / 2] with k % 32 == 0, got {tuple(codes.shape)} {codes.dtype}")
-    rows, k = codes.shape[0], 2 * codes.shape[1]
-    if tuple(scales.shape) != _scales_shape(rows, k) or scales.dtype != torch.uint8 or not scales.is_contiguous():
-        raise ValueError(f"{name} scales must be contiguous uint8 {_scales_shape(rows, k)}, got {tuple(scales.shape)} {scales.dtype}")
+def _operand(q: Mxfp4Rows, name: str) -> Mxfp4Rows:
+    """q if its tensors are those of its rows and k."""
+    codes, scales, rows, k = q
+    if rows < 0 or k < 0 or k % BLOCK:
+        raise ValueError(f"{name} has {rows} rows of {k} values: not a multiple of {BLOCK}")
+    for what, t, shape in zip(("codes", "scales"), (codes, scales), _shapes(rows, k)):
+        if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
+            raise ValueError(f"{name}'s {what} must be contiguous uint8 {shape} for {rows} rows of {k} values, got {tuple(t.shape)} {t.dtype}")
+        if t.numel() and t.data_ptr() % 16:
+            raise ValueError(f"{name}'s {what} must be 16-byte aligned")
     if scales.device != codes.device:
-        raise ValueError(f"{name} codes are on {codes.device}, its scales on {scales.device}")
-    if codes.numel() and (codes.data_ptr() % 16 or scales.data_ptr() % 16):
-        raise ValueError(f"{name} codes and scales must be 16-byte aligned")
-    return rows, k
+        raise ValueError(f"{name}'s codes are on {codes.device}, its scales on {scales.device}")
+    return q
 
 
 def _output(out: torch.Tensor | None, rows: int, cols: int, device, align: int) -> torch.Tensor:
@@ -68,43 +85,49 @@ def _output(out: torch.Tensor | None, rows: int, cols: int, device, align: int) 
     return out
 
 
-def quant_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """(codes uint8 [R, K / 2], scales uint8 [ceil(K / 128), R4, 4]) of bf16 rows [R, K], K % 32 == 0 (wf_mxfp4_quant).
+def quant_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
+    """bf16 rows [R, K], K % 32 == 0, quantized (wf_mxfp4_quant).
 
     Per block, s is the smallest power of two with max|x| < 7 s (2^-125 to 2^125), a code the nearest e2m1 number to x / s,
     an even code on a tie, at most 6.  A block that holds a NaN or an infinity reads back as NaN."""
     x = _rows(x, "x")
     R, K = x.shape
-    codes = torch.empty((R, K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_scales_shape(R, K), dtype=torch.uint8, device=x.device)
+    shape_c, shape_s = _shapes(R, K)
+    codes = torch.empty(shape_c, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(shape_s, dtype=torch.uint8, device=x.device)
     _lib.call_on(x.device, "wf_mxfp4_quant", x.data_ptr(), R, K, _ld(x), codes.data_ptr(), scales.data_ptr())
-    return codes, scales
+    return Mxfp4Rows(codes, scales, R, K)
 
 
-def dequant_mxfp4(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-    """The values of codes and scales as bf16 [R, K], exact (wf_mxfp4_dequant)."""
-    R, K = _operand(codes, scales, "the")
-    out = _output(out, R, K, codes.device, 8)
-    _lib.call_on(codes.device, "wf_mxfp4_dequant", codes.data_ptr(), scales.data_ptr(), R, K, out.data_ptr(), _ld(out))
+def dequant_mxfp4(codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values of quantized rows (the fields of :class:`Mxfp4Rows`) as bf16 [rows, k], exact (wf_mxfp4_dequant)."""
+    _operand(Mxfp4Rows(codes, scales, rows, k), "q")
+    out = _output(out, rows, k, codes.device, 8)
+    _lib.call_on(codes.device, "wf_mxfp4_dequant", codes.data_ptr(), scales.data_ptr(), rows, k, out.data_ptr(), _ld(out))
     return out
 
 
-def scales_to_rows(scales: torch.Tensor, rows: int, k: int) -> torch.Tensor:
-    """Scales of :func:`quant_mxfp4` as E8M0 bytes [rows, k / 32]."""
-    if tuple(scales.shape) != _scales_shape(rows, k) or k % BLOCK:
-        raise ValueError(f"scales of {rows} rows of {k} values have shape {_scales_shape(rows, k)}, got {tuple(scales.shape)}")
-    return scales.transpose(0, 1).flatten(1)[:rows, :k // BLOCK].contiguous()
+def to_rows(q: Mxfp4Rows) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes [rows, k / 2], E8M0 bytes [rows, k / 32]) of quantized rows."""
+    codes, scales, rows, k = _operand(q, "q")
+    codes = codes.permute(0, 3, 1, 2, 4).flatten(2).flatten(0, 1)
+    scales = scales.transpose(1, 2).flatten(2).flatten(0, 1)
+    return codes[:rows, :k // 2].contiguous(), scales[:rows, :k // BLOCK].contiguous()
 
 
-def scales_from_rows(scales: torch.Tensor) -> torch.Tensor:
-    """E8M0 bytes [rows, k / 32] in the kernels' layout."""
-    if scales.dim() != 2 or scales.dtype != torch.uint8:
-        raise ValueError(f"expected uint8 [rows, k / 32], got {tuple(scales.shape)} {scales.dtype}")
-    rows, blocks = scales.shape
-    g, rows4, _ = _scales_shape(rows, BLOCK * blocks)
-    out = torch.zeros((rows4, 4 * g), dtype=torch.uint8, device=scales.device)
-    out[:rows, :blocks] = scales
-    return out.view(rows4, g, 4).transpose(0, 1).contiguous()
+def from_rows(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4Rows:
+    """Codes uint8 [rows, k / 2] (the even value of a pair low) and E8M0 bytes uint8 [rows, k / 32] in the kernels' layout."""
+    if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"expected uint8 codes [rows, k / 2] and scales [rows, k / 32], got {tuple(codes.shape)} {codes.dtype} and "
+                         f"{tuple(scales.shape)} {scales.dtype}")
+    rows, k = codes.shape[0], 2 * codes.shape[1]
+    if k % BLOCK or tuple(scales.shape) != (rows, k // BLOCK) or scales.device != codes.device:
+        raise ValueError(f"codes of {rows} rows of {k} values on {codes.device} do not go with scales {tuple(scales.shape)} on {scales.device}")
+    (p, g, *_), _ = _shapes(rows, k)
+    wide_c, wide_s = codes.new_zeros((16 * p, 64 * g)), scales.new_zeros((16 * p, 4 * g))
+    wide_c[:rows, :k // 2], wide_s[:rows, :k // BLOCK] = codes, scales
+    return Mxfp4Rows(wide_c.view(p, 16, g, 4, 16).permute(0, 2, 3, 1, 4).contiguous(), wide_s.view(p, 16, g, 4).transpose(1, 2).contiguous(),
+                     rows, k)
 
 
 def _bias(bias: torch.Tensor | None, n: int, device) -> torch.Tensor | None:
@@ -114,17 +137,16 @@ def _bias(bias: torch.Tensor | None, n: int, device) -> torch.Tensor | None:
     return bias
 
 
-def gemm_mxfp4(a_codes: torch.Tensor, a_scales: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor,
-               bias: torch.Tensor | None = None, gelu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
-    """bf16 [M, N] = act(a [M, K] x w [N, K]^T + bias) of two operands of :func:`quant_mxfp4` (wf_gemm_mxfp4): fp32 sums,
-    act GELU(tanh) with ``gelu``, rounded once.  N must be a multiple of 4."""
-    M, K = _operand(a_codes, a_scales, "a")
-    N, kw = _operand(w_codes, w_scales, "w")
-    if kw != K or w_codes.device != a_codes.device:
-        raise ValueError(f"a has rows of {K} values on {a_codes.device}, w of {kw} on {w_codes.device}")
-    out = _output(out, M, N, a_codes.device, 4)
-    _lib.call_on(a_codes.device, "wf_gemm_mxfp4", a_codes.data_ptr(), a_scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(),
-                 M, N, K, _lib.ptr(_bias(bias, N, a_codes.device)), out.data_ptr(), _ld(out), _lib.GEMM_GELU_TANH if gelu else 0)
+def gemm_mxfp4(a: Mxfp4Rows, w: Mxfp4Rows, bias: torch.Tensor | None = None, gelu: bool = False,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 [M, N] = act(a [M, K] x w [N, K]^T + bias) of two quantized operands (wf_gemm_mxfp4): fp32 sums, act GELU(tanh)
+    with ``gelu``, rounded once.  N must be a multiple of 4."""
+    device = _operand(a, "a").codes.device
+    if _operand(w, "w").k != a.k or w.codes.device != device:
+        raise ValueError(f"a has rows of {a.k} values on {device}, w of {w.k} on {w.codes.device}")
+    out = _output(out, a.rows, w.rows, device, 4)
+    _lib.call_on(device, "wf_gemm_mxfp4", a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), a.rows,
+                 w.rows, a.k, _lib.ptr(_bias(bias, w.rows, device)), out.data_ptr(), _ld(out), _lib.GEMM_GELU_TANH if gelu else 0)
     return out
 
 
@@ -140,42 +162,43 @@ class WaveMxfp4Linear(nn.Module):
             raise ValueError("weight must be 2-D [out, in]")
         if not weight.is_cuda:
             raise ValueError("WaveMxfp4Linear quantizes on the GPU; move the weight to a GPU first")
-        self._take(*quant_mxfp4(self._checked(weight).detach().to(torch.bfloat16)), bias, gelu)
+        n, k = weight.shape
+        self._check_shape(n, k)
+        self._take(quant_mxfp4(weight.detach().to(torch.bfloat16)), bias, gelu)
 
     @staticmethod
-    def _checked(weight: torch.Tensor) -> torch.Tensor:
-        n, k = weight.shape
+    def _check_shape(n: int, k: int) -> None:
         if k % BLOCK or n % 4 or not k:
-            raise ValueError(f"unsupported linear shape {tuple(weight.shape)} (in % {BLOCK}, out % 4 required)")
-        return weight
+            raise ValueError(f"unsupported linear shape {(n, k)} (in % {BLOCK}, out % 4 required)")
 
     @classmethod
-    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None,
-                   gelu: bool = False) -> "WaveMxfp4Linear":
-        """A linear of a weight that is quantized already: codes uint8 [out, in / 2] and scales as :func:`quant_mxfp4` returns
-        them, or E8M0 bytes [out, in / 32]."""
+    def from_quantized(cls, weight: Mxfp4Rows, bias: torch.Tensor | None = None, gelu: bool = False) -> "WaveMxfp4Linear":
+        """A linear of a weight that is quantized already (:func:`quant_mxfp4`, or :func:`from_rows` of a checkpoint's)."""
         self = cls.__new__(cls)
         nn.Module.__init__(self)
-        if scales.dim() == 2:
-            scales = scales_from_rows(scales)
-        n, k = _operand(codes, scales, "weight")
-        cls._checked(codes.new_empty((n, k), device="meta"))
-        self._take(codes, scales, bias, gelu)
+        _operand(weight, "weight")
+        cls._check_shape(weight.rows, weight.k)
+        self._take(weight, bias, gelu)
         return self
 
-    def _take(self, codes, scales, bias, gelu) -> None:
+    def _take(self, weight: Mxfp4Rows, bias, gelu) -> None:
         self.out_dtype = torch.bfloat16
-        self.out_features, self.in_features = codes.shape[0], 2 * codes.shape[1]
-        self.register_buffer("w_codes", codes)
-        self.register_buffer("w_scales", scales)
+        self.out_features, self.in_features = weight.rows, weight.k
+        self.register_buffer("w_codes", weight.codes)
+        self.register_buffer("w_scales", weight.scales)
         if bias is not None:
-            bias = bias.detach().to(device=codes.device, dtype=torch.bfloat16).contiguous()
+            bias = bias.detach().to(device=weight.codes.device, dtype=torch.bfloat16).contiguous()
             if tuple(bias.shape) != (self.out_features,):
                 raise ValueError(f"bias has shape {tuple(bias.shape)}, the weight {self.out_features} rows")
             self.register_buffer("bias", bias)
         else:
             self.bias = None
         self.gelu = gelu
+
+    @property
+    def weight_rows(self) -> Mxfp4Rows:
+        """The quantized weight."""
+        return Mxfp4Rows(self.w_codes, self.w_scales, self.out_features, self.in_features)
 
     def _raw(self, x2: torch.Tensor) -> torch.Tensor:
         if x2.dim() != 2 or x2.shape[1] != self.in_features:
@@ -187,8 +210,9 @@ class WaveMxfp4Linear(nn.Module):
         y = torch.empty((M, self.out_features), dtype=torch.bfloat16, device=x2.device)
         codes = scales = None
         if M > _lib.MXFP4_FUSED_ROWS:
-            codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x2.device)
-            scales = torch.empty(_scales_shape(M, K), dtype=torch.uint8, device=x2.device)
+            shape_c, shape_s = _shapes(M, K)
+            codes = torch.empty(shape_c, dtype=torch.uint8, device=x2.device)
+            scales = torch.empty(shape_s, dtype=torch.uint8, device=x2.device)
         _lib.call_on(x2.device, "wf_mxfp4_linear", x2.data_ptr(), M, K, _ld(x2), self.w_codes.data_ptr(), self.w_scales.data_ptr(),
                      _lib.ptr(self.bias), self.out_features, y.data_ptr(), self.out_features,
                      _lib.GEMM_GELU_TANH if self.gelu else 0, _lib.ptr(codes), _lib.ptr(scales))
