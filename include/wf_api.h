@@ -443,9 +443,10 @@ int wf_attn_dense_bf16(const void* q, int64_t lq, int32_t n_heads,
  *               127) (fp32; wf_act_quant_i8's arithmetic per (token, head)),
  *               the codes as signed bytes;
  *   WF_KV_MXFP4 wf_mxfp4_quant's codes and scale bytes of the row's four
- *               blocks: codes u8 [pool_pages][page_tokens][n_kv_heads][64],
- *               and in the place of the fp32 scale of (page, head, row) its
- *               4 bytes (the pointers to scales point to those).  A byte of
+ *               blocks: codes u8 [pool_pages][n_kv_heads][page_tokens][64]
+ *               (head by head, unlike the others'), and in the place of the
+ *               fp32 scale of (page, head, row) its 4 bytes (the pointers to
+ *               scales point to those).  A byte of
  *               255, and 253 and 254, which append never writes, make the
  *               key one with a NaN scale.
  * ------------------------------------------------------------------- */

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
   struct Regs {
     u32x4 k[F::k_loads], v[F::k_loads];
     float fk, fv;
-    int ek[2], ev[2];  // MXFP4: the scale bytes of the lane's blocks
+    uint32_t ek[2], ev[2];  // MXFP4: the scale bytes of K's key 16 i + l16 and V's 16 i + lane / 4
     uint32_t bad;
   };
   // Where a tile's keys live: in one page (uniform; `n` of them to be read, the others read as zero), or each on its own.
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     bool there;
   };
   const int pt = a.geom.page_tokens;
-  const int64_t key_bytes = kDense ? a.ldkv * 2 : static_cast<int64_t>(a.n_kv_heads) * F::row_bytes;
+  const int64_t key_bytes = kDense ? a.ldkv * 2 : kMx ? F::row_bytes : static_cast<int64_t>(a.n_kv_heads) * F::row_bytes;
   const int64_t k_to_v = kDense ? reinterpret_cast<const uint8_t*>(a.v_dense) - reinterpret_cast<const uint8_t*>(a.k_dense)
                                 : a.v_codes - a.k_codes;
   const int64_t sk_to_sv = reinterpret_cast<const uint8_t*>(a.v_scales) - reinterpret_cast<const uint8_t*>(a.k_scales);
@@ -141,7 +141,11 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     page = uniform(page);
     const bool ok = page >= 0 && page < a.geom.pool_pages;
     const int pg = ok ? page : 0, r0 = static_cast<int>(at);
-    return Where{r0 + n <= pt, ok ? n : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * F::row_bytes,
+    if constexpr (kMx) {  // (codes are stored as scales are, head by head)
+      const int row = (pg * a.n_kv_heads + head) * pt + r0;
+      return Where{r0 + n <= pt, ok ? n : 0, a.k_codes + static_cast<int64_t>(row) * F::row_bytes, a.k_scales + row};
+    }
+    return Where{r0 + n <= pt, ok ? n : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * D,
                  a.k_scales + ((pg * a.n_kv_heads + head) * pt + r0)};
   };
   auto place = [&](int t0) __attribute__((always_inline)) -> Place {
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
     Place p{0, 0, false};
     int page, at;
     if (j < k_hi && pool_row(a.geom, t.b, j, page, at))
-      p = Place{(page * pt + at) * a.n_kv_heads + head, (page * a.n_kv_heads + head) * pt + at, true};
+      p = Place{kMx ? (page * a.n_kv_heads + head) * pt + at : (page * pt + at) * a.n_kv_heads + head, (page * a.n_kv_heads + head) * pt + at, true};
     return p;
   };
   // A lane's K bytes of key l16 of each 16: 16 g + 64 i .. + 15; its V bytes: 16 of row lane / C, C lanes to a row
@@ -168,11 +172,11 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
         const auto sk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(c.sk), 0, 4 * c.n, kWord3);
         const auto sv = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(c.sk) + sk_to_sv), 0, 4 * c.n, kWord3);
-        if constexpr (kMx) {  // block g of K's key 16 i + l16; block lane % 4 of V's key 16 i + lane / 4
+        if constexpr (kMx) {  // (whole words: a byte would be awaited where it is widened, with the tile's other loads)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            x.ek[i] = __builtin_amdgcn_raw_buffer_load_b8(sk, 64 * i + 4 * l16 + g4, 0, 0);
-            x.ev[i] = __builtin_amdgcn_raw_buffer_load_b8(sv, 64 * i + lane, 0, 0);
+            x.ek[i] = __builtin_amdgcn_raw_buffer_load_b32(sk, 64 * i + 4 * l16, 0, 0);
+            x.ev[i] = __builtin_amdgcn_raw_buffer_load_b32(sv, 64 * i + (lane & 60), 0, 0);
           }
         } else {
           x.fk = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sk, 4 * (lane & 31), 0, 0));
@@ -203,8 +207,8 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
       if constexpr (kMx) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          x.ek[i] = reinterpret_cast<const uint8_t*>(a.k_scales + __shfl(p.scale, 16 * i + l16))[g4];
-          x.ev[i] = reinterpret_cast<const uint8_t*>(a.v_scales + __shfl(p.scale, 16 * i + (lane >> 2)))[lane & 3];
+          x.ek[i] = reinterpret_cast<const uint32_t*>(a.k_scales)[__shfl(p.scale, 16 * i + l16)];
+          x.ev[i] = reinterpret_cast<const uint32_t*>(a.v_scales)[__shfl(p.scale, 16 * i + (lane >> 2))];
         }
       } else {
         x.fk = a.k_scales[p.scale];
@@ -315,6 +319,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
   float* fbuf = reinterpret_cast<float*>(vbuf + KT * F::v_pitch);
 
   v4f s[NB][2];
+  [[maybe_unused]] int ek[2], ev[2];
   // V and the factors to LDS, the scores.
   auto scores = [&](bool masked, Regs& x) __attribute__((always_inline)) {
     if (!kDense && x.bad) {  // keys past the range or without a page: zero K and V
@@ -324,26 +329,32 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
         if (x.bad >> (16 * (i / (F::k_loads / 2)) + l16) & 1u) x.k[i] = zero;
         if (x.bad >> (64 / C * i + lane / C) & 1u) x.v[i] = zero;
         if constexpr (kMx) {
-          if (x.bad >> (16 * i + l16) & 1u) x.ek[i] = 127;
-          if (x.bad >> (16 * i + (lane >> 2)) & 1u) x.ev[i] = 127;
+          if (x.bad >> (16 * i + l16) & 1u) x.ek[i] = 0;
+          if (x.bad >> (16 * i + (lane >> 2)) & 1u) x.ev[i] = 0;
         }
       }
       if (x.bad >> (lane & 31) & 1u) x.fk = x.fv = 0.f;
     }
     if constexpr (kMx) {
+      // The lane's bytes: block g4 of K's keys, block lane % 4 of V's.
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ek[i] = static_cast<int>((x.ek[i] >> (8 * g4)) & 0xffu);
+        ev[i] = static_cast<int>((x.ev[i] >> (8 * (lane & 3))) & 0xffu);
+      }
       // A NaN scale of V, which a weight of zero would not silence, becomes one of K: the score of the key is NaN, and is
       // hidden from the rows that do not see it.
-      if (__ballot(max(max(x.ek[0], x.ek[1]), max(x.ev[0], x.ev[1])) >= kMxNan)) {
+      if (__ballot(max(max(ek[0], ek[1]), max(ev[0], ev[1])) >= kMxNan)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint64_t v_nan = __ballot(x.ev[i] >= kMxNan);
-          if (x.ek[i] >= kMxNan || (v_nan >> (4 * l16) & 15u)) x.ek[i] = mx::kNanE;
-          if (x.ev[i] >= kMxNan) x.ev[i] = 127;
+          const uint64_t v_nan = __ballot(ev[i] >= kMxNan);
+          if (ek[i] >= kMxNan || (v_nan >> (4 * l16) & 15u)) ek[i] = mx::kNanE;
+          if (ev[i] >= kMxNan) ev[i] = 127;
         }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float s = mx::scale_of(x.ev[i]);
+        const float s = mx::scale_of(ev[i]);
         uint4* p = reinterpret_cast<uint4*>(vbuf + (16 * i + (lane >> 2)) * F::v_pitch + 64 * (lane & 3));
 #pragma unroll
         for (int e = 0; e < 4; ++e) p[e] = mx::decode8(x.v[i][e], s);
@@ -399,9 +410,9 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
           qb = __builtin_bit_cast(v8i, *reinterpret_cast<u32x4(*)[2]>(&q[2]));
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qb, s[n][b], kFormat, 0, 0, kMx ? x.ek[b] : 127, 0, q_scale[n] - 4);
+        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qb, s[n][b], kFormat, 0, 0, kMx ? ek[b] : 127, 0, q_scale[n] - 4);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qa, s[n][b], kFormat, 0, 0, kMx ? x.ek[b] : 127, 0, q_scale[n]);
+        for (int b = 0; b < 2; ++b) s[n][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[b], qa, s[n][b], kFormat, 0, 0, kMx ? ek[b] : 127, 0, q_scale[n]);
       }
       return;
     }

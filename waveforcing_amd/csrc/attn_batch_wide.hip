@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   };
   const int pt = a.geom.page_tokens;
   const int32_t* table = a.geom.tables + static_cast<int64_t>(t.b) * a.geom.ld_table;
-  const int64_t key_bytes = static_cast<int64_t>(a.n_kv_heads) * L::row_bytes;
+  const int64_t key_bytes = kMx ? L::row_bytes : static_cast<int64_t>(a.n_kv_heads) * L::row_bytes;
   const int64_t k_to_v = a.v_codes - a.k_codes;
   const int64_t sk_to_sv = reinterpret_cast<const uint8_t*>(a.v_scales) - reinterpret_cast<const uint8_t*>(a.k_scales);
   auto cursor_at = [&](int tile) __attribute__((always_inline)) -> Cursor {
@@ -173,7 +173,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     asm volatile("" ::"s"(page));  // awaited here, not among the LDS reads of the tile
     const bool ok = page >= 0 && page < a.geom.pool_pages;
     const int pg = ok ? page : 0, r0 = static_cast<int>(at);
-    return Cursor{r0, min(pt - r0, BKV), ok ? BKV : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * L::row_bytes,
+    if constexpr (kMx) {  // (codes are stored as scales are, head by head)
+      const int row = (pg * a.n_kv_heads + head) * pt + r0;
+      return Cursor{r0, min(pt - r0, BKV), ok ? BKV : 0, a.k_codes + static_cast<int64_t>(row) * L::row_bytes, a.k_scales + row};
+    }
+    return Cursor{r0, min(pt - r0, BKV), ok ? BKV : 0, a.k_codes + (static_cast<int64_t>(pg * pt + r0) * a.n_kv_heads + head) * D,
                   a.k_scales + ((pg * a.n_kv_heads + head) * pt + r0)};
   };
   auto cursor_next = [&](const Cursor& c, int tile) __attribute__((always_inline)) -> Cursor {
@@ -219,7 +223,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       x.sk = x.sv = 0.f;
       if (page_key >= 0 && page_key < a.geom.pool_pages) {
         const int at = static_cast<int>(jk - a.geom.page.div(jk) * a.geom.page.d);
-        const int64_t off = static_cast<int64_t>((page_key * pt + at) * a.n_kv_heads + head) * L::row_bytes + L::row_bytes / 8 * schunk;
+        const int64_t off = kMx ? static_cast<int64_t>((page_key * a.n_kv_heads + head) * pt + at) * L::row_bytes + 8 * schunk
+                                : static_cast<int64_t>((page_key * pt + at) * a.n_kv_heads + head) * D + 16 * schunk;
         const int sc = (page_key * a.n_kv_heads + head) * pt + at;
         x.k0 = *reinterpret_cast<const codes_t*>(a.k_codes + off);
         x.v0 = *reinterpret_cast<const codes_t*>(a.v_codes + off);

@@ -13,7 +13,7 @@
 // maximum that gives a also tells a row that holds one: it is stored as scale NaN and zero codes, and reads back as NaN
 // whole in every format, instead of as a finite row of a scale that its other values set.
 //
-// MXFP4 rows: 64 bytes of codes and 4 scale bytes, in the place of the fp32 scale.  A block of 32 values is two lanes' (one DPP
+// MXFP4 rows: 64 bytes of codes, a head's one after the other in a page, and 4 scale bytes, in the place of the fp32 scale.  A block of 32 values is two lanes' (one DPP
 // step), a lane's 16 codes are 8 bytes, and the four blocks' bytes meet in two more steps.
 //
 // Four chunks of 4680 rows of 12 heads: append 40-41 us (4.3 TB/s of 174 MB), gather 30 us (5.8); 64 single rows 4 us
@@ -45,6 +45,7 @@ struct KvBatchArgs {
 };
 
 // The (row, head) of this lane's group and where it lives in the pool; false: nowhere.  All lanes take part.
+template <bool MX>
 __device__ inline bool place(const KvBatchArgs& a, uint32_t blk, int& row, int& head, int64_t& code_row, int64_t& scale) {
   uint32_t t, h;
   a.heads.divmod(blk * kRowsPerBlock + (threadIdx.x >> 3), t, h);
@@ -56,6 +57,7 @@ __device__ inline bool place(const KvBatchArgs& a, uint32_t blk, int& row, int& 
   if (!pool_row(a.geom, b, a.geom.kv_lens[b] - a.geom.cu[b + 1] + row, page, at)) return false;
   code_row = (static_cast<int64_t>(page) * a.geom.page_tokens + at) * a.n_heads + head;
   scale = (static_cast<int64_t>(page) * a.n_heads + head) * a.geom.page_tokens + at;
+  if constexpr (MX) code_row = scale;
   return true;
 }
 
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvBatchArgs a) {
   if (!item(a, blk, which)) return;
   int row, head;
   int64_t code_row = 0, scale_at = 0;
-  const bool ok = place(a, blk, row, head, code_row, scale_at);
+  const bool ok = place<FMT == WF_KV_MXFP4>(a, blk, row, head, code_row, scale_at);
   const uint32_t lane8 = threadIdx.x & 7u;
   uint4 x = make_uint4(0, 0, 0, 0), y = x;
   if (ok) {
@@ -162,7 +164,7 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(KvBatchArgs a) {
   if (!item(a, blk, which)) return;
   int row, head;
   int64_t code_row = 0, scale_at = 0;
-  const bool ok = place(a, blk, row, head, code_row, scale_at);
+  const bool ok = place<FMT == WF_KV_MXFP4>(a, blk, row, head, code_row, scale_at);
   if (!ok && (!a.fresh || row >= a.n_rows)) return;
   const uint32_t lane8 = threadIdx.x & 7u;
   uint4* p = reinterpret_cast<uint4*>(a.dst[which] + static_cast<int64_t>(row) * a.ld + head * kHeadDim) + lane8 * 2;

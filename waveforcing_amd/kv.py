@@ -104,6 +104,7 @@ class Fp8PagePool:
 
     format = _lib.KV_E4M3
     row_bytes = 128                        # codes of a (token, head)
+    head_major = False                     # a page's codes are stored head by head
     scale_type, scale_dims = torch.float32, ()   # a (token, head)'s scales
 
     def __init__(
@@ -122,9 +123,13 @@ class Fp8PagePool:
         self.page_tokens = page_tokens
         self.device = torch.device(device)
         shape_c = (pool_pages, page_tokens, n_heads, self.row_bytes)
+        if self.head_major:
+            shape_c = (pool_pages, n_heads, page_tokens, self.row_bytes)
         shape_s = (pool_pages, n_heads, page_tokens, *self.scale_dims)
         self.k_codes = torch.zeros(shape_c, dtype=torch.uint8, device=self.device)
         self.v_codes = torch.zeros(shape_c, dtype=torch.uint8, device=self.device)
+        if self.head_major:
+            self.k_codes, self.v_codes = self.k_codes.transpose(1, 2), self.v_codes.transpose(1, 2)
         self.k_scales = torch.zeros(shape_s, dtype=self.scale_type, device=self.device)
         self.v_scales = torch.zeros(shape_s, dtype=self.scale_type, device=self.device)
         self._cache_ptrs()
@@ -305,11 +310,13 @@ class Mxfp4PagePool(Int8PagePool):
         codes  uint8 [pool_pages, page_tokens, H, 64]
         scales uint8 [pool_pages, H, page_tokens, 4]
 
+    The codes are stored head by head (``k_codes`` and ``v_codes`` are views of [pool_pages, H, page_tokens, 64]): a row is half
+    a cache line, and the attention reads one head's rows one after the other.
     A value is off by up to a sixth of itself (half a step of e2m1) where 8-bit codes keep 4 to 8 bits.  Written, read and
     attended through :class:`PagedBatch`."""
 
     format = _lib.KV_MXFP4
-    row_bytes = 64
+    row_bytes, head_major = 64, True
     scale_type, scale_dims = torch.uint8, (4,)
 
     @staticmethod

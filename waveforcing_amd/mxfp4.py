@@ -43,16 +43,20 @@ def _shapes(rows: int, k: int) -> tuple[tuple, tuple]:
     return (p, g, 4, 16, 16), (p, g, 16, 4)
 
 
-def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
-    """bf16 rows [R, K] (K % 32 == 0) on a GPU, as the kernels read them; a copy if their strides or address do not allow it."""
+def _rows(x: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int]:
+    """(rows, R, K, row stride) of bf16 rows [R, K] (K % 32 == 0), as the kernels read them; a copy if their strides or address
+    do not allow it."""
     if x.dim() != 2 or x.dtype != torch.bfloat16:
         raise ValueError(f"{name} must be bf16 [rows, k], got {tuple(x.shape)} {x.dtype}")
-    if x.shape[1] % BLOCK:
-        raise ValueError(f"{name} has rows of {x.shape[1]} values: not a multiple of {BLOCK}")
     rows, k = x.shape
-    if rows and k and (x.stride(1) != 1 or x.data_ptr() % 16 or (rows > 1 and (x.stride(0) % 8 or not k <= x.stride(0) < 1 << 26))):
-        x = dense(x)
-    return x
+    if k % BLOCK:
+        raise ValueError(f"{name} has rows of {k} values: not a multiple of {BLOCK}")
+    ld, dense_values = x.stride()
+    if rows <= 1:
+        ld = k   # (one row has no stride)
+    if rows and k and (dense_values != 1 or x.data_ptr() % 16 or ld % 8 or not k <= ld < 1 << 26):
+        return dense(x), rows, k, k
+    return x, rows, k, ld
 
 
 def _ld(x: torch.Tensor) -> int:
@@ -90,12 +94,12 @@ def quant_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
 
     Per block, s is the smallest power of two with max|x| < 7 s (2^-125 to 2^125), a code the nearest e2m1 number to x / s,
     an even code on a tie, at most 6.  A block that holds a NaN or an infinity reads back as NaN."""
-    x = _rows(x, "x")
-    R, K = x.shape
+    x, R, K, ld = _rows(x, "x")
     shape_c, shape_s = _shapes(R, K)
-    codes = torch.empty(shape_c, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(shape_s, dtype=torch.uint8, device=x.device)
-    _lib.call_on(x.device, "wf_mxfp4_quant", x.data_ptr(), R, K, _ld(x), codes.data_ptr(), scales.data_ptr())
+    device = x.device
+    codes = torch.empty(shape_c, dtype=torch.uint8, device=device)
+    scales = torch.empty(shape_s, dtype=torch.uint8, device=device)
+    _lib.call_on(device, "wf_mxfp4_quant", x.data_ptr(), R, K, ld, codes.data_ptr(), scales.data_ptr())
     return Mxfp4Rows(codes, scales, R, K)
 
 
@@ -201,27 +205,29 @@ class WaveMxfp4Linear(nn.Module):
         return Mxfp4Rows(self.w_codes, self.w_scales, self.out_features, self.in_features)
 
     def _raw(self, x2: torch.Tensor) -> torch.Tensor:
-        if x2.dim() != 2 or x2.shape[1] != self.in_features:
-            raise ValueError(f"input width {x2.shape[-1]} != in_features {self.in_features}")
-        if x2.device != self.w_codes.device:
-            raise ValueError(f"x is on {x2.device}, the weight on {self.w_codes.device}")
-        x2 = _rows(x2, "x")
-        M, K = x2.shape
-        y = torch.empty((M, self.out_features), dtype=torch.bfloat16, device=x2.device)
+        x2, M, K, ld = _rows(x2, "x")
+        n, buffers = self.out_features, self._buffers   # (their own dict: a module's attributes cost a search each)
+        w, bias, device = buffers["w_codes"], buffers.get("bias"), x2.device
+        if K != self.in_features:
+            raise ValueError(f"input width {K} != in_features {self.in_features}")
+        if device != w.device:
+            raise ValueError(f"x is on {device}, the weight on {w.device}")
+        y = torch.empty((M, n), dtype=torch.bfloat16, device=device)
         codes = scales = None
-        if M > _lib.MXFP4_FUSED_ROWS:
-            shape_c, shape_s = _shapes(M, K)
-            codes = torch.empty(shape_c, dtype=torch.uint8, device=x2.device)
-            scales = torch.empty(shape_s, dtype=torch.uint8, device=x2.device)
-        _lib.call_on(x2.device, "wf_mxfp4_linear", x2.data_ptr(), M, K, _ld(x2), self.w_codes.data_ptr(), self.w_scales.data_ptr(),
-                     _lib.ptr(self.bias), self.out_features, y.data_ptr(), self.out_features,
-                     _lib.GEMM_GELU_TANH if self.gelu else 0, _lib.ptr(codes), _lib.ptr(scales))
+        if M > _lib.MXFP4_FUSED_ROWS:   # one workspace: the quantized rows' codes, then their scales
+            panels = -(-M // 16) * -(-K // 128)
+            ws = torch.empty((1088 * panels,), dtype=torch.uint8, device=device)
+            codes = ws.data_ptr()
+            scales = codes + 1024 * panels
+        _lib.call_on(device, "wf_mxfp4_linear", x2.data_ptr(), M, K, ld, w.data_ptr(), buffers["w_scales"].data_ptr(),
+                     None if bias is None else bias.data_ptr(), n, y.data_ptr(), n, _lib.GEMM_GELU_TANH if self.gelu else 0, codes, scales)
         return y
 
     def forward(self, x: torch.Tensor):
+        if x.dim() == 2:
+            return self._raw(x), None
         shape = x.shape
-        y = self._raw(x.reshape(-1, shape[-1]))
-        return y.reshape(*shape[:-1], self.out_features), None
+        return self._raw(x.reshape(-1, shape[-1])).view(*shape[:-1], self.out_features), None
 
 
 def quantize_transformer_mxfp4(transformer: nn.Module, verbose: bool = False, scope: str | None = None,
