@@ -52,37 +52,37 @@ __device__ inline v16f mfma32(const v4i& w, const v4i& a, v16f c, int sw, int sa
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(w), widen(a), c, 4, 4, SEL, sw, SEL, sa);
 }
 
-// BM x BN outputs of a workgroup of WM x WN waves, ST stages.
-template <int BM_, int BN_, int WM_, int WN_, int ST_>
+// BM x BN outputs of a workgroup of WM x WN waves; steps of KG panels' depth (128 values each), ST stages of one.
+template <int BM_, int BN_, int WM_, int WN_, int KG_, int ST_>
 struct MxTile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KG = KG_, ST = ST_;
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
-  static constexpr int NBA = BM / 8 / NW, NBB = BN / 8 / NW;       // 1 KB DMA blocks of codes per wave and step
-  static constexpr int NSA = (BM + 127) / 128, NSB = (BN + 127) / 128;  // 1 KB DMA blocks of scales per step (64 rows: half used)
-  static constexpr int B_OFF = BM * BK, SA_OFF = B_OFF + BN * BK, SB_OFF = SA_OFF + NSA * 1024;
+  static constexpr int SUB = 2 * KG;                               // sub-steps of 64 values
+  static constexpr int NBA = BM / 16 * KG / NW, NBB = BN / 16 * KG / NW;  // 1 KB DMA blocks of codes per wave and step
+  static constexpr int NSA = (BM * KG + 255) / 256, NSB = (BN * KG + 255) / 256;  // and of scales per step, the last may be half used
+  static constexpr int B_OFF = BM * KG * 64, SA_OFF = B_OFF + BN * KG * 64, SB_OFF = SA_OFF + NSA * 1024;
   static constexpr int STAGE = SB_OFF + NSB * 1024;
   static constexpr int WCOLS = BN / WN, WPITCH = WCOLS * 2 + 16;
   static constexpr int EPI = BN * 4;                               // the bias as fp32
   static constexpr int LDS = ST * STAGE + EPI;
-  static_assert(NBA * 8 * NW == BM && NBB * 8 * NW == BN && NSA + NSB <= NW && NW % 2 == 0, "DMA blocks");
+  static_assert(NBA * 16 * NW == BM * KG && NBB * 16 * NW == BN * KG && NSA + NSB <= NW && NW % KG == 0, "DMA blocks");
   static_assert(NW * 2 * 32 * WPITCH <= ST * STAGE, "wave staging fits the stages");
   static_assert(LDS <= 160 * 1024, "LDS of one workgroup");
 };
-using TileBig = MxTile<256, 256, 2, 4, 2>;
-using TileStd = MxTile<128, 256, 2, 4, 3>;
-using TileMid = MxTile<128, 128, 2, 4, 3>;
-using TileHalf = MxTile<64, 128, 2, 2, 3>;
-using TileSmall = MxTile<64, 64, 2, 2, 3>;
+using TileBig = MxTile<256, 256, 2, 4, 1, 4>;  // (two stages of 256 values: 5-20 % slower)
+using TileStd = MxTile<128, 256, 2, 4, 2, 3>;
+using TileMid = MxTile<128, 128, 2, 4, 2, 3>;
+using TileHalf = MxTile<64, 128, 2, 2, 2, 3>;
+using TileSmall = MxTile<64, 64, 2, 2, 2, 4>;   // (three: up to 15 % slower over long K)
 
-constexpr int SUB = 4;       // sub-steps of a step, 64 values each
 constexpr uint32_t kFar = 0x7ffffff0u;
 
 // Tile t of rect r.
 template <typename T>
 __device__ __attribute__((always_inline)) inline void mx_tile(const MxArgs& p, const Rect& r, int t, uint8_t* lds) {
   constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN, NW = T::NW, MI = T::MI, NI = T::NI, ST = T::ST;
-  constexpr int NBA = T::NBA, NDMA = T::NBA + T::NBB, STAGE = T::STAGE, NS = T::NSA + T::NSB;
+  constexpr int KG = T::KG, SUB = T::SUB, NBA = T::NBA, NDMA = T::NBA + T::NBB, ND = NDMA + 1, STAGE = T::STAGE, NS = T::NSA + T::NSB;
   float* const epi = reinterpret_cast<float*>(lds + ST * STAGE);
 
   // in bands of GROUP_M tile rows
@@ -100,31 +100,32 @@ __device__ __attribute__((always_inline)) inline void mx_tile(const MxArgs& p, c
   const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a), 0, pa * groups * 1024, kBufferRsrcWord3);
   const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.w), 0, pw * groups * 1024, kBufferRsrcWord3);
 
-  // DMA block j of this wave: panel (j NW + wave) / 2 of the tile's rows, the step's first or second 128 values (wave % 2).
-  // Panels past the last row are past the buffer's end and read as zero.
-  const uint32_t doff_a = static_cast<uint32_t>(((m0 / 16 + wave / 2) * groups + (wave & 1)) * 1024 + 16 * lane);
-  const uint32_t doff_w = static_cast<uint32_t>(((n0 / 16 + wave / 2) * groups + (wave & 1)) * 1024 + 16 * lane);
-  // scales: wave i brings 1 KB (i % (NSA + NSB); the same bytes twice cost less than a branch in the loop), 128 bytes a panel
+  // DMA block j of this wave: panel (j NW + wave) / KG of the tile's rows, the step's 128 values (wave % KG).  Panels past the
+  // last row are past the buffer's end and read as zero.
+  const uint32_t doff_a = static_cast<uint32_t>(((m0 / 16 + wave / KG) * groups + wave % KG) * 1024 + 16 * lane);
+  const uint32_t doff_w = static_cast<uint32_t>(((n0 / 16 + wave / KG) * groups + wave % KG) * 1024 + 16 * lane);
+  // scales: wave i brings 1 KB (i % (NSA + NSB); the same bytes twice cost less than a branch in the loop), 64 KG bytes a panel
   const int sblk = wave % NS;
   const bool s_is_a = sblk < T::NSA;
   const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(s_is_a ? p.a_scales : p.w_scales), 0,
                                                     (s_is_a ? pa : pw) * groups * 64, kBufferRsrcWord3);
   const int sdst = T::SA_OFF + sblk * 1024;
-  const int spanel = (s_is_a ? sblk : sblk - T::NSA) * 8 + (lane >> 3), sgroup = (lane >> 2) & 1;
+  const int schunk = (s_is_a ? sblk : sblk - T::NSA) * 64 + lane, spanel = schunk / (4 * KG);
   // Offsets are unsigned: kFar more is out of every buffer's range.  (In scalar registers where they are uniform, not a vector
   // register for each block; and no branch in the loop.)
   const bool s_in = spanel < (s_is_a ? BM : BN) / 16;
-  const uint32_t soff = s_in ? static_cast<uint32_t>((((s_is_a ? m0 : n0) / 16 + spanel) * groups) * 64 + 16 * (lane & 7)) : kFar;
-  const uint32_t s_second = s_in && sgroup ? kFar : 0u;  // the words of the second 128 values
+  const uint32_t soff = s_in ? static_cast<uint32_t>((((s_is_a ? m0 : n0) / 16 + spanel) * groups) * 64 + 16 * (schunk % (4 * KG))) : kFar;
+  const uint32_t s_second = s_in && schunk % (4 * KG) >= 4 ? kFar : 0u;  // the words of the second 128 values
   auto dma = [&](auto J, int step, int stage) __attribute__((always_inline)) {
     constexpr int j = decltype(J)::value;
-    // (a last step of 128 values: nothing in the place of the second 128, not the next panel's first)
+    // (a last step of 128 values of 256: nothing in the place of the second 128, not the next panel's first)
     if constexpr (j == NDMA) {
-      const uint32_t half_step = __builtin_amdgcn_readfirstlane(2 * step + 1 < groups ? 0 : -1);
-      dma16(rs, lds + stage * STAGE + sdst, static_cast<int>(soff + static_cast<uint32_t>(step) * 128u + (half_step & s_second)));
+      uint32_t far = 0;
+      if constexpr (KG == 2) far = __builtin_amdgcn_readfirstlane(2 * step + 1 < groups ? 0 : -1) & s_second;
+      dma16(rs, lds + stage * STAGE + sdst, static_cast<int>(soff + static_cast<uint32_t>(step) * (64u * KG) + far));
     } else {
-      const uint32_t at = static_cast<uint32_t>((j < NBA ? j : j - NBA) * (NW / 2) * groups * 1024 + step * 2048);
-      const uint32_t by = __builtin_amdgcn_readfirstlane(2 * step + (wave & 1) < groups ? at : kFar);
+      const uint32_t at = static_cast<uint32_t>((j < NBA ? j : j - NBA) * (NW / KG) * groups * 1024 + step * (1024 * KG));
+      const uint32_t by = __builtin_amdgcn_readfirstlane(KG == 1 || 2 * step + (wave & 1) < groups ? at : kFar);
       if constexpr (j < NBA)
         dma16(ra, lds + stage * STAGE + (j * NW + wave) * 1024, static_cast<int>(doff_a + by));
       else
@@ -138,10 +139,11 @@ __device__ __attribute__((always_inline)) inline void mx_tile(const MxArgs& p, c
 
   // Fragments: a lane's 32 values of sub-step s are block 2 (s % 2) + half of its row in the panel of the step's first (s < 2)
   // or second 128 values
-  const int lane_a = (wm * (BM / WM) / 16 + (l32 >> 4)) * 2048 + half * 256 + (l32 & 15) * 16;
-  const int lane_b = T::B_OFF + (wn * (BN / WN) / 16 + (l32 >> 4)) * 2048 + half * 256 + (l32 & 15) * 16;
-  const int lane_sa = T::SA_OFF + (wm * (BM / WM) / 16 + (l32 >> 4)) * 128 + (l32 & 15) * 4;
-  const int lane_sb = T::SB_OFF + (wn * (BN / WN) / 16 + (l32 >> 4)) * 128 + (l32 & 15) * 4;
+  constexpr int PANEL = 1024 * KG, WORDS = 64 * KG;  // LDS bytes of a panel's codes and scales
+  const int lane_a = (wm * (BM / WM) / 16 + (l32 >> 4)) * PANEL + half * 256 + (l32 & 15) * 16;
+  const int lane_b = T::B_OFF + (wn * (BN / WN) / 16 + (l32 >> 4)) * PANEL + half * 256 + (l32 & 15) * 16;
+  const int lane_sa = T::SA_OFF + (wm * (BM / WM) / 16 + (l32 >> 4)) * WORDS + (l32 & 15) * 4;
+  const int lane_sb = T::SB_OFF + (wn * (BN / WN) / 16 + (l32 >> 4)) * WORDS + (l32 & 15) * 4;
 
   v16f acc[NI][MI];
 #pragma unroll
@@ -149,7 +151,8 @@ __device__ __attribute__((always_inline)) inline void mx_tile(const MxArgs& p, c
 #pragma unroll
     for (int i = 0; i < MI; ++i) acc[j][i] = v16f{};
   v4i fa[2][MI], fw[2][NI];
-  int sa[2][MI], sw[2][NI];  // by sub-steps 0, 1 and 2, 3 of a step
+  uint32_t sa_next[MI], sw_next[NI];  // scale words as they are read, and from the lane's byte on
+  int sa[MI], sw[NI];
   const int shift = 8 * half;
 
   constexpr int NFR = MI + NI;
@@ -158,32 +161,31 @@ __device__ __attribute__((always_inline)) inline void mx_tile(const MxArgs& p, c
     constexpr int o = decltype(O)::value, s = decltype(S)::value;
     const uint8_t* st = lds + stage * STAGE;
     if constexpr (o < MI)
-      fa[s & 1][o] = *reinterpret_cast<const v4i*>(st + lane_a + (s >> 1) * 1024 + (s & 1) * 512 + o * 4096);
+      fa[s & 1][o] = *reinterpret_cast<const v4i*>(st + lane_a + (s >> 1) * 1024 + (s & 1) * 512 + o * 2 * PANEL);
     else if constexpr (o < NFR)
-      fw[s & 1][o - MI] = *reinterpret_cast<const v4i*>(st + lane_b + (s >> 1) * 1024 + (s & 1) * 512 + (o - MI) * 4096);
+      fw[s & 1][o - MI] = *reinterpret_cast<const v4i*>(st + lane_b + (s >> 1) * 1024 + (s & 1) * 512 + (o - MI) * 2 * PANEL);
     else if constexpr (o < NFR + MI)
-      sa[s >> 1][o - NFR] = *reinterpret_cast<const int*>(st + lane_sa + (s >> 1) * 64 + (o - NFR) * 256);
+      sa_next[o - NFR] = *reinterpret_cast<const uint32_t*>(st + lane_sa + (s >> 1) * 64 + (o - NFR) * 2 * WORDS);
     else
-      sw[s >> 1][o - NFR - MI] = *reinterpret_cast<const int*>(st + lane_sb + (s >> 1) * 64 + (o - NFR - MI) * 256);
+      sw_next[o - NFR - MI] = *reinterpret_cast<const uint32_t*>(st + lane_sb + (s >> 1) * 64 + (o - NFR - MI) * 2 * WORDS);
   };
-  // The products of sub-step S and, spread between them, the reads of sub-step (S + 1) % 4 from rstage (RD) and the DMAs
+  // The products of sub-step S and, spread between them, the reads of sub-step (S + 1) % SUB from rstage (RD) and the DMAs
   // of slot SLOT (of SUB; two stages: all in slot 0) of step dstep into dstage (DM).
   auto substep = [&](auto S, int rstage, auto SLOT, int dstep, int dstage, auto RD, auto DM) __attribute__((always_inline)) {
     constexpr int s = decltype(S)::value, slot = decltype(SLOT)::value, nx = (s + 1) % SUB;
     constexpr bool rd = decltype(RD)::value, dm = decltype(DM)::value;
-    constexpr int ND = NDMA + 1;
-    constexpr int d_lo = ST == 3 ? (slot * ND + SUB - 1) / SUB : 0;
-    constexpr int d_hi = !dm ? d_lo : ST == 3 ? ((slot + 1) * ND + SUB - 1) / SUB : (slot == 0 ? ND : 0);
+    constexpr int d_lo = ST > 2 ? (slot * ND + SUB - 1) / SUB : 0;
+    constexpr int d_hi = !dm ? d_lo : ST > 2 ? ((slot + 1) * ND + SUB - 1) / SUB : (slot == 0 ? ND : 0);
     constexpr int NMF = MI * NI, NRD = rd ? (nx % 2 == 0 ? 2 * NFR : NFR) : 0, NOPS = NRD + d_hi - d_lo;
     if constexpr (s % 2 == 0) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) sa[s >> 1][i] = static_cast<int>(static_cast<uint32_t>(sa[s >> 1][i]) >> shift);
+      for (int i = 0; i < MI; ++i) sa[i] = static_cast<int>(sa_next[i] >> shift);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) sw[s >> 1][j] = static_cast<int>(static_cast<uint32_t>(sw[s >> 1][j]) >> shift);
+      for (int j = 0; j < NI; ++j) sw[j] = static_cast<int>(sw_next[j] >> shift);
     }
     static_for<NMF>([&](auto Q) {
       constexpr int q = decltype(Q)::value, jj = q / MI, ii = q % MI;
-      acc[jj][ii] = mfma32<2 * (s & 1)>(fw[s & 1][jj], fa[s & 1][ii], acc[jj][ii], sw[s >> 1][jj], sa[s >> 1][ii]);
+      acc[jj][ii] = mfma32<2 * (s & 1)>(fw[s & 1][jj], fa[s & 1][ii], acc[jj][ii], sw[jj], sa[ii]);
       constexpr int o_lo = (q * NOPS + NMF - 1) / NMF, o_hi = ((q + 1) * NOPS + NMF - 1) / NMF;
       static_for<o_hi - o_lo>([&](auto U) {
         constexpr int o = o_lo + decltype(U)::value;
@@ -201,68 +203,51 @@ __device__ __attribute__((always_inline)) inline void mx_tile(const MxArgs& p, c
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  // Stages 0 and 1; only stage 0 is waited for here (a wave's DMAs land in order).
-  const int nk = (groups + 1) / 2;
-  static_for<NDMA + 1>([&](auto J) { dma(J, 0, 0); });
-  if (nk > 1) static_for<NDMA + 1>([&](auto J) { dma(J, 1, 1); });
-  if (nk == 1)
-    wait_counts<0, 0>();
+  // The first steps; only step 0 is waited for here (a wave's DMAs land in order).
+  const int nk = (groups + KG - 1) / KG;
+  constexpr int FIRST = ST > 2 ? ST - 1 : 2;
+  static_for<FIRST>([&](auto I) {
+    if (decltype(I)::value < nk) static_for<ND>([&](auto J) { dma(J, decltype(I)::value, decltype(I)::value); });
+  });
+  if (nk >= FIRST)
+    wait_counts<(FIRST - 1) * ND, 0>();
   else
-    wait_counts<NDMA + 1, 0>();
+    wait_counts<0, 0>();
   barrier();
-  if constexpr (ST == 3) {  // slot 0 of step 2
-    if (nk >= 3) static_for<(NDMA + 1 + SUB - 1) / SUB>([&](auto J) { dma(J, 2, 2); });
+  if constexpr (ST > 2) {  // slot 0 of the next
+    if (nk >= ST) static_for<(ND + SUB - 1) / SUB>([&](auto J) { dma(J, ST - 1, ST - 1); });
   }
   static_for<2 * NFR>([&](auto O) { frag_read(O, ic<0>{}, 0); });
   __builtin_amdgcn_sched_barrier(0);
 
-  if constexpr (ST == 3) {
-    // Step kb: sub-steps 0 .. 2 fetch slots 1 .. 3 of step kb + 2 (PRE), the last one, behind the barrier that frees this
-    // step's stage, slot 0 of step kb + 3 (POST).  The last three steps are peeled: nothing past K is fetched.
-    int c0 = 0, c1 = 1, c2 = 2;
-    auto step = [&](int kb, auto PRE, auto POST, auto LAST) __attribute__((always_inline)) {
-      constexpr bool pre = decltype(PRE)::value, last = decltype(LAST)::value;
-      static_for<SUB - 1>([&](auto S) { substep(S, c0, ic<decltype(S)::value + 1>{}, kb + 2, c2, ic<1>{}, PRE); });
-      if constexpr (!last) {
-        // own reads of this stage done, own DMAs of step kb + 1 landed (of step kb + 2 all may be in flight)
-        if constexpr (pre)
-          wait_counts<NDMA + 1, 0>();
-        else
-          wait_counts<0, 0>();
-        barrier();
-      }
-      substep(ic<SUB - 1>{}, c1, ic<0>{}, kb + 3, c0, ic<!last>{}, POST);
-      const int c = c0;
-      c0 = c1;
-      c1 = c2;
-      c2 = c;
-    };
-    int kb = 0;
-    for (; kb < nk - 3; ++kb) step(kb, ic<1>{}, ic<1>{}, ic<0>{});
-    if (nk >= 3) step(kb++, ic<1>{}, ic<0>{}, ic<0>{});
-    if (nk >= 2) step(kb++, ic<0>{}, ic<0>{}, ic<0>{});
-    step(kb, ic<0>{}, ic<0>{}, ic<1>{});
-  } else {
-    // Two stages: the barrier before a step's last sub-step has every DMA landed and frees the step's stage, into which
-    // that sub-step fetches all of step kb + 2.
-    int c0 = 0, c1 = 1;
-    auto step = [&](int kb, auto POST, auto LAST) __attribute__((always_inline)) {
-      constexpr bool last = decltype(LAST)::value;
-      static_for<SUB - 1>([&](auto S) { substep(S, c0, ic<decltype(S)::value + 1>{}, 0, 0, ic<1>{}, ic<0>{}); });
-      if constexpr (!last) {
-        wait_counts<0, 0>();
-        barrier();
-      }
-      substep(ic<SUB - 1>{}, c1, ic<0>{}, kb + 2, c0, ic<!last>{}, POST);
-      const int c = c0;
-      c0 = c1;
-      c1 = c;
-    };
-    int kb = 0;
-    for (; kb < nk - 2; ++kb) step(kb, ic<1>{}, ic<0>{});
-    if (nk >= 2) step(kb++, ic<0>{}, ic<0>{});
-    step(kb, ic<0>{}, ic<1>{});
+  // Step kb.  Its last sub-step runs behind the barrier that frees the step's stage.  More than two stages: the sub-steps before
+  // it fetch slots 1 .. of step kb + ST - 1 (PRE) into the stage of kb - 1, it slot 0 of kb + ST (POST); two: it fetches all of
+  // kb + 2.  Only steps below nk are fetched, so the last ST are peeled.  WAIT: steps beyond kb + 1 that may be in flight.
+  int cur = 0;
+  auto step = [&](int kb, auto PRE, auto POST, auto WAIT, auto LAST) __attribute__((always_inline)) {
+    constexpr bool last = decltype(LAST)::value;
+    const int next = cur + 1 == ST ? 0 : cur + 1, before = cur == 0 ? ST - 1 : cur - 1;
+    static_for<SUB - 1>([&](auto S) { substep(S, cur, ic<decltype(S)::value + 1>{}, kb + ST - 1, before, ic<1>{}, PRE); });
+    if constexpr (!last) {
+      wait_counts<decltype(WAIT)::value * ND, 0>();
+      barrier();
+    }
+    substep(ic<SUB - 1>{}, next, ic<0>{}, kb + ST, cur, ic<!last>{}, POST);
+    cur = next;
+  };
+  constexpr bool kPre = ST > 2;
+  constexpr int kAhead = ST > 2 ? ST - 2 : 0;
+  int kb = 0;
+  for (; kb < nk - ST; ++kb) step(kb, ic<kPre>{}, ic<1>{}, ic<kAhead>{}, ic<0>{});
+  if constexpr (kPre) {
+    if (nk >= ST) step(kb++, ic<1>{}, ic<0>{}, ic<kAhead>{}, ic<0>{});
   }
+  constexpr int TAIL = ST > 2 ? ST - 2 : 1;
+  static_for<TAIL>([&](auto I) {
+    constexpr int w = TAIL - 1 - decltype(I)::value;
+    if (nk - kb >= w + 2) step(kb++, ic<0>{}, ic<0>{}, ic<w>{}, ic<0>{});
+  });
+  step(kb, ic<0>{}, ic<0>{}, ic<0>{}, ic<1>{});
 
   // Epilogue: every wave converts its sub-tile as 32-row slabs, through its own LDS area (two in turn), stored as whole row
   // segments.  Block (j, i), element (n, m): m = l32, n = 8 (r / 4) + 4 half + r % 4.
@@ -537,14 +522,14 @@ void launch_tiles(MxArgs p, hipStream_t stream) {
 }
 
 // What a tile costs, in us: `fixed` and `step` for each 256 values of K, with the chip's CUs all busy; `step2` where two share a
-// CU.  Single launches of 64 .. 4680 rows at K = 1536, 5120, 13824 (6, 20, 54 steps) measured, a round of tiles on all CUs: 256 x
-// 256 15, 38, 90 us; 128 x 256 9, 24, 57; 128 x 128 6.3, 16.7, 33; 64 x 128 4.5, 11.5, 26 (two to a CU 6, 17.5, 45); 64 x 64
-// 3.5, 8.6, 20.5 (two: 5, 12.6, 31).
+// CU.  From single launches of 128 .. 4680 rows at K = 1536, 5120, 13824 (6, 20, 54 steps), a round of tiles on all CUs: 256 x
+// 256 16, 36, 80 us; 128 x 256 9, 23, 54; 128 x 128 5.8, 14.4, 33; 64 x 128 5.2, 12, 25 (two to a CU 6, 17, 45); 64 x 64 2.8,
+// 8, 18 (two: 4.3, 12.5, 24-30).
 struct TileCost {
   int bm, bn;
   double fixed, step, step2;
 };
-constexpr TileCost kCost[] = {{256, 256, 5., 1.6, 0.}, {128, 256, 3., 1.02, 0.}, {128, 128, 2.5, 0.62, 0.}, {64, 128, 2., 0.46, 0.82}, {64, 64, 1.5, 0.37, 0.56}};
+constexpr TileCost kCost[] = {{256, 256, 8., 1.35, 0.}, {128, 256, 3., 0.96, 0.}, {128, 128, 2.2, 0.58, 0.}, {64, 128, 2., 0.44, 0.78}, {64, 64, 1., 0.32, 0.5}};
 
 double round_cost(const TileCost& c, int64_t tiles, int64_t steps, int64_t cus) {
   const int64_t rounds = (tiles + cus - 1) / cus;
@@ -555,7 +540,8 @@ double round_cost(const TileCost& c, int64_t tiles, int64_t steps, int64_t cus) 
 
 // The cheapest by these figures: one tile for the whole output, or whole rounds of 256 x 256 tiles (whole tile rows, then a
 // part of the next) and 128 x 256 or 128 x 128 ones over the rest, so that no round is mostly idle.  4680 x 13824 -> 5120, 380
-// large tiles on 256 CUs: 180 us in them alone, 173 in 740 of 128 x 256.
+// large tiles on 256 CUs: 178 us in them or in 740 of 128 x 256, 162 as 256 large ones and 248 (5120 -> 13824 194 and 180, -> 5120
+// 78 and 70).
 void launch_many(MxArgs p, hipStream_t stream) {
   const int64_t cus = device_cus(), steps = (p.K + 255) / 256;
   const Rect all{0, p.M, 0, p.N}, none{0, 0, 0, 0};
