@@ -9,8 +9,8 @@
 // constant from the lane's first.  The scales, a word a row and panel, come with their stage; the byte a lane needs is
 // 2 s + (its half) of the word: one shift a word, and the instruction's byte select.
 //
-// Few rows (gemm_mxfp4_few_kernel): bound by reading the weight once.  A workgroup takes 16 or 32 columns and all rows; its
-// waves split K and go without barriers, operands straight from memory, and add up in LDS in the order of the waves.  Up to
+// Few rows, or a small output (gemm_mxfp4_few_kernel): bound by reading the weight once, or by the way from the first load to
+// the last store.  A workgroup takes 16 or 32 columns (64 in one case) and 16 or 32 rows; its waves split K and go without barriers, operands straight from memory, and add up in LDS in the order of the waves.  Up to
 // WF_MXFP4_FUSED_ROWS rows the activations are quantized in the same kernel.
 #include <algorithm>
 #include <type_traits>
@@ -332,7 +332,7 @@ __device__ inline void wave_order() {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-constexpr int kFewRows = 64, kFusedRows = WF_MXFP4_FUSED_ROWS;
+constexpr int kFusedRows = WF_MXFP4_FUSED_ROWS;
 
 constexpr int kRun = 2;
 constexpr int kXPitch = 80;  // LDS bytes of a quantized row's 128 values (16 rows' 16-byte reads touch every bank alike)
@@ -371,6 +371,7 @@ __global__ __launch_bounds__(64 * W, OCC) void gemm_mxfp4_few_kernel(MxArgs p) {
     int sw[NC], sa[NB];
   };
   const int first = n0 / 16 * steps;  // panel
+  const int row_blocks = QUANT ? 0 : NB * static_cast<int>(blockIdx.y);  // before this workgroup's
   auto load = [&](int step, Regs& r) __attribute__((always_inline)) {
     const int s = __builtin_amdgcn_readfirstlane(step);  // (in scalar registers, no vector register for each load's place)
     const bool there = s < steps;
@@ -388,7 +389,7 @@ __global__ __launch_bounds__(64 * W, OCC) void gemm_mxfp4_few_kernel(MxArgs p) {
     if constexpr (!QUANT) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const int panel = b * steps + s;
+        const int panel = (row_blocks + b) * steps + s;
         r.a[b] = __builtin_amdgcn_raw_buffer_load_b128(ra, (there ? panel * 1024 : kOutOfRange - 1024) + 16 * lane, 0, 0);
         r.sa[b] = __builtin_amdgcn_raw_buffer_load_b32(rsa, (there ? panel * 64 : kOutOfRange - 64) + 4 * l16, 0, 0);
       }
@@ -471,7 +472,7 @@ __global__ __launch_bounds__(64 * W, OCC) void gemm_mxfp4_few_kernel(MxArgs p) {
       v4f v = acc[b][c];
 #pragma unroll
       for (int i = 0; i < W - 1; ++i) v += part[(i * NB * NC + b * NC + c) * 64];
-      const int m = 16 * b + l16, n = n0 + 16 * c + 4 * g4;  // rows of the first operand, 4 to a lane: columns of y
+      const int m = 16 * (row_blocks + b) + l16, n = n0 + 16 * c + 4 * g4;  // rows of the first operand, 4 to a lane: columns of y
       if (m >= p.M || n >= p.N) continue;
       v[0] += bf16_lo_to_f32(bias[c].x), v[1] += bf16_hi_to_f32(bias[c].x), v[2] += bf16_lo_to_f32(bias[c].y), v[3] += bf16_hi_to_f32(bias[c].y);
       if (p.gelu) {
@@ -492,8 +493,8 @@ template <int NB, int XR>
 void launch_few(const MxArgs& p, hipStream_t stream) {
   auto go = [&](auto C, auto WAVES) {
     constexpr int NC = decltype(C)::value, W = decltype(WAVES)::value;
-    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<NB, NC, W, kDeep, 4, XR>), dim3(static_cast<uint32_t>((p.N + 16 * NC - 1) / (16 * NC))),
-                       dim3(64 * W), 0, stream, p);
+    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<NB, NC, W, kDeep, 4, XR>), dim3(static_cast<uint32_t>((p.N + 16 * NC - 1) / (16 * NC)),
+                       static_cast<uint32_t>((p.M + 16 * NB - 1) / (16 * NB))), dim3(64 * W), 0, stream, p);
   };
   const int cus = device_cus();
   if (p.N >= 32 * cus)
@@ -595,14 +596,17 @@ int launch_gemm(const MxArgs& p, hipStream_t stream) {
       launch_few<1, 2>(p, stream);
     else
       launch_few<1, 4>(p, stream);
-  } else if (p.M <= 16) {
-    launch_few<1, 0>(p, stream);
-  } else if (p.M <= 32) {
-    launch_few<2, 0>(p, stream);
-  } else if (p.M <= kFewRows) {
-    launch_few<4, 0>(p, stream);
   } else {
-    launch_many(p, stream);
+    // By the output's blocks of 16 x 16: some 6 to a CU and fewer are left to waves that split K, in blocks of 32 rows where
+    // there is one to a CU (us of 16 rows, 32 rows, tiles: 64 x 13824 -> 512 5.6, 6.0, 17; 200 x 13824 -> 512 7.9, 7.1, 17;
+    // 200 x 5120 -> 1536 8.6, 7.9, 9.1; 300 x 5120 -> 1536 11.3, 9.7, 9.5; 100 x 5120 -> 5120 12.0, 11.1, 10.2).
+    const int64_t blocks = static_cast<int64_t>((p.M + 15) / 16) * ((p.N + 15) / 16), cus = device_cus();
+    if (p.M <= 16 || blocks <= cus)
+      launch_few<1, 0>(p, stream);
+    else if (p.M <= 32 || blocks <= 6 * cus)
+      launch_few<2, 0>(p, stream);
+    else
+      launch_many(p, stream);
   }
   return check_launch("wf_gemm_mxfp4");
 }
