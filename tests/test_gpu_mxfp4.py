@@ -146,6 +146,19 @@ def test_strides_shapes_and_given_outputs(m):
     assert linear(x[:0])[0].shape == (0, n)
 
 
+def test_bias_out_of_a_larger_tensor_and_a_module_cast_to_another_type():
+    g = gen(8)
+    w, b = rows(100, 96, g, 0.1), rows(1, 131, g)[0]
+    for m in (3, 40, 200):
+        x = rows(m, 96, g)
+        for at in (0, 1, 3, 31):             # 2, 6 and 62 bytes into its storage too
+            check(mxfp4.WaveMxfp4Linear(w, b[at:at + 100])(x)[0], *om.product(exact(x), exact(w), b[at:at + 100]))
+        cast = mxfp4.WaveMxfp4Linear(w, b[:100]).float()
+        with pytest.raises(ValueError, match="bias has become torch.float32"):
+            cast(x)
+        same(cast.bfloat16()(x)[0], mxfp4.WaveMxfp4Linear(w, b[:100])(x)[0])
+
+
 @pytest.mark.parametrize("m", [1, 16, 33, 64, 130, 600])
 def test_nonfinite_rows_stay_by_themselves(m):
     g = gen(m)

@@ -107,7 +107,8 @@ def test_swap_refuses_what_the_others_refuse():
     ((16, 1, 64, 32, 16, 16, None), "bad sizes"),
     ((16, 1, 48, 48, 16, 16, None), "multiple of 32"),
     ((16, 1 << 28, 32, 32, 16, 16, None), "too large"),
-    ((16, 1, 32 << 21, 32 << 21, 16, 16, None), "too large"),
+    ((16, 1, 1 << 28, 1 << 28, 16, 16, None), "too large"),
+    ((16, 1 << 20, 1 << 20, 1 << 20, 16, 16, None), "too large"),
     ((None, 1, 32, 32, 16, 16, None), "null pointer"),
     ((8, 1, 32, 32, 16, 16, None), "16-byte aligned"),
     ((16, 1, 32, 36, 16, 16, None), "16-byte aligned"),

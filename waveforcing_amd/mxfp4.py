@@ -194,7 +194,7 @@ class WaveMxfp4Linear(nn.Module):
             bias = bias.detach().to(device=weight.codes.device, dtype=torch.bfloat16).contiguous()
             if tuple(bias.shape) != (self.out_features,):
                 raise ValueError(f"bias has shape {tuple(bias.shape)}, the weight {self.out_features} rows")
-            self.register_buffer("bias", bias)
+            self.register_buffer("bias", bias.clone() if bias.data_ptr() % 8 else bias)   # (a view of a larger tensor: the kernels read 8 bytes)
         else:
             self.bias = None
         self.gelu = gelu
@@ -212,6 +212,8 @@ class WaveMxfp4Linear(nn.Module):
             raise ValueError(f"input width {K} != in_features {self.in_features}")
         if device != w.device:
             raise ValueError(f"x is on {device}, the weight on {w.device}")
+        if bias is not None and bias.dtype != torch.bfloat16:
+            raise ValueError(f"the bias has become {bias.dtype}: keep the module in bf16")
         y = torch.empty((M, n), dtype=torch.bfloat16, device=device)
         codes = scales = None
         if M > _lib.MXFP4_FUSED_ROWS:   # one workspace: the quantized rows' codes, then their scales
