@@ -230,7 +230,7 @@ __device__ inline void split_q(const uint4& x, int e, uint2& q1, uint2& q2) {
 constexpr int kMxNan = mx::kMaxE + 1;
 // True when a byte of w is one.
 __device__ inline bool has_nan_scale(uint32_t w) {
-  return (w & 0xffu) >= kMxNan || (w >> 8 & 0xffu) >= kMxNan || (w >> 16 & 0xffu) >= kMxNan || (w >> 24) >= kMxNan;
+  return (((w & 0x7f7f7f7fu) + 0x01010101u * (256 - kMxNan)) & w & 0x80808080u) != 0;
 }
 
 // True when a byte of w is an e4m3 NaN code; the word with those bytes cleared.

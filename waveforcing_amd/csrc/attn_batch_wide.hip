@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     if constexpr (kMx) {
       // a NaN scale of K or V: that of all of K's blocks, so the score of the key is NaN for the rows that see it
       const uint32_t ek = f32_bits(x.sk), ev = f32_bits(x.sv);
-      const bool poison = has_nan_scale(ek) || has_nan_scale(ev);
+      const bool poison = has_nan_scale(ek) | has_nan_scale(ev);
       const float s = mx::scale_of(poison ? 127 : (ev >> (8 * (schunk >> 1))) & 0xffu);
       y.u = bits_f32(poison ? ~0u : ek);
       y.k0 = make_uint4(x.k0[0], x.k0[1], 0, 0);
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   v16f o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  float m_use = -INFINITY;  // the row's maximum in the exponents, log2 units
+  float m_use = kMx && !row_ok ? 0.f : -INFINITY;  // the row's maximum in the exponents, log2 units (MXFP4: a row that is not there has one)
   float l_run = 0.f;        // this half's row sum
   float neg_m = kMx ? 0.f : kShift;
 
