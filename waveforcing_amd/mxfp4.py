@@ -68,10 +68,11 @@ def _operand(q: Mxfp4Rows, name: str) -> Mxfp4Rows:
     codes, scales, rows, k = q
     if rows < 0 or k < 0 or k % BLOCK:
         raise ValueError(f"{name} has {rows} rows of {k} values: not a multiple of {BLOCK}")
-    for what, t, shape in zip(("codes", "scales"), (codes, scales), _shapes(rows, k)):
-        if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
+    shape_c, shape_s = _shapes(rows, k)
+    for what, t, shape in ("codes", codes, shape_c), ("scales", scales, shape_s):
+        if t.shape != shape or t.dtype != torch.uint8 or not t.is_contiguous():
             raise ValueError(f"{name}'s {what} must be contiguous uint8 {shape} for {rows} rows of {k} values, got {tuple(t.shape)} {t.dtype}")
-        if t.numel() and t.data_ptr() % 16:
+        if t.data_ptr() % 16:   # (0 where nothing is there)
             raise ValueError(f"{name}'s {what} must be 16-byte aligned")
     if scales.device != codes.device:
         raise ValueError(f"{name}'s codes are on {codes.device}, its scales on {scales.device}")
@@ -97,8 +98,7 @@ def quant_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
     x, R, K, ld = _rows(x, "x")
     shape_c, shape_s = _shapes(R, K)
     device = x.device
-    codes = torch.empty(shape_c, dtype=torch.uint8, device=device)
-    scales = torch.empty(shape_s, dtype=torch.uint8, device=device)
+    codes, scales = x.new_empty(shape_c, dtype=torch.uint8), x.new_empty(shape_s, dtype=torch.uint8)
     _lib.call_on(device, "wf_mxfp4_quant", x.data_ptr(), R, K, ld, codes.data_ptr(), scales.data_ptr())
     return Mxfp4Rows(codes, scales, R, K)
 
