@@ -46,7 +46,7 @@ def limit(position: int, kv_len: int, block: int) -> int:
     return kv_len if block == 0 else min(kv_len, (position // block + 1) * block)
 
 
-def attend(q, k, v, limits, scale, q_error=None):
+def attend(q, k, v, limits, scale):
     """Rows q [n, heads, 128] over keys k, v [t, key heads, 128] (64 bits); row i sees the keys before limits[i].
 
     Returns (out, bound): the output and how far a bf16 output of fp32 arithmetic with bf16 weights may be from it.
@@ -56,8 +56,6 @@ def attend(q, k, v, limits, scale, q_error=None):
     the fp32 sums of 128 products of the parts run in any order (256 roundings of 2^-24 of twice the sum of the
     magnitudes: 2^-15); 2^-20 more for the exponential, and 2^-14 for the fp32 running sums over the keys (up to
     2^10 tiles' roundings).  The quotient of two sums doubles e.  The result is rounded to bf16 once: 2^-8.
-    q_error [n, heads, 128]: how far the values of q themselves may be off where they are held in fewer bits; each adds
-    itself times |k|.
 
     Two absolute terms come with fp16 (many rows), whose numbers are 2^-24 apart below 2^-14, half a step 2^-25.  A
     weight times its key's scale of V is held as 64 times its ratio to the largest such product M that the row has
@@ -81,8 +79,6 @@ def attend(q, k, v, limits, scale, q_error=None):
         s = q[:, h] @ kg.t().contiguous() * scale
         e = (2.0 ** -17.8 * q[:, h].abs().amax(-1, keepdim=True) * kz.abs().sum(-1)
              + 2.0 ** -15 * (q[:, h].abs() @ kz.abs().t().contiguous())) * scale
-        if q_error is not None:
-            e = e + q_error[:, h] @ kz.abs().t().contiguous() * scale
         e = e.masked_fill(~seen, 0).amax(-1, keepdim=True) if len(key) else torch.zeros_like(q[:, h, :1])
         s = s.masked_fill(~seen, float("-inf"))
         w = torch.zeros_like(s)

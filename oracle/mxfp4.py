@@ -90,15 +90,3 @@ def cached(codes, scales, pages, n, page_tokens):
         return torch.zeros((0, codes.shape[2], 128), dtype=torch.float64, device=codes.device)
     ids = torch.tensor(pages[:-(-n // page_tokens)], dtype=torch.int64, device=codes.device)
     return values(unpack(codes[ids]), scales[ids].transpose(1, 2)).reshape(-1, codes.shape[2], 128)[:n]
-
-
-def query_error(q):
-    """How far many rows' queries [..., 128] may be off as they multiply MXFP4 keys.
-
-    A block of 32 is held as 2^e (a + b / 16), a and b the nearest e2m3 numbers (steps of 1/8 below 2, 1/4 below 4, 1/2 up to
-    7.5), with max|q| in [4, 8) 2^e, e at least -122.  Of a number of [1, 8) 2^e, whose last bit is 2^-7 to 2^-5, b / 16 has
-    all that a leaves.  Below, a leaves at most 1/16, which b / 16 has in steps of 2^-7: off by at most 2^-8."""
-    blocks = q.double().unflatten(-1, (-1, 32))
-    top = blocks.abs().amax(-1, keepdim=True)
-    unit = torch.exp2(torch.frexp(top).exponent.double() - 3).clamp(min=2.0 ** -122)
-    return torch.where((blocks != 0) & (blocks.abs() < unit), 2.0 ** -8 * unit, 0.0).flatten(-2)

@@ -72,19 +72,12 @@ def check(out, ref, bound):
     assert float(off.max()) <= 0, f"off by {float((out - ref).abs().nan_to_num(0).max()):.3g}, over the bound by {float(off.max()):.3g}"
 
 
-def attend(q, k, v, lim, scale, most):
-    """ob.attend; ``most``: rows of the batch's longest sequence, times their heads a key head more than 64 or not."""
-    wide = most * (q.shape[1] // k.shape[1]) > 64
-    return ob.attend(q, k, v, lim, scale, om.query_error(q) if wide else None)
-
-
 def check_paged(out, q, pool, batch, block, scale=SCALE):
     at = 0
     for b, (t, n) in enumerate(zip(batch.kv_lens, batch.new_lens)):
         if n:
             lim = [ob.limit(t - n + i, t, block) for i in range(n)]
-            check(out[at:at + n], *attend(q[at:at + n], cached(pool, batch, b, "k"), cached(pool, batch, b, "v"), lim, scale,
-                                          max(batch.new_lens)))
+            check(out[at:at + n], *ob.attend(q[at:at + n], cached(pool, batch, b, "k"), cached(pool, batch, b, "v"), lim, scale))
         at += n
 
 
@@ -188,7 +181,7 @@ def test_missing_pages_take_no_other_pages_scales(new):
         zk, zv = cached(pool, batch, 0, "k"), cached(pool, batch, 0, "v")
         zk[page:2 * page] = 0
         zv[page:2 * page] = 0
-        check(out, *attend(q, zk, zv, [200] * new, SCALE, new))
+        check(out, *ob.attend(q, zk, zv, [200] * new, SCALE))
 
 
 # --------------------------------------------------------------- attention

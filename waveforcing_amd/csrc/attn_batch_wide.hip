@@ -53,36 +53,6 @@ constexpr float kMostMx = 0x1p20f;  // of bf16 weights, whose bits do not go by 
 constexpr int kRun = 2;  // neighbouring row tiles that one XCD takes, which read the same keys (1: 0.7 % slower, 4: 2.5 %)
 static_assert(kThreads == BKV * 8, "one thread per key and 16 values of its row");
 
-// 32 values of a row of Q as the sum of two e2m3 parts (4 bits and a sign, steps of 1/8 up to 2, 7.5 at most), the second under
-// 1/16 of the first's power of two: with 2^e the one that puts the largest value in [4, 8), q = 2^e (q1 + q2 / 16), exact where
-// |q| >= 2^e, off by at most 2^-8 2^e below.  Returns the scale bytes, q1's and, shifted by 16, q2's; 255 for a NaN or an infinity.
-__device__ inline uint32_t split_q6(const uint4 (&x)[4], v8i& q1, v8i& q2) {
-  typedef uint32_t v6u __attribute__((ext_vector_type(6)));
-  typedef uint32_t v16u __attribute__((ext_vector_type(16)));
-  typedef __bf16 v32bf __attribute__((ext_vector_type(32)));
-  v16u w;
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[4 * i] = x[i].x, w[4 * i + 1] = x[i].y, w[4 * i + 2] = x[i].z, w[4 * i + 3] = x[i].w;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, max(w[4 * i + j] & 0x7fffu, w[4 * i + j] >> 16 & 0x7fffu));
-  }
-  const uint32_t e1 = max(static_cast<int>(top >> 7) - 2, 5), e2 = e1 - 4;
-  const v6u c1 = __builtin_amdgcn_cvt_scalef32_pk32_fp6_bf16(__builtin_bit_cast(v32bf, w), mx::scale_of(e1));
-  const v16u d = __builtin_bit_cast(v16u, __builtin_amdgcn_cvt_scalef32_pk32_bf16_fp6(c1, mx::scale_of(e1)));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {  // (what is left has at most 8 bits, those of q)
-    const float lo = bf16_lo_to_f32(w[i]) - bf16_lo_to_f32(d[i]), hi = bf16_hi_to_f32(w[i]) - bf16_hi_to_f32(d[i]);
-    w[i] = f32_bits(lo) >> 16 | (f32_bits(hi) & 0xffff0000u);
-  }
-  const v6u c2 = __builtin_amdgcn_cvt_scalef32_pk32_fp6_bf16(__builtin_bit_cast(v32bf, w), mx::scale_of(e2));
-#pragma unroll
-  for (int i = 0; i < 6; ++i) q1[i] = static_cast<int>(c1[i]), q2[i] = static_cast<int>(c2[i]);
-  q1[6] = q1[7] = q2[6] = q2[7] = 0;
-  return top >= 0x7f80u ? 0x00ff00ffu : e1 | e2 << 16;
-}
-
 template <int SRC>
 struct Lds {
   static constexpr bool mx = SRC == SRC_MXFP4;
@@ -325,27 +295,21 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // ---- Q, the second operand of the scores, for the whole kernel
   v8bf qb[kCodes ? 1 : 8];
   v8i q1[kCodes ? 2 : 1], q2[kCodes ? 2 : 1];
-  int q_scale = 127;     // E8M0 scales: e4m3, q1's; MXFP4, those of q1[0], q1[1], q2[0] and q2[1] for the lane's 32 values
+  int q_scale = 127;     // e4m3: E8M0 scale of q1
   {
     const uint16_t* qp = a.q + static_cast<int64_t>(t.row0 + static_cast<int>(qi)) * a.ldq + (head * a.group + static_cast<int>(gi)) * D;
     uint4 raw[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      // codes: values 64 (i / 4) + 32 half + 8 (i % 4) .. + 7; else 16 i + 8 half .. + 7
-      raw[i] = *reinterpret_cast<const uint4*>(qp + (kCodes ? 64 * (i >> 2) + 32 * half + 8 * (i & 3) : 16 * i + 8 * half));
+      // e4m3: values 64 (i / 4) + 32 half + 8 (i % 4) .. + 7; MXFP4, where the lanes of K hold 32 values in a row and the fp8
+      // operand's first and last 16 bytes belong to different blocks: 64 (i / 4) + 32 (i / 2 % 2) + 16 half + 8 (i % 2) .. + 7;
+      // else 16 i + 8 half .. + 7
+      raw[i] = *reinterpret_cast<const uint4*>(qp + (kMx ? 64 * (i >> 2) + 32 * ((i >> 1) & 1) + 16 * half + 8 * (i & 1) : kCodes ? 64 * (i >> 2) + 32 * half + 8 * (i & 3) : 16 * i + 8 * half));
       if (!row_ok) raw[i] = make_uint4(0, 0, 0, 0);
     }
     if constexpr (!kCodes) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) qb[i] = __builtin_bit_cast(v8bf, raw[i]);
-    } else if constexpr (kMx) {
-      q_scale = 0;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const uint4 x[4] = {raw[4 * m], raw[4 * m + 1], raw[4 * m + 2], raw[4 * m + 3]};
-        const uint32_t e = split_q6(x, q1[m], q2[m]);
-        q_scale |= static_cast<int>(e << (8 * m));
-      }
     } else {
       float amax = 0.f;
 #pragma unroll
@@ -434,11 +398,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int m = i >> 2, b = i & 1;
-          if constexpr (kMx) {  // (the small part first; the scale bytes of Q are chosen by constants)
-            s[b] = i == 0 || i == 1 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][0], q2[0], s[b], 4, 2, 0, ke[b], 2, q_scale)
-                   : i < 4          ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][0], q1[0], s[b], 4, 2, 0, ke[b], 0, q_scale)
-                   : i < 6          ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][1], q2[1], s[b], 4, 2, 2, ke[b], 3, q_scale)
-                                    : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][1], q1[1], s[b], 4, 2, 2, ke[b], 1, q_scale);
+          if constexpr (kMx) {
+            const v8i& q = i & 2 ? q1[m] : q2[m];
+            const int e = i & 2 ? q_scale : q_scale - 4;
+            s[b] = m ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q, s[b], 4, 0, 2, ke[b], 0, e)
+                     : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q, s[b], 4, 0, 0, ke[b], 0, e);
           } else if (i & 2) {
             s[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf[b][m], q1[m], s[b], 0, 0, 0, 127, 0, q_scale);
           } else {
