@@ -498,11 +498,13 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads,
  * a chunk).  Rows without a key are zero; a row of q that holds a NaN or an
  * infinity is NaN, and so are the rows that see a key with a scale of K or V
  * that is NaN or infinite; no NaN or infinity of a key reaches a row that does
- * not see it.  softmax_scale is not negative.  fp32 scores (of e4m3 keys from
- * q held to 2^-13 of its row's largest value), softmax and sums.  Up to 64 (row, head) rows of a
- * sequence per key head the weights p_j s_v[j] are held in 16 significant
- * bits; with more, in 11 (fp16: those below 2^-20 of the largest that the row
- * sees lose bits, and so do all where the scales of V are below 2^-100).
+ * not see it.  softmax_scale is not negative.  fp32 scores (of e4m3 and MXFP4
+ * keys from q held to 2^-13 of its row's largest value), softmax and sums.
+ * Up to 64 (row, head) rows of a sequence per key head the weights p_j s_v[j]
+ * are held in 16 significant bits; with more, in 11 (fp16: those below 2^-20
+ * of the largest that the row sees lose bits, and so do all where the scales
+ * of V are below 2^-100).  MXFP4: the weights p_j alone, in 16 bits and, with
+ * more rows, in 8 (bf16).
  * max_new and max_kv bound the sequences' rows and keys; they choose the
  * split, and with it the order of the sums, and results stay right where the
  * device's lengths pass them.  ws: ws_bytes of scratch, 16-byte aligned, at

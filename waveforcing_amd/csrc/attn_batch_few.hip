@@ -1,6 +1,6 @@
 // Batched attention, few rows: up to 64 (row, head) rows of a sequence over one key head (single tokens, a few drafted
 // ones, grouped heads).  The cache is read once and little is computed, so HBM bounds it: 264 bytes a key of an 8-bit
-// cache, 512 of a dense one.
+// cache, 136 of an MXFP4 one, 512 of a dense one.
 //
 // A workgroup owns a tile of 16 or 32 rows, one key head and one range of the keys; every wave takes each W-th tile
 // of 32 keys of the range by itself (no barrier in the loop).  Its loads are one tile ahead: a tile's K leaves its
@@ -17,8 +17,15 @@
 // codes of both formats exact in bf16.  The scales are applied in fp32, s_k c to the scores and s_v to the weights, and
 // the weights go in as the sum of two bf16 (16 significant bits; the matrix cores are idle most of the time anyway).
 //
+// MXFP4 keys go to the scaled product as codes with their scale bytes, a lane's 32 values of a head one block of a row, against Q in
+// the two e4m3 parts in the order that the codes have (the lanes of a 4-bit and of an 8-bit operand hold different values);
+// V goes to LDS as bf16 with its scale, one conversion for two codes, exact for every scale that append writes, so no factor is
+// left for the scores or the weights.  The scale words are loaded whole, one a key: as single bytes, widened as soon as they
+// arrive, they made each tile wait for its own loads.
+//
 // Measured: 64 single tokens of 40 heads over 8 key heads and 8192 keys each 219-224 us (4.9-5.1 TB/s), 256 over 2048 208 us
-// (5.3), 12 over 37440 of 12 heads 272 us (5.2).  With 17 to 64 rows the vector work bounds it: 48 sequences of 25 rows
+// (5.3), 12 over 37440 of 12 heads 272 us (5.2); the first over MXFP4 keys 124 us (4.6; over 32768 keys 5.0; two tiles ahead or a
+// fourth wave 0-4 %).  With 17 to 64 rows the vector work bounds it: 48 sequences of 25 rows
 // over 8192 keys of 8 heads 189 us (4.4), of 60 rows 322 us.
 #include "attn_batch.hpp"
 

@@ -10,20 +10,29 @@
 // 3 x 4680 rows over up to 37440 keys of 12 heads: 2.17-2.23 ms, 0.97 PFLOP/s (one sequence at a time, csrc/attn_paged.hip: 1.0
 // PFLOP/s with bf16 keys and weights).  Of the cycles in which a CU has work (85 % of the kernel's) the matrix cores are busy
 // 51 % and the vector unit issues 59 %, the matrix instructions' own 5 % among them.  Over 18720 keys 1.10 PFLOP/s on
-// zeros and 0.98 on N(0, 1) data, int8 0.97 and 0.88: instructions first, power close behind.
+// zeros and 0.98 on N(0, 1) data, int8 0.97 and 0.88: instructions first, power close behind.  MXFP4 3 x 4680 rows over 37440
+// keys 2.47 ms (1.31 PFLOP/s; int8 3.53), 8 x 1024 rows of 32 heads over 8192 keys of 8 0.82 ms (1.34; int8 1.12).  Of its time
+// staging takes a fifth (the writes to LDS most of it), the exponentials an eighth; weights among the wave's own products,
+// in place of the other wave's, were even, and with that the waves half a tile apart 60 % slower (they spill).
 //
 // What is rounded, and where:
 //   e4m3 keys  the codes go to the fp8 matrix cores as they are, Q as the sum of two e4m3 parts under a power-of-two scale
 //              of the row: q = 2^e (q1 + q2 / 16), exact where q's last bit is not below 2^-13 of 2^e (|q| < 2^8 2^e);
 //              the product is that of the codes with Q in fp32, and s_k c multiplies the score in fp32.  Staging K costs
 //              no conversion and half the LDS.
+//   MXFP4 keys the codes go in as they are too, with their scale bytes, against the same parts of Q (in the order that the lanes of a
+//              4-bit operand have); c multiplies the score in fp32.  Q in two 6-bit parts, at the 4-bit rate, was 2.5-4 % faster
+//              and off by up to 2^-10 of a block's largest (error against 64 bits 2.0e-3 for 1.6e-3); in three, exact to 1/128 of
+//              it, 2-4 % slower, the registers' doing.
 //   int8 keys  the codes are exact in bf16, as Q is.
-//   V          the codes are exact in fp16.
+//   V          the codes are exact in fp16; MXFP4 as bf16 with its scale, exact.
 //   weights    fp16(p s_v), the product in fp32: 11 significant bits, eight times finer than bf16.  p is relative to a reference
 //              of the row, set by the p s_v of the keys that it sees: the largest so far is between 2^6 and 2^15, so bits are
 //              lost below 2^-20 of it, 2^-31 of it at most.  (The scale in V instead, under an exponent that the tile shares,
 //              saves an instruction a score, but there a key that a row does not see, or gives no weight, takes the bits of
 //              those that it does.)  The row sum adds the p in fp32.
+//              MXFP4: bf16(p), 8 bits at any size, since V has its scales' range; a reference that keeps the sums of a tile below
+//              2^20 is all they need, so for most tiles the weights are an exponential, a sum and half a conversion a score.
 // A NaN or infinite scale makes the key's score NaN and its weight of V zero, so the rows that see the key become NaN and
 // no others; in tiles that some row does not see whole, so does a NaN code of V.
 #include <utility>
@@ -304,7 +313,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       // e4m3: values 64 (i / 4) + 32 half + 8 (i % 4) .. + 7; MXFP4, where the lanes of K hold 32 values in a row and the fp8
       // operand's first and last 16 bytes belong to different blocks: 64 (i / 4) + 32 (i / 2 % 2) + 16 half + 8 (i % 2) .. + 7;
       // else 16 i + 8 half .. + 7
-      raw[i] = *reinterpret_cast<const uint4*>(qp + (kMx ? 64 * (i >> 2) + 32 * ((i >> 1) & 1) + 16 * half + 8 * (i & 1) : kCodes ? 64 * (i >> 2) + 32 * half + 8 * (i & 3) : 16 * i + 8 * half));
+      raw[i] = *reinterpret_cast<const uint4*>(qp + (kMx      ? 64 * (i >> 2) + 32 * ((i >> 1) & 1) + 16 * half + 8 * (i & 1)
+                                                     : kCodes ? 64 * (i >> 2) + 32 * half + 8 * (i & 3)
+                                                              : 16 * i + 8 * half));
       if (!row_ok) raw[i] = make_uint4(0, 0, 0, 0);
     }
     if constexpr (!kCodes) {
@@ -339,7 +350,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   v16f o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  float m_use = kMx && !row_ok ? 0.f : -INFINITY;  // the row's maximum in the exponents, log2 units (MXFP4: a row that is not there has one)
+  float m_use = kMx && !row_ok ? 0.f : -INFINITY;  // the row's maximum, log2 units (MXFP4: a row that is not there has one)
   float l_run = 0.f;        // this half's row sum
   float neg_m = kMx ? 0.f : kShift;
 
