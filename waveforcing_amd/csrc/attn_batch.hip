@@ -2,7 +2,8 @@
 // over ragged dense bf16 keys.
 //
 //   out[i, h] = sum_j w_j V[j, g] / sum_j w_j,   w_j = exp(scale <Q[i, h], K[j, g]>),   g = h / (n_heads / n_kv_heads)
-//   over the keys j < lim(i) of the row's sequence; K = code_k s_k and V = code_v s_v are products of fp32 numbers (MXFP4: s by blocks of 32).
+//   over the keys j < lim(i) of the row's sequence; K = code_k s_k and V = code_v s_v are products of fp32 numbers (MXFP4: s by
+//   blocks of 32).
 //   lim = kv_len without a block; min(kv_len, (p / block + 1) block) with one, p = kv_len - new + i the row's position.
 //   A row without keys is zero.
 //

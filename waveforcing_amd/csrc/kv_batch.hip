@@ -15,8 +15,8 @@
 //
 //   MXFP4: mxfp4_codec.hpp's, a block of 32 values in two lanes (one DPP step), a lane's 16 codes 8 bytes; the four blocks'
 //   scale bytes meet in two more steps and take the place of the fp32 scale.  A head's rows of 64 bytes follow one another in
-//   a page: half lines of one head are read and written whole only together (position by position, a head's rows as the other
-//   formats have them, the attention read them at half the rate).
+//   a page, two to a cache line (as the other formats have them, position by position, the attention, which reads one head's,
+//   took half of every line).
 //
 // Four chunks of 4680 rows of 12 heads: append 40-41 us (4.3 TB/s of 174 MB), gather 30 us (5.8), MXFP4 33 and 29 (4.4 and 5.1
 // TB/s of 146 MB); 64 single rows 4 us each, the launch.
