@@ -501,13 +501,17 @@ void launch_few(const MxArgs& p, hipStream_t stream) {
     hipLaunchKernelGGL((gemm_mxfp4_few_kernel<NB, NC, W, kDeep, 4, XR>), dim3(static_cast<uint32_t>((p.N + 16 * NC - 1) / (16 * NC)),
                        static_cast<uint32_t>((p.M + 16 * NB - 1) / (16 * NB))), dim3(64 * W), 0, stream, p);
   };
+  // The waves set the order of the sums (the columns do not), so rows quantized here and quantized ones, which are to give the
+  // same results, have as many: 8 for 9 to 16 rows, whichever they are (16 quantized rows in 4 and 8 waves: 5120 -> 13824 9.2,
+  // 9.9 us, 5120 -> 8192 7.5, 6.7).
   const int cus = device_cus();
-  if (p.N >= 32 * cus)
-    if constexpr (XR == 4)  // (the rows are quantized anew by every workgroup: 16 x 5120 -> 13824 12.9 us in columns of 32, 11.5 of 64)
-      go(ic<4>{}, ic<8>{});
-    else
-      go(ic<2>{}, ic<4>{});
-  else if (p.N >= 20 * cus)
+  const bool wide = p.N >= 32 * cus;
+  if constexpr (XR == 4) {  // (the rows are quantized anew by every workgroup: 16 x 5120 -> 13824 12.9 us in columns of 32, 11.5 of 64)
+    if (wide) return go(ic<4>{}, ic<8>{});
+  } else {
+    if (wide && (NB > 1 || p.M <= 8)) return go(ic<2>{}, ic<4>{});
+  }
+  if (wide || p.N >= 20 * cus)
     go(ic<2>{}, ic<8>{});
   else
     go(ic<1>{}, ic<8>{});
