@@ -491,9 +491,11 @@ __global__ __launch_bounds__(64 * W, OCC) void gemm_mxfp4_few_kernel(MxArgs p) {
 constexpr int kDeep = 2;  // (3 or 4 turns in flight: 5-25 % slower at one row, even at 64)
 
 // Columns and waves of a workgroup.  Enough columns that the rows are not read too often, enough waves that the weight is on
-// its way everywhere: some 6 waves to a CU.  16 x 5120 -> 13824 in columns of 16, 32, 64: 10.5, 9.9, 9.6 us (its product alone);
-// 1 x 13824 -> 5120 12.5, 10.3, 15.0; 1 x 1536 -> 1536 2.9, 3.3, 4.2; in 4, 8, 16 waves 1 x 5120 -> 13824 9.1, 9.4, 10.3,
-// 13824 -> 5120 (columns of 16) 14.4, 10.4, 11.7.
+// its way everywhere: some 6 waves to a CU.  Columns of 32 from the width on whose workgroups of 16 columns are more than the CUs,
+// so that some CU has two (us in columns of 16, of 32; 256 CUs): 16 rows x 13824 -> 4096 13.5, 16.0; -> 4608 21.8, 16.0; -> 5120 21.6, 15.7;
+// 16 x 1536 -> 4096 3.8, 4.2; -> 4608 4.8, 4.4; 1 x 13824 -> 4096 9.6, 10.2; -> 4608 10.6, 10.2; -> 5120 11.6, 10.4; 1 x 1536 -> 1536 2.9, 3.2;
+// -> 4608 3.4, 3.5.  At 32 columns a CU and more, 16 x 5120 -> 13824 in columns of 32 and 64: 9.9, 9.7; in 4, 8, 16 waves 1 x 5120 -> 13824
+// 9.1, 9.4, 10.3; 13824 -> 5120 (columns of 16) 14.4, 10.4, 11.7.
 template <int NB, int XR>
 void launch_few(const MxArgs& p, hipStream_t stream) {
   auto go = [&](auto C, auto WAVES) {
@@ -511,7 +513,7 @@ void launch_few(const MxArgs& p, hipStream_t stream) {
   } else {
     if (wide && (NB > 1 || p.M <= 8)) return go(ic<2>{}, ic<4>{});
   }
-  if (wide || p.N >= 20 * cus)
+  if (p.N > 16 * cus)
     go(ic<2>{}, ic<8>{});
   else
     go(ic<1>{}, ic<8>{});
