@@ -20,7 +20,7 @@
 // MXFP4 keys go to the scaled product as codes with their scale bytes, a lane's 32 values of a head one block of a row, against Q in
 // the two e4m3 parts in the order that the codes have (the lanes of a 4-bit and of an 8-bit operand hold different values);
 // V goes to LDS as bf16 with its scale, one conversion for two codes, exact for every scale that append writes, so no factor is
-// left for the scores or the weights.  The scale words are loaded whole, one a key: as single bytes, widened as soon as they
+// left for the scores or the weights; those have room for V of any scale (attn_batch.hpp: headroom).  The scale words are loaded whole, one a key: as single bytes, widened as soon as they
 // arrive, they made each tile wait for its own loads.
 //
 // Measured: 64 single tokens of 40 heads over 8 key heads and 8192 keys each 219-224 us (4.9-5.1 TB/s), 256 over 2048 208 us
@@ -313,7 +313,8 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
   }
 
   v4f o[NB][8];
-  float m[NB], l[NB];
+  float m[NB], l[NB];  // the row's reference, at most kTau below its maximum (MXFP4: above by `above`), and its lanes' sums
+  const float above = kMx ? headroom(lim_max) : 0.f;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     m[n] = -INFINITY;
@@ -472,6 +473,7 @@ __global__ __launch_bounds__(64 * W, (Form<SRC, NB>::waves)) void attn_few_kerne
       }
       float mt = fmaxf(fmaxf(fmaxf(x8[0], x8[1]), fmaxf(x8[2], x8[3])), fmaxf(fmaxf(x8[4], x8[5]), fmaxf(x8[6], x8[7])));
       mt = max16(max32(mt));
+      if constexpr (kMx) mt += above;
       const bool fire = mt > m[n] + kTau;
       if (__ballot(fire)) {
         const float m_new = fire ? mt : m[n];

@@ -31,8 +31,9 @@
 //              lost below 2^-20 of it, 2^-31 of it at most.  (The scale in V instead, under an exponent that the tile shares,
 //              saves an instruction a score, but there a key that a row does not see, or gives no weight, takes the bits of
 //              those that it does.)  The row sum adds the p in fp32.
-//              MXFP4: bf16(p), 8 bits at any size, since V has its scales' range; a reference that keeps the sums of a tile below
-//              2^20 is all they need, so for most tiles the weights are an exponential, a sum and half a conversion a score.
+//              MXFP4: bf16(p), 8 bits at any size, since V has its scales' range; the reference lies so far above the row's maximum
+//              that the sum of all p is at most 1 (attn_batch.hpp: headroom), and moves where a tile's sum passes 2^14 times the
+//              weight of the maximum: so for most tiles the weights are an exponential, a sum and half a conversion a score.
 // A NaN or infinite scale makes the key's score NaN and its weight of V zero, so the rows that see the key become NaN and
 // no others; in tiles that some row does not see whole, so does a NaN code of V.
 #include <utility>
@@ -58,7 +59,7 @@ constexpr int kXcds = 8;
 constexpr float kShift = 6.f, kGrow = 9.f, kFloor = -80.f;
 constexpr _Float16 kMost = 32768.f;
 constexpr float kMostSum = 0x1p95f;
-constexpr float kMostMx = 0x1p20f;  // of bf16 weights, whose bits do not go by their size: the sum of a tile's
+constexpr float kMostMx = 14.f;  // of bf16 weights, whose bits do not go by their size: log2 of a tile's sum over the row's largest weight
 constexpr int kRun = 2;  // neighbouring row tiles that one XCD takes, which read the same keys (1: 0.7 % slower, 4: 2.5 %)
 static_assert(kThreads == BKV * 8, "one thread per key and 16 values of its row");
 
@@ -350,9 +351,10 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   v16f o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  float m_use = kMx && !row_ok ? 0.f : -INFINITY;  // the row's maximum, log2 units (MXFP4: a row that is not there has one)
+  const float above = kMx ? headroom(lim_max) : 0.f, most = kMx ? __builtin_amdgcn_exp2f(kMostMx - above) : 0.f;
+  float m_use = kMx && !row_ok ? above : -INFINITY;  // the row's maximum, log2 units (MXFP4: and `above`; a row that is not there has one)
   float l_run = 0.f;        // this half's row sum
-  float neg_m = kMx ? 0.f : kShift;
+  float neg_m = !kMx ? kShift : row_ok ? 0.f : -above;
 
   // Stages (bytes in LDS) of the tiles t - 1, t and t + 1.
   int st_prev = 0, st_cur = L::stage, st_next = 2 * L::stage;
@@ -531,7 +533,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
     // (NaN needs no other reference; m_use is -inf until the row has seen a key, and its weights count for nothing)
     auto moves = [&]() __attribute__((always_inline)) {
       if constexpr (kMx)
-        return l_tile > kMostMx || m_use == -INFINITY;
+        return l_tile > most || m_use == -INFINITY;
       else
         return top[0] > kMost || top[1] > kMost || l_tile > kMostSum || m_use == -INFINITY;
     };
@@ -557,6 +559,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
         }
       }
       mt = max32(mt);
+      if constexpr (kMx) mt += above;
       const bool fire = m_use == -INFINITY || mt - m_use > kGrow;
       const float m_new = fire ? fmaxf(m_use, mt) : m_use;
       // (in two steps: a sum of small scales' p may be large, and still count where the step as one is below 2^-126)
