@@ -503,10 +503,12 @@ int wf_attn_batch_workspace(int64_t n_rows, int32_t n_heads,
  * Up to 64 (row, head) rows of a sequence per key head the weights p_j s_v[j]
  * are held in 16 significant bits; with more, in 11 (fp16: those below 2^-20
  * of the largest that the row sees lose bits, and so do all where the scales
- * of V are below 2^-100).  MXFP4: the weights p_j alone, in 16 bits and, with
- * more rows, in 8 (bf16); finite results for V of every finite scale, and
- * values of V below 2^-80 may lose bits.  (e4m3 and int8, up to 64 rows: sums
- * of p_j |V| in fp32, finite for |V| below 2^118 / max_kv.)
+ * of V are below 2^-100).  MXFP4: the weights p_j alone, in 16 bits; with
+ * more rows in 11 (fp16, as above) where every scale of V among the keys of a
+ * workgroup's rows is 2^-19 to 2^12 or a zero block's, else in 8 (bf16).
+ * Results are finite for V of every finite scale; values of V below 2^-80 may
+ * lose bits.  (e4m3 and int8, up to 64 rows: fp32 sums of p_j |V|, finite for
+ * |V| below 2^118 / max_kv.)
  * max_new and max_kv bound the sequences' rows and keys; they choose the
  * split, and with it the order of the sums, and results stay right where the
  * device's lengths pass them.  ws: ws_bytes of scratch, 16-byte aligned, at

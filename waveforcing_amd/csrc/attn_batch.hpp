@@ -150,10 +150,10 @@ __device__ inline int used_splits(const Args& a, int lim) {
   return min(a.n_splits, max(lim - 1, 0) / a.split_keys + 1);
 }
 
-// MXFP4 keys: V carries its scales, up to 6 * 2^125 a value, so the sum of a row's weights, before it divides the result, must not
-// pass 1.  The row's reference is this many powers of two above its maximum: a weight is at most 2^9 times that of the maximum where a
-// new one is taken (2^8, in tiles of few rows), a tile's 32 weights in a lane at most 2^14, and there are n of them.  (Products of
-// weights and values below 2^-126 lose bits: with 2^15 keys, values below some 2^-80.)
+// MXFP4 keys with V as bf16, which carries its scales, up to 6 * 2^125 a value: the sum of a row's weights, before it divides the result,
+// must not pass 1.  The row's reference is this many powers of two above its maximum: n keys, whose weights grow to at most 2^9 times
+// that of the maximum before a new one is taken, or a tile's 32 in a lane to a sum of 2^14.  (Products of weights and values
+// below 2^-126 lose bits: with 2^15 keys, values below some 2^-80.)
 __device__ inline float headroom(int n) { return static_cast<float>(10 + 32 - __clz(max(n, 1) - 1)); }
 
 // 1 / sum of a row's weights.  A row that sees keys and whose weights are all zero has scores of -inf only (an infinite q, or

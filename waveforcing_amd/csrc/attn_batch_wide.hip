@@ -25,15 +25,18 @@
 //              and off by up to 2^-10 of a block's largest (error against 64 bits 2.0e-3 for 1.6e-3); in three, exact to 1/128 of
 //              it, 2-4 % slower, the registers' doing.
 //   int8 keys  the codes are exact in bf16, as Q is.
-//   V          the codes are exact in fp16; MXFP4 as bf16 with its scale, exact.
+//   V          the codes are exact in fp16; MXFP4 with its scale, exact, as fp16 or as bf16 (below).
 //   weights    fp16(p s_v), the product in fp32: 11 significant bits, eight times finer than bf16.  p is relative to a reference
 //              of the row, set by the p s_v of the keys that it sees: the largest so far is between 2^6 and 2^15, so bits are
 //              lost below 2^-20 of it, 2^-31 of it at most.  (The scale in V instead, under an exponent that the tile shares,
 //              saves an instruction a score, but there a key that a row does not see, or gives no weight, takes the bits of
 //              those that it does.)  The row sum adds the p in fp32.
-//              MXFP4: bf16(p), 8 bits at any size, since V has its scales' range; the reference lies so far above the row's maximum
-//              that the sum of all p is at most 1 (attn_batch.hpp: headroom), and moves where a tile's sum passes 2^14 times the
-//              weight of the maximum: so for most tiles the weights are an exponential, a sum and half a conversion a score.
+//              MXFP4: fp16(p) where every scale of V in the workgroup's range of keys is 2^-19 .. 2^12, which a look at them shows first
+//              (V of N(0, 1) has 2^-1 and 2^0).  Else bf16(p), 8 bits at any size: the reference then lies so far above the row's maximum
+//              that the sum of all p is at most 1 (attn_batch.hpp: headroom), and V may have any scale.  The reference moves where a tile's sum
+//              passes a bound, so for most tiles the weights are an exponential, a sum and half a conversion a score.  (bf16 alone: 2 % less
+//              time over 3 x 37440 keys, 3.5 % over 8 x 8192, and an error of 2.3e-3 against 64 bits where fp16 gives 1.67e-3 and the
+//              rounding of the results 1.66e-3: N(0, 1) rows over 4096 keys.)
 // A NaN or infinite scale makes the key's score NaN and its weight of V zero, so the rows that see the key become NaN and
 // no others; in tiles that some row does not see whole, so does a NaN code of V.
 #include <utility>
@@ -59,7 +62,11 @@ constexpr int kXcds = 8;
 constexpr float kShift = 6.f, kGrow = 9.f, kFloor = -80.f;
 constexpr _Float16 kMost = 32768.f;
 constexpr float kMostSum = 0x1p95f;
-constexpr float kMostMx = 14.f;  // of bf16 weights, whose bits do not go by their size: log2 of a tile's sum over the row's largest weight
+// MXFP4: fp16 holds V of the scale bytes kNearE .. + 31, 0.5 * 2^-19 to 6 * 2^12.  bf16 weights, whose bits do not go by their size, may
+// grow by 2^kMostBf16 (a tile's sum).
+constexpr int kNearE = 108;
+constexpr float kMostBf16 = 14.f;
+constexpr int kScan = 4;  // loads of scales of a thread on their way
 constexpr int kRun = 2;  // neighbouring row tiles that one XCD takes, which read the same keys (1: 0.7 % slower, 4: 2.5 %)
 static_assert(kThreads == BKV * 8, "one thread per key and 16 values of its row");
 
@@ -103,6 +110,14 @@ __device__ inline uint2 i8_bf16(uint32_t w) {
                     cvt_bf16x2(static_cast<float>(static_cast<int8_t>(w >> 16)), static_cast<float>(static_cast<int8_t>(w >> 24))));
 }
 
+// 8 MXFP4 codes as 8 fp16 under s.
+__device__ inline uint4 decode8_f16(uint32_t c, float s) {
+  return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 0)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 1)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 2)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 3)));
+}
+
 __device__ inline uint32_t cvt_f16x2(float lo, float hi) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   const f2 v = {lo, hi};
@@ -111,32 +126,18 @@ __device__ inline uint32_t cvt_f16x2(float lo, float hi) {
 
 __device__ inline bool finite(float v) { return (f32_bits(v) & 0x7f800000u) != 0x7f800000u; }
 
-// SMALL: pages of fewer than 64 positions, where every lane finds its own key's page.
-template <int SRC, bool SMALL>
-__global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
+// The work of one item.  SMALL: pages of fewer than 64 positions, where every lane finds its own key's page.  F16: V and the weights are
+// fp16, else bf16.
+template <int SRC, bool SMALL, bool F16>
+__device__ __attribute__((always_inline)) inline void attend_tile(const Args& a, const Tile& t, int w, int head, int split, int splits,
+                                                                  int lim_max, int lim_min, uint8_t* lds) {
   using L = Lds<SRC>;
   constexpr bool kCodes = L::codes, kMx = L::mx;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[L::bytes];
-
-  if (blockIdx.x >= a.clear_from) return clear_rest<kThreads>(a);
+  static_assert(F16 || kMx, "the other formats have fp16");
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
-
-  // Item: runs of kRun neighbouring row tiles go to the XCDs in turn (workgroups are dealt to them round-robin), the
-  // heads of a run one after the other.  The last tiles of a sequence, whose causal rows see most, come first in every
-  // head, so that little is left at the end (two clips of 7 frames: 10 % less time than with a head after the other).
-  const int runs = (a.n_tiles + kRun - 1) / kRun;
-  const int xcd = static_cast<int>(blockIdx.x) % kXcds, slot = static_cast<int>(blockIdx.x) / kXcds;
-  const int i_run = (slot / kRun) * kXcds + xcd;
-  const int head = i_run % a.n_kv_heads, rs = i_run / a.n_kv_heads;
-  const int w = a.n_tiles - 1 - (rs % runs) * kRun - slot % kRun, split = a.n_splits - 1 - rs / runs;
-  Tile t;
-  if (w < 0 || split < 0 || !find_tile<false>(a, w, t)) return;
-  const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
-  const int splits = used_splits(a, lim_max);
-  if (split >= splits) return;
   const int k_lo = split * a.split_keys;
   const int k_hi = uniform(split == splits - 1 ? lim_max : k_lo + a.split_keys);
   const int tile_lo = k_lo / BKV, tile_hi = (k_hi + BKV - 1) / BKV;
@@ -257,8 +258,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       const float s = mx::scale_of(poison ? 127 : (ev >> (8 * (schunk >> 1))) & 0xffu);
       y.u = bits_f32(poison ? ~0u : ek);
       y.k0 = make_uint4(x.k0[0], x.k0[1], 0, 0);
-      y.v0 = mx::decode8(x.v0[0], s);
-      y.v1 = mx::decode8(x.v0[1], s);
+      y.v0 = F16 ? decode8_f16(x.v0[0], s) : mx::decode8(x.v0[0], s);
+      y.v1 = F16 ? decode8_f16(x.v0[1], s) : mx::decode8(x.v0[1], s);
     } else {
     bool poison = !finite(x.sv) || !finite(x.sk);  // the score is NaN for the rows that see the key, the weight of V zero for the others
     if constexpr (SRC == SRC_E4M3 && decltype(PARTIAL)::value) {
@@ -351,7 +352,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   v16f o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  const float above = kMx ? headroom(lim_max) : 0.f, most = kMx ? __builtin_amdgcn_exp2f(kMostMx - above) : 0.f;
+  const float above = F16 ? -kShift : headroom(lim_max), most = F16 ? static_cast<float>(kMost) : __builtin_amdgcn_exp2f(kMostBf16 - above);
   float m_use = kMx && !row_ok ? above : -INFINITY;  // the row's maximum, log2 units (MXFP4: and `above`; a row that is not there has one)
   float l_run = 0.f;        // this half's row sum
   float neg_m = !kMx ? kShift : row_ok ? 0.f : -above;
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
       const uint4 w = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
-        if constexpr (kMx)
+        if constexpr (!F16)
           o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, vf[k & 1][db]), __builtin_bit_cast(v8bf, w), o[db], 0, 0, 0);
         else
           o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[k & 1][db]), __builtin_bit_cast(v8h, w), o[db], 0, 0, 0);
@@ -392,8 +393,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
   // wave may see none of t, or the tile to be loaded may span pages; without it the half is one block of instructions.
   float4 uf[2], sf[2];
   int ke[2];  // MXFP4: the scale bytes of key l32 of each 32, from the lane's first one on
-  auto read_u = [&](int stage, int j) __attribute__((always_inline)) {
-    if constexpr (kMx) return;  // factors and scales of V of the keys 8 j + 4 half + 0 .. 3
+  auto read_u = [&](int stage, int j) __attribute__((always_inline)) {  // factors and scales of V of the keys 8 j + 4 half + 0 .. 3
+    if constexpr (kMx) return;  // (it has neither)
     const float* us = reinterpret_cast<const float*>(lds + stage + L::u_off) + 8 * j + 4 * half;
     uf[j & 1] = *reinterpret_cast<const float4*>(us);
     sf[j & 1] = *reinterpret_cast<const float4*>(us + BKV);
@@ -506,7 +507,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
           const float p = __builtin_amdgcn_exp2f(fmaf(x, factor(a.c, x), neg_m)), q = __builtin_amdgcn_exp2f(fmaf(z, factor(a.c, z), neg_m));
           l_tile += p;
           l_tile += q;
-          pw[j] = cvt_bf16x2(p, q);
+          pw[j] = F16 ? cvt_f16x2(p, q) : cvt_bf16x2(p, q);
         }
         return;
       }
@@ -683,6 +684,80 @@ __global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
                                 (head * a.group + static_cast<int>(gj)) * D + 4 * l32) = v;
     }
   }
+}
+
+// True where a byte of four scales of V is not kNearE .. + 31.  The smallest scale, a zero block's, no scale at all and what stands for
+// NaN are no such byte: V reads as zero there, or is not used.
+__device__ inline bool far_scale(uint32_t w) {
+  bool far = false;
+  if (((w + 0x01010101u * (128 - kNearE)) & 0xe0e0e0e0u) != 0x80808080u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = static_cast<int>((w >> (8 * i)) & 0xffu);
+      far |= e > mx::kMinE && e < kMxNan && (e < kNearE || e >= kNearE + 32);
+    }
+  }
+  return far;
+}
+
+// MXFP4: whether a key of [k_lo, k_hi) has such a scale.  Every thread takes part; flag: a place in LDS that is free behind it.  N keys of a page
+// at a time, which start at a multiple of N.
+template <int N>
+__device__ inline bool far_scales(const Args& a, const Tile& t, int head, int k_lo, int k_hi, uint32_t* flag) {
+  typedef unsigned int word_t __attribute__((ext_vector_type(N)));
+  const int32_t* table = a.geom.tables + static_cast<int64_t>(t.b) * a.geom.ld_table;
+  bool far = false;
+  if (threadIdx.x == 0) *flag = 0;
+  for (int j0 = k_lo + N * static_cast<int>(threadIdx.x); a.geom.ld_table && j0 < k_hi; j0 += kScan * N * kThreads) {
+    word_t w[kScan];
+    bool ok[kScan];
+#pragma unroll
+    for (int i = 0; i < kScan; ++i) {  // (no branch: the loads of all of them on their way)
+      const uint32_t j = static_cast<uint32_t>(min(j0 + i * N * kThreads, (k_hi - 1) / N * N)), lp = a.geom.page.div(j);
+      const int page = table[min(static_cast<int>(lp), a.geom.ld_table - 1)];
+      ok[i] = lp < static_cast<uint32_t>(a.geom.ld_table) && page >= 0 && page < a.geom.pool_pages;
+      const int at = ((ok[i] ? page : 0) * a.n_kv_heads + head) * a.geom.page_tokens + static_cast<int>(j - lp * a.geom.page.d);
+      w[i] = *reinterpret_cast<const word_t*>(reinterpret_cast<const uint32_t*>(a.v_scales) + at);
+    }
+#pragma unroll
+    for (int i = 0; i < kScan; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) far |= ok[i] && j0 + i * N * kThreads + e < k_hi && far_scale(w[i][e]);
+  }
+  __syncthreads();
+  if (far) *flag = 1;
+  __syncthreads();
+  const bool any = uniform(static_cast<int>(*flag)) != 0;
+  __syncthreads();
+  return any;
+}
+
+template <int SRC, bool SMALL>
+__global__ __launch_bounds__(kThreads, 1) void attn_wide_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[Lds<SRC>::bytes];
+
+  if (blockIdx.x >= a.clear_from) return clear_rest<kThreads>(a);
+  // Item: runs of kRun neighbouring row tiles go to the XCDs in turn (workgroups are dealt to them round-robin), the
+  // heads of a run one after the other.  The last tiles of a sequence, whose causal rows see most, come first in every
+  // head, so that little is left at the end (two clips of 7 frames: 10 % less time than with a head after the other).
+  const int runs = (a.n_tiles + kRun - 1) / kRun;
+  const int xcd = static_cast<int>(blockIdx.x) % kXcds, slot = static_cast<int>(blockIdx.x) / kXcds;
+  const int i_run = (slot / kRun) * kXcds + xcd;
+  const int head = i_run % a.n_kv_heads, rs = i_run / a.n_kv_heads;
+  const int w = a.n_tiles - 1 - (rs % runs) * kRun - slot % kRun, split = a.n_splits - 1 - rs / runs;
+  Tile t;
+  if (w < 0 || split < 0 || !find_tile<false>(a, w, t)) return;
+  const int lim_max = tile_max(a, t), lim_min = tile_min(a, t);
+  const int splits = used_splits(a, lim_max);
+  if (split >= splits) return;
+  if constexpr (SRC == SRC_MXFP4) {
+    const int k_lo = split * a.split_keys, k_hi = split == splits - 1 ? lim_max : k_lo + a.split_keys;
+    uint32_t* flag = reinterpret_cast<uint32_t*>(lds);
+    if (a.geom.page_tokens % 4 == 0 && (reinterpret_cast<uintptr_t>(a.v_scales) & 15u) == 0 ? far_scales<4>(a, t, head, k_lo, k_hi, flag)
+                                                                                          : far_scales<1>(a, t, head, k_lo, k_hi, flag))
+      return attend_tile<SRC, SMALL, false>(a, t, w, head, split, splits, lim_max, lim_min, lds);
+  }
+  attend_tile<SRC, SMALL, true>(a, t, w, head, split, splits, lim_max, lim_min, lds);
 }
 
 }  // namespace
