@@ -708,12 +708,13 @@ __device__ inline bool far_scales(const Args& a, const Tile& t, int head, int k_
   const int32_t* table = a.geom.tables + static_cast<int64_t>(t.b) * a.geom.ld_table;
   bool far = false;
   if (threadIdx.x == 0) *flag = 0;
-  for (int j0 = k_lo + N * static_cast<int>(threadIdx.x); a.geom.ld_table && j0 < k_hi; j0 += kScan * N * kThreads) {
+  const uint32_t end = static_cast<uint32_t>(k_hi);  // (positions past it stay below 2^32)
+  for (uint32_t j0 = static_cast<uint32_t>(k_lo) + N * threadIdx.x; a.geom.ld_table && j0 < end; j0 += kScan * N * kThreads) {
     word_t w[kScan];
     bool ok[kScan];
 #pragma unroll
     for (int i = 0; i < kScan; ++i) {  // (no branch: the loads of all of them on their way)
-      const uint32_t j = static_cast<uint32_t>(min(j0 + i * N * kThreads, (k_hi - 1) / N * N)), lp = a.geom.page.div(j);
+      const uint32_t j = min(j0 + i * N * kThreads, (end - 1) / N * N), lp = a.geom.page.div(j);
       const int page = table[min(static_cast<int>(lp), a.geom.ld_table - 1)];
       ok[i] = lp < static_cast<uint32_t>(a.geom.ld_table) && page >= 0 && page < a.geom.pool_pages;
       const int at = ((ok[i] ? page : 0) * a.n_kv_heads + head) * a.geom.page_tokens + static_cast<int>(j - lp * a.geom.page.d);
@@ -722,7 +723,7 @@ __device__ inline bool far_scales(const Args& a, const Tile& t, int head, int k_
 #pragma unroll
     for (int i = 0; i < kScan; ++i)
 #pragma unroll
-      for (int e = 0; e < N; ++e) far |= ok[i] && j0 + i * N * kThreads + e < k_hi && far_scale(w[i][e]);
+      for (int e = 0; e < N; ++e) far |= ok[i] && j0 + i * N * kThreads + e < end && far_scale(w[i][e]);
   }
   __syncthreads();
   if (far) *flag = 1;
