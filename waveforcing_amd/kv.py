@@ -312,8 +312,8 @@ class Mxfp4PagePool(Int8PagePool):
 
     The codes are stored head by head (``k_codes`` and ``v_codes`` are views of [pool_pages, H, page_tokens, 64]): a row is half
     a cache line, and the attention reads one head's rows one after the other.
-    A value is off by up to a sixth of itself (half a step of e2m1) where 8-bit codes keep 4 to 8 bits.  Written, read and
-    attended through :class:`PagedBatch`."""
+    Under a block's scale s a value is off by up to half a step of e2m1: s / 4 below 2 s, where up to s / 4 becomes zero, and a
+    fifth of itself above; 8-bit codes keep 4 to 8 bits.  Written, read and attended through :class:`PagedBatch`."""
 
     format = _lib.KV_MXFP4
     row_bytes, head_major = 64, True
