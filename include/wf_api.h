@@ -317,7 +317,10 @@ int wf_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales,
  * with flags & WF_GEMM_GELU_TANH, in fp32 (rounded once).  A scale byte of
  * 255 makes its row of a (of w: its column of y) NaN.  k % 32 == 0; n, ldy %
  * 4 == 0; codes and scales 16-byte, y and bias 8-byte aligned; codes of an
- * operand fewer than 2^31 bytes.  Reads whole panels.  The order of the sums goes by the sizes. */
+ * operand fewer than 2^31 bytes.  Reads whole panels: the codes and scale bytes
+ * of values past k must be zero, as the layout says (a scale byte of 255 there
+ * makes the row NaN); those of rows past the last may be anything.  The order
+ * of the sums goes by the sizes. */
 int wf_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scales,
                   const uint8_t* w, const uint8_t* w_scales, int64_t m,
                   int64_t n, int64_t k, const void* bias, void* y,

@@ -30,7 +30,7 @@ class Mxfp4Rows(NamedTuple):
 
     codes uint8 [P, G, 4, 16, 16]: byte j of (p, g, b, r) holds the values 128 g + 32 b + 2 j (low half) and the next (high
     half) of row 16 p + r; scales uint8 [P, G, 16, 4]: byte b of (p, g, r) is the E8M0 byte of the values 128 g + 32 b .. + 31
-    of that row.  Both are zero where there is no such row or value."""
+    of that row.  Both are zero where there is no such row or value; the product relies on that of values past k, not of rows."""
 
     codes: torch.Tensor
     scales: torch.Tensor
