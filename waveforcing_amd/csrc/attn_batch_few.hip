@@ -26,7 +26,9 @@
 // Measured: 64 single tokens of 40 heads over 8 key heads and 8192 keys each 219-224 us (4.9-5.1 TB/s), 256 over 2048 208 us
 // (5.3), 12 over 37440 of 12 heads 272 us (5.2); the first over MXFP4 keys 124 us (4.6; over 32768 keys 5.0; two tiles ahead or a
 // fourth wave 0-4 %).  With 17 to 64 rows the vector work bounds it: 48 sequences of 25 rows
-// over 8192 keys of 8 heads 189 us (4.4), of 60 rows 322 us.
+// over 8192 keys of 8 heads 184-189 us (4.4-4.5), of 60 rows 318-322 us; over MXFP4 keys 128-135 us (3.2-3.3 of 428 MB) and 234-248:
+// no unit is full (the vector unit issues in 52 % of the cycles, the matrix cores are busy in 29 %), each tile's chain of steps is; above
+// 32 rows a second tile of rows reads and decodes the cache again.
 #include "attn_batch.hpp"
 
 namespace wf {

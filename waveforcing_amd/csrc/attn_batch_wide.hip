@@ -11,8 +11,8 @@
 // PFLOP/s with bf16 keys and weights).  Of the cycles in which a CU has work (85 % of the kernel's) the matrix cores are busy
 // 51 % and the vector unit issues 59 %, the matrix instructions' own 5 % among them.  Over 18720 keys 1.10 PFLOP/s on
 // zeros and 0.98 on N(0, 1) data, int8 0.97 and 0.88: instructions first, power close behind.  MXFP4 3 x 4680 rows over 37440
-// keys 2.47 ms (1.31 PFLOP/s; int8 3.53), 8 x 1024 rows of 32 heads over 8192 keys of 8 0.82 ms (1.34; int8 1.12).  Of its time
-// staging takes a fifth (the writes to LDS most of it), the exponentials an eighth; weights among the wave's own products,
+// keys 2.46-2.50 ms (1.29-1.31 PFLOP/s; int8 3.47), 8 x 1024 rows of 32 heads over 8192 keys of 8 0.83 ms (1.33; int8 1.10).  Of its
+// time staging takes a fifth (the writes to LDS most of it), the exponentials an eighth; weights among the wave's own products,
 // in place of the other wave's, were even, and with that the waves half a tile apart 60 % slower (they spill).
 //
 // What is rounded, and where:
@@ -22,8 +22,7 @@
 //              no conversion and half the LDS.
 //   MXFP4 keys the codes go in as they are too, with their scale bytes, against the same parts of Q (in the order that the lanes of a
 //              4-bit operand have); c multiplies the score in fp32.  Q in two 6-bit parts, at the 4-bit rate, was 2.5-4 % faster
-//              and off by up to 2^-10 of a block's largest (error against 64 bits 2.0e-3 for 1.6e-3); in three, exact to 1/128 of
-//              it, 2-4 % slower, the registers' doing.
+//              and off by up to 2^-10 of a block's largest; in three 2-4 % slower, the registers' doing.
 //   int8 keys  the codes are exact in bf16, as Q is.
 //   V          the codes are exact in fp16; MXFP4 with its scale, exact, as fp16 or as bf16 (below).
 //   weights    fp16(p s_v), the product in fp32: 11 significant bits, eight times finer than bf16.  p is relative to a reference
@@ -31,12 +30,13 @@
 //              lost below 2^-20 of it, 2^-31 of it at most.  (The scale in V instead, under an exponent that the tile shares,
 //              saves an instruction a score, but there a key that a row does not see, or gives no weight, takes the bits of
 //              those that it does.)  The row sum adds the p in fp32.
-//              MXFP4: fp16(p) where every scale of V in the workgroup's range of keys is 2^-19 .. 2^12, which a look at them shows first
-//              (V of N(0, 1) has 2^-1 and 2^0).  Else bf16(p), 8 bits at any size: the reference then lies so far above the row's maximum
-//              that the sum of all p is at most 1 (attn_batch.hpp: headroom), and V may have any scale.  The reference moves where a tile's sum
-//              passes a bound, so for most tiles the weights are an exponential, a sum and half a conversion a score.  (bf16 alone: 2 % less
-//              time over 3 x 37440 keys, 3.5 % over 8 x 8192, and an error of 2.3e-3 against 64 bits where fp16 gives 1.67e-3 and the
-//              rounding of the results 1.66e-3: N(0, 1) rows over 4096 keys.)
+//              MXFP4: fp16(p) where every scale of V in the workgroup's range of keys is 2^-19 .. 2^12 (a look at them first; V of
+//              N(0, 1) has 2^-1 and 2^0).  Else bf16(p), 8 bits at any size: the reference then lies so far above the row's maximum
+//              that the sum of all p is at most 1 (attn_batch.hpp: headroom), and V may have any scale.  The reference moves where
+//              a tile's sum passes a bound, so for most tiles the weights are an exponential, a sum and half a conversion a
+//              score.  bf16 alone took 2 % less time over 3 x 37440 keys, 3.5 % over 8 x 8192, and was off by 2.3e-3 where fp16
+//              is by 1.67e-3, the rounding of the results being 1.66e-3 (N(0, 1) rows over 4096 keys).  Rows of V under one scale
+//              each, whatever it is, with p s as over 8-bit codes: 0-2 % slower than the look, blocks far below the row's largest lost.
 // A NaN or infinite scale makes the key's score NaN and its weight of V zero, so the rows that see the key become NaN and
 // no others; in tiles that some row does not see whole, so does a NaN code of V.
 #include <utility>

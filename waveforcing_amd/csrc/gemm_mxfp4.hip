@@ -4,13 +4,13 @@
 //
 // Many rows (gemm_mxfp4_kernel): the K loop of the 8-bit products (gemm_w8a8.hip), whose 128 bytes of a row are here 256
 // values: operands by DMA into LDS, three stages (the 256-row tile and the smallest: four), a step of four sub-steps (the
-// 256-row tile: two), the next sub-step's fragments read and a later step's DMAs issued between the matrix instructions.  A panel (16 rows x 128 values, 1 KB in the
-// order of the lanes) is one DMA, and 16 lanes' fragments are 256 bytes in a row: no swizzle, and every place in LDS is a
-// constant from the lane's first.  The scales, a word a row and panel, come with their stage; the byte a lane needs is
-// 2 s + (its half) of the word: one shift a word, and the instruction's byte select.
+// 256-row tile: two), the next sub-step's fragments read and a later step's DMAs issued between the matrix instructions.  A panel
+// (16 rows x 128 values, 1 KB in the order of the lanes) is one DMA, and 16 lanes' fragments are 256 bytes in a row: no swizzle,
+// and every place in LDS is a constant from the lane's first.  The scales, a word a row and panel, come with their stage; the
+// byte a lane needs is 2 s + (its half) of the word: one shift a word, and the instruction's byte select.
 //
 // It is bound by the matrix cores and the power limit: 16384^3 at 4.9 PFLOP/s on N(0, 1) operands, 7.6 on zeros; 4680 x 13824 -> 5120
-// 158-162 us by box (4.1-4.2; whole rounds of 256 x 256 tiles, then smaller ones), 5120 -> 13824 173-180 (3.7-3.8).
+// 155-162 us by box (4.1-4.3; whole rounds of 256 x 256 tiles, then smaller ones), 5120 -> 13824 173-180 (3.7-3.8).
 //
 // Few rows, or a small output (gemm_mxfp4_few_kernel): bound by reading the weight once, or by the way from the first load to
 // the last store.  A workgroup takes 16 or 32 columns (64 in one case) and 16 or 32 rows; its waves split K and go without
