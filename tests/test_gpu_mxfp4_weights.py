@@ -123,3 +123,28 @@ def test_far_scales_that_no_row_sees_change_nothing(page):
     batch.tables[1, 0] = pool.pool_pages               # no page: zeros, whatever the others hold
     out = backend.attn_paged_batch(q, batch, block=1)
     assert torch.equal(out[:100], clean[:100]) and bool((out[100:100 + min(page, 150)] == 0).all())
+
+
+def test_captured_attention_follows_the_scales():
+    """A captured call replayed while V's scales leave what fp16 holds and come back, on two streams' graphs in turn."""
+    pool, batch, g = make(2, 64, [900, 200], [150, 70], 11)
+    q = queries(batch.n_new, 4, g)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        backend.attn_paged_batch(q, batch, block=1)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(backend.attn_paged_batch(q, batch, block=1))
+    for byte in (125, 200, 125, 60, 252, 125):
+        pool.v_scales[batch.pages[0][3], :, 17, 1] = byte
+        q.copy_(queries(batch.n_new, 4, g))
+        want = backend.attn_paged_batch(q, batch, block=1)
+        check(want, q, pool, batch, 1)
+        torch.cuda.synchronize()
+        for i, graph in enumerate(graphs):
+            with torch.cuda.stream(side if i else torch.cuda.current_stream()):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
